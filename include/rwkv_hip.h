@@ -562,6 +562,93 @@ int rwkv7_backward_f32(void* stream, int B, int T, int H,
                        const float* s, const float* sa,
                        float* dr, float* dw, float* dk, float* dv, float* da, float* db);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Sequence mixers beside the WKV family, without a counterpart in the reference: an elementwise gated recurrence, attention,
+ * and the attention of one new token over a paged cache.  Their arguments come in a struct.  Strides are counted in elements,
+ * the innermost dimension is dense, tensors named without strides are dense; a pointer is aligned to its element type unless
+ * said otherwise. */
+enum { RWKV_DTYPE_BF16 = 0, RWKV_DTYPE_FP16 = 1, RWKV_DTYPE_FP32 = 2 };
+enum { RWKV_GATE_SIGMOID = 0, RWKV_GATE_LOG = 1 };
+
+/* Gated recurrence, channel by channel:  h_t = a_t h_{t-1} + u_t,  y_t = h_t,
+ * a_t = sigmoid(w_t) or exp(w_t) (gate), u_t = (1 - a_t) x_t (tied) or x_t.  h_{-1} is h0, or 0 where that is NULL.
+ * doc (may be NULL): a token with doc < 0 is padding, y is 0 there and the state passes by it; a real token whose predecessor has
+ * another doc starts from a state of 0.  w, x, y (and dy, dw, dx) are of `dtype`, states are fp32; h0 and hT may be the same memory.
+ * The forward keeps in `saved` (may be NULL) what the backward needs beside w, x and doc; both may need a workspace. */
+typedef struct rwkv_grec_args {
+    int dtype, gate, tied;
+    int B, T, C;
+    const void* w;                    /* [B,T,C] with strides */
+    int64_t w_sb, w_st;
+    const void* x;                    /* [B,T,C] with strides */
+    int64_t x_sb, x_st;
+    const float* h0;                  /* [B,C] or NULL */
+    const int* doc;                   /* [B,T] or NULL */
+    void* y;                          /* forward: [B,T,C] */
+    float* hT;                        /* forward: [B,C] */
+    float* saved;                     /* 16-byte aligned */
+    size_t saved_bytes;
+    const void* dy;                   /* backward: [B,T,C] or NULL (zeros) */
+    const float* dhT;                 /* backward: [B,C] or NULL (zeros) */
+    void* dw;                         /* backward: [B,T,C] */
+    void* dx;                         /* backward: [B,T,C] */
+    float* dh0;                       /* backward: [B,C] or NULL */
+    void* workspace;                  /* 16-byte aligned */
+    size_t workspace_bytes;
+} rwkv_grec_args;
+size_t rwkv_grec_saved_bytes(int B, int T, int C);
+size_t rwkv_grec_workspace_bytes(int B, int T, int C);
+int rwkv_grec_forward(void* stream, const rwkv_grec_args* args);
+int rwkv_grec_backward(void* stream, const rwkv_grec_args* args);
+
+/* Attention.  The Tq queries are the last of the Tk positions: query i stands at p = Tk - Tq + i.  Key head of head h: h Hk / H.
+ * s = scale q.k;  s = cap tanh(s / cap) where cap > 0;  s -= slopes[h] |p - j|;  y = softmax(s) v over the visible keys j:
+ * all of them, or with `causal` those with j <= p or j < prefix[b]; with doc only those of the query's own doc, and none where that is
+ * negative.  A query that sees nothing has y = 0.  N is a multiple of 8 up to 128; q, k, v are bf16 or fp16, 16-byte aligned with strides
+ * that are multiples of 8.  y_rest (may be NULL): what y lost when it was rounded, for the backward; lse: log of the sum of exp(s), [B,H,Tq]. */
+typedef struct rwkv_attn_args {
+    int dtype, causal;
+    int B, Tq, Tk, H, Hk, N;
+    float scale, cap;
+    const void *q, *k, *v;            /* [B,Tq,H,N], [B,Tk,Hk,N], [B,Tk,Hk,N] with strides */
+    int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+    const float* slopes;              /* [H] or NULL */
+    const int* doc;                   /* [B,Tk] or NULL */
+    const int* prefix;                /* [B] or NULL */
+    void* y;                          /* [B,Tq,H,N], 16-byte aligned; forward: written, backward: read */
+    void* y_rest;                     /* [B,Tq,H,N], 16-byte aligned */
+    float* lse;                       /* [B,H,Tq]; forward: may be NULL */
+    const void* dy;                   /* backward: [B,Tq,H,N], 16-byte aligned */
+    void *dq, *dk, *dv;               /* backward: dense, 16-byte aligned */
+    void* workspace;                  /* backward; 16-byte aligned */
+    size_t workspace_bytes;
+} rwkv_attn_args;
+size_t rwkv_attn_backward_workspace_bytes(int B, int Tq, int H);
+int rwkv_attn_forward(void* stream, const rwkv_attn_args* args);
+int rwkv_attn_backward(void* stream, const rwkv_attn_args* args);
+
+/* Attention of one new token a sequence over a cache in pages: sequence b has lens[b] tokens, the new one's position is lens[b] - 1, token t
+ * is row t % page of page table[b][t / page].  Scores and key heads as above.  lens[b] <= 0: y = 0; more tokens than the table has
+ * pages for are not seen; tokens of a page whose number is not in 0 .. P-1 are not seen.  k, v (may be NULL): the new token's key and value,
+ * which are written to the cache at lens[b] - 1 and seen; a page that is written belongs to one sequence.  page is a power of two. */
+typedef struct rwkv_paged_args {
+    int dtype;
+    int B, H, Hk, N, P, page, M;
+    float scale, cap;
+    const void* q;                    /* [B,H,N], 16-byte aligned */
+    void *k_pages, *v_pages;          /* [P,page,Hk,N] with strides, 16-byte aligned, strides multiples of 8 */
+    int64_t k_sp, k_st, k_sh, v_sp, v_st, v_sh;
+    const int* table;                 /* [B,M] */
+    const int* lens;                  /* [B] */
+    const float* slopes;              /* [H] or NULL */
+    const void *k, *v;                /* [B,Hk,N], 16-byte aligned, or both NULL */
+    void* y;                          /* [B,H,N], 16-byte aligned */
+    void* workspace;                  /* 16-byte aligned */
+    size_t workspace_bytes;
+} rwkv_paged_args;
+size_t rwkv_paged_workspace_bytes(int B, int H, int Hk, int N, int page, int M);
+int rwkv_paged_attn(void* stream, const rwkv_paged_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,7 +18,7 @@ _INCLUDE = os.path.join(_ROOT, "include")
 LIB_PATH = os.path.join(_HERE, "librwkv_hip.so")
 HASH_PATH = LIB_PATH + ".srchash"        # digest of the sources the library was built from (content, not mtime)
 
-SOURCES = ["abi.hip", "wkv56.hip", "wkv6_fwd.hip", "wkv6_bwd_a.hip", "wkv6_bwd_b.hip", "wkv6_fwd_f.hip", "wkv6_bwd_f.hip", "wkv6_local.hip", "wkv4.hip", "timex.hip", "wkv5_f32.hip", "wkv5_bf.hip", "rwkv7.hip", "rwkv7_chunk.hip"]
+SOURCES = ["abi.hip", "wkv56.hip", "wkv6_fwd.hip", "wkv6_bwd_a.hip", "wkv6_bwd_b.hip", "wkv6_fwd_f.hip", "wkv6_bwd_f.hip", "wkv6_local.hip", "wkv4.hip", "timex.hip", "wkv5_f32.hip", "wkv5_bf.hip", "rwkv7.hip", "rwkv7_chunk.hip", "grec.hip", "attn.hip", "paged.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
@@ -117,6 +117,20 @@ _I = ctypes.c_int
 _F = ctypes.c_float
 _Z = ctypes.c_size_t
 _U = ctypes.c_uint
+_L = ctypes.c_int64
+
+
+def _struct(name, *groups):
+    """A ctypes structure of the header: (type, names) pairs in its order."""
+    return type(name, (ctypes.Structure,), {"_fields_": [(n, t) for t, names in groups for n in names.split()]})
+
+
+GrecArgs = _struct("GrecArgs", (_I, "dtype gate tied B T C"), (_P, "w"), (_L, "w_sb w_st"), (_P, "x"), (_L, "x_sb x_st"), (_P, "h0 doc y hT saved"), (_Z, "saved_bytes"),
+                   (_P, "dy dhT dw dx dh0 workspace"), (_Z, "workspace_bytes"))
+AttnArgs = _struct("AttnArgs", (_I, "dtype causal B Tq Tk H Hk N"), (_F, "scale cap"), (_P, "q k v"), (_L, "q_sb q_st q_sh k_sb k_st k_sh v_sb v_st v_sh"),
+                   (_P, "slopes doc prefix y y_rest lse dy dq dk dv workspace"), (_Z, "workspace_bytes"))
+PagedArgs = _struct("PagedArgs", (_I, "dtype B H Hk N P page M"), (_F, "scale cap"), (_P, "q k_pages v_pages"), (_L, "k_sp k_st k_sh v_sp v_st v_sh"),
+                    (_P, "table lens slopes k v y workspace"), (_Z, "workspace_bytes"))
 
 # name -> (restype, argtypes): one row per symbol in include/rwkv_hip.h
 SIGNATURES = {
@@ -212,6 +226,15 @@ SIGNATURES = {
     "rwkv7_state_backward_f32": (_I, [_P, _I, _I, _I] + [_P] * 16),
     "rwkv7_forward_f32": (_I, [_P, _I, _I, _I] + [_P] * 9),
     "rwkv7_backward_f32": (_I, [_P, _I, _I, _I] + [_P] * 15),
+    "rwkv_grec_saved_bytes": (_Z, [_I, _I, _I]),
+    "rwkv_grec_workspace_bytes": (_Z, [_I, _I, _I]),
+    "rwkv_grec_forward": (_I, [_P, ctypes.POINTER(GrecArgs)]),
+    "rwkv_grec_backward": (_I, [_P, ctypes.POINTER(GrecArgs)]),
+    "rwkv_attn_backward_workspace_bytes": (_Z, [_I, _I, _I]),
+    "rwkv_attn_forward": (_I, [_P, ctypes.POINTER(AttnArgs)]),
+    "rwkv_attn_backward": (_I, [_P, ctypes.POINTER(AttnArgs)]),
+    "rwkv_paged_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I]),
+    "rwkv_paged_attn": (_I, [_P, ctypes.POINTER(PagedArgs)]),
 }
 
 

@@ -484,6 +484,219 @@ Tensor rwkv7_op(const Tensor& r, const Tensor& w, const Tensor& k, const Tensor&
     return Rwkv7::apply(r, w, k, v, a, b, flags, flat, wants_grad({&r, &w, &k, &v, &a, &b}))[0];
 }
 
+// --------------------------------------------------------------------------------------------- gated recurrence, attention, paged attention
+using Maybe = c10::optional<Tensor>;
+Tensor or_none(const Maybe& t) { return t.has_value() ? *t : Tensor(); }
+int dtype_of(const Tensor& t, const char* n, bool with_f32) {
+    const auto d = t.scalar_type();
+    require(d == BF || d == torch::kFloat16 || (with_f32 && d == F32), std::string(n) + ".dtype must be torch.bfloat16" + (with_f32 ? ", torch.float16 or torch.float32" : " or torch.float16") + ", got " + str(d));
+    return d == BF ? RWKV_DTYPE_BF16 : (d == F32 ? RWKV_DTYPE_FP32 : RWKV_DTYPE_FP16);
+}
+// one device, one dtype, a dense innermost dimension
+void check_rows(std::initializer_list<std::pair<const Tensor*, const char*>> ts, const Tensor& first) {
+    for (const auto& t : ts) {
+        const Tensor& x = *t.first;
+        const std::string n = t.second;
+        require(x.is_cuda() && first.is_cuda(), "tensors must live on a HIP device: there is no CPU path");
+        require(x.device() == first.device(), n + " is on " + x.device().str() + ", expected " + first.device().str());
+        require(x.scalar_type() == first.scalar_type(), n + ".dtype must be " + str(first.scalar_type()) + ", got " + str(x.scalar_type()));
+        require(x.stride(-1) == 1 || x.size(-1) == 1, n + " must be dense in its last dimension");
+    }
+}
+// an optional dense tensor of a given shape beside `first`
+void check_side(const Tensor& x, const char* n, c10::ScalarType dt, at::IntArrayRef shape, const Tensor& first) {
+    if (!x.defined()) return;
+    check({{&x, n}}, dt, first);
+    require(x.sizes() == shape, std::string(n) + " has the wrong shape");
+}
+// the strides of a dimension of size 1 are arbitrary: 0 for the kernels' checks
+int64_t stride_of(const Tensor& x, int64_t d) { return x.size(d) == 1 ? 0 : x.stride(d); }
+void once_only(const char* n) {
+    if (c10::GradMode::is_enabled()) fail(std::string(n) + " has no second derivatives: its backward cannot run with create_graph");
+}
+
+rwkv_grec_args grec_args(const Tensor& w, const Tensor& x, int64_t gate, bool tied) {
+    rwkv_grec_args a{};
+    a.dtype = dtype_of(w, "w", true);
+    a.gate = static_cast<int>(gate);
+    a.tied = tied;
+    a.B = i32(w.size(0)); a.T = i32(w.size(1)); a.C = i32(w.size(2));
+    a.w = w.data_ptr(); a.w_sb = stride_of(w, 0); a.w_st = stride_of(w, 1);
+    a.x = x.data_ptr(); a.x_sb = stride_of(x, 0); a.x_st = stride_of(x, 1);
+    return a;
+}
+struct Grec : Function<Grec> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& w, const Tensor& x, const Maybe& h0_, const Maybe& doc_, int64_t gate, bool tied, bool grad) {
+        const Tensor h0 = or_none(h0_), doc = or_none(doc_);
+        require(w.dim() == 3 && x.sizes() == w.sizes(), "w and x are [B,T,C]");
+        check_rows({{&w, "w"}, {&x, "x"}}, w);
+        const int64_t B = w.size(0), T = w.size(1), C = w.size(2);
+        check_side(h0, "h0", F32, {B, C}, w);
+        check_side(doc, "doc", torch::kInt32, {B, T}, w);
+        const Guard guard(w.device());
+        rwkv_grec_args a = grec_args(w, x, gate, tied);
+        Tensor y = at::empty({B, T, C}, w.options()), hT = at::empty({B, C}, w.options().dtype(F32)), saved;
+        a.h0 = P(h0); a.doc = P(doc); a.y = P(y); a.hT = P(hT);
+        if (grad) {
+            a.saved_bytes = rwkv_grec_saved_bytes(a.B, a.T, a.C);
+            saved = bytes(w, a.saved_bytes);
+            a.saved = P(saved);
+        }
+        a.workspace_bytes = rwkv_grec_workspace_bytes(a.B, a.T, a.C);
+        const Tensor ws = a.workspace_bytes > 0 ? bytes(w, a.workspace_bytes) : Tensor();
+        a.workspace = P(ws);
+        ok(rwkv_grec_forward(stream_of(w), &a));
+        if (grad) ctx->save_for_backward({w, x, doc, saved});
+        put(ctx, {{"gate", gate}, {"tied", tied}, {"state", h0.defined()}});
+        ctx->set_materialize_grads(false);
+        return {y, hT};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        once_only("gated_recurrence");
+        const auto s = ctx->get_saved_variables();
+        const Tensor &w = s[0], &x = s[1], &doc = s[2], &saved = s[3];
+        const Tensor dy = g[0].defined() ? g[0].contiguous() : Tensor(), dhT = g[1].defined() ? g[1].contiguous() : Tensor();
+        const Guard guard(w.device());
+        rwkv_grec_args a = grec_args(w, x, get(ctx, "gate"), get(ctx, "tied") != 0);
+        Tensor dw = at::empty(w.sizes(), w.options()), dx = at::empty(w.sizes(), w.options());
+        Tensor dh0 = get(ctx, "state") ? at::empty({a.B, a.C}, w.options().dtype(F32)) : Tensor();
+        a.doc = P(doc); a.saved = P(saved); a.saved_bytes = saved.numel();
+        a.dy = P(dy); a.dhT = P(dhT); a.dw = P(dw); a.dx = P(dx); a.dh0 = P(dh0);
+        a.workspace_bytes = rwkv_grec_workspace_bytes(a.B, a.T, a.C);
+        const Tensor ws = a.workspace_bytes > 0 ? bytes(w, a.workspace_bytes) : Tensor();
+        a.workspace = P(ws);
+        ok(rwkv_grec_backward(stream_of(w), &a));
+        return {dw, dx, dh0, NONE, NONE, NONE, NONE};
+    }
+};
+std::tuple<Tensor, Tensor> grec_op(const Tensor& w, const Tensor& x, const Maybe& h0, const Maybe& doc, int64_t gate, bool tied) {
+    const Tensor h = or_none(h0);
+    variable_list o = Grec::apply(w, x, h0, doc, gate, tied, wants_grad({&w, &x}) || (h.defined() && wants_grad({&h})));
+    return {o[0], o[1]};
+}
+Tensor grec_step_op(const Tensor& w, const Tensor& x, const Tensor& h, const Tensor& out, int64_t gate, bool tied) {
+    require(!wants_grad({&w, &x, &h, &out}), "STEP has no gradients: call it under torch.no_grad()");
+    require(w.dim() == 2 && x.sizes() == w.sizes(), "w and x are [B,C]");
+    const Tensor w3 = w.unsqueeze(1), x3 = x.unsqueeze(1);
+    check_rows({{&w, "w"}, {&x, "x"}}, w);
+    check_side(h, "h", F32, w.sizes(), w);
+    check_side(out, "out", F32, w.sizes(), w);
+    const Guard guard(w.device());
+    rwkv_grec_args a = grec_args(w3, x3, gate, tied);
+    Tensor y = at::empty(w.sizes(), w.options());
+    a.h0 = P(h); a.hT = P(out); a.y = P(y);
+    a.workspace_bytes = rwkv_grec_workspace_bytes(a.B, a.T, a.C);
+    const Tensor ws = a.workspace_bytes > 0 ? bytes(w, a.workspace_bytes) : Tensor();
+    a.workspace = P(ws);
+    ok(rwkv_grec_forward(stream_of(w), &a));
+    return y;
+}
+
+float scale_of(const c10::optional<double>& scale, int64_t N) { return static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(N))); }
+rwkv_attn_args attn_args(const Tensor& q, const Tensor& k, const Tensor& v, double cap, double scale, bool causal) {
+    rwkv_attn_args a{};
+    a.dtype = dtype_of(q, "q", false);
+    a.causal = causal;
+    a.B = i32(q.size(0)); a.Tq = i32(q.size(1)); a.H = i32(q.size(2)); a.N = i32(q.size(3));
+    a.Tk = i32(k.size(1)); a.Hk = i32(k.size(2));
+    a.scale = static_cast<float>(scale); a.cap = static_cast<float>(cap);
+    a.q = q.data_ptr(); a.q_sb = stride_of(q, 0); a.q_st = stride_of(q, 1); a.q_sh = stride_of(q, 2);
+    a.k = k.data_ptr(); a.k_sb = stride_of(k, 0); a.k_st = stride_of(k, 1); a.k_sh = stride_of(k, 2);
+    a.v = v.data_ptr(); a.v_sb = stride_of(v, 0); a.v_st = stride_of(v, 1); a.v_sh = stride_of(v, 2);
+    return a;
+}
+struct Attn : Function<Attn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& doc_, const Maybe& prefix_, const Maybe& slopes_, double cap,
+                          double scale, bool causal, bool grad) {
+        const Tensor doc = or_none(doc_), prefix = or_none(prefix_), slopes = or_none(slopes_);
+        const int64_t B = q.size(0), Tq = q.size(1), H = q.size(2), N = q.size(3), Tk = k.size(1);
+        check_side(doc, "doc", torch::kInt32, {B, Tk}, q);
+        check_side(prefix, "prefix", torch::kInt32, {B}, q);
+        check_side(slopes, "slopes", F32, {H}, q);
+        const Guard guard(q.device());
+        rwkv_attn_args a = attn_args(q, k, v, cap, scale, causal);
+        Tensor y = at::empty({B, Tq, H, N}, q.options()), rest, lse;
+        a.doc = P(doc); a.prefix = P(prefix); a.slopes = P(slopes); a.y = P(y);
+        if (grad) {
+            rest = at::empty_like(y);
+            lse = at::empty({B, H, Tq}, q.options().dtype(F32));
+            a.y_rest = P(rest); a.lse = P(lse);
+        }
+        ok(rwkv_attn_forward(stream_of(q), &a));
+        if (grad) ctx->save_for_backward({q, k, v, doc, prefix, slopes, y, rest, lse});
+        ctx->saved_data["cap"] = cap;
+        ctx->saved_data["scale"] = scale;
+        put(ctx, {{"causal", causal}});
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        once_only("attention");
+        const auto s = ctx->get_saved_variables();
+        const Tensor &q = s[0], &k = s[1], &v = s[2], &y = s[6], &rest = s[7], &lse = s[8], dy = g[0].contiguous();
+        const Guard guard(q.device());
+        rwkv_attn_args a = attn_args(q, k, v, ctx->saved_data["cap"].toDouble(), ctx->saved_data["scale"].toDouble(), get(ctx, "causal") != 0);
+        Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
+        a.doc = P(s[3]); a.prefix = P(s[4]); a.slopes = P(s[5]); a.y = P(y); a.y_rest = P(rest); a.lse = P(lse);
+        a.dy = P(dy); a.dq = P(dq); a.dk = P(dk); a.dv = P(dv);
+        a.workspace_bytes = rwkv_attn_backward_workspace_bytes(a.B, a.Tq, a.H);
+        const Tensor ws = bytes(q, a.workspace_bytes);
+        a.workspace = P(ws);
+        ok(rwkv_attn_backward(stream_of(q), &a));
+        return {dq, dk, dv, NONE, NONE, NONE, NONE, NONE, NONE, NONE};
+    }
+};
+Tensor attention_op(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& doc, const Maybe& prefix, const Maybe& slopes, double cap,
+                    c10::optional<double> scale, bool causal) {
+    require(q.dim() == 4 && k.dim() == 4 && v.sizes() == k.sizes(), "q is [B,Tq,H,N], k and v are [B,Tk,Hk,N]");
+    check_rows({{&q, "q"}, {&k, "k"}, {&v, "v"}}, q);
+    const int64_t N = q.size(3);
+    require(k.size(0) == q.size(0) && k.size(3) == N && k.size(1) >= q.size(1), "q is [B,Tq,H,N], k and v are [B,Tk,Hk,N] with Tk >= Tq");
+    require(k.size(2) > 0 && q.size(2) % k.size(2) == 0, "H must be a multiple of Hk");
+    require(N >= 8 && N <= MAX_HEAD && N % 8 == 0, "the head size must be a multiple of 8 up to 128");
+    require(causal || !prefix.has_value(), "prefix goes with causal");
+    require(cap >= 0.0 && std::isfinite(cap), "cap must be 0 or positive");
+    const float sc = scale_of(scale, N);
+    require(sc > 0.f && std::isfinite(sc), "scale must be positive");
+    require(!slopes.has_value() || !wants_grad({&*slopes}), "slopes have no gradient");
+    return Attn::apply(q, k, v, doc, prefix, slopes, cap, static_cast<double>(sc), causal, wants_grad({&q, &k, &v}));
+}
+
+Tensor paged_op(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& lens, const Maybe& k_, const Maybe& v_, const Maybe& slopes_,
+                double cap, c10::optional<double> scale) {
+    const Tensor k = or_none(k_), v = or_none(v_), slopes = or_none(slopes_);
+    require(!wants_grad({&q, &kp, &vp}) && !(k.defined() && wants_grad({&k})) && !(v.defined() && wants_grad({&v})), "paged_attention has no gradients: call it under torch.no_grad()");
+    require(q.dim() == 3 && kp.dim() == 4 && vp.sizes() == kp.sizes(), "q is [B,H,N], k_pages and v_pages are [P,page,Hk,N]");
+    const int64_t B = q.size(0), H = q.size(1), N = q.size(2), page = kp.size(1), Hk = kp.size(2);
+    check({{&q, "q"}}, q.scalar_type(), q);
+    check_rows({{&q, "q"}, {&kp, "k_pages"}, {&vp, "v_pages"}}, q);
+    require(kp.size(3) == N && Hk > 0 && H % Hk == 0, "H must be a multiple of Hk, and the head size that of the pages");
+    require(N >= 8 && N <= MAX_HEAD && N % 8 == 0, "the head size must be a multiple of 8 up to 128");
+    require(page > 0 && (page & (page - 1)) == 0, "page must be a power of two");
+    require(table.dim() == 2, "table is [B,M]");
+    check_side(table, "table", torch::kInt32, {B, table.size(1)}, q);
+    check_side(lens, "lens", torch::kInt32, {B}, q);
+    check_side(slopes, "slopes", F32, {H}, q);
+    require(k.defined() == v.defined(), "k and v go together");
+    check_side(k, "k", q.scalar_type(), {B, Hk, N}, q);
+    check_side(v, "v", q.scalar_type(), {B, Hk, N}, q);
+    require(cap >= 0.0 && std::isfinite(cap), "cap must be 0 or positive");
+    const Guard guard(q.device());
+    rwkv_paged_args a{};
+    a.dtype = dtype_of(q, "q", false);
+    a.B = i32(B); a.H = i32(H); a.Hk = i32(Hk); a.N = i32(N); a.P = i32(kp.size(0)); a.page = i32(page); a.M = i32(table.size(1));
+    a.scale = scale_of(scale, N); a.cap = static_cast<float>(cap);
+    require(a.scale > 0.f && std::isfinite(a.scale), "scale must be positive");
+    a.k_sp = stride_of(kp, 0); a.k_st = stride_of(kp, 1); a.k_sh = stride_of(kp, 2);
+    a.v_sp = stride_of(vp, 0); a.v_st = stride_of(vp, 1); a.v_sh = stride_of(vp, 2);
+    Tensor y = at::empty({B, H, N}, q.options());
+    a.q = P(q); a.k_pages = P(kp); a.v_pages = P(vp); a.table = P(table); a.lens = P(lens); a.slopes = P(slopes); a.k = P(k); a.v = P(v); a.y = P(y);
+    a.workspace_bytes = rwkv_paged_workspace_bytes(a.B, a.H, a.Hk, a.N, a.page, a.M);
+    const Tensor ws = a.workspace_bytes > 0 ? bytes(q, a.workspace_bytes) : Tensor();
+    a.workspace = P(ws);
+    ok(rwkv_paged_attn(stream_of(q), &a));
+    return y;
+}
+
 }  // namespace
 
 void bind_autograd(py::module_& m) {
@@ -498,4 +711,8 @@ void bind_autograd(py::module_& m) {
     ops.def("rwkv7_passing", &rwkv7_passing_op);
     ops.def("rwkv7_state", &rwkv7_state_op);
     ops.def("rwkv7", &rwkv7_op);
+    ops.def("gated_recurrence", &grec_op);
+    ops.def("gated_recurrence_step", &grec_step_op);
+    ops.def("attention", &attention_op);
+    ops.def("paged_attention", &paged_op);
 }

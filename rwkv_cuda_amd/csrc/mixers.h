@@ -1,0 +1,19 @@
+// What the gated recurrence, attention and paged attention share: the element types, and their conversions, which round to nearest even.
+#pragma once
+
+#include "common.h"
+
+namespace rwkv {
+
+struct bf16_t { uint16_t bits; };
+typedef _Float16 half_t;
+
+DEVINL float to_f(bf16_t x) { return bf2f(x.bits); }
+DEVINL float to_f(half_t x) { return static_cast<float>(x); }
+DEVINL float to_f(float x) { return x; }
+template <class E> DEVINL E from_f(float x) {
+    if constexpr (std::is_same_v<E, bf16_t>) return {f2bf(x)};
+    else return static_cast<E>(x);
+}
+
+}  // namespace rwkv

@@ -1,0 +1,183 @@
+"""GPU: attention against its 64-bit definition, with bounds element by element."""
+import pytest
+import torch
+
+from oracle import mixers as O
+from rwkv_cuda_amd import attention as A
+from _gpu_util import DEV
+from _mixers_util import DT, doc_ids, graph_of, randn, within
+
+pytestmark = pytest.mark.gpu
+
+
+def inputs(B, Tq, Tk, H, Hk, N, dt, seed=0, scale=1.0):
+    return [randn(*s, seed=seed + i, scale=scale).to(dt).to(DEV) for i, s in enumerate([(B, Tq, H, N), (B, Tk, Hk, N), (B, Tk, Hk, N), (B, Tq, H, N)])]
+
+
+def check(q, k, v, dy, seen=None, **how):
+    """`seen`: the tensors that the oracle gets instead of q, k, v."""
+    t = [z.detach().requires_grad_(True) for z in (q, k, v)]
+    y = A.RUN_CUDA(*t, **how)
+    assert y.is_contiguous() and y.dtype == q.dtype
+    grads = torch.autograd.grad([y], t, [dy])
+    with torch.no_grad():
+        assert torch.equal(y, A.RUN_CUDA(q, k, v, **how))
+    torch.cuda.synchronize()
+    want = O.attention(*(seen or (q, k, v)), dy=dy, **how)
+    for n, got in zip(["y", "dq", "dk", "dv"], [y] + list(grads)):
+        within(n, got, want[n])
+
+
+SHAPES = [(1, 1, 1, 1, 1, 64), (2, 1, 70, 2, 1, 64), (1, 2, 2, 2, 2, 128), (2, 31, 31, 2, 1, 64), (1, 32, 33, 4, 1, 128), (2, 64, 64, 1, 1, 64), (1, 65, 65, 3, 3, 64),
+          (1, 100, 227, 4, 2, 128), (2, 127, 127, 2, 2, 128), (1, 129, 129, 8, 1, 64), (1, 255, 300, 2, 1, 96), (1, 257, 257, 2, 2, 80), (2, 300, 300, 2, 1, 40), (1, 200, 200, 2, 2, 8),
+          (1, 520, 520, 6, 2, 128), (1, 777, 777, 2, 2, 64), (1, 5, 1500, 4, 2, 64)]
+
+
+@pytest.mark.parametrize("B,Tq,Tk,H,Hk,N", SHAPES)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("causal", [True, False])
+def test_against_the_definition(lib, B, Tq, Tk, H, Hk, N, dtype, causal):
+    print(f"\n{B} {Tq} {Tk} {H} {Hk} {N} {dtype} {causal}", flush=True)
+    check(*inputs(B, Tq, Tk, H, Hk, N, DT[dtype]), causal=causal)
+
+
+HOW = {"cap": dict(cap=2.0), "bias": dict(bias=True), "cap and bias": dict(cap=5.0, bias=True), "wide bias": dict(bias=True, causal=False), "prefix": dict(prefix=True),
+       "prefix and bias": dict(prefix=True, bias=True), "two documents": dict(doc="two"), "many documents": dict(doc="many"), "padding": dict(doc="padded"),
+       "single tokens": dict(doc="one"), "ids that come back": dict(doc="back"), "wide documents": dict(doc="padded", causal=False),
+       "all": dict(doc="padded", prefix=True, cap=3.0, bias=True)}
+
+
+@pytest.mark.parametrize("how", list(HOW))
+@pytest.mark.parametrize("B,Tq,Tk,H,Hk,N,dtype", [(2, 90, 90, 2, 1, 64, "bf16"), (3, 200, 333, 4, 2, 128, "fp16"), (2, 400, 400, 2, 2, 64, "bf16"), (2, 1, 150, 2, 1, 128, "bf16")])
+def test_masks_caps_and_biases(lib, how, B, Tq, Tk, H, Hk, N, dtype):
+    print(f"\n{how} {B} {Tq} {Tk} {H} {Hk} {N} {dtype}", flush=True)
+    o = dict(HOW[how])
+    if o.pop("bias", False):
+        o["slopes"] = torch.exp2(-torch.arange(1.0, H + 1)).to(DEV)
+    if "doc" in o:
+        o["doc"] = doc_ids(B, Tk, o["doc"], seed=Tk).to(DEV)
+    if o.pop("prefix", False):
+        o["prefix"] = torch.tensor([Tk // 3, Tk + 5, 0][:B], dtype=torch.int32, device=DEV)
+    check(*inputs(B, Tq, Tk, H, Hk, N, DT[dtype], seed=7), **o)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_large_scores(lib, dtype):
+    """Scores in the hundreds, of either sign: nothing overflows, and rows that are one key's alone."""
+    q, k, v, dy = inputs(1, 150, 150, 2, 2, 64, DT[dtype], seed=3, scale=8.0)
+    check(q, k, v, dy, scale=1.0)
+    check(q, k, v, dy, scale=1.0, cap=30.0)
+    check(q, -k.abs(), v, dy, scale=1.0)
+
+
+def test_views_of_one_projection(lib):
+    B, T, H, Hk, N = 2, 140, 4, 2, 64
+    x = randn(B, T, (H + 2 * Hk) * N, seed=5).to(torch.bfloat16).to(DEV)
+    q, k, v = (z.unflatten(2, (-1, N)) for z in x.split([H * N, Hk * N, Hk * N], 2))
+    dy = randn(B, T, H, N, seed=6).to(torch.bfloat16).to(DEV)
+    check(q, k, v, dy)
+    heads_first = [z.transpose(1, 2).contiguous().transpose(1, 2) for z in (q, k, v)]
+    check(*heads_first, dy)
+    y = A.RUN_CUDA(q, k, v)
+    assert torch.equal(y, A.RUN_CUDA(*heads_first)) and torch.equal(y, A.RUN_CUDA(*(z.contiguous() for z in (q, k, v))))
+    one = x[:, :, :N].unsqueeze(2).expand(B, T, H, N)                # a broadcast query: its gradient is the sum over the heads
+    t = [z.detach().requires_grad_(True) for z in (x[:, :, :N].contiguous(), k, v)]
+    y = A.RUN_CUDA(t[0].unsqueeze(2).expand(B, T, H, N), t[1], t[2])
+    got = torch.autograd.grad([y], t, [dy])
+    t2 = [z.detach().contiguous().requires_grad_(True) for z in (one, k, v)]
+    want = torch.autograd.grad([A.RUN_CUDA(*t2)], t2, [dy])
+    assert torch.equal(got[0], want[0].sum(2)) and torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_padding_of_any_value_reaches_nothing(lib, value):
+    B, T, H, Hk, N = 2, 190, 2, 1, 64
+    q, k, v, dy = inputs(B, T, T, H, Hk, N, torch.bfloat16, seed=11)
+    doc = torch.zeros(B, T, dtype=torch.int32, device=DEV)
+    doc[0, 150:] = -1
+    doc[1, :20] = -1
+    doc[1, 77:99] = -2
+    clean = [z.masked_fill((doc < 0)[:, :, None, None], 0.0) for z in (q, k, v, dy)]
+    dirty = [z.masked_fill((doc < 0)[:, :, None, None], value) for z in (q, k, v, dy)]
+    for causal in (True, False):
+        results = []
+        for z in (clean, dirty):
+            t = [a.detach().requires_grad_(True) for a in z[:3]]
+            y = A.RUN_CUDA(*t, doc=doc, causal=causal)
+            results.append([y.detach()] + list(torch.autograd.grad([y], t, [z[3]])))
+        for n, a, b in zip(["y", "dq", "dk", "dv"], *results):
+            assert torch.equal(a, b), n
+            assert not a[doc < 0].any(), n
+
+
+def test_the_same_bits_every_time_and_a_rows_own(lib):
+    """Each row of a batch is what it is alone."""
+    q, k, v, dy = inputs(3, 333, 333, 4, 2, 64, torch.bfloat16, seed=13)
+
+    def once(q, k, v, dy):
+        t = [z.detach().requires_grad_(True) for z in (q, k, v)]
+        y = A.RUN_CUDA(*t, cap=20.0)
+        return [y.detach()] + list(torch.autograd.grad([y], t, [dy]))
+    want = once(q, k, v, dy)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(want, once(q, k, v, dy)))
+    for b in range(3):
+        assert all(torch.equal(a[b:b + 1], c) for a, c in zip(want, once(*(z[b:b + 1] for z in (q, k, v, dy)))))
+
+
+def test_captured_and_replayed(lib):
+    q, k, v, dy = inputs(2, 310, 310, 4, 2, 128, torch.bfloat16, seed=17)
+    doc = doc_ids(2, 310, "two", seed=1).to(DEV)
+    t = [z.detach().clone().requires_grad_(True) for z in (q, k, v)]
+
+    def once():
+        y = A.RUN_CUDA(*t, doc=doc)
+        return [y.detach()] + list(torch.autograd.grad([y], t, [dy]))
+    (g1, o1), (g2, o2) = graph_of(once), graph_of(once)
+    for i in range(4):
+        with torch.no_grad():
+            for j, z in enumerate(t):
+                z.copy_(randn(*z.shape, seed=50 + 10 * i + j).to(z.dtype))
+            doc.copy_(doc_ids(2, 310, "padded" if i % 2 else "two", seed=i))
+        want = [z.clone() for z in once()]
+        g1.replay()
+        g2.replay()
+        torch.cuda.synchronize()
+        for o in (o1, o2):
+            assert all(torch.equal(a, b) for a, b in zip(want, o)), i
+
+
+def test_two_streams_at_once(lib):
+    cases = [inputs(2, 600, 600, 4, 4, 64, torch.bfloat16, seed=s) for s in (1, 2)]
+    want = [A.RUN_CUDA(*c[:3]) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(4):
+        got = []
+        for c, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                got.append(A.RUN_CUDA(*c[:3]))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_long_keys_and_tensors_beyond_2_31_elements(lib):
+    """A few queries of the end of a long text, of which the last part has a document of its own; the heads lie far apart."""
+    Tk, N = 70001, 64
+    k = torch.zeros(1, Tk, 1, N, device=DEV, dtype=torch.bfloat16)
+    k[:] = randn(Tk, 1, N, seed=1).to(DEV)
+    v = randn(1, Tk, 1, N, seed=2).to(torch.bfloat16).to(DEV)
+    q = randn(1, 3, 2, N, seed=3).to(torch.bfloat16).to(DEV)
+    doc = torch.zeros(1, Tk, dtype=torch.int32, device=DEV)
+    dy = randn(1, 3, 2, N, seed=4).to(torch.bfloat16).to(DEV)
+    check(q, k, v, dy)
+    doc[:, 69000:] = 1
+    check(q, k, v, dy, doc=doc)
+    big = torch.empty(2, Tk, 16 * 1024, device=DEV, dtype=torch.bfloat16)
+    assert big.numel() > 1 << 31
+    K, V = big[..., :N].unsqueeze(2), big[..., -N:].unsqueeze(2)
+    K.copy_(k.expand(2, -1, -1, -1))
+    V.copy_(v.expand(2, -1, -1, -1))
+    got = A.RUN_CUDA(q.expand(2, -1, -1, -1).contiguous(), K, V)
+    want = A.RUN_CUDA(q, k, v)
+    assert torch.equal(got[:1], want) and torch.equal(got[1:], want)
