@@ -181,7 +181,7 @@ template <class E> int attn_run(hipStream_t st, const rwkv_attn_args& p, bool ba
     const dim3 rows(p.Tq, p.H, p.B), block(64);
     float* delta = static_cast<float*>(p.workspace);
     if (!backward) {
-        hipLaunchKernelGGL((attn_rows_plain<E, false>), rows, block, 0, st, p, nullptr);
+        return launch_attn_fwd(st, p);
     } else {
         hipLaunchKernelGGL((attn_delta_plain<E>), rows, block, 0, st, p, delta);
         hipLaunchKernelGGL((attn_rows_plain<E, true>), rows, block, 0, st, p, delta);

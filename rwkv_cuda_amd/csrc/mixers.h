@@ -16,4 +16,7 @@ template <class E> DEVINL E from_f(float x) {
     else return static_cast<E>(x);
 }
 
+// attn_fwd.hip (arguments checked)
+int launch_attn_fwd(hipStream_t st, const rwkv_attn_args& p);
+
 }  // namespace rwkv
