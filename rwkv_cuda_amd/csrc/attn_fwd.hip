@@ -215,7 +215,7 @@ __global__ __launch_bounds__(256, QT * D > 128 ? 1 : 2) void attn_fwd(const rwkv
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
             store32<E>(o[z][d], f, static_cast<E*>(p.y) + at, p.y_rest ? static_cast<E*>(p.y_rest) + at : nullptr, 32 * d, p.N, on);
-        if (p.lse && on && hi == 0) p.lse[(wide(b) * p.H + h) * p.Tq + i] = sum == 0.f ? -INFINITY : fmaf(m[z], mul, __builtin_amdgcn_logf(sum)) / LOG2E;
+        if (p.lse && on && hi == 0) p.lse[(wide(b) * p.H + h) * p.Tq + i] = sum == 0.f ? -INFINITY : fmaf(m[z], mul, __builtin_amdgcn_logf(sum));
     }
 }
 

@@ -16,7 +16,8 @@ template <class E> DEVINL E from_f(float x) {
     else return static_cast<E>(x);
 }
 
-// attn_fwd.hip (arguments checked)
+// attn_fwd.hip, attn_bwd.hip (arguments checked)
 int launch_attn_fwd(hipStream_t st, const rwkv_attn_args& p);
+int launch_attn_bwd(hipStream_t st, const rwkv_attn_args& p);
 
 }  // namespace rwkv
