@@ -98,11 +98,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const rwkv_attn_args p, const 
         const int j0 = t * TILE, n = p.Tk - j0;
         ks.load(kbase + j0 * p.k_st, n, static_cast<int>(p.k_st) * 2, p.N);
         vs.load(vbase + j0 * p.v_st, n, static_cast<int>(p.v_st) * 2, p.N);
-        if constexpr (DOC) {
-            next_doc = tid < TILE && tid < n ? doc[j0 + tid] : -1;
-#pragma unroll
-            for (int s = 0; s < ks.STEPS; ++s) ks.keep(s, doc[min(j0 + ks.row + s * ks.STEP_ROWS, p.Tk - 1)] >= 0);      // the keys of padding may be anything
-        }
+        if constexpr (DOC) next_doc = lane < n ? doc[j0 + lane] : -1;
     };
     int par = 0;
     for (int w0 = 0; w0 < tiles; w0 += WINDOW) {
@@ -113,14 +109,15 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const rwkv_attn_args p, const 
             __syncthreads();
         }
         const auto skip = [&](int t) {
-            if constexpr (DOC) while (t < w1 && kind[t - w0] == 0) ++t;
-            return __builtin_amdgcn_readfirstlane(t);
+            if constexpr (DOC) return next_tile(kind, t, w0, w1);
+            return t;
         };
         int t = skip(w0);
         if (t < w1) load(t);
         while (t < w1) {
             const lds_t kb = lds + par * BUF, vb = kb + Plane<D>::BYTES;
-            ks.store(kb);
+            if constexpr (DOC) ks.store(kb, __ballot(next_doc >= 0));
+            else ks.store(kb);
             vs.store(vb);
             if (DOC && tid < TILE) key_doc[par][tid] = next_doc;
             const int now = t, j0 = t * TILE;
@@ -244,15 +241,7 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_dkv(const rwkv_att
             if (!on || next_lse == -INFINITY) next_lse = INFINITY, next_delta = 0.f;     // a row that is not there or sees nothing: weights of 0
             next_lse -= SHIFT<E>;
         }
-        if constexpr (DOC) {
-            next_doc = on ? max(doc[shift + i0 + tid], -1) : -1;     // no padding is any other's document
-#pragma unroll
-            for (int s = 0; s < qs.STEPS; ++s) {                 // the rows of padding may be anything
-                const bool there = doc[min(shift + i0 + qs.row + s * qs.STEP_ROWS, p.Tk - 1)] >= 0;
-                qs.keep(s, there);
-                ys.keep(s, there);
-            }
-        }
+        if constexpr (DOC) next_doc = lane < n ? max(doc[shift + i0 + lane], -1) : -1;     // no padding is any other's document
     };
     int par = 0;
     for (int w0 = first; w0 < tiles; w0 += WINDOW) {
@@ -263,16 +252,16 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_dkv(const rwkv_att
             __syncthreads();
         }
         const auto skip = [&](int t) {
-            if constexpr (DOC) while (t < w1 && kind[t - w0] == 0) ++t;
-            return __builtin_amdgcn_readfirstlane(t);
+            if constexpr (DOC) return next_tile(kind, t, w0, w1);
+            return t;
         };
         const int begin = skip(w0);
         int t = begin, h = hk * G;
         if (t < w1) load(h, t);
         while (t < w1) {
             const lds_t qb = lds + par * BUF, yb = qb + Plane<D>::BYTES;
-            qs.store(qb);
-            ys.store(yb);
+            if constexpr (DOC) qs.store(qb, __ballot(next_doc >= 0)), ys.store(yb, __ballot(next_doc >= 0));
+            else qs.store(qb), ys.store(yb);
             if (tid < TILE) {
                 row_lse[par][tid] = next_lse;
                 row_delta[par][tid] = next_delta;

@@ -87,14 +87,7 @@ __global__ __launch_bounds__(256, QT * D > 128 ? 1 : 2) void attn_fwd(const rwkv
         const int j0 = t * TILE, rows = p.Tk - j0;
         ks.load(kbase + j0 * p.k_st, rows, static_cast<int>(p.k_st) * 2, p.N);
         vs.load(vbase + j0 * p.v_st, rows, static_cast<int>(p.v_st) * 2, p.N);
-        if constexpr (DOC) {
-            next_doc = tid < TILE && tid < rows ? doc[j0 + tid] : -1;
-#pragma unroll
-            for (int i = 0; i < vs.STEPS; ++i) {                 // the values of padding may be anything: they are multiplied by weights of 0
-                const int r = vs.row + i * vs.STEP_ROWS;
-                vs.keep(i, doc[min(j0 + r, p.Tk - 1)] >= 0);
-            }
-        }
+        if constexpr (DOC) next_doc = lane < rows ? doc[j0 + lane] : -1;
     };
 
     int par = 0;
@@ -106,15 +99,16 @@ __global__ __launch_bounds__(256, QT * D > 128 ? 1 : 2) void attn_fwd(const rwkv
             __syncthreads();
         }
         const auto skip = [&](int t) {
-            if constexpr (DOC) while (t < w1 && kind[t - w0] == 0) ++t;
-            return __builtin_amdgcn_readfirstlane(t);
+            if constexpr (DOC) return next_tile(kind, t, w0, w1);
+            return t;
         };
         int t = skip(w0);
         if (t < w1) load(t);
         while (t < w1) {
             const lds_t kb = lds + par * BUF, vb = kb + Plane<D>::BYTES;
             ks.store(kb);
-            vs.store(vb);
+            if constexpr (DOC) vs.store(vb, __ballot(next_doc >= 0));
+            else vs.store(vb);
             if (DOC && tid < TILE) key_doc[par][tid] = next_doc;
             const int now = t, j0 = t * TILE;
             t = skip(t + 1);

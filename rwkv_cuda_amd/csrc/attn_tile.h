@@ -118,13 +118,20 @@ template <int D, int THREADS> struct Stage {
             x[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, off == 0x7ffffff0 || r >= rows ? 0x7ffffff0 : r * step + off, 0, 0));
         }
     }
-    DEVINL void keep(const int i, const bool on) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[i][e] = on ? x[i][e] : 0u;
-    }
     DEVINL void store(const lds_t base) const {
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) lds_st(base + to + i * STEP_ROWS * Plane<D>::ROW, x[i]);
+    }
+    // only the rows whose bit is set: those of padding may hold anything and count as zeros
+    DEVINL void store(const lds_t base, const uint64_t rows) const {
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            const bool on = rows >> (row + i * STEP_ROWS) & 1;
+            u32x4 z = x[i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[e] = on ? z[e] : 0u;
+            lds_st(base + to + i * STEP_ROWS * Plane<D>::ROW, z);
+        }
     }
 };
 
@@ -186,7 +193,7 @@ struct Scorer {
 constexpr int WINDOW = 1024;
 DEVINL void classify(uint8_t* kind, const int* doc, const int first_tile, const int tiles, const int T, const int lo, const int hi, const bool uniform, const int waves) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    constexpr int AHEAD = 4;
+    constexpr int AHEAD = 8;
     for (int i0 = wave * AHEAD; i0 < tiles; i0 += waves * AHEAD) {
         int d[AHEAD];
 #pragma unroll
@@ -200,6 +207,16 @@ DEVINL void classify(uint8_t* kind, const int* doc, const int first_tile, const 
             if (lane == 0 && i0 + e < tiles) kind[i0 + e] = !any ? 0 : (all && uniform ? 2 : 1);
         }
     }
+}
+
+// the first tile from `t` on (below `end`) that is looked at; `kind` begins with tile w0
+DEVINL int next_tile(const uint8_t* kind, int t, const int w0, const int end) {
+    const int lane = threadIdx.x & 63;
+    for (; t < end; t += 64) {
+        const uint64_t some = __ballot(t + lane < end && kind[t + lane - w0] != 0);
+        if (some) return __builtin_amdgcn_readfirstlane(t + __builtin_ctzll(some));
+    }
+    return end;
 }
 
 }  // namespace
