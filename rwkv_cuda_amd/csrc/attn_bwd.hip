@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const rwkv_attn_args p, const 
     const float pos = static_cast<float>(shift + i);
     const int64_t stat = (wide(b) * p.H + h) * p.Tq + (real ? i : 0);
     const float lse = lim >= 0 ? p.lse[stat] : INFINITY, dlt = lim >= 0 ? delta[stat] : 0.f;
-    int lim_lo = lim, lim_hi = lim, dlo = real ? qdoc : INT_MAX, dhi = real ? qdoc : -1;
+    int lim_lo = lim, lim_hi = lim, dlo = real && qdoc >= 0 ? qdoc : INT_MAX, dhi = real ? qdoc : -1;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
         lim_lo = min(lim_lo, __shfl_xor(lim_lo, m, 64));
@@ -197,10 +197,9 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_dkv(const rwkv_att
     u32x4 k[D / 16], v[D / 16];
     load_rows<E, D>(k, static_cast<const E*>(p.k) + b * p.k_sb + (real ? j : 0) * p.k_st + hk * p.k_sh, real, p.N);
     load_rows<E, D>(v, static_cast<const E*>(p.v) + b * p.v_sb + (real ? j : 0) * p.v_st + hk * p.v_sh, real, p.N);
-    int kdoc = DOC && real ? doc[j] : -2;
-    if (kdoc < 0) kdoc = -2;
-    const int from = !p.causal || j < reach ? 0 : j;             // the first position that sees the key
-    int from_lo = real ? from : INT_MAX, from_hi = real ? from : 0, dlo = real ? kdoc : INT_MAX, dhi = real ? kdoc : -1;
+    const int kdoc = DOC && real ? doc[j] : 0;
+    const int from = kdoc < 0 ? INT_MAX : (!p.causal || j < reach ? 0 : j);            // the first position that sees the key; none that sees padding
+    int from_lo = real ? from : INT_MAX, from_hi = real ? from : 0, dlo = real && kdoc >= 0 ? kdoc : INT_MAX, dhi = real ? kdoc : -1;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
         from_lo = min(from_lo, __shfl_xor(from_lo, m, 64));
@@ -241,7 +240,7 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_dkv(const rwkv_att
             if (!on || next_lse == -INFINITY) next_lse = INFINITY, next_delta = 0.f;     // a row that is not there or sees nothing: weights of 0
             next_lse -= SHIFT<E>;
         }
-        if constexpr (DOC) next_doc = lane < n ? max(doc[shift + i0 + lane], -1) : -1;     // no padding is any other's document
+        if constexpr (DOC) next_doc = lane < n ? doc[shift + i0 + lane] : -1;
     };
     int par = 0;
     for (int w0 = first; w0 < tiles; w0 += WINDOW) {

@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256, QT * D > 128 ? 1 : 2) void attn_fwd(const rwkv
         pos[z] = static_cast<float>(shift + i);
         lim_lo = min(lim_lo, lim[z]);
         lim_hi = max(lim_hi, lim[z]);
-        if (on) dlo = min(dlo, qdoc[z]), dhi = max(dhi, qdoc[z]);
+        if (on && qdoc[z] >= 0) dlo = min(dlo, qdoc[z]), dhi = max(dhi, qdoc[z]);      // (padding sees nothing: lim is below every key)
     }
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
