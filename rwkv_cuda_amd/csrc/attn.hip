@@ -25,8 +25,11 @@ int check_attn(const rwkv_attn_args* p, bool backward) {
     if (backward) {
         if (const int rc = check_ptrs({p->dy, p->dq, p->dk, p->dv, p->y_rest})) return rc;
         if (p->lse == nullptr) return RWKV_ERR_NULL;
-        if (p->workspace == nullptr || !aligned16(p->workspace) || p->workspace_bytes < rwkv_attn_backward_workspace_bytes(p->B, p->Tq, p->H)) return RWKV_ERR_WORKSPACE;
-    } else if (!aligned16(p->y_rest)) return RWKV_ERR_ALIGN;
+        if (p->workspace == nullptr || !aligned16(p->workspace) || p->workspace_bytes < rwkv_attn_workspace_bytes(p->B, p->Tq, p->Tk, p->H, p->doc != nullptr, 1)) return RWKV_ERR_WORKSPACE;
+    } else {
+        if (!aligned16(p->y_rest)) return RWKV_ERR_ALIGN;
+        if (p->doc != nullptr && (p->workspace == nullptr || !aligned16(p->workspace) || p->workspace_bytes < rwkv_attn_workspace_bytes(p->B, p->Tq, p->Tk, p->H, 1, 0))) return RWKV_ERR_WORKSPACE;
+    }
     for (const void* q : {static_cast<const void*>(p->slopes), static_cast<const void*>(p->doc), static_cast<const void*>(p->prefix), static_cast<const void*>(p->lse)})
         if (reinterpret_cast<uintptr_t>(q) & 3) return RWKV_ERR_ALIGN;
     return RWKV_OK;
@@ -43,9 +46,12 @@ int attn_any(void* stream, const rwkv_attn_args* p, bool backward) {
 
 extern "C" {
 
-size_t rwkv_attn_backward_workspace_bytes(int B, int Tq, int H) {
-    if (B <= 0 || Tq <= 0 || H <= 0) return 0;
-    return static_cast<size_t>(B) * Tq * H * sizeof(float);
+// the documents of tiles of 64 keys (16 bytes each), in the backward also of tiles of queries, and a sum of each query and head
+size_t rwkv_attn_workspace_bytes(int B, int Tq, int Tk, int H, int doc, int backward) {
+    if (B <= 0 || Tq <= 0 || Tk < Tq || H <= 0) return 0;
+    size_t n = doc ? static_cast<size_t>(B) * ((static_cast<int64_t>(Tk) + 63) / 64) * 16 : 0;
+    if (backward) n += (doc ? static_cast<size_t>(B) * ((static_cast<int64_t>(Tq) + 63) / 64) * 16 : 0) + static_cast<size_t>(B) * Tq * H * sizeof(float);
+    return n;
 }
 int rwkv_attn_forward(void* stream, const rwkv_attn_args* args) { return rwkv::attn_any(stream, args, false); }
 int rwkv_attn_backward(void* stream, const rwkv_attn_args* args) { return rwkv::attn_any(stream, args, true); }

@@ -9,6 +9,18 @@ namespace {
 template <class E> constexpr float SHIFT = std::is_same_v<E, bf16_t> ? 0.f : 8.f;
 template <class E> constexpr float UNSHIFT = std::is_same_v<E, bf16_t> ? 1.f : 1.f / 256.f;
 
+__global__ __launch_bounds__(256) void attn_ranges(const int* doc, const int T, const int first, const int tiles, Range* out) {
+    const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, b = blockIdx.y;
+    if (t >= tiles) return;
+    const int64_t j = first + wide(t) * TILE + lane;
+    const int d = j < T ? doc[wide(b) * T + j] : -1;
+    int lo = d < 0 ? INT_MAX : d, hi = max(d, -1);
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) lo = min(lo, __shfl_xor(lo, m, 64)), hi = max(hi, __shfl_xor(hi, m, 64));
+    const bool whole = __ballot(d >= 0) == ~0ull;
+    if (lane == 0) out[wide(b) * tiles + t] = {lo, hi, whole, 0};
+}
+
 // delta = sum over the channels of dy y, y as the forward had it before it was rounded; a row has D / 8 lanes
 template <class E, int D> __global__ __launch_bounds__(256) void attn_delta(const rwkv_attn_args p, float* delta) {
     constexpr int LANES = D / 8;
@@ -34,12 +46,10 @@ template <class E, int D> __global__ __launch_bounds__(256) void attn_delta(cons
 
 // dQ: 4 waves of 32 queries over the keys that any of them sees; S^T = K Q^T and dP^T = V dY^T, dQ^T += K^T dS^T
 template <class E, int D, bool CAP, bool BIAS, bool DOC>
-__global__ __launch_bounds__(256, 2) void attn_dq(const rwkv_attn_args p, const float* delta, const int blocks_q, const int per_xcd) {
+__global__ __launch_bounds__(256, 2) void attn_dq(const rwkv_attn_args p, const float* delta, const Range* ranges, const int blocks_q, const int per_xcd) {
     constexpr int QB = 128;
     __shared__ __align__(16) char smem[4 * Plane<D>::BYTES];
-    __shared__ uint8_t kind[WINDOW];
     __shared__ __align__(16) int key_doc[2][TILE];
-    __shared__ int docs_lo[4], docs_hi[4];
     const int id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
     if (id >= wide(blocks_q) * p.H * p.B) return;
     const int bh = id / blocks_q, q0 = (blocks_q - 1 - id % blocks_q) * QB, b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
@@ -63,23 +73,16 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const rwkv_attn_args p, const 
     const float pos = static_cast<float>(shift + i);
     const int64_t stat = (wide(b) * p.H + h) * p.Tq + (real ? i : 0);
     const float lse = lim >= 0 ? p.lse[stat] : INFINITY, dlt = lim >= 0 ? delta[stat] : 0.f;
-    int lim_lo = lim, lim_hi = lim, dlo = real && qdoc >= 0 ? qdoc : INT_MAX, dhi = real ? qdoc : -1;
-#pragma unroll
-    for (int m = 1; m < 32; m <<= 1) {
-        lim_lo = min(lim_lo, __shfl_xor(lim_lo, m, 64));
-        lim_hi = max(lim_hi, __shfl_xor(lim_hi, m, 64));
-        dlo = min(dlo, __shfl_xor(dlo, m, 64));
-        dhi = max(dhi, __shfl_xor(dhi, m, 64));
-    }
-    lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
-    lim_hi = __builtin_amdgcn_readfirstlane(lim_hi);
-    bool uniform = true;
+    const int row_lo = q0 + __builtin_amdgcn_readfirstlane(wave) * 32;
+    // the last key that all of the wave's queries see, and one that none behind sees
+    const int lim_lo = __ballot(lim < 0) != 0ull ? -1 : (p.causal ? max(shift + row_lo, reach) : p.Tk - 1);
+    const int lim_hi = row_lo >= p.Tq ? -1 : (p.causal ? max(shift + min(row_lo + 31, p.Tq - 1), reach) : p.Tk - 1);
+    int dlo = 0, dhi = 0;                                        // the documents of the block's queries (and of what shares their tiles)
     if constexpr (DOC) {
-        if (lane == 0) docs_lo[wave] = dlo, docs_hi[wave] = dhi;
-        __syncthreads();
-        dlo = min(min(docs_lo[0], docs_lo[1]), min(docs_lo[2], docs_lo[3]));
-        dhi = max(max(docs_hi[0], docs_hi[1]), max(docs_hi[2], docs_hi[3]));
-        uniform = dlo == dhi;
+        ranges += b * tiles_of(p.Tk);
+        const int t0 = (shift + q0) / TILE, t1 = (shift + min(q0 + QB, p.Tq) - 1) / TILE;
+        dlo = INT_MAX, dhi = -1;
+        for (int x = t0; x <= t1; ++x) dlo = min(dlo, ranges[x].lo), dhi = max(dhi, ranges[x].hi);
     }
     const int last = p.causal ? max(min(q0 + QB, p.Tq) - 1 + shift, reach) : p.Tk - 1;
     const int tiles = last / TILE + 1;
@@ -100,33 +103,21 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const rwkv_attn_args p, const 
         vs.load(vbase + j0 * p.v_st, n, static_cast<int>(p.v_st) * 2, p.N);
         if constexpr (DOC) next_doc = lane < n ? doc[j0 + lane] : -1;
     };
-    int par = 0;
-    for (int w0 = 0; w0 < tiles; w0 += WINDOW) {
-        const int w1 = min(tiles, w0 + WINDOW);
-        if constexpr (DOC) {
-            __syncthreads();
-            classify(kind, doc, w0, w1 - w0, p.Tk, dlo, dhi, uniform, 4);
-            __syncthreads();
-        }
-        const auto skip = [&](int t) {
-            if constexpr (DOC) return next_tile(kind, t, w0, w1);
-            return t;
-        };
-        int t = skip(w0);
-        if (t < w1) load(t);
-        while (t < w1) {
+    Walk<DOC> walk(ranges, dlo, dhi, 0, tiles);
+    if (walk.t < tiles) load(walk.t);
+    for (int par = 0; walk.t < tiles; par ^= 1) {
             const lds_t kb = lds + par * BUF, vb = kb + Plane<D>::BYTES;
             if constexpr (DOC) ks.store(kb, __ballot(next_doc >= 0));
             else ks.store(kb);
             vs.store(vb);
             if (DOC && tid < TILE) key_doc[par][tid] = next_doc;
-            const int now = t, j0 = t * TILE;
-            t = skip(t + 1);
+            const int j0 = walk.t * TILE;
+            const bool part = !walk.whole;
+            walk.next();
             __syncthreads();
-            if (t < w1) load(t);
-            const int part = DOC ? kind[now - w0] : 2;
+            if (walk.t < tiles) load(walk.t);
             if (j0 <= lim_hi) {
-                const bool masked = part != 2 || j0 + TILE - 1 > lim_lo;
+                const bool masked = part || j0 + TILE - 1 > lim_lo;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     f32x16 s = f32x16{}, dp = f32x16{};
@@ -166,8 +157,6 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const rwkv_attn_args p, const 
                         for (int d = 0; d < D / 32; ++d) g[d] = mma<E>(cols(kb, 2 * e + c, d), w[c], g[d]);
                 }
             }
-            par ^= 1;
-        }
     }
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) store32<E>(g[d], p.scale, static_cast<E*>(p.dq) + row, nullptr, 32 * d, p.N, real);
@@ -176,13 +165,11 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const rwkv_attn_args p, const 
 // dK, dV: 4 waves of 32 keys over the queries, of all heads that share them, that see any of them; S = Q K^T and dP = dY V^T,
 // dV^T += dY^T P, dK^T += Q^T dS
 template <class E, int D, bool CAP, bool BIAS, bool DOC>
-__global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_dkv(const rwkv_attn_args p, const float* delta, const int blocks_k, const int per_xcd) {
+__global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_dkv(const rwkv_attn_args p, const float* delta, const Range* key_ranges, const Range* ranges, const int blocks_k, const int per_xcd) {
     constexpr int KB = 128;
     __shared__ __align__(16) char smem[4 * Plane<D>::BYTES];
-    __shared__ uint8_t kind[WINDOW];
     __shared__ __align__(16) int row_doc[2][TILE];
     __shared__ __align__(16) float row_lse[2][TILE], row_delta[2][TILE];
-    __shared__ int docs_lo[4], docs_hi[4];
     const int id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
     if (id >= wide(blocks_k) * p.Hk * p.B) return;
     const int bh = id / blocks_k, k0 = id % blocks_k * KB, b = bh / p.Hk, hk = bh % p.Hk, G = p.H / p.Hk;
@@ -199,23 +186,16 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_dkv(const rwkv_att
     load_rows<E, D>(v, static_cast<const E*>(p.v) + b * p.v_sb + (real ? j : 0) * p.v_st + hk * p.v_sh, real, p.N);
     const int kdoc = DOC && real ? doc[j] : 0;
     const int from = kdoc < 0 ? INT_MAX : (!p.causal || j < reach ? 0 : j);            // the first position that sees the key; none that sees padding
-    int from_lo = real ? from : INT_MAX, from_hi = real ? from : 0, dlo = real && kdoc >= 0 ? kdoc : INT_MAX, dhi = real ? kdoc : -1;
-#pragma unroll
-    for (int m = 1; m < 32; m <<= 1) {
-        from_lo = min(from_lo, __shfl_xor(from_lo, m, 64));
-        from_hi = max(from_hi, __shfl_xor(from_hi, m, 64));
-        dlo = min(dlo, __shfl_xor(dlo, m, 64));
-        dhi = max(dhi, __shfl_xor(dhi, m, 64));
-    }
-    from_lo = __builtin_amdgcn_readfirstlane(from_lo);
-    from_hi = __builtin_amdgcn_readfirstlane(from_hi);
-    bool uniform = true;
+    const int key_lo = k0 + __builtin_amdgcn_readfirstlane(wave) * 32, key_hi = min(key_lo + 31, p.Tk - 1);
+    // the first position that sees any of the wave's keys, and one from which on all see them
+    const int from_lo = key_lo >= p.Tk ? INT_MAX : (!p.causal || key_lo < reach ? 0 : key_lo);
+    const int from_hi = __ballot(kdoc < 0) != 0ull ? INT_MAX : (!p.causal || key_hi < reach ? 0 : key_hi);
+    int dlo = 0, dhi = 0;                                        // the documents of the block's keys
     if constexpr (DOC) {
-        if (lane == 0) docs_lo[wave] = dlo, docs_hi[wave] = dhi;
-        __syncthreads();
-        dlo = min(min(docs_lo[0], docs_lo[1]), min(docs_lo[2], docs_lo[3]));
-        dhi = max(max(docs_hi[0], docs_hi[1]), max(docs_hi[2], docs_hi[3]));
-        uniform = dlo == dhi;
+        key_ranges += b * tiles_of(p.Tk) + k0 / TILE;
+        ranges += b * tiles_of(p.Tq);
+        dlo = key_ranges[0].lo, dhi = key_ranges[0].hi;
+        if (k0 + TILE < p.Tk) dlo = min(dlo, key_ranges[1].lo), dhi = max(dhi, key_ranges[1].hi);
     }
     const int first = !p.causal || k0 < reach ? 0 : max(0, k0 - shift) / TILE, tiles = (p.Tq + TILE - 1) / TILE;
 
@@ -242,22 +222,11 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_dkv(const rwkv_att
         }
         if constexpr (DOC) next_doc = lane < n ? doc[shift + i0 + lane] : -1;
     };
-    int par = 0;
-    for (int w0 = first; w0 < tiles; w0 += WINDOW) {
-        const int w1 = min(tiles, w0 + WINDOW);
-        if constexpr (DOC) {
-            __syncthreads();
-            classify(kind, doc + shift, w0, w1 - w0, p.Tq, dlo, dhi, uniform, 4);
-            __syncthreads();
-        }
-        const auto skip = [&](int t) {
-            if constexpr (DOC) return next_tile(kind, t, w0, w1);
-            return t;
-        };
-        const int begin = skip(w0);
-        int t = begin, h = hk * G;
-        if (t < w1) load(h, t);
-        while (t < w1) {
+    int h = hk * G, par = 0;
+    Walk<DOC> walk(ranges, dlo, dhi, first, tiles);
+    if (walk.t < tiles) load(h, walk.t);
+    const Walk<DOC> start = walk;
+    while (walk.t < tiles) {
             const lds_t qb = lds + par * BUF, yb = qb + Plane<D>::BYTES;
             if constexpr (DOC) qs.store(qb, __ballot(next_doc >= 0)), ys.store(yb, __ballot(next_doc >= 0));
             else qs.store(qb), ys.store(yb);
@@ -266,16 +235,16 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_dkv(const rwkv_att
                 row_delta[par][tid] = next_delta;
                 if (DOC) row_doc[par][tid] = next_doc;
             }
-            const int now = t, i0 = t * TILE;
+            const int i0 = walk.t * TILE;
+            const bool part = !walk.whole;
             const Scorer sc(p, h);
             const float mul = CAP || BIAS ? 1.f : sc.unit;
-            t = skip(t + 1);
-            if (t >= w1 && h + 1 < hk * G + G) t = begin, ++h;
+            walk.next();
+            if (walk.t >= tiles && h + 1 < hk * G + G) walk = start, ++h;
             __syncthreads();
-            if (t < w1) load(h, t);
-            const int part = DOC ? kind[now - w0] : 2;
+            if (walk.t < tiles) load(h, walk.t);
             if (shift + i0 + TILE - 1 >= from_lo) {
-                const bool masked = part != 2 || shift + i0 < from_hi;
+                const bool masked = part || shift + i0 < from_hi;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     f32x16 s = f32x16{}, dp = f32x16{};
@@ -327,7 +296,6 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_dkv(const rwkv_att
                 }
             }
             par ^= 1;
-        }
     }
     const int64_t row = ((wide(b) * p.Tk + (real ? j : 0)) * p.Hk + hk) * p.N;
 #pragma unroll
@@ -338,15 +306,21 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_dkv(const rwkv_att
 }
 
 template <class E, int D> int run(hipStream_t st, const rwkv_attn_args& p) {
-    float* delta = static_cast<float*>(p.workspace);
+    // the documents of tiles of keys, of tiles of queries, and delta
+    Range *key_ranges = static_cast<Range*>(p.workspace), *ranges = key_ranges + (p.doc ? p.B * tiles_of(p.Tk) : 0);
+    float* delta = reinterpret_cast<float*>(ranges + (p.doc ? p.B * tiles_of(p.Tq) : 0));
+    if (p.doc) {
+        launch_attn_ranges(st, p.doc, p.B, p.Tk, 0, key_ranges);
+        launch_attn_ranges(st, p.doc, p.B, p.Tk, p.Tk - p.Tq, ranges);
+    }
     const int64_t rows = wide(p.B) * p.Tq * p.H, row_blocks = (rows * (D / 8) + 255) / 256;
     const int blocks_q = (p.Tq + 127) / 128, blocks_k = (p.Tk + 127) / 128;
     const int64_t per_q = (wide(blocks_q) * p.H * p.B + 7) / 8, per_k = (wide(blocks_k) * p.Hk * p.B + 7) / 8;
     if (row_blocks > INT_MAX || per_q * 8 > INT_MAX || per_k * 8 > INT_MAX) return RWKV_ERR_SHAPE;
     hipLaunchKernelGGL((attn_delta<E, D>), dim3(static_cast<unsigned>(row_blocks)), dim3(256), 0, st, p, delta);
     const auto go = [&](auto dq, auto dkv) {
-        hipLaunchKernelGGL(dkv, dim3(static_cast<unsigned>(per_k * 8)), dim3(256), 0, st, p, delta, blocks_k, static_cast<int>(per_k));
-        hipLaunchKernelGGL(dq, dim3(static_cast<unsigned>(per_q * 8)), dim3(256), 0, st, p, delta, blocks_q, static_cast<int>(per_q));
+        hipLaunchKernelGGL(dkv, dim3(static_cast<unsigned>(per_k * 8)), dim3(256), 0, st, p, delta, key_ranges, ranges, blocks_k, static_cast<int>(per_k));
+        hipLaunchKernelGGL(dq, dim3(static_cast<unsigned>(per_q * 8)), dim3(256), 0, st, p, delta, key_ranges, blocks_q, static_cast<int>(per_q));
         return launch_status();
     };
     const auto masks = [&](auto cap, auto bias) {
@@ -361,6 +335,11 @@ template <class E, int D> int run(hipStream_t st, const rwkv_attn_args& p) {
 template <class E> int run_any(hipStream_t st, const rwkv_attn_args& p) { return p.N <= 64 ? run<E, 64>(st, p) : run<E, 128>(st, p); }
 
 }  // namespace
+
+void launch_attn_ranges(hipStream_t st, const int* doc, int B, int T, int first, Range* out) {
+    const int tiles = static_cast<int>(tiles_of(T - first));
+    hipLaunchKernelGGL(attn_ranges, dim3((tiles + 3) / 4, B), dim3(256), 0, st, doc, T, first, tiles, out);
+}
 
 int launch_attn_bwd(hipStream_t st, const rwkv_attn_args& p) { return p.dtype == RWKV_DTYPE_BF16 ? run_any<bf16_t>(st, p) : run_any<half_t>(st, p); }
 

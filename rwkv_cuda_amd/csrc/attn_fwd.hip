@@ -1,4 +1,4 @@
-// Attention forward on the matrix cores.  A workgroup has 4 waves of 32 QT queries of one head each and walks over the keys that any of
+// Attention forward on the matrix cores.  A workgroup has 4 waves of 32 queries of one head each and walks over the keys that any of
 // them sees, 64 at a time: S^T = K Q^T, one pass of the softmax with the running maximum and sum of a lane's query, O^T += V^T P^T.
 #include "attn_tile.h"
 
@@ -8,227 +8,245 @@ namespace {
 // The maximum that weights are taken relative to follows the running one only when that has grown by 2^GROWTH: sums and weights stay far from fp32's
 // and fp16's ends, and the accumulators are rarely scaled.
 constexpr float GROWTH = 8.f;
+using yes = std::true_type;
+using no = std::false_type;
+constexpr int READS = 6;
 
-template <class E, int D, int QT, bool CAP, bool BIAS, bool DOC>
-__global__ __launch_bounds__(256, QT * D > 128 ? 1 : 2) void attn_fwd(const rwkv_attn_args p, const int blocks_q, const int per_xcd) {
-    constexpr int QB = 128 * QT;
-    __shared__ __align__(16) char smem[4 * Plane<D>::BYTES];
-    __shared__ uint8_t kind[WINDOW];
-    __shared__ __align__(16) int key_doc[2][TILE];
-    __shared__ int docs_lo[4], docs_hi[4];
+template <class E, int D, bool CAP, bool BIAS, bool DOC>
+__global__ __launch_bounds__(256, 2) void attn_fwd(const rwkv_attn_args p, const Range* ranges, const int blocks_q, const int per_xcd) {
+    constexpr int QB = 128;
+    // two planes of keys and of values (below 64 KB: what M0 can name), and the documents of two tiles
+    constexpr int PLANES = 4 * Plane<D>::BYTES;
+    __shared__ __align__(16) char smem[PLANES + (DOC ? 8 * TILE : 0)];
+    int* const key_doc = reinterpret_cast<int*>(smem + PLANES);
     const int id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
     const int64_t all = wide(blocks_q) * p.H * p.B;
     if (id >= all) return;
     const int bh = id / blocks_q, q0 = (blocks_q - 1 - id % blocks_q) * QB, b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5;
     const lds_t lds = lds_of(smem);
-    constexpr lds_t BUF = 2 * Plane<D>::BYTES;
+    constexpr int BUF = 2 * Plane<D>::BYTES;
 
     const E* kbase = static_cast<const E*>(p.k) + b * p.k_sb + hk * p.k_sh;
     const E* vbase = static_cast<const E*>(p.v) + b * p.v_sb + hk * p.v_sh;
     const int* doc = DOC ? p.doc + wide(b) * p.Tk : nullptr;
     const int shift = p.Tk - p.Tq, reach = p.prefix ? min(p.prefix[b], p.Tk) - 1 : -1;
 
-    u32x4 q[QT][D / 16];
-    int lim[QT], qdoc[QT];
-    float pos[QT];
-    int lim_lo = INT_MAX, lim_hi = -1, dlo = INT_MAX, dhi = -1;
-#pragma unroll
-    for (int z = 0; z < QT; ++z) {
-        const int i = q0 + (wave * QT + z) * 32 + (lane & 31);
-        const bool on = i < p.Tq;
-        load_rows<E, D>(q[z], static_cast<const E*>(p.q) + b * p.q_sb + (on ? i : 0) * p.q_st + h * p.q_sh, on, p.N);
-        qdoc[z] = DOC && on ? doc[shift + i] : 0;
-        lim[z] = !on || qdoc[z] < 0 ? -1 : (p.causal ? max(shift + i, reach) : p.Tk - 1);
-        pos[z] = static_cast<float>(shift + i);
-        lim_lo = min(lim_lo, lim[z]);
-        lim_hi = max(lim_hi, lim[z]);
-        if (on && qdoc[z] >= 0) dlo = min(dlo, qdoc[z]), dhi = max(dhi, qdoc[z]);      // (padding sees nothing: lim is below every key)
-    }
-#pragma unroll
-    for (int m = 1; m < 32; m <<= 1) {
-        lim_lo = min(lim_lo, __shfl_xor(lim_lo, m, 64));
-        lim_hi = max(lim_hi, __shfl_xor(lim_hi, m, 64));
-        dlo = min(dlo, __shfl_xor(dlo, m, 64));
-        dhi = max(dhi, __shfl_xor(dhi, m, 64));
-    }
-    lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
-    lim_hi = __builtin_amdgcn_readfirstlane(lim_hi);
-    bool uniform = true;
+    const int i = q0 + wave * 32 + (lane & 31);
+    const bool real = i < p.Tq;
+    u32x4 q[D / 16];
+    load_rows<E, D>(q, static_cast<const E*>(p.q) + b * p.q_sb + (real ? i : 0) * p.q_st + h * p.q_sh, real, p.N);
+    const int qdoc = DOC && real ? doc[shift + i] : 0;
+    const int lim = !real || qdoc < 0 ? -1 : (p.causal ? max(shift + i, reach) : p.Tk - 1);      // the last key that the query sees; padding sees none
+    const float pos = static_cast<float>(shift + i);
+    const int row_lo = q0 + __builtin_amdgcn_readfirstlane(wave) * 32, pos_lo = shift + row_lo;
+    // the last key that all of the wave's queries see
+    const int lim_lo = __ballot(lim < 0) != 0ull ? -1 : (p.causal ? max(pos_lo, reach) : p.Tk - 1);
+    int dlo = 0, dhi = 0;                                        // the documents of the block's queries (and of what shares their tiles)
     if constexpr (DOC) {
-        if (lane == 0) docs_lo[wave] = dlo, docs_hi[wave] = dhi;
-        __syncthreads();
-        dlo = min(min(docs_lo[0], docs_lo[1]), min(docs_lo[2], docs_lo[3]));
-        dhi = max(max(docs_hi[0], docs_hi[1]), max(docs_hi[2], docs_hi[3]));
-        uniform = dlo == dhi;
+        ranges += b * tiles_of(p.Tk);
+        const int t0 = (shift + q0) / TILE, t1 = (shift + min(q0 + QB, p.Tq) - 1) / TILE;
+        dlo = INT_MAX, dhi = -1;
+        for (int x = t0; x <= t1; ++x) dlo = min(dlo, ranges[x].lo), dhi = max(dhi, ranges[x].hi);
     }
     // the last key that the block's last query sees
     const int last = p.causal ? max(min(q0 + QB, p.Tq) - 1 + shift, reach) : p.Tk - 1;
     const int tiles = last / TILE + 1;
 
-    const RowReader<D> krow(lane);
-    const ColReader<D> vcol(lane);
-    Stage<D, 256> ks(tid, p.N), vs(tid, p.N);
+    RowReader<D> krow(lane);
+    ColReader<D> vcol(lane);
+    krow.move(lds);
+    vcol.move(lds + Plane<D>::BYTES);
+    const Fetch<D, 4> fetch(tid, p.N);
     const Scorer sc(p, h);
     const float mul = CAP || BIAS ? 1.f : sc.unit;
 
-    f32x16 o[QT][D / 32];
-    float m[QT], l[QT];
+    f32x16 o[D / 32], sa, sb;
+    u32x4 pa[2], pb[2];
+    float m = -INFINITY, l = 0.f, f;
 #pragma unroll
-    for (int z = 0; z < QT; ++z) {
-        m[z] = -INFINITY;
-        l[z] = 0.f;
+    for (int d = 0; d < D / 32; ++d) o[d] = f32x16{};
+    // the scores of half e (32 keys) of a tile
+    const auto scores = [&](f32x16& s, const int e) {
+        s = f32x16{};
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d) o[z][d] = f32x16{};
-    }
-
-    int next_doc = -1;
-    const auto load = [&](const int t) {
-        const int j0 = t * TILE, rows = p.Tk - j0;
-        ks.load(kbase + j0 * p.k_st, rows, static_cast<int>(p.k_st) * 2, p.N);
-        vs.load(vbase + j0 * p.v_st, rows, static_cast<int>(p.v_st) * 2, p.N);
-        if constexpr (DOC) next_doc = lane < rows ? doc[j0 + lane] : -1;
+        for (int c = 0; c < D / 16; ++c) s = mma<E>(krow(0, e, c), q[c], s);
     };
-
-    int par = 0;
-    for (int w0 = 0; w0 < tiles; w0 += WINDOW) {
-        const int w1 = min(tiles, w0 + WINDOW);
-        if constexpr (DOC) {
-            __syncthreads();
-            classify(kind, doc, w0, w1 - w0, p.Tk, dlo, dhi, uniform, 4);
-            __syncthreads();
-        }
-        const auto skip = [&](int t) {
-            if constexpr (DOC) return next_tile(kind, t, w0, w1);
-            return t;
-        };
-        int t = skip(w0);
-        if (t < w1) load(t);
-        while (t < w1) {
-            const lds_t kb = lds + par * BUF, vb = kb + Plane<D>::BYTES;
-            ks.store(kb);
-            if constexpr (DOC) vs.store(vb, __ballot(next_doc >= 0));
-            else vs.store(vb);
-            if (DOC && tid < TILE) key_doc[par][tid] = next_doc;
-            const int now = t, j0 = t * TILE;
-            t = skip(t + 1);
-            __syncthreads();
-            if (t < w1) load(t);
-            const int part = DOC ? kind[now - w0] : 2;
-            if (j0 <= lim_hi) {
-                const bool masked = part != 2 || j0 + TILE - 1 > lim_lo;
-                f32x16 s[QT][2];
+    // capped, biased, and -inf where a query does not see a key; `ahead`: keys may stand behind a query
+    const auto bound = [&](f32x16& s, const int j0, const int e, const int slot, const bool masked, const bool ahead) {
+        if constexpr (CAP || BIAS) {
+            const float dist = pos - static_cast<float>(j0 + 4 * hi + 32 * e);
+            if (!BIAS || ahead) {
 #pragma unroll
-                for (int z = 0; z < QT; ++z) s[z][0] = s[z][1] = f32x16{};
+                for (int r = 0; r < 16; ++r) s[r] = sc.t<CAP, BIAS>(s[r], sc.squash<CAP>(s[r]), dist - (8 * (r >> 2) + (r & 3)));
+            } else {
+                const float far = -sc.slope * dist + (CAP ? sc.out : 0.f);
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int c = 0; c < D / 16; ++c) {
-                        const u32x4 kf = krow(kb, e, c);
-#pragma unroll
-                        for (int z = 0; z < QT; ++z) s[z][e] = mma<E>(kf, q[z][c], s[z][e]);
-                    }
-                __builtin_amdgcn_sched_barrier(0);
-                u32x4 w[QT][4];
-#pragma unroll
-                for (int z = 0; z < QT; ++z) {
-                    if constexpr (CAP || BIAS) {
-                        const float dist = pos[z] - static_cast<float>(j0 + 4 * hi);
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) s[z][e][r] = sc.t<CAP, BIAS>(s[z][e][r], sc.squash<CAP>(s[z][e][r]), dist - (32 * e + 8 * (r >> 2) + (r & 3)));
-                    }
-                    if (masked) {
-                        const int room = lim[z] - j0 - 4 * hi;                  // the keys are j0 + 4 hi + n
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-#pragma unroll
-                            for (int g = 0; g < 4; ++g) {
-                                u32x4 kd;
-                                if constexpr (DOC) kd = *reinterpret_cast<const u32x4*>(&key_doc[par][32 * e + 8 * g + 4 * hi]);
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    bool on = 32 * e + 8 * g + i <= room;
-                                    if constexpr (DOC) on = on && static_cast<int>(kd[i]) == qdoc[z];
-                                    s[z][e][4 * g + i] = on ? s[z][e][4 * g + i] : -INFINITY;
-                                }
-                            }
-                    }
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[z][e][r]);
-                    top = fmaxf(top, other_half(top));
-                    const bool grown = (top - m[z]) * mul > GROWTH;              // always at a query's first key, never while it has seen none (-inf and -inf)
-                    if (__ballot(grown) != 0ull) {
-                        const float to = grown ? top : m[z], f = grown ? __builtin_amdgcn_exp2f((m[z] - to) * mul) : 1.f;
-                        m[z] = to;
-                        l[z] *= f;
-#pragma unroll
-                        for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) o[z][d][r] *= f;
-                    }
-                    const float base = m[z] == -INFINITY ? 0.f : -m[z] * mul;
-                    float sum = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const float x = __builtin_amdgcn_exp2f(fmaf(s[z][e][r], mul, base));
-                            sum += x;
-                            s[z][e][r] = x;
-                        }
-                        w[z][2 * e] = as_operand<E>(s[z][e], 0);
-                        w[z][2 * e + 1] = as_operand<E>(s[z][e], 1);
-                    }
-                    l[z] += sum;
+                for (int r = 0; r < 16; ++r) {
+                    const float near = fmaf(sc.slope, 8 * (r >> 2) + (r & 3), far);
+                    s[r] = CAP ? fmaf(sc.squash<CAP>(s[r]), -2.f * sc.out, near) : fmaf(s[r], sc.unit, near);
                 }
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int d = 0; d < D / 32; ++d) {
-                        const u32x4 vf = vcol(vb, c, d);
-#pragma unroll
-                        for (int z = 0; z < QT; ++z) o[z][d] = mma<E>(vf, w[z][c], o[z][d]);
-                    }
             }
-            par ^= 1;
         }
-    }
-
+        if (masked) {
+            asm volatile("");                                    // (a branch: few tiles come here)
+            const int room = lim - j0 - 4 * hi - 32 * e;
 #pragma unroll
-    for (int z = 0; z < QT; ++z) {
-        const int i = q0 + (wave * QT + z) * 32 + (lane & 31);
-        const float sum = l[z] + other_half(l[z]), f = sum == 0.f ? 0.f : 1.f / sum;
-        const bool on = i < p.Tq;
-        const int64_t at = ((wide(b) * p.Tq + (on ? i : 0)) * p.H + h) * p.N;
+            for (int g = 0; g < 4; ++g) {
+                u32x4 kd;
+                if constexpr (DOC) kd = *reinterpret_cast<const u32x4*>(key_doc + slot * TILE + 32 * e + 8 * g + 4 * hi);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    bool on = 8 * g + i <= room;
+                    if constexpr (DOC) on = on && static_cast<int>(kd[i]) == qdoc;
+                    s[4 * g + i] = on ? s[4 * g + i] : -INFINITY;
+                }
+            }
+        }
+    };
+    // the weights of 32 keys; what was summed before counts f times
+    const auto weights = [&](f32x16& s, u32x4 (&w)[2]) {
+        float top = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+        top = fmaxf(top, other_half(top));
+        const bool grown = (top - m) * mul > GROWTH;             // always at a query's first key, never while it has seen none (-inf and -inf)
+        const float to = grown ? top : m;
+        f = grown ? __builtin_amdgcn_exp2f((m - to) * mul) : 1.f;
+        m = to;
+        const float base = to == -INFINITY ? 0.f : -to * mul;
+        float sum = l * f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float x = __builtin_amdgcn_exp2f(CAP || BIAS ? s[r] + base : fmaf(s[r], mul, base));
+            sum += x;
+            s[r] = x;
+        }
+        l = sum;
+        w[0] = as_operand<E>(s, 0);
+        w[1] = as_operand<E>(s, 1);
+        here(w[0]);
+        here(w[1]);
+        here(l);
+        return __ballot(grown) != 0ull;
+    };
+    const auto add = [&](const u32x4 (&w)[2], const int e) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) o[d] = mma<E>(vcol(0, 2 * e + c, d), w[c], o[d]);
+    };
+    const auto rescale = [&]() {
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
-            store32<E>(o[z][d], f, static_cast<E*>(p.y) + at, p.y_rest ? static_cast<E*>(p.y_rest) + at : nullptr, 32 * d, p.N, on);
-        if (p.lse && on && hi == 0) p.lse[(wide(b) * p.H + h) * p.Tq + i] = sum == 0.f ? -INFINITY : fmaf(m[z], mul, __builtin_amdgcn_logf(sum));
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] *= f;
+    };
+    // scores of one half and values of another, in turn, and the weights of the one between them beside
+    const auto all_three = [&](f32x16& ahead, f32x16& now, const u32x4 (&wold)[2], u32x4 (&wnow)[2], const int e) {
+        __builtin_amdgcn_sched_barrier(0);
+        ahead = f32x16{};
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+            ahead = mma<E>(krow(0, e, c), q[c], ahead);
+            o[c % (D / 32)] = mma<E>(vcol(0, 2 * e + c / (D / 32), c % (D / 32)), wold[c / (D / 32)], o[c % (D / 32)]);
+        }
+        const bool grown = weights(now, wnow);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);  // LDS reads ahead of the products
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 72 * 8 / D, 0);
+            __builtin_amdgcn_sched_group_barrier(0x400, 16 * 8 / D, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (grown) rescale();
+    };
+
+    // Tiles go through in halves of 32 keys, three halves at a time: while the weights of one are made, the matrix cores make the scores of the next and
+    // add the values of the one before, in one stretch of code.  The keys of a tile are therefore in LDS one tile before its values.
+    int next_doc = -1;
+    const auto fetch_keys = [&](const int t, const int slot) {
+        const int j0 = t * TILE, rows = p.Tk - j0;
+        fetch.template operator()<false>(lds + slot * BUF, kbase + j0 * p.k_st, rows, static_cast<int>(p.k_st) * 2, p.N, 0);
+        if constexpr (DOC) next_doc = lane < rows ? doc[j0 + lane] : -1;
+    };
+    // (the values of padding may be anything: zeros instead)
+    const auto fetch_values = [&](const int t, const int slot, const uint64_t real) {
+        fetch.template operator()<DOC>(lds + slot * BUF + Plane<D>::BYTES, vbase + t * TILE * p.v_st, p.Tk - t * TILE, static_cast<int>(p.v_st) * 2, p.N, real);
+    };
+    Walk<DOC> walk(ranges, dlo, dhi, 0, tiles);
+    if (walk.t < tiles) {
+        int t = walk.t;
+        bool whole = walk.whole;
+        fetch_keys(t, 0);
+        if (DOC && tid < TILE) key_doc[tid] = next_doc;
+        const uint64_t there = DOC ? __ballot(next_doc >= 0) : 0;
+        arrived();
+        __syncthreads();
+        fetch_values(t, 0, there);
+        walk.next();
+        if (walk.t < tiles) fetch_keys(walk.t, 1);
+        const auto is_masked = [&]() { return !whole || t * TILE + TILE - 1 > lim_lo; };
+        const auto is_ahead = [&]() { return t * TILE + TILE - 1 > pos_lo; };
+        scores(sa, 0);
+        scores(sb, 1);
+        bound(sa, t * TILE, 0, 0, is_masked(), is_ahead());
+        bound(sb, t * TILE, 1, 0, is_masked(), is_ahead());
+        if (weights(sa, pa)) rescale();
+        int par = 0, step = BUF;
+        const auto meet = [&]() {                                // what is under way has come, for all waves
+            if (DOC && walk.t < tiles && tid < TILE) key_doc[(par ^ 1) * TILE + tid] = next_doc;
+            arrived();
+            __syncthreads();
+        };
+        meet();
+        while (walk.t < tiles) {
+            t = walk.t;
+            whole = walk.whole;
+            walk.next();
+            fetch_values(t, par ^ 1, DOC ? __ballot(next_doc >= 0) : 0);
+            if (walk.t < tiles) fetch_keys(walk.t, par);
+            krow.move(step);
+            const bool masked = is_masked(), ahead = is_ahead();
+            all_three(sa, sb, pa, pb, 0);
+            bound(sa, t * TILE, 0, par ^ 1, masked, ahead);
+            all_three(sb, sa, pb, pa, 1);
+            bound(sb, t * TILE, 1, par ^ 1, masked, ahead);
+            vcol.move(step);
+            par ^= 1;
+            step = -step;
+            meet();
+        }
+        add(pa, 0);
+        if (weights(sb, pb)) rescale();
+        add(pb, 1);
     }
+
+    const float sum = l + other_half(l), inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t at = ((wide(b) * p.Tq + (real ? i : 0)) * p.H + h) * p.N;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) store32<E>(o[d], inv, static_cast<E*>(p.y) + at, p.y_rest ? static_cast<E*>(p.y_rest) + at : nullptr, 32 * d, p.N, real);
+    if (p.lse && real && hi == 0) p.lse[(wide(b) * p.H + h) * p.Tq + i] = sum == 0.f ? -INFINITY : fmaf(m, mul, __builtin_amdgcn_logf(sum));
 }
 
-template <class E, int D, int QT> int run(hipStream_t st, const rwkv_attn_args& p) {
-    const int blocks_q = (p.Tq + 128 * QT - 1) / (128 * QT);
+template <class E, int D> int run(hipStream_t st, const rwkv_attn_args& p) {
+    const int blocks_q = (p.Tq + 127) / 128;
     const int64_t all = wide(blocks_q) * p.H * p.B, per = (all + 7) / 8;
     if (per * 8 > INT_MAX) return RWKV_ERR_SHAPE;
     const dim3 grid(static_cast<unsigned>(per * 8)), block(256);
-    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, p, blocks_q, static_cast<int>(per)); return launch_status(); };
+    Range* ranges = static_cast<Range*>(p.workspace);
+    if (p.doc) launch_attn_ranges(st, p.doc, p.B, p.Tk, 0, ranges);
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, p, ranges, blocks_q, static_cast<int>(per)); return launch_status(); };
     const auto masks = [&](auto cap, auto bias) {
-        return p.doc ? go(attn_fwd<E, D, QT, decltype(cap)::value, decltype(bias)::value, true>) : go(attn_fwd<E, D, QT, decltype(cap)::value, decltype(bias)::value, false>);
+        return p.doc ? go(attn_fwd<E, D, decltype(cap)::value, decltype(bias)::value, true>) : go(attn_fwd<E, D, decltype(cap)::value, decltype(bias)::value, false>);
     };
-    using yes = std::true_type;
-    using no = std::false_type;
     if (p.cap > 0.f) return p.slopes ? masks(yes{}, yes{}) : masks(yes{}, no{});
     return p.slopes ? masks(no{}, yes{}) : masks(no{}, no{});
 }
 template <class E> int run_any(hipStream_t st, const rwkv_attn_args& p) {
-    return p.N <= 64 ? run<E, 64, 1>(st, p) : run<E, 128, 1>(st, p);
+    return p.N <= 64 ? run<E, 64>(st, p) : run<E, 128>(st, p);
 }
 
 }  // namespace

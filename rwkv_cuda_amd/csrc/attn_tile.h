@@ -61,40 +61,51 @@ DEVINL float other_half(const float x) {                        // lane ^ 32's
     return __uint_as_float((threadIdx.x & 32) ? s[0] : s[1]);
 }
 
-// A matrix in LDS: `rows` rows of D values in 16-byte pieces, piece c of row r at place c ^ swap(r).  16 lanes that read one piece of 16
-// rows, and 16 lanes that read four pieces of four rows, both touch every bank once.
+// A matrix of 64 rows of D values in LDS.  A kilobyte (4 rows of 128 values, 8 of 64) is what a wave brings at once; kilobytes lie 16 or 32 bytes further apart
+// than their size, and piece c (16 bytes) of a row is at place c ^ swap(row).  So 16 lanes that read one piece of 16 rows, and 16 lanes that read four pieces of
+// four rows, touch every bank once, and most of an address is a constant: a lane keeps one for every bit of the piece's number that is swapped.
 template <int D> struct Plane {
-    static constexpr int ROW = 2 * D, PIECES = D / 8, BYTES = TILE * ROW;
-    static DEVINL int swap(const int r) { return D == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : (((r >> 1) & 1) << 2) | ((r >> 2) & 3); }
-    static DEVINL lds_t at(const int r, const int c) { return r * ROW + ((c ^ swap(r)) << 4); }
+    static constexpr int ROW = 2 * D, ROWS = 512 / D, STEP = D == 128 ? 1040 : 1056, BYTES = TILE / ROWS * STEP;
+    static DEVINL int swap(const int r) { return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2 | ((r >> 2) & 1); }
+    static DEVINL lds_t at(const int r, const int c) { return r / ROWS * STEP + r % ROWS * ROW + ((c ^ swap(r)) << 4); }
 };
-// rows of a Plane as the first operand with the channels along the contraction: lane = row, `a` the addresses for row lane & 31
+// rows of a Plane as the first operand with the channels along the contraction: lane = row, `a` the addresses for row lane & 31 and channels 32 n
 template <int D> struct RowReader {
-    lds_t a[D / 16];
+    lds_t a[D / 32];
     DEVINL RowReader(const int lane) {
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) a[s] = Plane<D>::at(lane & 31, 2 * s + (lane >> 5));
+        for (int n = 0; n < D / 32; ++n) a[n] = Plane<D>::at(lane & 31, 4 * n + (lane >> 5));
     }
-    DEVINL u32x4 operator()(const lds_t base, const int rows32, const int s) const { return lds_ld<u32x4>(a[s] + base + rows32 * 32 * Plane<D>::ROW); }
+    DEVINL u32x4 operator()(const lds_t base, const int rows32, const int s) const { return lds_ld<u32x4>(a[s / 2] + base + rows32 * (32 / Plane<D>::ROWS) * Plane<D>::STEP + s % 2 * 32); }
+    DEVINL void move(const int by) {
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n) a[n] += by;
+    }
 };
 // ... with the rows along the contraction, in accumulator order: lane = channel of a block of 32
 template <int D> struct ColReader {
-    lds_t a[D / 32][2];
+    lds_t a[D / 32];
     DEVINL ColReader(const int lane) {
         const int l = lane & 15, r = 4 * (lane >> 5) + (l >> 2);
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) a[d][e] = Plane<D>::at(r + 8 * e, 4 * d + 2 * ((lane >> 4) & 1) + ((l & 3) >> 1)) + 8 * (l & 1);
+        for (int d = 0; d < D / 32; ++d) a[d] = Plane<D>::at(r, 4 * d + 2 * ((lane >> 4) & 1) + ((l & 3) >> 1)) + 8 * (l & 1);
     }
     DEVINL u32x4 operator()(const lds_t base, const int rows16, const int d) const {
         typedef v4s __attribute__((address_space(3))) * ptr;
-        const lds_t o = base + rows16 * 16 * Plane<D>::ROW;
-        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(a[d][0] + o)), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(a[d][1] + o));
+        constexpr int EIGHT = 8 / Plane<D>::ROWS * Plane<D>::STEP;  // eight rows
+        const lds_t o = a[d] + base + rows16 * 2 * EIGHT;
+        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(o)), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(o + EIGHT));
         const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
         return u32x4{x[0], x[1], y[0], y[1]};
     }
+    DEVINL void move(const int by) {
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) a[d] += by;
+    }
 };
+// keeps an operand where the program has it made: left to itself the compiler moves it to its use, behind the products that it should run beside
+DEVINL void here(u32x4& x) { asm volatile("" : "+v"(x)); }
+DEVINL void here(float& x) { asm volatile("" : "+v"(x)); }
 
 // The way of a tile of 64 rows from memory to LDS: a piece of 16 bytes a thread and step, zeros behind the last row and the last channel
 // (the buffer's bounds), and for rows that are to count as zeros.
@@ -120,7 +131,7 @@ template <int D, int THREADS> struct Stage {
     }
     DEVINL void store(const lds_t base) const {
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) lds_st(base + to + i * STEP_ROWS * Plane<D>::ROW, x[i]);
+        for (int i = 0; i < STEPS; ++i) lds_st(base + to + i * (STEP_ROWS / Plane<D>::ROWS) * Plane<D>::STEP, x[i]);
     }
     // only the rows whose bit is set: those of padding may hold anything and count as zeros
     DEVINL void store(const lds_t base, const uint64_t rows) const {
@@ -130,10 +141,42 @@ template <int D, int THREADS> struct Stage {
             u32x4 z = x[i];
 #pragma unroll
             for (int e = 0; e < 4; ++e) z[e] = on ? z[e] : 0u;
-            lds_st(base + to + i * STEP_ROWS * Plane<D>::ROW, z);
+            lds_st(base + to + i * (STEP_ROWS / Plane<D>::ROWS) * Plane<D>::STEP, z);
         }
     }
 };
+
+// The same without a stop in registers: 16 bytes a lane from memory straight to LDS, a wave's 1024 bytes in the order of its lanes, so that each lane
+// fetches the piece whose place it is.  The compiler does not count these loads: arrived() before the barrier behind which they are read.  Of the waves of a
+// workgroup each brings every WAVES-th kilobyte.
+template <int D, int WAVES> struct Fetch {
+    static constexpr int LANES = D / 8, ROWS = Plane<D>::ROWS, STEPS = TILE / (ROWS * WAVES);
+    static constexpr uint32_t NOWHERE = 0x7ffffff0u;             // beyond all bounds: such lanes bring zeros
+    uint32_t row, off;
+    DEVINL Fetch(const int tid, const int N) {
+        const int lane = tid & 63;
+        row = (tid >> 6) * ROWS + lane / LANES;
+        const int piece = (lane % LANES) ^ Plane<D>::swap(row);
+        off = 8 * piece < N ? 16 * piece : NOWHERE;
+    }
+    // `rows` rows `step` bytes apart to the plane at `to`; of those only the ones whose bit is set
+    template <bool SOME> DEVINL void operator()(const lds_t to, const void* first, const int rows, const int step, const int N, const uint64_t which) const {
+        const buf_t b = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(first), 0, rows > 0 ? (rows - 1) * step + 2 * N : 0, 0x00027000);
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        uint32_t first_off = off;
+        asm volatile("" : "+v"(first_off));                     // (offsets are made anew: kept, they would be spilled, and a reload waits for all that is under way)
+        const bool on = first_off != NOWHERE;
+        first_off += on ? row * step : 0;
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            uint32_t o = first_off + (on ? i * ROWS * WAVES * step : 0);
+            if (SOME) o = which >> (row + i * ROWS * WAVES) & 1 ? o : NOWHERE;
+            // (M0 is read one wait state after it is written)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(to + (i * WAVES + wave) * Plane<D>::STEP), "v"(o), "s"(b) : "memory");
+        }
+    }
+};
+DEVINL void arrived() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
 
 // An accumulator [channel][row of the output] times `f`, rounded, to 32 channels of the lane's row (and what the rounding lost to `rest`).
 // Lanes l and l + 32 exchange halves so that each has eight consecutive channels to store.
@@ -188,36 +231,47 @@ struct Scorer {
     }
 };
 
-// Which tiles of 64 positions a block whose rows have documents lo .. hi has to look at: 0 none of its tokens, 1 some, 2 all of them and of its rows
-// one document.  Written for a window of tiles to LDS.
-constexpr int WINDOW = 1024;
-DEVINL void classify(uint8_t* kind, const int* doc, const int first_tile, const int tiles, const int T, const int lo, const int hi, const bool uniform, const int waves) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    constexpr int AHEAD = 8;
-    for (int i0 = wave * AHEAD; i0 < tiles; i0 += waves * AHEAD) {
-        int d[AHEAD];
-#pragma unroll
-        for (int e = 0; e < AHEAD; ++e) {
-            const int64_t j = wide(first_tile + i0 + e) * TILE + lane;
-            d[e] = i0 + e < tiles && j < T ? doc[j] : -1;
-        }
-#pragma unroll
-        for (int e = 0; e < AHEAD; ++e) {
-            const bool any = __ballot(d[e] >= 0 && d[e] >= lo && d[e] <= hi) != 0ull, all = __ballot(d[e] == lo) == ~0ull;
-            if (lane == 0 && i0 + e < tiles) kind[i0 + e] = !any ? 0 : (all && uniform ? 2 : 1);
+__host__ __device__ __forceinline__ int64_t tiles_of(const int T) { return (wide(T) + TILE - 1) / TILE; }
+// The tiles below `end` that hold tokens of documents lo .. hi, in order, and whether each is whole and all of the one document lo (= hi).  Without documents: all.
+template <bool DOC> struct Walk {
+    const Range* ranges;
+    int lo, hi, end, base;
+    uint64_t some, full;                                        // of tiles base .. base + 63
+    int t;                                                      // the next tile, `end` behind the last
+    bool whole;
+    DEVINL Walk(const Range* ranges, const int lo, const int hi, const int first, const int end) : ranges(ranges), lo(lo), hi(hi), end(end), base(first), some(0), full(0), t(first), whole(true) {
+        if constexpr (DOC) {
+            look();
+            settle();
+        } else t = min(first, end);
+    }
+    DEVINL void look() {
+        const int i = base + static_cast<int>(threadIdx.x & 63);
+        Range r = {INT_MAX, -1, 0, 0};
+        if (i < end) r = ranges[i];
+        some = __ballot(r.lo <= hi && r.hi >= lo);
+        full = __ballot(r.whole && r.lo == lo && r.hi == lo && lo == hi);
+    }
+    DEVINL void settle() {                                      // to the first tile from t on
+        for (;;) {
+            if (t >= end) { t = end; return; }
+            if (t - base >= 64) { base = t; look(); }
+            const uint64_t left = some >> (t - base);
+            if (left) {
+                t += __builtin_ctzll(left);
+                whole = full >> (t - base) & 1;
+                return;
+            }
+            t = base + 64;
         }
     }
-}
-
-// the first tile from `t` on (below `end`) that is looked at; `kind` begins with tile w0
-DEVINL int next_tile(const uint8_t* kind, int t, const int w0, const int end) {
-    const int lane = threadIdx.x & 63;
-    for (; t < end; t += 64) {
-        const uint64_t some = __ballot(t + lane < end && kind[t + lane - w0] != 0);
-        if (some) return __builtin_amdgcn_readfirstlane(t + __builtin_ctzll(some));
+    DEVINL void next() {
+        ++t;
+        if constexpr (DOC) settle();
+        else asm volatile("" : "+s"(t));                        // (no sums of the tile's number kept from one to the next: they cost registers)
     }
-    return end;
-}
+};
 
 }  // namespace
+
 }  // namespace rwkv

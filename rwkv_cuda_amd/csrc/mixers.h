@@ -16,6 +16,14 @@ template <class E> DEVINL E from_f(float x) {
     else return static_cast<E>(x);
 }
 
+// The documents of a tile of 64 positions, made by a kernel of its own before the others.
+struct Range {
+    int lo, hi;                                                 // of the tokens that are no padding; INT_MAX and -1 without one
+    int whole;                                                  // 64 tokens, none of them padding
+    int unused;
+};
+// attn_bwd.hip: tile i of `out`'s row b has positions first + 64 i .. of doc's row b, below T
+void launch_attn_ranges(hipStream_t st, const int* doc, int B, int T, int first, Range* out);
 // attn_fwd.hip, attn_bwd.hip (arguments checked)
 int launch_attn_fwd(hipStream_t st, const rwkv_attn_args& p);
 int launch_attn_bwd(hipStream_t st, const rwkv_attn_args& p);
