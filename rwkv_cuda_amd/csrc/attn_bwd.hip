@@ -48,14 +48,16 @@ template <class E, int D> __global__ __launch_bounds__(256) void attn_delta(cons
 template <class E, int D, bool CAP, bool BIAS, bool DOC>
 __global__ __launch_bounds__(256, 2) void attn_dq(const rwkv_attn_args p, const float* delta, const Range* ranges, const int blocks_q, const int per_xcd) {
     constexpr int QB = 128;
-    __shared__ __align__(16) char smem[4 * Plane<D>::BYTES];
-    __shared__ __align__(16) int key_doc[2][TILE];
+    constexpr int PLANES = 4 * Plane<D>::BYTES;
+    constexpr int SLOPE_VALUS = 4 + (CAP ? 6 : 0) + (BIAS ? 2 : 0), SLOPE_TRANS = CAP ? 3 : 1;      // instructions of a pair
+    __shared__ __align__(16) char smem[PLANES + (DOC ? 8 * TILE : 0)];      // two planes of keys and of values, and the documents of two tiles
+    int* const key_doc = reinterpret_cast<int*>(smem + PLANES);
     const int id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
     if (id >= wide(blocks_q) * p.H * p.B) return;
     const int bh = id / blocks_q, q0 = (blocks_q - 1 - id % blocks_q) * QB, b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5;
     const lds_t lds = lds_of(smem);
-    constexpr lds_t BUF = 2 * Plane<D>::BYTES;
+    constexpr int BUF = 2 * Plane<D>::BYTES;
 
     const E* kbase = static_cast<const E*>(p.k) + b * p.k_sb + hk * p.k_sh;
     const E* vbase = static_cast<const E*>(p.v) + b * p.v_sb + hk * p.v_sh;
@@ -87,9 +89,11 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const rwkv_attn_args p, const 
     const int last = p.causal ? max(min(q0 + QB, p.Tq) - 1 + shift, reach) : p.Tk - 1;
     const int tiles = last / TILE + 1;
 
-    const RowReader<D> rows(lane);
-    const ColReader<D> cols(lane);
-    Stage<D, 256> ks(tid, p.N), vs(tid, p.N);
+    RowReader<D> rows(lane);
+    ColReader<D> cols(lane);
+    rows.move(lds);
+    cols.move(lds);
+    const Fetch<D, 4> fetch(tid, p.N);
     const Scorer sc(p, h);
     const float mul = CAP || BIAS ? 1.f : sc.unit;
     f32x16 g[D / 32];
@@ -97,66 +101,90 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const rwkv_attn_args p, const 
     for (int d = 0; d < D / 32; ++d) g[d] = f32x16{};
 
     int next_doc = -1;
-    const auto load = [&](const int t) {
+    const auto bring = [&](const int t, const int slot) {
         const int j0 = t * TILE, n = p.Tk - j0;
-        ks.load(kbase + j0 * p.k_st, n, static_cast<int>(p.k_st) * 2, p.N);
-        vs.load(vbase + j0 * p.v_st, n, static_cast<int>(p.v_st) * 2, p.N);
+        fetch.template operator()<false>(lds + slot * BUF, kbase + j0 * p.k_st, n, static_cast<int>(p.k_st) * 2, p.N, 0);
+        fetch.template operator()<false>(lds + slot * BUF + Plane<D>::BYTES, vbase + j0 * p.v_st, n, static_cast<int>(p.v_st) * 2, p.N, 0);
         if constexpr (DOC) next_doc = lane < n ? doc[j0 + lane] : -1;
     };
-    Walk<DOC> walk(ranges, dlo, dhi, 0, tiles);
-    if (walk.t < tiles) load(walk.t);
-    for (int par = 0; walk.t < tiles; par ^= 1) {
-            const lds_t kb = lds + par * BUF, vb = kb + Plane<D>::BYTES;
-            if constexpr (DOC) ks.store(kb, __ballot(next_doc >= 0));
-            else ks.store(kb);
-            vs.store(vb);
-            if (DOC && tid < TILE) key_doc[par][tid] = next_doc;
-            const int j0 = walk.t * TILE;
-            const bool part = !walk.whole;
-            walk.next();
-            __syncthreads();
-            if (walk.t < tiles) load(walk.t);
-            if (j0 <= lim_hi) {
-                const bool masked = part || j0 + TILE - 1 > lim_lo;
+    // half e of a tile: scores and the gradients of the weights
+    const auto products = [&](f32x16& s, f32x16& dp, const int e) {
+        s = dp = f32x16{};
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    f32x16 s = f32x16{}, dp = f32x16{};
+        for (int c = 0; c < D / 16; ++c) {
+            s = mma<E>(rows(0, e, c), q[c], s);
+            dp = mma<E>(rows(Plane<D>::BYTES, e, c), dy[c], dp);
+        }
+    };
+    // the gradients of the scores, in s
+    const auto slopes = [&](f32x16& s, const f32x16& dp, const int j) {
+        const float dist = pos - static_cast<float>(j + 4 * hi);
 #pragma unroll
-                    for (int c = 0; c < D / 16; ++c) s = mma<E>(rows(kb, e, c), q[c], s);
+        for (int r = 0; r < 16; ++r) {
+            const float x = s[r], sq = sc.squash<CAP>(x);
+            float ds = __builtin_amdgcn_exp2f(fmaf(sc.t<CAP, BIAS>(x, sq, dist - (8 * (r >> 2) + (r & 3))), mul, -lse)) * (dp[r] - dlt);
+            if constexpr (CAP) ds *= 4.f * sq * (1.f - sq);
+            s[r] = ds;
+        }
+    };
+    const auto mask = [&](f32x16& s, const int j0, const int e, const int slot) {
+        asm volatile("");                                        // (a branch: few tiles come here)
+        const int room = lim - j0 - 4 * hi - 32 * e;
 #pragma unroll
-                    for (int c = 0; c < D / 16; ++c) dp = mma<E>(rows(vb, e, c), dy[c], dp);
-                    __builtin_amdgcn_sched_barrier(0);
-                    const float dist = pos - static_cast<float>(j0 + 4 * hi + 32 * e);
+        for (int n = 0; n < 4; ++n) {
+            u32x4 kd;
+            if constexpr (DOC) kd = *reinterpret_cast<const u32x4*>(key_doc + slot * TILE + 32 * e + 8 * n + 4 * hi);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const float x = s[r], sq = sc.squash<CAP>(x);
-                        const float w = __builtin_amdgcn_exp2f(fmaf(sc.t<CAP, BIAS>(x, sq, dist - (8 * (r >> 2) + (r & 3))), mul, -lse));
-                        float ds = w * (dp[r] - dlt);
-                        if constexpr (CAP) ds *= 4.f * sq * (1.f - sq);
-                        s[r] = ds;
-                    }
-                    if (masked) {
-                        const int room = lim - j0 - 4 * hi - 32 * e;
-#pragma unroll
-                        for (int n = 0; n < 4; ++n) {
-                            u32x4 kd;
-                            if constexpr (DOC) kd = *reinterpret_cast<const u32x4*>(&key_doc[par][32 * e + 8 * n + 4 * hi]);
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                bool on = 8 * n + r <= room;
-                                if constexpr (DOC) on = on && static_cast<int>(kd[r]) == qdoc;
-                                s[4 * n + r] = on ? s[4 * n + r] : 0.f;
-                            }
-                        }
-                    }
-                    const u32x4 w[2] = {as_operand<E>(s, 0), as_operand<E>(s, 1)};
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int d = 0; d < D / 32; ++d) g[d] = mma<E>(cols(kb, 2 * e + c, d), w[c], g[d]);
-                }
+            for (int r = 0; r < 4; ++r) {
+                bool on = 8 * n + r <= room;
+                if constexpr (DOC) on = on && static_cast<int>(kd[r]) == qdoc;
+                s[4 * n + r] = on ? s[4 * n + r] : 0.f;
             }
+        }
+    };
+    const auto add = [&](const u32x4 (&w)[2], const int e) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) g[d] = mma<E>(cols(0, 2 * e + c, d), w[c], g[d]);
+    };
+    Walk<DOC> walk(ranges, dlo, dhi, 0, tiles);
+    if (walk.t < tiles) bring(walk.t, 0);
+    int par = 0, step = BUF;
+    while (walk.t < tiles) {
+        const int j0 = walk.t * TILE;
+        const bool part = !walk.whole;
+        if (DOC && tid < TILE) key_doc[par * TILE + tid] = next_doc;
+        arrived();
+        __syncthreads();
+        walk.next();
+        if (walk.t < tiles) bring(walk.t, par ^ 1);
+        if (DOC && part) clear_padding<D>(lds + par * BUF, key_doc + par * TILE);
+        if (j0 <= lim_hi) {
+            const bool masked = part || j0 + TILE - 1 > lim_lo;
+            f32x16 s0, s1, p0, p1;
+            u32x4 w[2];
+            products(s0, p0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            products(s1, p1, 1);
+            slopes(s0, p0, j0);
+            beside<2 * D / 16, D / 8, SLOPE_VALUS * 16, SLOPE_TRANS * 16>();
+            __builtin_amdgcn_sched_barrier(0);
+            if (masked) mask(s0, j0, 0, par);
+            w[0] = as_operand<E>(s0, 0), w[1] = as_operand<E>(s0, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            add(w, 0);
+            slopes(s1, p1, j0 + 32);
+            beside<D / 16, D / 8, SLOPE_VALUS * 16, SLOPE_TRANS * 16>();
+            __builtin_amdgcn_sched_barrier(0);
+            if (masked) mask(s1, j0, 1, par);
+            w[0] = as_operand<E>(s1, 0), w[1] = as_operand<E>(s1, 1);
+            add(w, 1);
+        }
+        rows.move(step);
+        cols.move(step);
+        step = -step;
+        par ^= 1;
     }
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) store32<E>(g[d], p.scale, static_cast<E*>(p.dq) + row, nullptr, 32 * d, p.N, real);
@@ -164,26 +192,39 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const rwkv_attn_args p, const 
 
 // dK, dV: 4 waves of 32 keys over the queries, of all heads that share them, that see any of them; S = Q K^T and dP = dY V^T,
 // dV^T += dY^T P, dK^T += Q^T dS
-template <class E, int D, bool CAP, bool BIAS, bool DOC>
-__global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_dkv(const rwkv_attn_args p, const float* delta, const Range* key_ranges, const Range* ranges, const int blocks_k, const int per_xcd) {
-    constexpr int KB = 128;
-    __shared__ __align__(16) char smem[4 * Plane<D>::BYTES];
-    __shared__ __align__(16) int row_doc[2][TILE];
-    __shared__ __align__(16) float row_lse[2][TILE], row_delta[2][TILE];
+//
+// With heads of 128 the two sums take half of a wave's 256 registers and the keys a quarter of the rest: the values are read from LDS.  There a workgroup has 8 waves
+// (256 keys; two waves a SIMD), or 4 where there are few workgroups.
+template <class E, int D, int WAVES, bool CAP, bool BIAS, bool DOC>
+__global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void attn_dkv(const rwkv_attn_args p, const float* delta, const Range* key_ranges, const Range* ranges, const int blocks_k, const int per_xcd) {
+    constexpr int KB = 32 * WAVES, PLANES = 4 * Plane<D>::BYTES, VALUES = D == 128 ? KB / TILE * Plane<D>::BYTES : 0;
+    constexpr int VALUS = 5 + (CAP ? 6 : 0) + (BIAS ? 2 : 0), TRANS = CAP ? 3 : 1;      // instructions of a pair
+    // two planes of queries and of dY (below 64 KB: what M0 can name), lse, delta and documents of two tiles, the values of the block's keys
+    __shared__ __align__(16) char smem[PLANES + 6 * 4 * TILE + VALUES];
+    float *const row_lse = reinterpret_cast<float*>(smem + PLANES), *const row_delta = row_lse + 2 * TILE;
+    int* const row_doc = reinterpret_cast<int*>(row_delta + 2 * TILE);
     const int id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
     if (id >= wide(blocks_k) * p.Hk * p.B) return;
     const int bh = id / blocks_k, k0 = id % blocks_k * KB, b = bh / p.Hk, hk = bh % p.Hk, G = p.H / p.Hk;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5;
     const lds_t lds = lds_of(smem);
-    constexpr lds_t BUF = 2 * Plane<D>::BYTES;
+    constexpr int BUF = 2 * Plane<D>::BYTES;
 
     const int shift = p.Tk - p.Tq, reach = p.prefix ? min(p.prefix[b], p.Tk) : 0;
     const int* doc = DOC ? p.doc + wide(b) * p.Tk : nullptr;
     const int j = k0 + wave * 32 + (lane & 31);
     const bool real = j < p.Tk;
-    u32x4 k[D / 16], v[D / 16];
-    load_rows<E, D>(k, static_cast<const E*>(p.k) + b * p.k_sb + (real ? j : 0) * p.k_st + hk * p.k_sh, real, p.N);
-    load_rows<E, D>(v, static_cast<const E*>(p.v) + b * p.v_sb + (real ? j : 0) * p.v_st + hk * p.v_sh, real, p.N);
+    const E *kbase = static_cast<const E*>(p.k) + b * p.k_sb + hk * p.k_sh, *vbase = static_cast<const E*>(p.v) + b * p.v_sb + hk * p.v_sh;
+    u32x4 k[D / 16], v[D == 128 ? 1 : D / 16];
+    load_rows<E, D>(k, kbase + (real ? j : 0) * p.k_st, real, p.N);
+    if constexpr (D == 64) load_rows<E, D>(v, vbase + (real ? j : 0) * p.v_st, real, p.N);
+    else
+        for (int x = tid; x < KB * D / 8; x += 64 * WAVES) {
+            const int r = x / (D / 8), c = x % (D / 8);
+            u32x4 z = {0, 0, 0, 0};
+            if (k0 + r < p.Tk && 8 * c < p.N) z = *reinterpret_cast<const u32x4*>(vbase + (k0 + r) * p.v_st + 8 * c);
+            lds_st(lds + PLANES + 6 * 4 * TILE + r / TILE * Plane<D>::BYTES + Plane<D>::at(r % TILE, c), z);
+        }
     const int kdoc = DOC && real ? doc[j] : 0;
     const int from = kdoc < 0 ? INT_MAX : (!p.causal || j < reach ? 0 : j);            // the first position that sees the key; none that sees padding
     const int key_lo = k0 + __builtin_amdgcn_readfirstlane(wave) * 32, key_hi = min(key_lo + 31, p.Tk - 1);
@@ -194,108 +235,156 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_dkv(const rwkv_att
     if constexpr (DOC) {
         key_ranges += b * tiles_of(p.Tk) + k0 / TILE;
         ranges += b * tiles_of(p.Tq);
-        dlo = key_ranges[0].lo, dhi = key_ranges[0].hi;
-        if (k0 + TILE < p.Tk) dlo = min(dlo, key_ranges[1].lo), dhi = max(dhi, key_ranges[1].hi);
+        dlo = INT_MAX, dhi = -1;
+        for (int x = 0; x < KB / TILE && k0 + x * TILE < p.Tk; ++x) dlo = min(dlo, key_ranges[x].lo), dhi = max(dhi, key_ranges[x].hi);
     }
     const int first = !p.causal || k0 < reach ? 0 : max(0, k0 - shift) / TILE, tiles = (p.Tq + TILE - 1) / TILE;
 
-    const RowReader<D> rows(lane);
-    const ColReader<D> cols(lane);
-    Stage<D, 256> qs(tid, p.N), ys(tid, p.N);
+    RowReader<D> rows(lane);
+    ColReader<D> cols(lane);
+    rows.move(lds);
+    cols.move(lds);
+    const lds_t values = lds + PLANES + 6 * 4 * TILE + wave / 2 * Plane<D>::BYTES;
+    const RowReader<D> vrows(lane);
+    const Fetch<D, WAVES> fetch(tid, p.N);
     f32x16 gk[D / 32], gv[D / 32];
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) gk[d] = gv[d] = f32x16{};
 
     int next_doc = -1;
     float next_lse = 0.f, next_delta = 0.f;
-    const auto load = [&](const int h, const int t) {
+    const auto bring = [&](const int h, const int t, const int slot) {
         const int i0 = t * TILE, n = p.Tq - i0;
-        qs.load(static_cast<const E*>(p.q) + b * p.q_sb + i0 * p.q_st + h * p.q_sh, n, static_cast<int>(p.q_st) * 2, p.N);
-        ys.load(static_cast<const E*>(p.dy) + ((wide(b) * p.Tq + i0) * p.H + h) * p.N, n, p.H * p.N * 2, p.N);
-        const bool on = tid < TILE && tid < n;
+        fetch.template operator()<false>(lds + slot * BUF, static_cast<const E*>(p.q) + b * p.q_sb + i0 * p.q_st + h * p.q_sh, n, static_cast<int>(p.q_st) * 2, p.N, 0);
+        fetch.template operator()<false>(lds + slot * BUF + Plane<D>::BYTES, static_cast<const E*>(p.dy) + ((wide(b) * p.Tq + i0) * p.H + h) * p.N, n, p.H * p.N * 2, p.N, 0);
         if (tid < TILE) {
+            const bool on = tid < n;
             const int64_t stat = (wide(b) * p.H + h) * p.Tq + (on ? i0 + tid : 0);
             next_lse = p.lse[stat];
-            next_delta = delta[stat] * UNSHIFT<E>;
-            if (!on || next_lse == -INFINITY) next_lse = INFINITY, next_delta = 0.f;     // a row that is not there or sees nothing: weights of 0
-            next_lse -= SHIFT<E>;
+            next_delta = delta[stat];
+            if constexpr (DOC) next_doc = on ? doc[shift + i0 + tid] : -1;
         }
-        if constexpr (DOC) next_doc = lane < n ? doc[shift + i0 + lane] : -1;
     };
-    int h = hk * G, par = 0;
-    Walk<DOC> walk(ranges, dlo, dhi, first, tiles);
-    if (walk.t < tiles) load(h, walk.t);
-    const Walk<DOC> start = walk;
-    while (walk.t < tiles) {
-            const lds_t qb = lds + par * BUF, yb = qb + Plane<D>::BYTES;
-            if constexpr (DOC) qs.store(qb, __ballot(next_doc >= 0)), ys.store(yb, __ballot(next_doc >= 0));
-            else qs.store(qb), ys.store(yb);
-            if (tid < TILE) {
-                row_lse[par][tid] = next_lse;
-                row_delta[par][tid] = next_delta;
-                if (DOC) row_doc[par][tid] = next_doc;
+    const auto note = [&](const int t, const int slot) {
+        if (tid < TILE) {
+            const bool off = t * TILE + tid >= p.Tq || next_lse == -INFINITY;            // a row that is not there or sees nothing: weights of 0
+            row_lse[slot * TILE + tid] = off ? INFINITY : next_lse - SHIFT<E>;
+            row_delta[slot * TILE + tid] = off ? 0.f : next_delta * UNSHIFT<E>;
+            if (DOC) row_doc[slot * TILE + tid] = next_doc;
+        }
+    };
+    const auto products = [&](f32x16& s, f32x16& dp, const int e) {
+        s = dp = f32x16{};
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+            s = mma<E>(rows(0, e, c), k[c], s);
+            if constexpr (D == 64) dp = mma<E>(rows(Plane<D>::BYTES, e, c), v[c], dp);
+            else dp = mma<E>(rows(Plane<D>::BYTES, e, c), vrows(values, wave & 1, c), dp);
+        }
+    };
+    // weights in s, gradients of the scores in dp
+    const auto slopes = [&](const Scorer& sc, f32x16& s, f32x16& dp, const int i0, const int e, const int slot) {
+        const float dist = static_cast<float>(shift + i0 + 4 * hi + 32 * e) - static_cast<float>(j), mul = CAP || BIAS ? 1.f : sc.unit;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const int o = slot * TILE + 32 * e + 8 * n + 4 * hi;
+            const float4 ls = *reinterpret_cast<const float4*>(row_lse + o), dl = *reinterpret_cast<const float4*>(row_delta + o);
+            const float lse[4] = {ls.x, ls.y, ls.z, ls.w}, dlt[4] = {dl.x, dl.y, dl.z, dl.w};
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int at = 4 * n + r;
+                const float x = s[at], sq = sc.squash<CAP>(x);
+                const float w = __builtin_amdgcn_exp2f(fmaf(sc.t<CAP, BIAS>(x, sq, dist + (8 * n + r)), mul, -lse[r]));
+                float ds = w * (SHIFT<E> == 0.f ? dp[at] - dlt[r] : fmaf(dp[at], UNSHIFT<E>, -dlt[r]));
+                if constexpr (CAP) ds *= 4.f * sq * (1.f - sq);
+                s[at] = w;
+                dp[at] = ds;
             }
-            const int i0 = walk.t * TILE;
-            const bool part = !walk.whole;
-            const Scorer sc(p, h);
-            const float mul = CAP || BIAS ? 1.f : sc.unit;
-            walk.next();
-            if (walk.t >= tiles && h + 1 < hk * G + G) walk = start, ++h;
-            __syncthreads();
-            if (walk.t < tiles) load(h, walk.t);
-            if (shift + i0 + TILE - 1 >= from_lo) {
-                const bool masked = part || shift + i0 < from_hi;
+        }
+    };
+    const auto mask = [&](f32x16& s, f32x16& dp, const int i0, const int e, const int slot) {
+        asm volatile("");                                        // (a branch: few tiles come here)
+        const int need = from - shift - i0 - 4 * hi - 32 * e;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            u32x4 rd;
+            if constexpr (DOC) rd = *reinterpret_cast<const u32x4*>(row_doc + slot * TILE + 32 * e + 8 * n + 4 * hi);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                bool on = 8 * n + r >= need;
+                if constexpr (DOC) on = on && static_cast<int>(rd[r]) == kdoc;
+                s[4 * n + r] = on ? s[4 * n + r] : 0.f;
+                dp[4 * n + r] = on ? dp[4 * n + r] : 0.f;
+            }
+        }
+    };
+    const auto add = [&](const u32x4 (&w)[2], const u32x4 (&ds)[2], const int e) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) {
+                gv[d] = mma<E>(cols(Plane<D>::BYTES, 2 * e + c, d), w[c], gv[d]);
+                gk[d] = mma<E>(cols(0, 2 * e + c, d), ds[c], gk[d]);
+            }
+    };
+    int h = hk * G, par = 0, step = BUF;
+    Walk<DOC> walk(ranges, dlo, dhi, first, tiles);
+    const Walk<DOC> start = walk;
+    if (walk.t < tiles) bring(h, walk.t, 0);
+    while (walk.t < tiles) {
+        const int i0 = walk.t * TILE;
+        const bool part = !walk.whole;
+        const Scorer sc(p, h);
+        note(walk.t, par);
+        arrived();
+        __syncthreads();
+        walk.next();
+        if (walk.t >= tiles && h + 1 < hk * G + G) walk = start, ++h;
+        if (walk.t < tiles) bring(h, walk.t, par ^ 1);
+        if (DOC && part) {
+            clear_padding<D, WAVES>(lds + par * BUF, row_doc + par * TILE);
+            clear_padding<D, WAVES>(lds + par * BUF + Plane<D>::BYTES, row_doc + par * TILE);
+        }
+        if (shift + i0 + TILE - 1 >= from_lo) {
+            const bool masked = part || shift + i0 < from_hi;
+            u32x4 w[2], ds[2];
+            if constexpr (D == 64) {
+                f32x16 s0, s1, p0, p1;
+                products(s0, p0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                products(s1, p1, 1);
+                slopes(sc, s0, p0, i0, 0, par);
+                beside<2 * D / 16, D / 8 + 8, VALUS * 16, TRANS * 16>();
+                __builtin_amdgcn_sched_barrier(0);
+                if (masked) mask(s0, p0, i0, 0, par);
+                w[0] = as_operand<E>(s0, 0), w[1] = as_operand<E>(s0, 1), ds[0] = as_operand<E>(p0, 0), ds[1] = as_operand<E>(p0, 1);
+                __builtin_amdgcn_sched_barrier(0);
+                add(w, ds, 0);
+                slopes(sc, s1, p1, i0, 1, par);
+                beside<2 * D / 16, D / 4 + 8, VALUS * 16, TRANS * 16>();
+                __builtin_amdgcn_sched_barrier(0);
+                if (masked) mask(s1, p1, i0, 1, par);
+                w[0] = as_operand<E>(s1, 0), w[1] = as_operand<E>(s1, 1), ds[0] = as_operand<E>(p1, 0), ds[1] = as_operand<E>(p1, 1);
+                add(w, ds, 1);
+            } else {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    f32x16 s = f32x16{}, dp = f32x16{};
-#pragma unroll
-                    for (int c = 0; c < D / 16; ++c) s = mma<E>(rows(qb, e, c), k[c], s);
-#pragma unroll
-                    for (int c = 0; c < D / 16; ++c) dp = mma<E>(rows(yb, e, c), v[c], dp);
+                    f32x16 s, dp;
+                    products(s, dp, e);
                     __builtin_amdgcn_sched_barrier(0);
-                    const float dist = static_cast<float>(shift + i0 + 4 * hi + 32 * e) - static_cast<float>(j);
-                    const int need = from - shift - i0 - 4 * hi - 32 * e;
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const float4 ls = *reinterpret_cast<const float4*>(&row_lse[par][32 * e + 8 * n + 4 * hi]), dl = *reinterpret_cast<const float4*>(&row_delta[par][32 * e + 8 * n + 4 * hi]);
-                        const float lse[4] = {ls.x, ls.y, ls.z, ls.w}, dlt[4] = {dl.x, dl.y, dl.z, dl.w};
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int at = 4 * n + r;
-                            const float x = s[at], sq = sc.squash<CAP>(x);
-                            const float w = __builtin_amdgcn_exp2f(fmaf(sc.t<CAP, BIAS>(x, sq, dist + (8 * n + r)), mul, -lse[r]));
-                            float ds = w * fmaf(dp[at], UNSHIFT<E>, -dlt[r]);
-                            if constexpr (CAP) ds *= 4.f * sq * (1.f - sq);
-                            s[at] = w;
-                            dp[at] = ds;
-                        }
-                    }
-                    if (masked) {
-#pragma unroll
-                        for (int n = 0; n < 4; ++n) {
-                            u32x4 rd;
-                            if constexpr (DOC) rd = *reinterpret_cast<const u32x4*>(&row_doc[par][32 * e + 8 * n + 4 * hi]);
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                bool on = 8 * n + r >= need;
-                                if constexpr (DOC) on = on && static_cast<int>(rd[r]) == kdoc;
-                                s[4 * n + r] = on ? s[4 * n + r] : 0.f;
-                                dp[4 * n + r] = on ? dp[4 * n + r] : 0.f;
-                            }
-                        }
-                    }
-                    const u32x4 w[2] = {as_operand<E>(s, 0), as_operand<E>(s, 1)}, ds[2] = {as_operand<E>(dp, 0), as_operand<E>(dp, 1)};
+                    slopes(sc, s, dp, i0, e, par);
+                    if (masked) mask(s, dp, i0, e, par);
+                    w[0] = as_operand<E>(s, 0), w[1] = as_operand<E>(s, 1), ds[0] = as_operand<E>(dp, 0), ds[1] = as_operand<E>(dp, 1);
                     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int d = 0; d < D / 32; ++d) {
-                            gv[d] = mma<E>(cols(yb, 2 * e + c, d), w[c], gv[d]);
-                            gk[d] = mma<E>(cols(qb, 2 * e + c, d), ds[c], gk[d]);
-                        }
+                    add(w, ds, e);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            par ^= 1;
+        }
+        rows.move(step);
+        cols.move(step);
+        step = -step;
+        par ^= 1;
     }
     const int64_t row = ((wide(b) * p.Tk + (real ? j : 0)) * p.Hk + hk) * p.N;
 #pragma unroll
@@ -314,18 +403,22 @@ template <class E, int D> int run(hipStream_t st, const rwkv_attn_args& p) {
         launch_attn_ranges(st, p.doc, p.B, p.Tk, p.Tk - p.Tq, ranges);
     }
     const int64_t rows = wide(p.B) * p.Tq * p.H, row_blocks = (rows * (D / 8) + 255) / 256;
-    const int blocks_q = (p.Tq + 127) / 128, blocks_k = (p.Tk + 127) / 128;
+    // heads of 128: 256 keys a workgroup where these are enough for the card's 256 CUs
+    const bool eight = D == 128 && wide(p.B) * p.Hk * ((p.Tk + 255) / 256) >= 256;
+    const int blocks_q = (p.Tq + 127) / 128, blocks_k = eight ? (p.Tk + 255) / 256 : (p.Tk + 127) / 128;
     const int64_t per_q = (wide(blocks_q) * p.H * p.B + 7) / 8, per_k = (wide(blocks_k) * p.Hk * p.B + 7) / 8;
     if (row_blocks > INT_MAX || per_q * 8 > INT_MAX || per_k * 8 > INT_MAX) return RWKV_ERR_SHAPE;
     hipLaunchKernelGGL((attn_delta<E, D>), dim3(static_cast<unsigned>(row_blocks)), dim3(256), 0, st, p, delta);
     const auto go = [&](auto dq, auto dkv) {
-        hipLaunchKernelGGL(dkv, dim3(static_cast<unsigned>(per_k * 8)), dim3(256), 0, st, p, delta, key_ranges, ranges, blocks_k, static_cast<int>(per_k));
+        hipLaunchKernelGGL(dkv, dim3(static_cast<unsigned>(per_k * 8)), dim3(eight ? 512 : 256), 0, st, p, delta, key_ranges, ranges, blocks_k, static_cast<int>(per_k));
         hipLaunchKernelGGL(dq, dim3(static_cast<unsigned>(per_q * 8)), dim3(256), 0, st, p, delta, key_ranges, blocks_q, static_cast<int>(per_q));
         return launch_status();
     };
     const auto masks = [&](auto cap, auto bias) {
         constexpr bool C = decltype(cap)::value, S = decltype(bias)::value;
-        return p.doc ? go(attn_dq<E, D, C, S, true>, attn_dkv<E, D, C, S, true>) : go(attn_dq<E, D, C, S, false>, attn_dkv<E, D, C, S, false>);
+        constexpr int W = D == 128 ? 8 : 4;
+        if (p.doc) return go(attn_dq<E, D, C, S, true>, eight ? attn_dkv<E, D, W, C, S, true> : attn_dkv<E, D, 4, C, S, true>);
+        return go(attn_dq<E, D, C, S, false>, eight ? attn_dkv<E, D, W, C, S, false> : attn_dkv<E, D, 4, C, S, false>);
     };
     using yes = std::true_type;
     using no = std::false_type;

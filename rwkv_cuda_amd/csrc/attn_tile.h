@@ -107,47 +107,8 @@ template <int D> struct ColReader {
 DEVINL void here(u32x4& x) { asm volatile("" : "+v"(x)); }
 DEVINL void here(float& x) { asm volatile("" : "+v"(x)); }
 
-// The way of a tile of 64 rows from memory to LDS: a piece of 16 bytes a thread and step, zeros behind the last row and the last channel
-// (the buffer's bounds), and for rows that are to count as zeros.
-template <int D, int THREADS> struct Stage {
-    static constexpr int STEPS = TILE * D / 8 / THREADS, STEP_ROWS = THREADS / (D / 8);
-    u32x4 x[STEPS];
-    int row, off;                                               // the thread's first row, and its bytes within a row (beyond all bounds: no such channel)
-    lds_t to;
-    DEVINL Stage(const int tid, const int N) {
-        row = tid / (D / 8);
-        const int c = tid % (D / 8);
-        off = 8 * c < N ? 16 * c : 0x7ffffff0;
-        to = Plane<D>::at(row, c);
-    }
-    // rows from `first` on, `rows` of them there, `step` bytes apart
-    DEVINL void load(const void* first, const int rows, const int step, const int N) {
-        const buf_t b = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(first), 0, rows > 0 ? (rows - 1) * step + 2 * N : 0, 0x00027000);
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            const int r = row + i * STEP_ROWS;
-            x[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, off == 0x7ffffff0 || r >= rows ? 0x7ffffff0 : r * step + off, 0, 0));
-        }
-    }
-    DEVINL void store(const lds_t base) const {
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) lds_st(base + to + i * (STEP_ROWS / Plane<D>::ROWS) * Plane<D>::STEP, x[i]);
-    }
-    // only the rows whose bit is set: those of padding may hold anything and count as zeros
-    DEVINL void store(const lds_t base, const uint64_t rows) const {
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            const bool on = rows >> (row + i * STEP_ROWS) & 1;
-            u32x4 z = x[i];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) z[e] = on ? z[e] : 0u;
-            lds_st(base + to + i * (STEP_ROWS / Plane<D>::ROWS) * Plane<D>::STEP, z);
-        }
-    }
-};
-
-// The same without a stop in registers: 16 bytes a lane from memory straight to LDS, a wave's 1024 bytes in the order of its lanes, so that each lane
-// fetches the piece whose place it is.  The compiler does not count these loads: arrived() before the barrier behind which they are read.  Of the waves of a
+// The way of a tile of 64 rows from memory straight to LDS: 16 bytes a lane, a wave's 1024 bytes in the order of its lanes, so that each lane fetches the piece whose
+// place it is.  Rows behind the last and channels behind N come as zeros (the buffer's bounds).  The compiler does not count these loads: arrived() before the barrier behind which they are read.  Of the waves of a
 // workgroup each brings every WAVES-th kilobyte.
 template <int D, int WAVES> struct Fetch {
     static constexpr int LANES = D / 8, ROWS = Plane<D>::ROWS, STEPS = TILE / (ROWS * WAVES);
@@ -176,6 +137,25 @@ template <int D, int WAVES> struct Fetch {
         }
     }
 };
+// Rows of padding may hold anything, and count as zeros where rows are summed.  Called by all of a workgroup's threads; the barrier behind it is here.
+template <int D, int WAVES = 4> DEVINL void clear_padding(const lds_t plane, const int* docs) {
+    constexpr int SHARE = WAVES;                                // threads of a row
+    const int r = threadIdx.x / SHARE;
+    if (docs[r] < 0)
+        for (int c = threadIdx.x % SHARE; c < D / 8; c += SHARE) lds_st(plane + Plane<D>::at(r, c), u32x4{0, 0, 0, 0});
+    __syncthreads();
+}
+// The order of what stands before it: a product, and its part of the LDS reads and of the other instructions.
+template <int PRODUCTS, int READS, int VALUS, int TRANS> DEVINL void beside() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int c = 0; c < PRODUCTS; ++c) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, (READS + PRODUCTS - 1) / PRODUCTS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, (VALUS + PRODUCTS - 1) / PRODUCTS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x400, (TRANS + PRODUCTS - 1) / PRODUCTS, 0);
+    }
+}
 DEVINL void arrived() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
 
 // An accumulator [channel][row of the output] times `f`, rounded, to 32 channels of the lane's row (and what the rounding lost to `rest`).
