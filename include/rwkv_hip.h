@@ -621,10 +621,10 @@ typedef struct rwkv_attn_args {
     float* lse;                       /* [B,H,Tq]; forward: may be NULL */
     const void* dy;                   /* backward: [B,Tq,H,N], 16-byte aligned */
     void *dq, *dk, *dv;               /* backward: dense, 16-byte aligned */
-    void* workspace;                  /* 16-byte aligned; the forward needs one with doc only */
+    void* workspace;                  /* 16-byte aligned */
     size_t workspace_bytes;
 } rwkv_attn_args;
-size_t rwkv_attn_workspace_bytes(int B, int Tq, int Tk, int H, int doc, int backward);      /* doc, backward: 0 or 1 */
+size_t rwkv_attn_workspace_bytes(int B, int Tq, int Tk, int H, int Hk, int N, int doc, int backward);      /* doc, backward: 0 or 1; 0: none is needed */
 int rwkv_attn_forward(void* stream, const rwkv_attn_args* args);
 int rwkv_attn_backward(void* stream, const rwkv_attn_args* args);
 

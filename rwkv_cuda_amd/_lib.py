@@ -230,7 +230,7 @@ SIGNATURES = {
     "rwkv_grec_workspace_bytes": (_Z, [_I, _I, _I]),
     "rwkv_grec_forward": (_I, [_P, ctypes.POINTER(GrecArgs)]),
     "rwkv_grec_backward": (_I, [_P, ctypes.POINTER(GrecArgs)]),
-    "rwkv_attn_workspace_bytes": (_Z, [_I] * 6),
+    "rwkv_attn_workspace_bytes": (_Z, [_I] * 8),
     "rwkv_attn_forward": (_I, [_P, ctypes.POINTER(AttnArgs)]),
     "rwkv_attn_backward": (_I, [_P, ctypes.POINTER(AttnArgs)]),
     "rwkv_paged_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I]),

@@ -1,6 +1,8 @@
 // Attention with capped scores, distance bias, documents and prefixes: the entry points (the arguments are explained in rwkv_hip.h).  Kernels:
 // attn_fwd.hip, attn_bwd.hip.  Backward, with p the softmax's weights, dp = dy.v and delta = dy.y:  ds = p (dp - delta) (1 - tanh^2);
 // dv = p^T dy;  dq = scale ds k;  dk = scale ds^T q.
+#include <algorithm>
+
 #include "common.h"
 #include "mixers.h"
 
@@ -16,6 +18,31 @@ bool wide_rows(const rwkv_attn_args& p) {
     for (const int64_t s : {p.q_st, p.k_st, p.v_st, static_cast<int64_t>(p.H) * p.N}) if (s < 0 || s >= 1 << 24) return true;
     return false;
 }
+}  // namespace
+
+// A CU runs two workgroups of attn_fwd with heads of 128, four with heads of 64.  B1 Tq512 Tk16384 H32 N128, 128 workgroups: 0.30 ms whole, PIECE ms in four parts.
+// attn_dkv: B1 T3001 H32 Hk8 N128 with five documents, 192 workgroups: 0.30 ms whole, GROUP ms in four groups.
+AttnPlan attn_plan(int B, int Tq, int Tk, int H, int Hk, int N, bool doc) {
+    const int64_t width = N <= 64 ? 64 : 128, tiles = (static_cast<int64_t>(Tk) + 63) / 64;
+    const auto blocks = [](int64_t n, int64_t of) { return (n + of - 1) / of; };
+    AttnPlan a{};
+    const int64_t queries = blocks(Tq, 128) * H * B, room = width == 64 ? 1024 : 512;
+    a.query_parts = static_cast<int>(std::max<int64_t>(1, std::min({room / queries, tiles / 8, int64_t{16}})));
+    const int G = H / Hk;
+    const int64_t keys = blocks(Tk, width == 64 ? 128 : 256) * Hk * B, want = width == 64 ? 512 : 256;
+    a.key_parts = 1;
+    for (int x = 2; x <= G; ++x)
+        if (G % x == 0 && keys * a.key_parts < want) a.key_parts = x;
+    a.eight = width == 128 && keys * a.key_parts >= 256;
+    a.ranges = doc ? static_cast<size_t>(B) * tiles * sizeof(Range) : 0;
+    a.forward = a.ranges + (a.query_parts > 1 ? static_cast<size_t>(B) * H * Tq * a.query_parts * (width + 4) * sizeof(float) : 0);
+    a.backward = a.ranges + (doc ? static_cast<size_t>(B) * blocks(Tq, 64) * sizeof(Range) : 0) + (static_cast<size_t>(B) * Tq * H * sizeof(float) + 15) / 16 * 16 +
+                 (a.key_parts > 1 ? 2 * static_cast<size_t>(a.key_parts) * B * Tk * Hk * N * sizeof(float) : 0);
+    return a;
+}
+
+namespace {
+
 int check_attn(const rwkv_attn_args* p, bool backward) {
     if (p == nullptr) return RWKV_ERR_NULL;
     if ((p->dtype != RWKV_DTYPE_BF16 && p->dtype != RWKV_DTYPE_FP16) || p->B <= 0 || p->Tq <= 0 || p->Tk < p->Tq || p->H <= 0 || p->Hk <= 0 || p->H % p->Hk != 0 ||
@@ -25,10 +52,11 @@ int check_attn(const rwkv_attn_args* p, bool backward) {
     if (backward) {
         if (const int rc = check_ptrs({p->dy, p->dq, p->dk, p->dv, p->y_rest})) return rc;
         if (p->lse == nullptr) return RWKV_ERR_NULL;
-        if (p->workspace == nullptr || !aligned16(p->workspace) || p->workspace_bytes < rwkv_attn_workspace_bytes(p->B, p->Tq, p->Tk, p->H, p->doc != nullptr, 1)) return RWKV_ERR_WORKSPACE;
+        if (p->workspace == nullptr || !aligned16(p->workspace) || p->workspace_bytes < attn_plan(p->B, p->Tq, p->Tk, p->H, p->Hk, p->N, p->doc != nullptr).backward) return RWKV_ERR_WORKSPACE;
     } else {
         if (!aligned16(p->y_rest)) return RWKV_ERR_ALIGN;
-        if (p->doc != nullptr && (p->workspace == nullptr || !aligned16(p->workspace) || p->workspace_bytes < rwkv_attn_workspace_bytes(p->B, p->Tq, p->Tk, p->H, 1, 0))) return RWKV_ERR_WORKSPACE;
+        const size_t need = attn_plan(p->B, p->Tq, p->Tk, p->H, p->Hk, p->N, p->doc != nullptr).forward;
+        if (need > 0 && (p->workspace == nullptr || !aligned16(p->workspace) || p->workspace_bytes < need)) return RWKV_ERR_WORKSPACE;
     }
     for (const void* q : {static_cast<const void*>(p->slopes), static_cast<const void*>(p->doc), static_cast<const void*>(p->prefix), static_cast<const void*>(p->lse)})
         if (reinterpret_cast<uintptr_t>(q) & 3) return RWKV_ERR_ALIGN;
@@ -46,12 +74,10 @@ int attn_any(void* stream, const rwkv_attn_args* p, bool backward) {
 
 extern "C" {
 
-// the documents of tiles of 64 keys (16 bytes each), in the backward also of tiles of queries, and a sum of each query and head
-size_t rwkv_attn_workspace_bytes(int B, int Tq, int Tk, int H, int doc, int backward) {
-    if (B <= 0 || Tq <= 0 || Tk < Tq || H <= 0) return 0;
-    size_t n = doc ? static_cast<size_t>(B) * ((static_cast<int64_t>(Tk) + 63) / 64) * 16 : 0;
-    if (backward) n += (doc ? static_cast<size_t>(B) * ((static_cast<int64_t>(Tq) + 63) / 64) * 16 : 0) + static_cast<size_t>(B) * Tq * H * sizeof(float);
-    return n;
+size_t rwkv_attn_workspace_bytes(int B, int Tq, int Tk, int H, int Hk, int N, int doc, int backward) {
+    if (B <= 0 || Tq <= 0 || Tk < Tq || H <= 0 || Hk <= 0 || H % Hk != 0 || N <= 0 || N > 128) return 0;
+    const rwkv::AttnPlan a = rwkv::attn_plan(B, Tq, Tk, H, Hk, N, doc != 0);
+    return backward ? a.backward : a.forward;
 }
 int rwkv_attn_forward(void* stream, const rwkv_attn_args* args) { return rwkv::attn_any(stream, args, false); }
 int rwkv_attn_backward(void* stream, const rwkv_attn_args* args) { return rwkv::attn_any(stream, args, true); }

@@ -196,7 +196,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const rwkv_attn_args p, const 
 // With heads of 128 the two sums take half of a wave's 256 registers and the keys a quarter of the rest: the values are read from LDS.  There a workgroup has 8 waves
 // (256 keys; two waves a SIMD), or 4 where there are few workgroups.
 template <class E, int D, int WAVES, bool CAP, bool BIAS, bool DOC>
-__global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void attn_dkv(const rwkv_attn_args p, const float* delta, const Range* key_ranges, const Range* ranges, const int blocks_k, const int per_xcd) {
+__global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void attn_dkv(const rwkv_attn_args p, const float* delta, const Range* key_ranges, const Range* ranges, const int blocks_k, const int per_xcd, const int parts, float* part) {
     constexpr int KB = 32 * WAVES, PLANES = 4 * Plane<D>::BYTES, VALUES = D == 128 ? KB / TILE * Plane<D>::BYTES : 0;
     constexpr int VALUS = 5 + (CAP ? 6 : 0) + (BIAS ? 2 : 0), TRANS = CAP ? 3 : 1;      // instructions of a pair
     // two planes of queries and of dY (below 64 KB: what M0 can name), lse, delta and documents of two tiles, the values of the block's keys
@@ -204,8 +204,9 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void at
     float *const row_lse = reinterpret_cast<float*>(smem + PLANES), *const row_delta = row_lse + 2 * TILE;
     int* const row_doc = reinterpret_cast<int*>(row_delta + 2 * TILE);
     const int id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-    if (id >= wide(blocks_k) * p.Hk * p.B) return;
-    const int bh = id / blocks_k, k0 = id % blocks_k * KB, b = bh / p.Hk, hk = bh % p.Hk, G = p.H / p.Hk;
+    if (id >= wide(blocks_k) * parts * p.Hk * p.B) return;
+    const int bh = id / (blocks_k * parts), mine = id / blocks_k % parts, k0 = id % blocks_k * KB, b = bh / p.Hk, hk = bh % p.Hk, G = p.H / p.Hk / parts;
+    const int first_head = (hk * parts + mine) * G;              // of G that the block does
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5;
     const lds_t lds = lds_of(smem);
     constexpr int BUF = 2 * Plane<D>::BYTES;
@@ -327,7 +328,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void at
                 gk[d] = mma<E>(cols(0, 2 * e + c, d), ds[c], gk[d]);
             }
     };
-    int h = hk * G, par = 0, step = BUF;
+    int h = first_head, par = 0, step = BUF;
     Walk<DOC> walk(ranges, dlo, dhi, first, tiles);
     const Walk<DOC> start = walk;
     if (walk.t < tiles) bring(h, walk.t, 0);
@@ -339,7 +340,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void at
         arrived();
         __syncthreads();
         walk.next();
-        if (walk.t >= tiles && h + 1 < hk * G + G) walk = start, ++h;
+        if (walk.t >= tiles && h + 1 < first_head + G) walk = start, ++h;
         if (walk.t < tiles) bring(h, walk.t, par ^ 1);
         if (DOC && part) {
             clear_padding<D, WAVES>(lds + par * BUF, row_doc + par * TILE);
@@ -387,6 +388,20 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void at
         par ^= 1;
     }
     const int64_t row = ((wide(b) * p.Tk + (real ? j : 0)) * p.Hk + hk) * p.N;
+    if (parts > 1) {
+        const int64_t size = wide(p.B) * p.Tk * p.Hk * p.N;
+        float* to = part + 2 * mine * size + row;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const int c = 32 * d + 8 * n + 4 * hi;
+                if (!real || c >= p.N) continue;
+                *reinterpret_cast<float4*>(to + c) = make_float4(gk[d][4 * n], gk[d][4 * n + 1], gk[d][4 * n + 2], gk[d][4 * n + 3]);
+                *reinterpret_cast<float4*>(to + size + c) = make_float4(gv[d][4 * n], gv[d][4 * n + 1], gv[d][4 * n + 2], gv[d][4 * n + 3]);
+            }
+        return;
+    }
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) {
         store32<E>(gk[d], p.scale, static_cast<E*>(p.dk) + row, nullptr, 32 * d, p.N, real);
@@ -394,23 +409,41 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void at
     }
 }
 
+// adds the groups of heads: eight values a thread, y = 0 for dK, 1 for dV
+template <class E> __global__ __launch_bounds__(256) void attn_dkv_sum(const rwkv_attn_args p, const int parts, const float* part) {
+    const int64_t size = wide(p.B) * p.Tk * p.Hk * p.N, at = (blockIdx.x * wide(256) + threadIdx.x) * 8;
+    if (at >= size) return;
+    float s[8] = {};
+    for (int i = 0; i < parts; ++i) {
+        const float4* x = reinterpret_cast<const float4*>(part + (2 * i + blockIdx.y) * size + at);
+        const float4 a = x[0], b = x[1];
+        s[0] += a.x, s[1] += a.y, s[2] += a.z, s[3] += a.w, s[4] += b.x, s[5] += b.y, s[6] += b.z, s[7] += b.w;
+    }
+    const float f = blockIdx.y ? UNSHIFT<E> : p.scale;
+    *reinterpret_cast<u32x4*>(static_cast<E*>(blockIdx.y ? p.dv : p.dk) + at) =
+        u32x4{pack2<E>(s[0] * f, s[1] * f), pack2<E>(s[2] * f, s[3] * f), pack2<E>(s[4] * f, s[5] * f), pack2<E>(s[6] * f, s[7] * f)};
+}
+
 template <class E, int D> int run(hipStream_t st, const rwkv_attn_args& p) {
-    // the documents of tiles of keys, of tiles of queries, and delta
+    const int64_t rows = wide(p.B) * p.Tq * p.H, row_blocks = (rows * (D / 8) + 255) / 256;
+    const AttnPlan plan = attn_plan(p.B, p.Tq, p.Tk, p.H, p.Hk, p.N, p.doc != nullptr);
+    const bool eight = plan.eight;
+    const int blocks_q = (p.Tq + 127) / 128, blocks_k = eight ? (p.Tk + 255) / 256 : (p.Tk + 127) / 128;
+    const int64_t per_q = (wide(blocks_q) * p.H * p.B + 7) / 8, per_k = (wide(blocks_k) * plan.key_parts * p.Hk * p.B + 7) / 8;
+    const int64_t sums = (wide(p.B) * p.Tk * p.Hk * p.N / 8 + 255) / 256;
+    if (row_blocks > INT_MAX || per_q * 8 > INT_MAX || per_k * 8 > INT_MAX || (plan.key_parts > 1 && sums > INT_MAX)) return RWKV_ERR_SHAPE;
+    // the documents of tiles of keys and of tiles of queries, delta, the sums of groups of heads
     Range *key_ranges = static_cast<Range*>(p.workspace), *ranges = key_ranges + (p.doc ? p.B * tiles_of(p.Tk) : 0);
     float* delta = reinterpret_cast<float*>(ranges + (p.doc ? p.B * tiles_of(p.Tq) : 0));
+    float* part = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + plan.backward) - (plan.key_parts > 1 ? 2 * plan.key_parts * wide(p.B) * p.Tk * p.Hk * p.N : 0);
     if (p.doc) {
         launch_attn_ranges(st, p.doc, p.B, p.Tk, 0, key_ranges);
         launch_attn_ranges(st, p.doc, p.B, p.Tk, p.Tk - p.Tq, ranges);
     }
-    const int64_t rows = wide(p.B) * p.Tq * p.H, row_blocks = (rows * (D / 8) + 255) / 256;
-    // heads of 128: 256 keys a workgroup where these are enough for the card's 256 CUs
-    const bool eight = D == 128 && wide(p.B) * p.Hk * ((p.Tk + 255) / 256) >= 256;
-    const int blocks_q = (p.Tq + 127) / 128, blocks_k = eight ? (p.Tk + 255) / 256 : (p.Tk + 127) / 128;
-    const int64_t per_q = (wide(blocks_q) * p.H * p.B + 7) / 8, per_k = (wide(blocks_k) * p.Hk * p.B + 7) / 8;
-    if (row_blocks > INT_MAX || per_q * 8 > INT_MAX || per_k * 8 > INT_MAX) return RWKV_ERR_SHAPE;
     hipLaunchKernelGGL((attn_delta<E, D>), dim3(static_cast<unsigned>(row_blocks)), dim3(256), 0, st, p, delta);
     const auto go = [&](auto dq, auto dkv) {
-        hipLaunchKernelGGL(dkv, dim3(static_cast<unsigned>(per_k * 8)), dim3(eight ? 512 : 256), 0, st, p, delta, key_ranges, ranges, blocks_k, static_cast<int>(per_k));
+        hipLaunchKernelGGL(dkv, dim3(static_cast<unsigned>(per_k * 8)), dim3(eight ? 512 : 256), 0, st, p, delta, key_ranges, ranges, blocks_k, static_cast<int>(per_k), plan.key_parts, part);
+        if (plan.key_parts > 1) hipLaunchKernelGGL((attn_dkv_sum<E>), dim3(static_cast<unsigned>(sums), 2), dim3(256), 0, st, p, plan.key_parts, part);
         hipLaunchKernelGGL(dq, dim3(static_cast<unsigned>(per_q * 8)), dim3(256), 0, st, p, delta, key_ranges, blocks_q, static_cast<int>(per_q));
         return launch_status();
     };

@@ -12,17 +12,18 @@ using yes = std::true_type;
 using no = std::false_type;
 constexpr int READS = 6;
 
+// parts > 1: the block does one part of the keys, and leaves sums and maxima in `part` for attn_join.
 template <class E, int D, bool CAP, bool BIAS, bool DOC>
-__global__ __launch_bounds__(256, 2) void attn_fwd(const rwkv_attn_args p, const Range* ranges, const int blocks_q, const int per_xcd) {
+__global__ __launch_bounds__(256, 2) void attn_fwd(const rwkv_attn_args p, const Range* ranges, const int blocks_q, const int per_xcd, const int parts, float* part) {
     constexpr int QB = 128;
     // two planes of keys and of values (below 64 KB: what M0 can name), and the documents of two tiles
     constexpr int PLANES = 4 * Plane<D>::BYTES;
     __shared__ __align__(16) char smem[PLANES + (DOC ? 8 * TILE : 0)];
     int* const key_doc = reinterpret_cast<int*>(smem + PLANES);
     const int id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-    const int64_t all = wide(blocks_q) * p.H * p.B;
+    const int64_t all = wide(blocks_q) * parts * p.H * p.B;
     if (id >= all) return;
-    const int bh = id / blocks_q, q0 = (blocks_q - 1 - id % blocks_q) * QB, b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
+    const int bh = id / (blocks_q * parts), mine = id % parts, q0 = (blocks_q - 1 - id / parts % blocks_q) * QB, b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5;
     const lds_t lds = lds_of(smem);
     constexpr int BUF = 2 * Plane<D>::BYTES;
@@ -51,7 +52,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd(const rwkv_attn_args p, const
     }
     // the last key that the block's last query sees
     const int last = p.causal ? max(min(q0 + QB, p.Tq) - 1 + shift, reach) : p.Tk - 1;
-    const int tiles = last / TILE + 1;
+    const int all_tiles = last / TILE + 1, first_tile = static_cast<int>(wide(all_tiles) * mine / parts), tiles = static_cast<int>(wide(all_tiles) * (mine + 1) / parts);
 
     RowReader<D> krow(lane);
     ColReader<D> vcol(lane);
@@ -176,7 +177,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd(const rwkv_attn_args p, const
     const auto fetch_values = [&](const int t, const int slot, const uint64_t real) {
         fetch.template operator()<DOC>(lds + slot * BUF + Plane<D>::BYTES, vbase + t * TILE * p.v_st, p.Tk - t * TILE, static_cast<int>(p.v_st) * 2, p.N, real);
     };
-    Walk<DOC> walk(ranges, dlo, dhi, 0, tiles);
+    Walk<DOC> walk(ranges, dlo, dhi, first_tile, tiles);
     if (walk.t < tiles) {
         int t = walk.t;
         bool whole = walk.whole;
@@ -225,20 +226,64 @@ __global__ __launch_bounds__(256, 2) void attn_fwd(const rwkv_attn_args p, const
     }
 
     const float sum = l + other_half(l), inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (parts > 1) {
+        if (!real) return;
+        float* to = part + (((wide(b) * p.H + h) * p.Tq + i) * parts + mine) * (D + 4);
+        if (hi == 0) to[0] = m * mul, to[1] = sum;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) *reinterpret_cast<float4*>(to + 4 + 32 * d + 8 * g + 4 * hi) = make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+        return;
+    }
     const int64_t at = ((wide(b) * p.Tq + (real ? i : 0)) * p.H + h) * p.N;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) store32<E>(o[d], inv, static_cast<E*>(p.y) + at, p.y_rest ? static_cast<E*>(p.y_rest) + at : nullptr, 32 * d, p.N, real);
     if (p.lse && real && hi == 0) p.lse[(wide(b) * p.H + h) * p.Tq + i] = sum == 0.f ? -INFINITY : fmaf(m, mul, __builtin_amdgcn_logf(sum));
 }
 
+// joins the parts of a query: D / 4 lanes, four channels each
+template <class E, int D> __global__ __launch_bounds__(256) void attn_join(const rwkv_attn_args p, const int parts, const float* part) {
+    constexpr int LANES = D / 4;
+    const int64_t row = blockIdx.x * wide(256 / LANES) + threadIdx.x / LANES;       // of [B,H,Tq]
+    const int c = threadIdx.x % LANES * 4;
+    if (row >= wide(p.B) * p.H * p.Tq || c >= p.N) return;
+    const float* from = part + row * parts * (D + 4);
+    float top = -INFINITY;
+    for (int i = 0; i < parts; ++i) top = fmaxf(top, from[i * (D + 4)]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < parts; ++i) {
+        const float* x = from + i * (D + 4);
+        const float f = __builtin_amdgcn_exp2f(x[0] - base);
+        const float4 o = *reinterpret_cast<const float4*>(x + 4 + c);
+        sum = fmaf(x[1], f, sum);
+        y[0] = fmaf(o.x, f, y[0]), y[1] = fmaf(o.y, f, y[1]), y[2] = fmaf(o.z, f, y[2]), y[3] = fmaf(o.w, f, y[3]);
+    }
+    const float f = sum == 0.f ? 0.f : 1.f / sum;
+    const int i = row % p.Tq, h = row / p.Tq % p.H;
+    const int64_t at = ((row / p.Tq / p.H * p.Tq + i) * p.H + h) * p.N + c;
+    const u32x2 w = {pack2<E>(y[0] * f, y[1] * f), pack2<E>(y[2] * f, y[3] * f)};
+    *reinterpret_cast<u32x2*>(static_cast<E*>(p.y) + at) = w;
+    if (p.y_rest)
+        *reinterpret_cast<u32x2*>(static_cast<E*>(p.y_rest) + at) = u32x2{pack2<E>(y[0] * f - unpack_lo<E>(w[0]), y[1] * f - unpack_hi<E>(w[0])), pack2<E>(y[2] * f - unpack_lo<E>(w[1]), y[3] * f - unpack_hi<E>(w[1]))};
+    if (p.lse && c == 0) p.lse[row] = sum == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(sum);
+}
+
 template <class E, int D> int run(hipStream_t st, const rwkv_attn_args& p) {
     const int blocks_q = (p.Tq + 127) / 128;
-    const int64_t all = wide(blocks_q) * p.H * p.B, per = (all + 7) / 8;
-    if (per * 8 > INT_MAX) return RWKV_ERR_SHAPE;
+    const AttnPlan plan = attn_plan(p.B, p.Tq, p.Tk, p.H, p.Hk, p.N, p.doc != nullptr);
+    const int64_t all = wide(blocks_q) * plan.query_parts * p.H * p.B, per = (all + 7) / 8, join = (wide(p.B) * p.H * p.Tq * (D / 4) + 255) / 256;
+    if (per * 8 > INT_MAX || (plan.query_parts > 1 && join > INT_MAX)) return RWKV_ERR_SHAPE;
+    float* part = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + plan.ranges);
     const dim3 grid(static_cast<unsigned>(per * 8)), block(256);
     Range* ranges = static_cast<Range*>(p.workspace);
     if (p.doc) launch_attn_ranges(st, p.doc, p.B, p.Tk, 0, ranges);
-    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, p, ranges, blocks_q, static_cast<int>(per)); return launch_status(); };
+    const auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, block, 0, st, p, ranges, blocks_q, static_cast<int>(per), plan.query_parts, part);
+        if (plan.query_parts > 1) hipLaunchKernelGGL((attn_join<E, D>), dim3(static_cast<unsigned>(join)), block, 0, st, p, plan.query_parts, part);
+        return launch_status();
+    };
     const auto masks = [&](auto cap, auto bias) {
         return p.doc ? go(attn_fwd<E, D, decltype(cap)::value, decltype(bias)::value, true>) : go(attn_fwd<E, D, decltype(cap)::value, decltype(bias)::value, false>);
     };

@@ -622,7 +622,7 @@ struct Attn : Function<Attn> {
             lse = at::empty({B, H, Tq}, q.options().dtype(F32));
             a.y_rest = P(rest); a.lse = P(lse);
         }
-        a.workspace_bytes = rwkv_attn_workspace_bytes(a.B, a.Tq, a.Tk, a.H, doc.defined(), 0);
+        a.workspace_bytes = rwkv_attn_workspace_bytes(a.B, a.Tq, a.Tk, a.H, a.Hk, a.N, doc.defined(), 0);
         const Tensor ws = a.workspace_bytes > 0 ? bytes(q, a.workspace_bytes) : Tensor();
         a.workspace = P(ws);
         ok(rwkv_attn_forward(stream_of(q), &a));
@@ -641,7 +641,7 @@ struct Attn : Function<Attn> {
         Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
         a.doc = P(s[3]); a.prefix = P(s[4]); a.slopes = P(s[5]); a.y = P(y); a.y_rest = P(rest); a.lse = P(lse);
         a.dy = P(dy); a.dq = P(dq); a.dk = P(dk); a.dv = P(dv);
-        a.workspace_bytes = rwkv_attn_workspace_bytes(a.B, a.Tq, a.Tk, a.H, s[3].defined(), 1);
+        a.workspace_bytes = rwkv_attn_workspace_bytes(a.B, a.Tq, a.Tk, a.H, a.Hk, a.N, s[3].defined(), 1);
         const Tensor ws = bytes(q, a.workspace_bytes);
         a.workspace = P(ws);
         ok(rwkv_attn_backward(stream_of(q), &a));

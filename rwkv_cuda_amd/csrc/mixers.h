@@ -22,6 +22,14 @@ struct Range {
     int whole;                                                  // 64 tokens, none of them padding
     int unused;
 };
+// How the work of few queries or keys is spread over the card (a rule on sizes alone, for the kernels and for the size of their workspace).  `query_parts`: the keys of
+// a query in as many parts, joined by a kernel of its own; `key_parts`: the heads that share a key in as many groups, whose sums are added by a kernel of its own.
+struct AttnPlan {
+    int query_parts, key_parts;
+    bool eight;                                                 // heads of 128: 256 keys a workgroup of attn_dkv
+    size_t ranges, forward, backward;                           // bytes: documents of tiles; workspace of either direction
+};
+AttnPlan attn_plan(int B, int Tq, int Tk, int H, int Hk, int N, bool doc);
 // attn_bwd.hip: tile i of `out`'s row b has positions first + 64 i .. of doc's row b, below T
 void launch_attn_ranges(hipStream_t st, const int* doc, int B, int T, int first, Range* out);
 // attn_fwd.hip, attn_bwd.hip (arguments checked)

@@ -65,10 +65,13 @@ def test_attention_entry_points(lib, change, status):
 
 def test_attention_entry_points_of_one_direction(lib):
     assert lib.rwkv_attn_forward(None, None) == -2 and lib.rwkv_attn_forward(None, _attn(y_rest=P + 2)) == -3
-    need = lib.rwkv_attn_workspace_bytes(1, 4, 4, 2, 0, 1)
-    assert need > 0 and lib.rwkv_attn_workspace_bytes(1, 4, 4, 2, 0, 0) == 0 and lib.rwkv_attn_workspace_bytes(1, 5, 4, 2, 1, 1) == 0
-    with_doc = lib.rwkv_attn_workspace_bytes(1, 4, 4, 2, 1, 0)
-    assert with_doc > 0 and lib.rwkv_attn_workspace_bytes(1, 4, 4, 2, 1, 1) > need
+    size = lambda *a: lib.rwkv_attn_workspace_bytes(1, a[0], a[1], 2, 1, 64, a[2], a[3])
+    need = size(4, 4, 0, 1)
+    assert need > 0 and size(4, 4, 0, 0) == 0 and size(5, 4, 1, 1) == 0
+    with_doc = size(4, 4, 1, 0)
+    assert with_doc > 0 and size(4, 4, 1, 1) > need
+    parts = size(4, 70000, 0, 0)                                    # few queries, many keys: in parts
+    assert parts > 0 and lib.rwkv_attn_forward(None, _attn(Tk=70000, workspace_bytes=parts - 1)) == -4
     for change in (dict(workspace=None), dict(workspace=P + 8), dict(workspace_bytes=with_doc - 1)):
         assert lib.rwkv_attn_forward(None, _attn(doc=P, **change)) == -4, change
     for change, status in ((dict(dy=None), -2), (dict(dq=P + 2), -3), (dict(lse=None), -2), (dict(y_rest=None), -2), (dict(workspace=None), -4), (dict(workspace=P + 8), -4),
