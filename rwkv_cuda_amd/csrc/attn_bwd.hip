@@ -46,7 +46,7 @@ template <class E, int D> __global__ __launch_bounds__(256) void attn_delta(cons
 
 // dQ: 4 waves of 32 queries over the keys that any of them sees; S^T = K Q^T and dP^T = V dY^T, dQ^T += K^T dS^T
 template <class E, int D, bool CAP, bool BIAS, bool DOC>
-__global__ __launch_bounds__(256, 2) void attn_dq(const rwkv_attn_args p, const float* delta, const Range* ranges, const int blocks_q, const int per_xcd) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_dq(const rwkv_attn_args p, const float* delta, const Range* ranges, const int blocks_q, const int per_xcd) {
     constexpr int QB = 128;
     constexpr int PLANES = 4 * Plane<D>::BYTES;
     constexpr int SLOPE_VALUS = 4 + (CAP ? 6 : 0) + (BIAS ? 2 : 0), SLOPE_TRANS = CAP ? 3 : 1;      // instructions of a pair
@@ -117,15 +117,24 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const rwkv_attn_args p, const 
         }
     };
     // the gradients of the scores, in s
+    constexpr bool LINE = BIAS && !CAP;                          // the bias as slope (key - query), right where no key stands behind a query; `turn` makes it right elsewhere
+    const bool two_sided = LINE && (p.prefix != nullptr || !p.causal);
     const auto slopes = [&](f32x16& s, const f32x16& dp, const int j) {
-        const float dist = pos - static_cast<float>(j + 4 * hi);
+        const float dist = pos - static_cast<float>(j + 4 * hi), base = fmaf(-sc.slope, dist, -lse);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const float x = s[r], sq = sc.squash<CAP>(x);
-            float ds = __builtin_amdgcn_exp2f(fmaf(sc.t<CAP, BIAS>(x, sq, dist - (8 * (r >> 2) + (r & 3))), mul, -lse)) * (dp[r] - dlt);
+            const float t = LINE ? fmaf(x, sc.unit, fmaf(sc.slope, 8 * (r >> 2) + (r & 3), base)) : fmaf(sc.t<CAP, BIAS>(x, sq, dist - (8 * (r >> 2) + (r & 3))), mul, -lse);
+            float ds = __builtin_amdgcn_exp2f(t) * (dp[r] - dlt);
             if constexpr (CAP) ds *= 4.f * sq * (1.f - sq);
             s[r] = ds;
         }
+    };
+    const auto turn = [&](f32x16& s, const int j) {
+        asm volatile("");                                        // (a branch: few tiles come here)
+        const float over = static_cast<float>(j + 4 * hi) - pos, twice = 2.f * sc.slope / sc.unit;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(fmaxf(over + (8 * (r >> 2) + (r & 3)), 0.f), -twice, s[r]);
     };
     const auto mask = [&](f32x16& s, const int j0, const int e, const int slot) {
         asm volatile("");                                        // (a branch: few tiles come here)
@@ -148,29 +157,32 @@ __global__ __launch_bounds__(256, 2) void attn_dq(const rwkv_attn_args p, const 
 #pragma unroll
             for (int d = 0; d < D / 32; ++d) g[d] = mma<E>(cols(0, 2 * e + c, d), w[c], g[d]);
     };
-    Walk<DOC> walk(ranges, dlo, dhi, 0, tiles);
-    if (walk.t < tiles) bring(walk.t, 0);
+    Walk<DOC, false> walk(ranges, dlo, dhi, 0, tiles);
+    if (walk.more()) bring(walk.t, 0);
     int par = 0, step = BUF;
-    while (walk.t < tiles) {
+    while (walk.more()) {
         const int j0 = walk.t * TILE;
         const bool part = !walk.whole;
         if (DOC && tid < TILE) key_doc[par * TILE + tid] = next_doc;
         arrived();
         __syncthreads();
         walk.next();
-        if (walk.t < tiles) bring(walk.t, par ^ 1);
+        if (walk.more()) bring(walk.t, par ^ 1);
         if (DOC && part) clear_padding<D>(lds + par * BUF, key_doc + par * TILE);
         if (j0 <= lim_hi) {
             const bool masked = part || j0 + TILE - 1 > lim_lo;
             f32x16 s0, s1, p0, p1;
             u32x4 w[2];
+            const bool ahead = two_sided && j0 + TILE - 1 > shift + row_lo;
             products(s0, p0, 0);
+            if (ahead) turn(s0, j0);
             __builtin_amdgcn_sched_barrier(0);
             products(s1, p1, 1);
             slopes(s0, p0, j0);
             beside<2 * D / 16, D / 8, SLOPE_VALUS * 16, SLOPE_TRANS * 16>();
             __builtin_amdgcn_sched_barrier(0);
             if (masked) mask(s0, j0, 0, par);
+            if (ahead) turn(s1, j0 + 32);
             w[0] = as_operand<E>(s0, 0), w[1] = as_operand<E>(s0, 1);
             __builtin_amdgcn_sched_barrier(0);
             add(w, 0);
@@ -266,10 +278,12 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void at
             if constexpr (DOC) next_doc = on ? doc[shift + i0 + tid] : -1;
         }
     };
-    const auto note = [&](const int t, const int slot) {
+    constexpr bool LINE = BIAS && !CAP;                          // as in attn_dq
+    const bool two_sided = LINE && (p.prefix != nullptr || !p.causal);
+    const auto note = [&](const int t, const int slot, const float slope) {
         if (tid < TILE) {
             const bool off = t * TILE + tid >= p.Tq || next_lse == -INFINITY;            // a row that is not there or sees nothing: weights of 0
-            row_lse[slot * TILE + tid] = off ? INFINITY : next_lse - SHIFT<E>;
+            row_lse[slot * TILE + tid] = off ? INFINITY : (LINE ? fmaf(slope, tid, next_lse) : next_lse) - SHIFT<E>;      // with the query's part of the bias
             row_delta[slot * TILE + tid] = off ? 0.f : next_delta * UNSHIFT<E>;
             if (DOC) row_doc[slot * TILE + tid] = next_doc;
         }
@@ -286,6 +300,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void at
     // weights in s, gradients of the scores in dp
     const auto slopes = [&](const Scorer& sc, f32x16& s, f32x16& dp, const int i0, const int e, const int slot) {
         const float dist = static_cast<float>(shift + i0 + 4 * hi + 32 * e) - static_cast<float>(j), mul = CAP || BIAS ? 1.f : sc.unit;
+        const float base = sc.slope * (static_cast<float>(j) - static_cast<float>(shift + i0));
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
             const int o = slot * TILE + 32 * e + 8 * n + 4 * hi;
@@ -295,13 +310,20 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void at
             for (int r = 0; r < 4; ++r) {
                 const int at = 4 * n + r;
                 const float x = s[at], sq = sc.squash<CAP>(x);
-                const float w = __builtin_amdgcn_exp2f(fmaf(sc.t<CAP, BIAS>(x, sq, dist + (8 * n + r)), mul, -lse[r]));
+                const float t = LINE ? fmaf(x, sc.unit, base - lse[r]) : fmaf(sc.t<CAP, BIAS>(x, sq, dist + (8 * n + r)), mul, -lse[r]);
+                const float w = __builtin_amdgcn_exp2f(t);
                 float ds = w * (SHIFT<E> == 0.f ? dp[at] - dlt[r] : fmaf(dp[at], UNSHIFT<E>, -dlt[r]));
                 if constexpr (CAP) ds *= 4.f * sq * (1.f - sq);
                 s[at] = w;
                 dp[at] = ds;
             }
         }
+    };
+    const auto turn = [&](const Scorer& sc, f32x16& s, const int i) {
+        asm volatile("");                                        // (a branch: few tiles come here)
+        const float over = static_cast<float>(j) - static_cast<float>(shift + i + 4 * hi), twice = 2.f * sc.slope / sc.unit;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(fmaxf(over - (8 * (r >> 2) + (r & 3)), 0.f), -twice, s[r]);
     };
     const auto mask = [&](f32x16& s, f32x16& dp, const int i0, const int e, const int slot) {
         asm volatile("");                                        // (a branch: few tiles come here)
@@ -329,19 +351,19 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void at
             }
     };
     int h = first_head, par = 0, step = BUF;
-    Walk<DOC> walk(ranges, dlo, dhi, first, tiles);
-    const Walk<DOC> start = walk;
-    if (walk.t < tiles) bring(h, walk.t, 0);
-    while (walk.t < tiles) {
+    Walk<DOC, false> walk(ranges, dlo, dhi, first, tiles);
+    const Walk<DOC, false> start = walk;
+    if (walk.more()) bring(h, walk.t, 0);
+    while (walk.more()) {
         const int i0 = walk.t * TILE;
         const bool part = !walk.whole;
         const Scorer sc(p, h);
-        note(walk.t, par);
+        note(walk.t, par, sc.slope);
         arrived();
         __syncthreads();
         walk.next();
-        if (walk.t >= tiles && h + 1 < first_head + G) walk = start, ++h;
-        if (walk.t < tiles) bring(h, walk.t, par ^ 1);
+        if (!walk.more() && h + 1 < first_head + G) walk = start, ++h;
+        if (walk.more()) bring(h, walk.t, par ^ 1);
         if (DOC && part) {
             clear_padding<D, WAVES>(lds + par * BUF, row_doc + par * TILE);
             clear_padding<D, WAVES>(lds + par * BUF + Plane<D>::BYTES, row_doc + par * TILE);
@@ -349,15 +371,18 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void at
         if (shift + i0 + TILE - 1 >= from_lo) {
             const bool masked = part || shift + i0 < from_hi;
             u32x4 w[2], ds[2];
+            const bool ahead = two_sided && shift + i0 < k0 + KB - 1;
             if constexpr (D == 64) {
                 f32x16 s0, s1, p0, p1;
                 products(s0, p0, 0);
+                if (ahead) turn(sc, s0, i0);
                 __builtin_amdgcn_sched_barrier(0);
                 products(s1, p1, 1);
                 slopes(sc, s0, p0, i0, 0, par);
                 beside<2 * D / 16, D / 8 + 8, VALUS * 16, TRANS * 16>();
                 __builtin_amdgcn_sched_barrier(0);
                 if (masked) mask(s0, p0, i0, 0, par);
+                if (ahead) turn(sc, s1, i0 + 32);
                 w[0] = as_operand<E>(s0, 0), w[1] = as_operand<E>(s0, 1), ds[0] = as_operand<E>(p0, 0), ds[1] = as_operand<E>(p0, 1);
                 __builtin_amdgcn_sched_barrier(0);
                 add(w, ds, 0);
@@ -372,6 +397,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void at
                 for (int e = 0; e < 2; ++e) {
                     f32x16 s, dp;
                     products(s, dp, e);
+                    if (ahead) turn(sc, s, i0 + 32 * e);
                     __builtin_amdgcn_sched_barrier(0);
                     slopes(sc, s, dp, i0, e, par);
                     if (masked) mask(s, dp, i0, e, par);

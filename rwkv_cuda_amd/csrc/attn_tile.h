@@ -212,43 +212,46 @@ struct Scorer {
 };
 
 __host__ __device__ __forceinline__ int64_t tiles_of(const int T) { return (wide(T) + TILE - 1) / TILE; }
-// The tiles below `end` that hold tokens of documents lo .. hi, in order, and whether each is whole and all of the one document lo (= hi).  Without documents: all.
-template <bool DOC> struct Walk {
+// The tiles first .. end - 1 that hold tokens of documents lo .. hi, from the first on or, BACK, from the last, and whether each is whole and all of the one document
+// lo (= hi).  Without documents: all.
+template <bool DOC, bool BACK> struct Walk {
     const Range* ranges;
-    int lo, hi, end, base;
-    uint64_t some, full;                                        // of tiles base .. base + 63
-    int t;                                                      // the next tile, `end` behind the last
+    int lo, hi, first, count, base;                             // steps 0 .. count - 1; those from base on are in the masks
+    uint64_t some, full;
+    int u, t;                                                   // the step, and its tile
     bool whole;
-    DEVINL Walk(const Range* ranges, const int lo, const int hi, const int first, const int end) : ranges(ranges), lo(lo), hi(hi), end(end), base(first), some(0), full(0), t(first), whole(true) {
-        if constexpr (DOC) {
-            look();
-            settle();
-        } else t = min(first, end);
+    DEVINL Walk(const Range* ranges, const int lo, const int hi, const int first, const int end)
+        : ranges(ranges), lo(lo), hi(hi), first(first), count(max(0, end - first)), base(0), some(0), full(0), u(0), t(0), whole(true) {
+        if (DOC && count > 0) look();
+        settle();
     }
+    DEVINL bool more() const { return u < count; }
+    DEVINL int tile(const int step) const { return BACK ? first + count - 1 - step : first + step; }
     DEVINL void look() {
         const int i = base + static_cast<int>(threadIdx.x & 63);
         Range r = {INT_MAX, -1, 0, 0};
-        if (i < end) r = ranges[i];
+        if (i < count) r = ranges[tile(i)];
         some = __ballot(r.lo <= hi && r.hi >= lo);
         full = __ballot(r.whole && r.lo == lo && r.hi == lo && lo == hi);
     }
-    DEVINL void settle() {                                      // to the first tile from t on
-        for (;;) {
-            if (t >= end) { t = end; return; }
-            if (t - base >= 64) { base = t; look(); }
-            const uint64_t left = some >> (t - base);
-            if (left) {
-                t += __builtin_ctzll(left);
-                whole = full >> (t - base) & 1;
-                return;
+    DEVINL void settle() {                                      // to the first step from u on whose tile is looked at
+        if constexpr (DOC)
+            while (u < count) {
+                if (u - base >= 64) { base = u; look(); }
+                const uint64_t left = some >> (u - base);
+                if (left) {
+                    u += __builtin_ctzll(left);
+                    whole = full >> (u - base) & 1;
+                    break;
+                }
+                u = base + 64;
             }
-            t = base + 64;
-        }
+        t = tile(u);
     }
     DEVINL void next() {
-        ++t;
-        if constexpr (DOC) settle();
-        else asm volatile("" : "+s"(t));                        // (no sums of the tile's number kept from one to the next: they cost registers)
+        ++u;
+        if constexpr (!DOC) asm volatile("" : "+s"(u));         // (no sums of the tile's number kept from one to the next: they cost registers)
+        settle();
     }
 };
 
