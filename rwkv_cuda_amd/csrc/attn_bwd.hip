@@ -464,7 +464,8 @@ template <class E, int D> int run(hipStream_t st, const rwkv_attn_args& p) {
     float* part = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + plan.backward) - (plan.key_parts > 1 ? 2 * plan.key_parts * wide(p.B) * p.Tk * p.Hk * p.N : 0);
     if (p.doc) {
         launch_attn_ranges(st, p.doc, p.B, p.Tk, 0, key_ranges);
-        launch_attn_ranges(st, p.doc, p.B, p.Tk, p.Tk - p.Tq, ranges);
+        if (p.Tq == p.Tk) ranges = key_ranges;
+        else launch_attn_ranges(st, p.doc, p.B, p.Tk, p.Tk - p.Tq, ranges);
     }
     hipLaunchKernelGGL((attn_delta<E, D>), dim3(static_cast<unsigned>(row_blocks)), dim3(256), 0, st, p, delta);
     const auto go = [&](auto dq, auto dkv) {

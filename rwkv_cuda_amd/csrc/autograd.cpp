@@ -511,6 +511,22 @@ void check_side(const Tensor& x, const char* n, c10::ScalarType dt, at::IntArray
 }
 // the strides of a dimension of size 1 are arbitrary: 0 for the kernels' checks
 int64_t stride_of(const Tensor& x, int64_t d) { return x.size(d) == 1 ? 0 : x.stride(d); }
+// a gradient that may be a view from anywhere, for kernels that read 16 bytes at once
+Tensor on_16(const Tensor& x) { return reinterpret_cast<uintptr_t>(x.data_ptr()) & 15 ? x.clone() : x; }
+// whether two tensors have memory in common (or may have: the spans that they lie in)
+bool touch(const Tensor& a, const Tensor& b) {
+    if (!a.storage().is_alias_of(b.storage())) return false;
+    const auto span = [](const Tensor& x) {
+        int64_t last = 0;
+        for (int64_t d = 0; d < x.dim(); ++d) last += (x.size(d) - 1) * x.stride(d);
+        const char* p = static_cast<const char*>(x.data_ptr());
+        return std::make_pair(p, p + (last + 1) * static_cast<int64_t>(x.element_size()));
+    };
+    const auto s = span(a), t = span(b);
+    return s.first < t.second && t.first < s.second;
+}
+// a tensor that a kernel writes: a graph that has saved it finds out
+void written(const Tensor& x) { x.unsafeGetTensorImpl()->bump_version(); }
 void once_only(const char* n) {
     if (c10::GradMode::is_enabled()) fail(std::string(n) + " has no second derivatives: its backward cannot run with create_graph");
 }
@@ -581,6 +597,7 @@ Tensor grec_step_op(const Tensor& w, const Tensor& x, const Tensor& h, const Ten
     check_rows({{&w, "w"}, {&x, "x"}}, w);
     check_side(h, "h", F32, w.sizes(), w);
     check_side(out, "out", F32, w.sizes(), w);
+    require(!touch(out, w) && !touch(out, x) && (out.data_ptr() == h.data_ptr() || !touch(out, h)), "out must be h, or share no memory with w, x and h");
     const Guard guard(w.device());
     rwkv_grec_args a = grec_args(w3, x3, gate, tied);
     Tensor y = at::empty(w.sizes(), w.options());
@@ -589,6 +606,7 @@ Tensor grec_step_op(const Tensor& w, const Tensor& x, const Tensor& h, const Ten
     const Tensor ws = a.workspace_bytes > 0 ? bytes(w, a.workspace_bytes) : Tensor();
     a.workspace = P(ws);
     ok(rwkv_grec_forward(stream_of(w), &a));
+    written(out);
     return y;
 }
 
@@ -635,7 +653,7 @@ struct Attn : Function<Attn> {
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         once_only("attention");
         const auto s = ctx->get_saved_variables();
-        const Tensor &q = s[0], &k = s[1], &v = s[2], &y = s[6], &rest = s[7], &lse = s[8], dy = g[0].contiguous();
+        const Tensor &q = s[0], &k = s[1], &v = s[2], &y = s[6], &rest = s[7], &lse = s[8], dy = on_16(g[0].contiguous());
         const Guard guard(q.device());
         rwkv_attn_args a = attn_args(q, k, v, ctx->saved_data["cap"].toDouble(), ctx->saved_data["scale"].toDouble(), get(ctx, "causal") != 0);
         Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
@@ -657,7 +675,7 @@ Tensor attention_op(const Tensor& q, const Tensor& k, const Tensor& v, const May
     require(k.size(2) > 0 && q.size(2) % k.size(2) == 0, "H must be a multiple of Hk");
     require(N >= 8 && N <= MAX_HEAD && N % 8 == 0, "the head size must be a multiple of 8 up to 128");
     require(causal || !prefix.has_value(), "prefix goes with causal");
-    require(cap >= 0.0 && std::isfinite(cap), "cap must be 0 or positive");
+    require(cap == 0.0 || (cap >= 0x1p-20 && cap <= 4096.0), "cap must be 0, or from 2^-20 to 4096");
     const float sc = scale_of(scale, N);
     require(sc > 0.f && std::isfinite(sc), "scale must be positive");
     require(!slopes.has_value() || !wants_grad({&*slopes}), "slopes have no gradient");
@@ -682,7 +700,7 @@ Tensor paged_op(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tenso
     require(k.defined() == v.defined(), "k and v go together");
     check_side(k, "k", q.scalar_type(), {B, Hk, N}, q);
     check_side(v, "v", q.scalar_type(), {B, Hk, N}, q);
-    require(cap >= 0.0 && std::isfinite(cap), "cap must be 0 or positive");
+    require(cap == 0.0 || (cap >= 0x1p-20 && cap <= 4096.0), "cap must be 0, or from 2^-20 to 4096");
     const Guard guard(q.device());
     rwkv_paged_args a{};
     a.dtype = dtype_of(q, "q", false);
@@ -697,6 +715,7 @@ Tensor paged_op(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tenso
     const Tensor ws = a.workspace_bytes > 0 ? bytes(q, a.workspace_bytes) : Tensor();
     a.workspace = P(ws);
     ok(rwkv_paged_attn(stream_of(q), &a));
+    if (k.defined()) written(kp), written(vp);
     return y;
 }
 

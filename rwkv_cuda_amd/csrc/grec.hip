@@ -22,12 +22,10 @@ constexpr int S = 8, MAX_GROUPS = 16;
 inline int groups_of(int T) { const int g = (T + S - 1) / S; return g >= MAX_GROUPS ? MAX_GROUPS : (g + 1) / 2 * 2; }
 inline int tiles_of(int T) { return (T + S * groups_of(T) - 1) / (S * groups_of(T)); }
 
-// e^x; infinities are exact and a NaN stays one.  fp32: to about two roundings (x log2(e) in two parts).  16-bit inputs: x log2(e) rounded once, which is off by up to
-// half a rounding for every unit of x, far below what the input's own rounding means (0.233 -> 0.207 ms forward at B8 T4096 C4096, chained, with the addresses below).
-template <class E> DEVINL float exp_of(const float x, const float most) {
-    const float raw = x * 1.4426950408889634f, z = raw > most ? most : raw, e = __builtin_amdgcn_exp2f(z);
-    if constexpr (!std::is_same_v<E, float>) return e;
-    const float low = fmaf(x, 1.9259629911266175e-8f, fmaf(x, 1.4426950408889634f, -raw));
+// e^x to about two roundings (x log2(e) in two parts); infinities are exact and a NaN stays one
+DEVINL float exp_of(const float x, const float most) {
+    const float raw = x * 1.4426950408889634f, low = fmaf(x, 1.9259629911266175e-8f, fmaf(x, 1.4426950408889634f, -raw));
+    const float z = raw > most ? most : raw, e = __builtin_amdgcn_exp2f(z);
     return fmaf(e, fabsf(raw) < 115.f ? low * 0.6931471805599453f : 0.f, e);
 }
 // Two workgroups a CU and more: each goes through its column.  Fewer: the tiles are workgroups of their own.  Forward + backward in us, going through / chained, T 4096:
@@ -36,13 +34,13 @@ template <class E> DEVINL float exp_of(const float x, const float most) {
 inline bool chained(int B, int T, int C) { return tiles_of(T) > 1 && static_cast<int64_t>((C + 63) / 64) * B < 512; }
 
 // gate and its complement, both to fp32's accuracy
-template <class E, int GATE> DEVINL void gate_of(const float w, float& a, float& rest) {
+template <int GATE> DEVINL void gate_of(const float w, float& a, float& rest) {
     if constexpr (GATE == RWKV_GATE_SIGMOID) {
-        const float e = exp_of<E>(-w, 115.f);                       // below w = -80 the gate is 2^-115
+        const float e = exp_of(-w, 115.f);                       // below w = -80 the gate is 2^-115
         a = __builtin_amdgcn_rcpf(1.f + e);
         rest = e * a;
     } else {
-        a = exp_of<E>(w, INFINITY);
+        a = exp_of(w, INFINITY);
         rest = -expm1f(w);
     }
 }
@@ -219,7 +217,7 @@ __global__ __launch_bounds__(512, 4) void grec_fwd(const rwkv_grec_args p, const
                 u[i][e] = 0.f;
                 if (on) {
                     float rest;
-                    gate_of<E, GATE>(e ? Two<E>::hi(wr[i]) : Two<E>::lo(wr[i]), a[i][e], rest);
+                    gate_of<GATE>(e ? Two<E>::hi(wr[i]) : Two<E>::lo(wr[i]), a[i][e], rest);
                     const float z = e ? Two<E>::hi(xr[i]) : Two<E>::lo(xr[i]);
                     u[i][e] = TIED ? rest * z : z;
                     if (DOC && (first >> i & 1)) a[i][e] = __uint_as_float(CUT);
@@ -318,7 +316,7 @@ __global__ __launch_bounds__(512, 4) void grec_bwd(const rwkv_grec_args p, const
                 rest[i][e] = 0.f;
                 h[i][e] = 0.f;
                 if (on) {
-                    gate_of<E, GATE>(e ? Two<E>::hi(wr[i]) : Two<E>::lo(wr[i]), a[i][e], rest[i][e]);
+                    gate_of<GATE>(e ? Two<E>::hi(wr[i]) : Two<E>::lo(wr[i]), a[i][e], rest[i][e]);
                     const float z = e ? Two<E>::hi(xr[i]) : Two<E>::lo(xr[i]);
                     h[i][e] = TIED ? rest[i][e] * z : z;
                 }
@@ -421,7 +419,7 @@ __global__ __launch_bounds__(512, 4) void grec_bwd(const rwkv_grec_args p, const
 
 int check_grec(const rwkv_grec_args* p, bool backward) {
     if (p == nullptr) return RWKV_ERR_NULL;
-    if (p->dtype < 0 || p->dtype > RWKV_DTYPE_FP32 || p->gate < 0 || p->gate > RWKV_GATE_LOG || p->B <= 0 || p->T <= 0 || p->C <= 0 || p->B > 65535) return RWKV_ERR_SHAPE;
+    if (p->dtype < 0 || p->dtype > RWKV_DTYPE_FP32 || p->gate < 0 || p->gate > RWKV_GATE_LOG || p->B <= 0 || p->T <= 0 || p->C <= 0 || p->B > 65535 || p->T > INT_MAX - 65536 || p->C > INT_MAX - 65536) return RWKV_ERR_SHAPE;
     if (p->w == nullptr || p->x == nullptr) return RWKV_ERR_NULL;
     if (backward ? p->dw == nullptr || p->dx == nullptr || p->saved == nullptr : p->y == nullptr || p->hT == nullptr) return RWKV_ERR_NULL;
     const uintptr_t eb = p->dtype == RWKV_DTYPE_FP32 ? 3 : 1;

@@ -246,7 +246,7 @@ template <class E> int run_any(hipStream_t st, const rwkv_paged_args& p) { retur
 int check_paged(const rwkv_paged_args* p) {
     if (p == nullptr) return RWKV_ERR_NULL;
     if ((p->dtype != RWKV_DTYPE_BF16 && p->dtype != RWKV_DTYPE_FP16) || p->B <= 0 || p->H <= 0 || p->Hk <= 0 || p->H % p->Hk != 0 || p->N <= 0 || p->N > 128 || p->N % 8 != 0 ||
-        p->P <= 0 || p->M <= 0 || p->page <= 0 || (p->page & (p->page - 1)) != 0 || static_cast<int64_t>(p->M) * p->page > INT_MAX - 65536 || p->B > 65535 || p->H > 65535 || !(p->scale > 0.f) || !(p->cap >= 0.f)) return RWKV_ERR_SHAPE;
+        p->P <= 0 || p->M <= 0 || p->page <= 0 || (p->page & (p->page - 1)) != 0 || static_cast<int64_t>(p->M) * p->page > INT_MAX - 65536 || p->B > 65535 || p->H > 65535 || !scores_ok(p->scale, p->cap)) return RWKV_ERR_SHAPE;
     for (const int64_t s : {p->k_sp, p->k_st, p->k_sh, p->v_sp, p->v_st, p->v_sh}) if (s % 8 != 0) return RWKV_ERR_ALIGN;
     if (const int rc = check_ptrs({p->q, p->k_pages, p->v_pages, p->y})) return rc;
     if (p->table == nullptr || p->lens == nullptr || (p->k == nullptr) != (p->v == nullptr)) return RWKV_ERR_NULL;

@@ -33,5 +33,5 @@ def RUN_CUDA(w, x, h0=None, doc=None, gate="sigmoid", tied=True):
 
 def STEP(w, x, h, out=None, gate="sigmoid", tied=True):
     """One token a sequence, for serving: w, x [B,C], h [B,C] fp32.  Returns y [B,C]; the new state goes to `out`, or replaces h where
-    that is None.  No gradients."""
+    that is None; `out` is another memory than w, x and (unless it is h itself) h.  No gradients."""
     return ops().gated_recurrence_step(w, x, h, h if out is None else out, _gate(gate), tied)

@@ -2,7 +2,7 @@
 
     python -m rwkv_cuda_amd.run OP [check|benchmark] [--B n --T n --H n]
 
-    OP: wkv  depthwise_conv1d  wkv5  wkv5_bf16  wkv5a  wkv6  wkv6_state  rwkv7  rwkv7_fp32
+    OP: wkv  depthwise_conv1d  wkv5  wkv5_bf16  wkv5a  wkv6  wkv6_state  rwkv7  rwkv7_fp32  gated_recurrence  attention
 
 `check` runs the HIP op forward and backward (through the "strange loss" of the reference's checks,
 wkv6_state/run.py:171-172) beside a plain torch formula of the same op evaluated in fp32 on the same
@@ -94,6 +94,25 @@ def formula_rwkv7(s0, r, w, k, v, a, b):
     return torch.stack(ys, 1), S
 
 
+def formula_recurrence(w, x, h0):
+    """gated_recurrence with the sigmoid gate, tied: h_t = a h_{t-1} + (1 - a) x_t, a = sigmoid(w_t)."""
+    a = torch.sigmoid(w)
+    h, ys = h0, []
+    for t in range(w.shape[1]):
+        h = a[:, t] * h + (1 - a[:, t]) * x[:, t]
+        ys.append(h)
+    return torch.stack(ys, 1), h
+
+
+def formula_attention(q, k, v, slopes, cap):
+    """attention, causal, with capped scores and a distance bias; q [B,T,H,N], k, v [B,T,Hk,N]."""
+    T, G = q.shape[1], q.shape[2] // k.shape[2]
+    q, k, v = q.transpose(1, 2), *(z.repeat_interleave(G, 2).transpose(1, 2) for z in (k, v))
+    at = torch.arange(T, device=q.device)
+    s = cap * torch.tanh(q @ k.transpose(-1, -2) * q.shape[-1] ** -0.5 / cap) - slopes.view(-1, 1, 1) * (at[:, None] - at).abs()
+    return (torch.softmax(s.masked_fill(at > at[:, None], -torch.inf), -1) @ v).transpose(1, 2)
+
+
 # ---------------------------------------------------------------------------------------------
 # one case per op: inputs as the reference's checks draw them, the formula, the HIP op
 # ---------------------------------------------------------------------------------------------
@@ -107,7 +126,7 @@ def case(op, dev, B, T, H, bench=False):
     the op's dtype).  Outputs are tuples; every output enters the loss.  With bench=True the wkv6 decays are the
     per-channel uniform(-8, 1) of the reference's speed runs (wkv6_state/run.py:188,284) instead of the low-rank form,
     whose spread grows with C until every decay is 0 or 1."""
-    from . import depthwise_conv1d, rwkv7_fast_fused, wkv, wkv5, wkv5_bf16, wkv5a, wkv6, wkv6_state
+    from . import attention, depthwise_conv1d, gated_recurrence, rwkv7_fast_fused, wkv, wkv5, wkv5_bf16, wkv5a, wkv6, wkv6_state
     C = H * N
     bf = torch.bfloat16
     U = lambda lo, hi, *s: _uniform(dev, lo, hi, *s)
@@ -167,10 +186,19 @@ def case(op, dev, B, T, H, bench=False):
             y, sT = rwkv7_fast_fused.RWKV7_STATE_PASSING_CLAMPW_CUDA(s0.float(), *(flat(x) for x in (r, w, k, v, a, b)))
             return y.view(B, T, H, N), sT
         return names, t, formula_rwkv7, hip, torch.float32 if f32 else bf
+    if op == "gated_recurrence":
+        names, t = ["w", "x", "h0"], [rb(U(0, 4, B, T, C)), rb(U(-1, 1, B, T, C)), U(-1, 1, B, C)]
+        return names, t, formula_recurrence, lambda w, x, h0: gated_recurrence.RUN_CUDA(w, x, h0.float()), bf
+    if op == "attention":                            # two query heads to a key head where H is even
+        Hk = H // 2 if H % 2 == 0 else H
+        names, t = ["q", "k", "v"], [rb(U(-2, 2, B, T, H, N)), rb(U(-2, 2, B, T, Hk, N)), rb(U(-1, 1, B, T, Hk, N))]
+        slopes = torch.exp2(-8.0 * torch.arange(1, H + 1, device=dev) / H)
+        return names, t, lambda q, k, v: (formula_attention(q, k, v, slopes, 30.0),), \
+            lambda q, k, v: (attention.RUN_CUDA(q, k, v, slopes=slopes, cap=30.0),), bf
     raise SystemExit(f"unknown op {op!r}")
 
 
-OPS = ["wkv", "depthwise_conv1d", "wkv5", "wkv5_bf16", "wkv5a", "wkv6", "wkv6_state", "rwkv7", "rwkv7_fp32"]
+OPS = ["wkv", "depthwise_conv1d", "wkv5", "wkv5_bf16", "wkv5a", "wkv6", "wkv6_state", "rwkv7", "rwkv7_fp32", "gated_recurrence", "attention"]
 # err-ratio bars of `check`: bf16 outputs carry 2^-9 relative rounding; fp32 paths sum in a different order only
 BAR = {torch.bfloat16: 2e-2, torch.float32: 2e-4}
 
@@ -200,10 +228,10 @@ def check(op, dev, B, T, H, out=print):
     return worst, BAR[dtype]
 
 
-# the reference's benchmark shapes: (B, T, H)
+# the reference's benchmark shapes: (B, T, H); its wkv6 shape or the like for what it does not have
 BENCH_SHAPE = {"wkv": (4, 512, 12), "depthwise_conv1d": (32, 768, 12), "wkv5": (8, 4096, 64), "wkv5_bf16": (8, 4096, 32),
                "wkv5a": (8, 4096, 64), "wkv6": (8, 4096, 32), "wkv6_state": (8, 4096, 32), "rwkv7": (8, 1024, 64),
-               "rwkv7_fp32": (8, 1024, 64)}
+               "rwkv7_fp32": (8, 1024, 64), "gated_recurrence": (8, 4096, 64), "attention": (8, 4096, 32)}
 
 
 def benchmark(op, dev, B, T, H, out=print):

@@ -61,6 +61,30 @@ def test_masks_caps_and_biases(lib, how, B, Tq, Tk, H, Hk, N, dtype):
     check(*inputs(B, Tq, Tk, H, Hk, N, DT[dtype], seed=7), **o)
 
 
+@pytest.mark.parametrize("how", ["none", "cap", "bias", "wide bias", "all"])
+@pytest.mark.parametrize("B,Tq,Tk,H,Hk,N", [(4, 300, 300, 32, 32, 128), (2, 300, 411, 64, 16, 128), (4, 260, 260, 32, 32, 64), (2, 129, 129, 12, 2, 64)])
+def test_many_heads(lib, how, B, Tq, Tk, H, Hk, N):
+    """Workgroups enough for the large ones of heads of 128; heads in one group and in several."""
+    q, k, v, dy = inputs(B, Tq, Tk, H, Hk, N, torch.bfloat16, seed=71)
+    how = dict(HOW.get(how, {}))
+    if how.pop("bias", False):
+        how["slopes"] = torch.exp2(-8.0 * torch.arange(1, H + 1) / H).to(DEV)
+    if how.pop("prefix", False):
+        how["prefix"] = torch.tensor([Tk // 3, 5, 0, Tk + 9][:B], dtype=torch.int32, device=DEV)
+    if "doc" in how:
+        how["doc"] = doc_ids(B, Tk, how["doc"], seed=3).to(DEV)
+    check(q, k, v, dy, **how)
+
+
+def test_gradients_that_come_as_views_from_anywhere(lib):
+    q, k, v, dy = inputs(1, 70, 70, 2, 1, 64, torch.bfloat16, seed=75)
+    odd = torch.zeros(dy.numel() + 3, device=DEV, dtype=dy.dtype)[3:].view_as(dy).copy_(dy)
+    t = [z.requires_grad_(True) for z in (q, k, v)]
+    y = A.RUN_CUDA(*t)
+    got, want = (torch.autograd.grad(y, t, d, retain_graph=True) for d in (odd, dy))
+    assert odd.data_ptr() % 16 != 0 and all(torch.equal(g, w) for g, w in zip(got, want))
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 def test_large_scores(lib, dtype):
     """Scores in the hundreds, of either sign: nothing overflows, and rows that are one key's alone."""

@@ -53,6 +53,24 @@ def test_documents_and_padding(lib, kind, B, T, C, dtype, gate, tied):
     check(w, x, h0, doc_ids(B, T, kind, seed=T).to(DEV), gate, tied, dy, dhT)
 
 
+@pytest.mark.parametrize("B,T,C,kind", [(8, 300, 4096, None), (9, 270, 3649, None), (9, 390, 3650, "padded"), (16, 129, 2048, "many"), (9, 261, 3649, "two")])
+@pytest.mark.parametrize("dtype,gate,tied", [("bf16", "sigmoid", True), ("fp16", "log", False), ("fp32", "log", True)])
+def test_enough_columns_to_walk_through(lib, B, T, C, kind, dtype, gate, tied):
+    """512 columns of 64 channels and more."""
+    w, x, h0, dy, dhT = inputs(B, T, C, DT[dtype], gate, seed=90)
+    check(w, x, h0, None if kind is None else doc_ids(B, T, kind, seed=T).to(DEV), gate, tied, dy, dhT)
+
+
+def test_tokens_far_apart(lib):
+    """[T,B,C] in memory, a token 2^24 elements from the next: offsets within a tile beyond 32 bits."""
+    T, B, C = 66, 4096, 4096
+    w, x = (randn(T, 1, C, seed=s).to(torch.bfloat16).to(DEV).expand(T, B, C).contiguous().transpose(0, 1) for s in (1, 2))
+    assert w.stride(1) * w.element_size() * (T - 1) > 1 << 31
+    y, hT = G.RUN_CUDA(w, x)
+    want = G.RUN_CUDA(w[:1].contiguous(), x[:1].contiguous())
+    assert all(torch.equal(y[b], want[0][0]) and torch.equal(hT[b], want[1][0]) for b in (0, 1, 2047, 4095))
+
+
 @pytest.mark.parametrize("gate,tied", [("sigmoid", False), ("log", True)])
 def test_only_one_of_the_outputs_has_a_gradient(lib, gate, tied):
     w, x, h0, dy, dhT = inputs(2, 530, 68, torch.float16, gate, seed=20)

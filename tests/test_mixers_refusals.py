@@ -32,7 +32,7 @@ def _paged(**change):
 
 @pytest.mark.parametrize("change,status", [
     (dict(dtype=3), -1), (dict(dtype=-1), -1), (dict(gate=2), -1), (dict(B=0), -1), (dict(T=0), -1), (dict(C=-4), -1), (dict(B=65536), -1), (dict(w=None), -2), (dict(x=None), -2),
-    (dict(w=P + 1), -3), (dict(dtype=2, x=P + 2), -3), (dict(h0=P + 2), -3), (dict(doc=P + 1), -3)])
+    (dict(T=(1 << 31) - 1), -1), (dict(w=P + 1), -3), (dict(dtype=2, x=P + 2), -3), (dict(h0=P + 2), -3), (dict(doc=P + 1), -3)])
 def test_recurrence_entry_points(lib, change, status):
     assert lib.rwkv_grec_forward(None, _grec(**change)) == status
     need = lib.rwkv_grec_saved_bytes(2, 8, 4)
@@ -56,7 +56,8 @@ def test_recurrence_entry_points_of_one_direction(lib):
 
 @pytest.mark.parametrize("change,status", [
     (dict(dtype=2), -1), (dict(B=0), -1), (dict(Tq=0), -1), (dict(Tk=3), -1), (dict(H=3, Hk=2), -1), (dict(Hk=0), -1), (dict(N=132), -1), (dict(N=12), -1), (dict(N=136), -1),
-    (dict(scale=0.0), -1), (dict(scale=float("nan")), -1), (dict(cap=-1.0), -1), (dict(cap=float("nan")), -1), (dict(prefix=P, causal=0), -1), (dict(B=65536), -1), (dict(q_st=130), -3), (dict(k_sb=4), -3),
+    (dict(scale=0.0), -1), (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(cap=1e-9), -1), (dict(cap=4097.0), -1), (dict(Tk=(1 << 31) - 1), -1),
+    (dict(Tk=(1 << 24) + 1, slopes=P), -1), (dict(q_st=1 << 24), -1), (dict(v_st=-64), -1), (dict(cap=-1.0), -1), (dict(cap=float("nan")), -1), (dict(prefix=P, causal=0), -1), (dict(B=65536), -1), (dict(q_st=130), -3), (dict(k_sb=4), -3),
     (dict(v_sh=1), -3), (dict(q=None), -2), (dict(k=P + 8), -3), (dict(y=None), -2), (dict(doc=P + 2), -3), (dict(slopes=P + 1), -3), (dict(prefix=P + 2), -3), (dict(lse=P + 1), -3)])
 def test_attention_entry_points(lib, change, status):
     assert lib.rwkv_attn_forward(None, _attn(**change)) == status
@@ -81,7 +82,7 @@ def test_attention_entry_points_of_one_direction(lib):
 
 @pytest.mark.parametrize("change,status", [
     (dict(dtype=2), -1), (dict(B=0), -1), (dict(H=3, Hk=2), -1), (dict(N=12), -1), (dict(N=136), -1), (dict(P=0), -1), (dict(M=0), -1), (dict(page=0), -1), (dict(page=24), -1), (dict(page=-16), -1),
-    (dict(scale=-1.0), -1), (dict(cap=float("nan")), -1), (dict(k_sp=1028), -3), (dict(v_st=4), -3), (dict(q=None), -2), (dict(k_pages=None), -2), (dict(v_pages=P + 8), -3), (dict(table=None), -2),
+    (dict(scale=-1.0), -1), (dict(cap=float("nan")), -1), (dict(cap=1e-9), -1), (dict(cap=4097.0), -1), (dict(M=1 << 27), -1), (dict(k_sp=1028), -3), (dict(v_st=4), -3), (dict(q=None), -2), (dict(k_pages=None), -2), (dict(v_pages=P + 8), -3), (dict(table=None), -2),
     (dict(lens=None), -2), (dict(lens=P + 2), -3), (dict(k=P), -2), (dict(k=P, v=P + 8), -3), (dict(y=None), -2), (dict(slopes=P + 2), -3)])
 def test_paged_entry_point(lib, change, status):
     assert lib.rwkv_paged_attn(None, _paged(**change)) == status
@@ -123,6 +124,11 @@ def test_recurrence_refusals_on_the_device(lib):
         R(w[:, :0], x[:, :0])
     with pytest.raises(AssertionError):
         gated_recurrence.STEP(w[:, 0].requires_grad_(True), x[:, 0], h)
+    w, two = w.detach(), torch.zeros(3, 8, device="cuda")             # an `out` that shares memory with the other arguments, but is not h
+    for call in (lambda: gated_recurrence.STEP(w[:, 0], x[:, 0], two[:2], out=two[1:]), lambda: gated_recurrence.STEP(two[:2], x[:, 0], h, out=two[1:]),
+                 lambda: gated_recurrence.STEP(w[:, 0], two[1:], two[1:])):
+        with pytest.raises(AssertionError, match="memory"):
+            call()
     leaf = w.detach().requires_grad_(True)
     with pytest.raises(_lib.RwkvHipError, match="second derivatives"):
         torch.autograd.grad(R(leaf, x)[0].sum(), leaf, create_graph=True)
@@ -137,7 +143,7 @@ def test_attention_refusals_on_the_device(lib):
     slopes = torch.zeros(4, device="cuda")
     for call in (lambda: R(q.float(), k.float(), k.float()), lambda: R(q, k.half(), k), lambda: R(q, k[:, :3], k[:, :3]), lambda: R(q[:, :, :3], k, k), lambda: R(q, k[..., :32], k[..., :32]),
                  lambda: R(q[..., :60], k[..., :60], k[..., :60]), lambda: R(q, k, k, doc=i32(2, 4)), lambda: R(q, k, k, doc=i32(2, 6).long()), lambda: R(q, k, k, prefix=i32(3)),
-                 lambda: R(q, k, k, prefix=i32(2), causal=False), lambda: R(q, k, k, slopes=slopes[:2]), lambda: R(q, k, k, cap=-1.0), lambda: R(q, k, k, scale=0.0), lambda: R(q, k, k, cap=float("inf")),
+                 lambda: R(q, k, k, prefix=i32(2), causal=False), lambda: R(q, k, k, slopes=slopes[:2]), lambda: R(q, k, k, cap=-1.0), lambda: R(q, k, k, scale=0.0), lambda: R(q, k, k, cap=float("inf")), lambda: R(q, k, k, cap=1e-9), lambda: R(q, k, k, cap=5000.0),
                  lambda: R(q, k, k, slopes=slopes.clone().requires_grad_(True)), lambda: R(q.transpose(2, 3), k, k)):
         with pytest.raises(AssertionError):
             call()
