@@ -49,6 +49,13 @@ def test_against_the_definition(lib, lens, H, Hk, N, dtype, page):
     check(*cache(lens, H, Hk, N, page, DT[dtype]))
 
 
+@pytest.mark.parametrize("H,Hk,N,B", [(32, 32, 64, 17), (40, 8, 40, 64), (136, 8, 64, 35)])
+def test_many_heads(lib, H, Hk, N, B):
+    """Workgroups enough to be dealt out by eights of neighbouring heads, their number no multiple of the XCDs'; also with heads in chunks."""
+    lens = torch.randint(0, 300, (B,), generator=torch.Generator().manual_seed(H)).tolist()
+    check(*cache(lens, H, Hk, N, 16, torch.bfloat16, seed=61))
+
+
 @pytest.mark.parametrize("how", ["cap", "bias", "both", "scale"])
 def test_caps_and_biases(lib, how):
     H = 8
