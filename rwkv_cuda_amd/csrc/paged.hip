@@ -31,10 +31,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn(const rwkv_paged_arg
     constexpr int ROWS = 64 / (D / 8), VSTEPS = STEP / ROWS;        // rows of an access of a wave, accesses of 32 rows
     __shared__ __align__(16) char smem[WAVES * STEP * 2 * D];
     __shared__ float top_of[WAVES][HEADS], sum_of[WAVES][HEADS];
-    // `group` neighbouring heads (with their chunks) are a share; an XCD has whole shares
+    // `group` neighbouring heads (with their chunks) are a share, and an XCD has whole shares; 0: the pieces of a head one after the other
     const int slot = group > 1 ? blockIdx.x >> 3 : blockIdx.x, share = group > 1 ? slot / group * 8 + (blockIdx.x & 7) : slot;
     if (share >= shares) return;
-    const int of_piece = p.Hk * chunks / group, y = share % of_piece * group + slot % group, piece = share / of_piece % pieces;
+    const int heads = p.Hk * chunks, of_piece = heads / max(group, 1);
+    const int y = group == 0 ? share / pieces % heads : share % of_piece * group + slot % group, piece = group == 0 ? share % pieces : share / of_piece % pieces;
     const int b = share / of_piece / pieces, hk = y / chunks, chunk = y % chunks, G = p.H / p.Hk;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
     const int all = p.lens[b], n = tokens_of(p, b, shift), size = piece_of(n, pieces);
@@ -239,15 +240,20 @@ inline int pieces_of(int B, int H, int Hk, int page, int M) {
 // Rows of 128 bytes: eight neighbouring heads on one XCD, which then reads a kilobyte of a token.  B64, up to 4096 tokens, H32 Hk32 N64: 0.247 ms one by one, 0.226 in eights,
 // 0.233 in sixteens; B1 65536 tokens 0.123, 0.113, 0.113; B64 up to 4096 H32 Hk8 N64 0.063, 0.061, 0.060.  Rows of 256 bytes (B4 H64 Hk8 N128 0.299, 0.294; B16 up to 4096 H32 Hk8
 // N128 0.036, 0.041) gain nothing.
-inline int group_of(int N, int heads, int64_t blocks) { return N <= 64 && heads % 8 == 0 && blocks >= 64 * 8 ? 8 : 1; }
+// Otherwise the heads of a piece come one after the other, or where pieces are many the pieces of a head: B4 H64 Hk8 N128, 64 pieces, 0.299 ms and 0.285; B8, 32 pieces,
+// 0.150 and 0.143; B16, 16 pieces, 0.036 and 0.041.
+inline int group_of(int N, int heads, int pieces, int64_t blocks) {
+    if (N <= 64 && heads % 8 == 0 && blocks >= 64 * 8) return 8;
+    return pieces >= 32 ? 0 : 1;
+}
 inline int width_of(int N) { return N <= 64 ? 64 : 128; }
 
 template <class E, int D> int run(hipStream_t st, const rwkv_paged_args& p) {
     const int shift = __builtin_ctz(p.page), pieces = pieces_of(p.B, p.H, p.Hk, p.page, p.M), chunks = chunks_of(p.H, p.Hk);
     float* part = static_cast<float*>(p.workspace);
     const int64_t blocks = static_cast<int64_t>(pieces) * p.Hk * chunks * p.B;
-    const int group = group_of(p.N, p.Hk * chunks, blocks);
-    const int64_t shares = blocks / group, grid = group > 1 ? (shares + 7) / 8 * 8 * group : blocks;
+    const int group = group_of(p.N, p.Hk * chunks, pieces, blocks);
+    const int64_t shares = blocks / std::max(group, 1), grid = group > 1 ? (shares + 7) / 8 * 8 * group : blocks;
     if (grid > INT_MAX) return RWKV_ERR_SHAPE;
     hipLaunchKernelGGL((paged_attn<E, D>), dim3(static_cast<unsigned>(grid)), dim3(64 * WAVES), 0, st, p, shift, pieces, chunks, group, static_cast<int>(shares), part);
     if (pieces > 1) hipLaunchKernelGGL((paged_join<E, D>), dim3(p.H, p.B), dim3(256), 0, st, p, shift, pieces, part);
