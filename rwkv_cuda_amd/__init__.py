@@ -11,6 +11,12 @@ reference's own torch.autograd.Function interface.
     wkv6_state        WKV_6STATE.apply(B,T,C,H,r,k,v,w,u,s)          bf16
     rwkv7_fast_fused  RWKV7_STATE_PASSING_CLAMPW_CUDA(s0,r,w,k,v,a,b) -> (y, sT)
 
+and, without a counterpart there, what hybrid models put beside them:
+
+    gated_recurrence  RUN_CUDA(w,x,h0,doc) -> (y, hT), STEP(w,x,h)   bf16, fp16, fp32; elementwise linear recurrence
+    attention         RUN_CUDA(q,k,v,doc,prefix,slopes,cap)          bf16, fp16; shared key heads, documents, prefixes
+    paged_attention   RUN_CUDA(q,k_pages,v_pages,table,lens,k,v)     bf16, fp16; one token a sequence, for serving
+
 There is no CPU or eager fallback: the ops need the compiled library and a HIP device.
 """
 

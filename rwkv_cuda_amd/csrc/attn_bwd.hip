@@ -1,5 +1,9 @@
 // Attention backward on the matrix cores, without atomics: the weights are made again from the forward's lse, once by the workgroups that own
 // queries (dQ: three products a pair) and once by those that own keys (dK, dV: four), each sum in one wave's registers in a fixed order.
+//
+// Seven products where one kernel for all three would do with five: that one would have to add dQ from many workgroups, in an order that changes (atomics)
+// or through memory.  Bound by issue, as the forward.  bf16, causal: B2 T8192 H32 Hk8 N128 with a cap and prefixes dK dV 2.5 ms, dQ 1.95 ms; B8 T4096 H32 N64 with
+// slopes 1.55 ms (690 TFLOP/s) and 0.95 ms (860).
 #include "attn_tile.h"
 
 namespace rwkv {
@@ -9,6 +13,7 @@ namespace {
 template <class E> constexpr float SHIFT = std::is_same_v<E, bf16_t> ? 0.f : 8.f;
 template <class E> constexpr float UNSHIFT = std::is_same_v<E, bf16_t> ? 1.f : 1.f / 256.f;
 
+// lo .. hi of the documents of each tile's real tokens, and whether all of them are real (4 us at T3001: a launch)
 __global__ __launch_bounds__(256) void attn_ranges(const int* doc, const int T, const int first, const int tiles, Range* out) {
     const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, b = blockIdx.y;
     if (t >= tiles) return;
@@ -21,7 +26,7 @@ __global__ __launch_bounds__(256) void attn_ranges(const int* doc, const int T, 
     if (lane == 0) out[wide(b) * tiles + t] = {lo, hi, whole, 0};
 }
 
-// delta = sum over the channels of dy y, y as the forward had it before it was rounded; a row has D / 8 lanes
+// delta = sum over the channels of dy y, y as the forward had it before it was rounded; a row has D / 8 lanes.  Bound by memory: B8 T4096 H32 N64 0.073 ms, 405 MB, 5.5 TB/s.
 template <class E, int D> __global__ __launch_bounds__(256) void attn_delta(const rwkv_attn_args p, float* delta) {
     constexpr int LANES = D / 8;
     const int64_t row = (blockIdx.x * wide(256) + threadIdx.x) / LANES, rows = wide(p.B) * p.Tq * p.H;
@@ -45,6 +50,7 @@ template <class E, int D> __global__ __launch_bounds__(256) void attn_delta(cons
 }
 
 // dQ: 4 waves of 32 queries over the keys that any of them sees; S^T = K Q^T and dP^T = V dY^T, dQ^T += K^T dS^T
+// Three waves a SIMD with heads of 64, for 1 to 8 spilled registers where there is a bias (B8 T4096 H32 N64 with slopes, with the forward, 3.135 -> 3.086 ms).
 template <class E, int D, bool CAP, bool BIAS, bool DOC>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_dq(const rwkv_attn_args p, const float* delta, const Range* ranges, const int blocks_q, const int per_xcd) {
     constexpr int QB = 128;
@@ -206,7 +212,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_dq(const rwkv_attn_
 // dV^T += dY^T P, dK^T += Q^T dS
 //
 // With heads of 128 the two sums take half of a wave's 256 registers and the keys a quarter of the rest: the values are read from LDS.  There a workgroup has 8 waves
-// (256 keys; two waves a SIMD), or 4 where there are few workgroups.
+// (256 keys; two waves a SIMD), or 4 where there are few workgroups (B2 T8192 H32 N128: with the values in registers and 4 waves 4.4 ms, so 2.5).
 template <class E, int D, int WAVES, bool CAP, bool BIAS, bool DOC>
 __global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void attn_dkv(const rwkv_attn_args p, const float* delta, const Range* key_ranges, const Range* ranges, const int blocks_k, const int per_xcd, const int parts, float* part) {
     constexpr int KB = 32 * WAVES, PLANES = 4 * Plane<D>::BYTES, VALUES = D == 128 ? KB / TILE * Plane<D>::BYTES : 0;

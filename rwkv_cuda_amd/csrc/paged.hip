@@ -3,7 +3,9 @@
 // Bound by reading the cache: each of its rows is read once for all (up to 16) query heads that share it.  A workgroup takes a piece of a sequence's
 // tokens for one key head; its waves take 32 tokens in turn.  On v_mfma_f32_16x16x32 a lane holds one head's scores of eight tokens, S^T = K Q^T with
 // the keys as they come from memory, and the weights, packed, are the second operand of O^T += V^T P^T, whose first comes through LDS
-// (ds_read_b64_tr_b16).  Waves are joined in LDS, pieces by a second kernel.
+// (ds_read_b64_tr_b16).  Waves are joined in LDS, pieces by a second kernel.  The next 32 tokens' rows are on their way while these are worked on; the vector unit is busy
+// a third of the time.  bf16 B64 up to 4096 tokens (2111 on average) H32 Hk32 N64: 0.226 ms, 4.9 TB/s; fp16 B4 up to 131072 (91750) H64 Hk8 N128: 0.285 ms, 5.3 TB/s
+// (a read-only stream reaches 7.3).  Three or four workgroups a CU and tables in order or shuffled are the same to 5 percent; lengths that are equal take 0.204 of 0.226.
 #include <algorithm>
 #include <climits>
 
