@@ -26,6 +26,35 @@ __global__ __launch_bounds__(256) void attn_ranges(const int* doc, const int T, 
     if (lane == 0) out[wide(b) * tiles + t] = {lo, hi, whole, 0};
 }
 
+// The blocks of 128 queries (workgroup 0) and of `kb` keys (workgroup 1) in the order of their work: tiles that hold tokens of the block's documents, as the kernels
+// walk over them.  The order changes no result.  One workgroup counts, a wave a block, and ranks; at T3001 with five documents 4 us.
+__global__ __launch_bounds__(1024) void attn_order(const rwkv_attn_args p, const Range* keys, const Range* queries, const int q_items, int* q_order, const int k_items, int* k_order, const int kb) {
+    __shared__ int work[MAX_ORDER];
+    const bool for_keys = q_items == 0 || blockIdx.x == 1;
+    const int items = for_keys ? k_items : q_items, block = for_keys ? kb : 128, tk = static_cast<int>(tiles_of(p.Tk)), tq = static_cast<int>(tiles_of(p.Tq)), shift = p.Tk - p.Tq;
+    const int blocks = items / p.B, lane = threadIdx.x & 63;
+    for (int i = threadIdx.x >> 6; i < items; i += 16) {
+        const int b = i / blocks, at = i % blocks * block, end = min(at + block, for_keys ? p.Tk : p.Tq);
+        const int reach = p.prefix ? min(p.prefix[b], p.Tk) : 0;
+        const Range* own = keys + wide(b) * tk;
+        const Range* other = for_keys ? queries + wide(b) * tq : own;
+        int lo = INT_MAX, hi = -1;
+        for (int t = ((for_keys ? 0 : shift) + at) / TILE; t <= ((for_keys ? 0 : shift) + end - 1) / TILE; ++t) lo = min(lo, own[t].lo), hi = max(hi, own[t].hi);
+        const int first = for_keys && p.causal && at >= reach ? max(0, at - shift) / TILE : 0;
+        const int last = for_keys ? tq : (p.causal ? max(shift + end - 1, reach - 1) : p.Tk - 1) / TILE + 1;
+        int n = 0;
+        for (int t = first + lane; t < last; t += 64) n += other[t].lo <= hi && other[t].hi >= lo;
+        n = static_cast<int>(group_sum<64>(static_cast<float>(n)));
+        if (lane == 0) work[i] = n;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < items; i += 1024) {
+        int rank = 0;
+        for (int j = 0; j < items; ++j) rank += work[j] > work[i] || (work[j] == work[i] && j < i);
+        (for_keys ? k_order : q_order)[rank] = i;
+    }
+}
+
 // delta = sum over the channels of dy y, y as the forward had it before it was rounded; a row has D / 8 lanes.  Bound by memory: B8 T4096 H32 N64 0.073 ms, 405 MB, 5.5 TB/s.
 template <class E, int D> __global__ __launch_bounds__(256) void attn_delta(const rwkv_attn_args p, float* delta) {
     constexpr int LANES = D / 8;
@@ -52,15 +81,20 @@ template <class E, int D> __global__ __launch_bounds__(256) void attn_delta(cons
 // dQ: 4 waves of 32 queries over the keys that any of them sees; S^T = K Q^T and dP^T = V dY^T, dQ^T += K^T dS^T
 // Three waves a SIMD with heads of 64, for 1 to 8 spilled registers where there is a bias (B8 T4096 H32 N64 with slopes, with the forward, 3.135 -> 3.086 ms).
 template <class E, int D, bool CAP, bool BIAS, bool DOC>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_dq(const rwkv_attn_args p, const float* delta, const Range* ranges, const int blocks_q, const int per_xcd) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_dq(const rwkv_attn_args p, const float* delta, const Range* ranges, const int* order, const int blocks_q, const int per_xcd) {
     constexpr int QB = 128;
     constexpr int PLANES = 4 * Plane<D>::BYTES;
     constexpr int SLOPE_VALUS = 4 + (CAP ? 6 : 0) + (BIAS ? 2 : 0), SLOPE_TRANS = CAP ? 3 : 1;      // instructions of a pair
     __shared__ __align__(16) char smem[PLANES + (DOC ? 8 * TILE : 0)];      // two planes of keys and of values, and the documents of two tiles
     int* const key_doc = reinterpret_cast<int*>(smem + PLANES);
     const int id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-    if (id >= wide(blocks_q) * p.H * p.B) return;
-    const int bh = id / blocks_q, q0 = (blocks_q - 1 - id % blocks_q) * QB, b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
+    if ((DOC && order ? static_cast<int>(blockIdx.x) : id) >= wide(blocks_q) * p.H * p.B) return;
+    int b = id / blocks_q / p.H, h = id / blocks_q % p.H, q0 = (blocks_q - 1 - id % blocks_q) * QB;
+    if (DOC && order) {
+        const int item = order[blockIdx.x / p.H];
+        b = item / blocks_q, h = dealt(blockIdx.x % p.H, p.H), q0 = item % blocks_q * QB;
+    }
+    const int hk = h / (p.H / p.Hk);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5;
     const lds_t lds = lds_of(smem);
     constexpr int BUF = 2 * Plane<D>::BYTES;
@@ -214,7 +248,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_dq(const rwkv_attn_
 // With heads of 128 the two sums take half of a wave's 256 registers and the keys a quarter of the rest: the values are read from LDS.  There a workgroup has 8 waves
 // (256 keys; two waves a SIMD), or 4 where there are few workgroups (B2 T8192 H32 N128: with the values in registers and 4 waves 4.4 ms, so 2.5).
 template <class E, int D, int WAVES, bool CAP, bool BIAS, bool DOC>
-__global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void attn_dkv(const rwkv_attn_args p, const float* delta, const Range* key_ranges, const Range* ranges, const int blocks_k, const int per_xcd, const int parts, float* part) {
+__global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void attn_dkv(const rwkv_attn_args p, const float* delta, const Range* key_ranges, const Range* ranges, const int* order, const int blocks_k, const int per_xcd, const int parts, float* part) {
     constexpr int KB = 32 * WAVES, PLANES = 4 * Plane<D>::BYTES, VALUES = D == 128 ? KB / TILE * Plane<D>::BYTES : 0;
     constexpr int VALUS = 5 + (CAP ? 6 : 0) + (BIAS ? 2 : 0), TRANS = CAP ? 3 : 1;      // instructions of a pair
     // two planes of queries and of dY (below 64 KB: what M0 can name), lse, delta and documents of two tiles, the values of the block's keys
@@ -222,8 +256,13 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void at
     float *const row_lse = reinterpret_cast<float*>(smem + PLANES), *const row_delta = row_lse + 2 * TILE;
     int* const row_doc = reinterpret_cast<int*>(row_delta + 2 * TILE);
     const int id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-    if (id >= wide(blocks_k) * parts * p.Hk * p.B) return;
-    const int bh = id / (blocks_k * parts), mine = id / blocks_k % parts, k0 = id % blocks_k * KB, b = bh / p.Hk, hk = bh % p.Hk, G = p.H / p.Hk / parts;
+    if ((DOC && order ? static_cast<int>(blockIdx.x) : id) >= wide(blocks_k) * parts * p.Hk * p.B) return;
+    int b = id / (blocks_k * parts) / p.Hk, hk = id / (blocks_k * parts) % p.Hk, mine = id / blocks_k % parts, k0 = id % blocks_k * KB;
+    if (DOC && order) {
+        const int groups = p.Hk * parts, item = order[blockIdx.x / groups], c = dealt(blockIdx.x % groups, groups);
+        b = item / blocks_k, hk = c / parts, mine = c % parts, k0 = item % blocks_k * KB;
+    }
+    const int G = p.H / p.Hk / parts;
     const int first_head = (hk * parts + mine) * G;              // of G that the block does
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5;
     const lds_t lds = lds_of(smem);
@@ -464,20 +503,23 @@ template <class E, int D> int run(hipStream_t st, const rwkv_attn_args& p) {
     const int64_t per_q = (wide(blocks_q) * p.H * p.B + 7) / 8, per_k = (wide(blocks_k) * plan.key_parts * p.Hk * p.B + 7) / 8;
     const int64_t sums = (wide(p.B) * p.Tk * p.Hk * p.N / 8 + 255) / 256;
     if (row_blocks > INT_MAX || per_q * 8 > INT_MAX || per_k * 8 > INT_MAX || (plan.key_parts > 1 && sums > INT_MAX)) return RWKV_ERR_SHAPE;
-    // the documents of tiles of keys and of tiles of queries, delta, the sums of groups of heads
+    // the documents of tiles of keys and of tiles of queries, the orders, delta, the sums of groups of heads
     Range *key_ranges = static_cast<Range*>(p.workspace), *ranges = key_ranges + (p.doc ? p.B * tiles_of(p.Tk) : 0);
-    float* delta = reinterpret_cast<float*>(ranges + (p.doc ? p.B * tiles_of(p.Tq) : 0));
+    char* at = reinterpret_cast<char*>(ranges + (p.doc ? p.B * tiles_of(p.Tq) : 0));
+    int *q_order = plan.q_items > 0 ? reinterpret_cast<int*>(at) : nullptr, *k_order = plan.k_items > 0 ? reinterpret_cast<int*>(at + plan.q_order) : nullptr;
+    float* delta = reinterpret_cast<float*>(at + plan.q_order + plan.k_order);
     float* part = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + plan.backward) - (plan.key_parts > 1 ? 2 * plan.key_parts * wide(p.B) * p.Tk * p.Hk * p.N : 0);
     if (p.doc) {
         launch_attn_ranges(st, p.doc, p.B, p.Tk, 0, key_ranges);
         if (p.Tq == p.Tk) ranges = key_ranges;
         else launch_attn_ranges(st, p.doc, p.B, p.Tk, p.Tk - p.Tq, ranges);
+        if (q_order || k_order) launch_attn_order(st, p, key_ranges, ranges, plan, q_order, k_order);
     }
     hipLaunchKernelGGL((attn_delta<E, D>), dim3(static_cast<unsigned>(row_blocks)), dim3(256), 0, st, p, delta);
     const auto go = [&](auto dq, auto dkv) {
-        hipLaunchKernelGGL(dkv, dim3(static_cast<unsigned>(per_k * 8)), dim3(eight ? 512 : 256), 0, st, p, delta, key_ranges, ranges, blocks_k, static_cast<int>(per_k), plan.key_parts, part);
+        hipLaunchKernelGGL(dkv, dim3(static_cast<unsigned>(per_k * 8)), dim3(eight ? 512 : 256), 0, st, p, delta, key_ranges, ranges, k_order, blocks_k, static_cast<int>(per_k), plan.key_parts, part);
         if (plan.key_parts > 1) hipLaunchKernelGGL((attn_dkv_sum<E>), dim3(static_cast<unsigned>(sums), 2), dim3(256), 0, st, p, plan.key_parts, part);
-        hipLaunchKernelGGL(dq, dim3(static_cast<unsigned>(per_q * 8)), dim3(256), 0, st, p, delta, key_ranges, blocks_q, static_cast<int>(per_q));
+        hipLaunchKernelGGL(dq, dim3(static_cast<unsigned>(per_q * 8)), dim3(256), 0, st, p, delta, key_ranges, q_order, blocks_q, static_cast<int>(per_q));
         return launch_status();
     };
     const auto masks = [&](auto cap, auto bias) {
@@ -498,6 +540,11 @@ template <class E> int run_any(hipStream_t st, const rwkv_attn_args& p) { return
 void launch_attn_ranges(hipStream_t st, const int* doc, int B, int T, int first, Range* out) {
     const int tiles = static_cast<int>(tiles_of(T - first));
     hipLaunchKernelGGL(attn_ranges, dim3((tiles + 3) / 4, B), dim3(256), 0, st, doc, T, first, tiles, out);
+}
+
+void launch_attn_order(hipStream_t st, const rwkv_attn_args& p, const Range* keys, const Range* queries, const AttnPlan& plan, int* q_order, int* k_order) {
+    const int q = q_order ? plan.q_items : 0, k = k_order ? plan.k_items : 0;
+    hipLaunchKernelGGL(attn_order, dim3((q > 0) + (k > 0)), dim3(1024), 0, st, p, keys, queries, q, q_order, k, k_order, plan.eight ? 256 : 128);
 }
 
 int launch_attn_bwd(hipStream_t st, const rwkv_attn_args& p) { return p.dtype == RWKV_DTYPE_BF16 ? run_any<bf16_t>(st, p) : run_any<half_t>(st, p); }

@@ -19,16 +19,21 @@ constexpr int READS = 6;
 
 // parts > 1: the block does one part of the keys, and leaves sums and maxima in `part` for attn_join.
 template <class E, int D, bool CAP, bool BIAS, bool DOC>
-__global__ __launch_bounds__(256, 2) void attn_fwd(const rwkv_attn_args p, const Range* ranges, const int blocks_q, const int per_xcd, const int parts, float* part) {
+__global__ __launch_bounds__(256, 2) void attn_fwd(const rwkv_attn_args p, const Range* ranges, const int* order, const int blocks_q, const int per_xcd, const int parts, float* part) {
     constexpr int QB = 128;
     // two planes of keys and of values (below 64 KB: what M0 can name), and the documents of two tiles
     constexpr int PLANES = 4 * Plane<D>::BYTES;
     __shared__ __align__(16) char smem[PLANES + (DOC ? 8 * TILE : 0)];
     int* const key_doc = reinterpret_cast<int*>(smem + PLANES);
-    const int id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+    const int id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3), mine = id % parts;
     const int64_t all = wide(blocks_q) * parts * p.H * p.B;
-    if (id >= all) return;
-    const int bh = id / (blocks_q * parts), mine = id % parts, q0 = (blocks_q - 1 - id / parts % blocks_q) * QB, b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
+    if ((DOC && order ? static_cast<int>(blockIdx.x) : id) >= all) return;
+    int b = id / (blocks_q * parts) / p.H, h = id / (blocks_q * parts) % p.H, q0 = (blocks_q - 1 - id / parts % blocks_q) * QB;
+    if (DOC && order) {
+        const int item = order[blockIdx.x / p.H];
+        b = item / blocks_q, h = dealt(blockIdx.x % p.H, p.H), q0 = item % blocks_q * QB;
+    }
+    const int hk = h / (p.H / p.Hk);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5;
     const lds_t lds = lds_of(smem);
     constexpr int BUF = 2 * Plane<D>::BYTES;
@@ -288,12 +293,14 @@ template <class E, int D> int run(hipStream_t st, const rwkv_attn_args& p) {
     const AttnPlan plan = attn_plan(p.B, p.Tq, p.Tk, p.H, p.Hk, p.N, p.doc != nullptr);
     const int64_t all = wide(blocks_q) * plan.query_parts * p.H * p.B, per = (all + 7) / 8, join = (wide(p.B) * p.H * p.Tq * (D / 4) + 255) / 256;
     if (per * 8 > INT_MAX || (plan.query_parts > 1 && join > INT_MAX)) return RWKV_ERR_SHAPE;
-    float* part = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + plan.ranges);
+    int* order = plan.q_items > 0 ? reinterpret_cast<int*>(static_cast<char*>(p.workspace) + plan.ranges) : nullptr;
+    float* part = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + plan.ranges + plan.q_order);
     const dim3 grid(static_cast<unsigned>(per * 8)), block(256);
     Range* ranges = static_cast<Range*>(p.workspace);
     if (p.doc) launch_attn_ranges(st, p.doc, p.B, p.Tk, 0, ranges);
+    if (order) launch_attn_order(st, p, ranges, ranges, plan, order, nullptr);
     const auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, block, 0, st, p, ranges, blocks_q, static_cast<int>(per), plan.query_parts, part);
+        hipLaunchKernelGGL(kernel, grid, block, 0, st, p, ranges, order, blocks_q, static_cast<int>(per), plan.query_parts, part);
         if (plan.query_parts > 1) hipLaunchKernelGGL((attn_join<E, D>), dim3(static_cast<unsigned>(join)), block, 0, st, p, plan.query_parts, part);
         return launch_status();
     };

@@ -211,6 +211,8 @@ struct Scorer {
     }
 };
 
+// head (or group) c of n of an item whose blocks follow each other: neighbours to one XCD where that comes out even
+DEVINL int dealt(const int c, const int n) { return n % 8 == 0 ? (c & 7) * (n >> 3) + (c >> 3) : c; }
 __host__ __device__ __forceinline__ int64_t tiles_of(const int T) { return (wide(T) + TILE - 1) / TILE; }
 // The tiles first .. end - 1 that hold tokens of documents lo .. hi, from the first on or, BACK, from the last, and whether each is whole and all of the one document
 // lo (= hi).  Without documents: all.

@@ -30,11 +30,15 @@ struct Range {
 struct AttnPlan {
     int query_parts, key_parts;
     bool eight;                                                 // heads of 128: 256 keys a workgroup of attn_dkv
-    size_t ranges, forward, backward;                           // bytes: documents of tiles; workspace of either direction
+    int q_items, k_items;                                       // blocks of queries, of keys, that are ordered by their work (0: they are not)
+    size_t ranges, q_order, k_order, forward, backward;         // bytes: documents of tiles; the orders; workspace of either direction
 };
+constexpr int MAX_ORDER = 1024;
 AttnPlan attn_plan(int B, int Tq, int Tk, int H, int Hk, int N, bool doc);
 // attn_bwd.hip: tile i of `out`'s row b has positions first + 64 i .. of doc's row b, below T
 void launch_attn_ranges(hipStream_t st, const int* doc, int B, int T, int first, Range* out);
+// attn_bwd.hip: the blocks of queries and of keys, of which either may be null, in the order of their work
+void launch_attn_order(hipStream_t st, const rwkv_attn_args& p, const Range* keys, const Range* queries, const AttnPlan& plan, int* q_order, int* k_order);
 // attn_fwd.hip, attn_bwd.hip (arguments checked)
 int launch_attn_fwd(hipStream_t st, const rwkv_attn_args& p);
 int launch_attn_bwd(hipStream_t st, const rwkv_attn_args& p);

@@ -76,6 +76,19 @@ def test_many_heads(lib, how, B, Tq, Tk, H, Hk, N):
     check(q, k, v, dy, **how)
 
 
+@pytest.mark.parametrize("how", ["many documents", "padding", "ids that come back", "wide documents", "all"])
+@pytest.mark.parametrize("B,Tq,Tk,H,Hk,N,dtype", [(3, 520, 600, 64, 16, 128, "bf16"), (4, 390, 390, 40, 40, 64, "fp16"), (4, 450, 450, 33, 11, 64, "bf16")])
+def test_more_blocks_of_documents_than_run_at_once(lib, how, B, Tq, Tk, H, Hk, N, dtype):
+    """Blocks of queries and of keys in the order of their work."""
+    o = dict(HOW[how])
+    if o.pop("bias", False):
+        o["slopes"] = torch.exp2(-8.0 * torch.arange(1, H + 1) / H).to(DEV)
+    if o.pop("prefix", False):
+        o["prefix"] = torch.tensor([Tk // 3, 5, 0, Tk + 9][:B], dtype=torch.int32, device=DEV)
+    o["doc"] = doc_ids(B, Tk, o["doc"], seed=5).to(DEV)
+    check(*inputs(B, Tq, Tk, H, Hk, N, DT[dtype], seed=81), **o)
+
+
 def test_gradients_that_come_as_views_from_anywhere(lib):
     q, k, v, dy = inputs(1, 70, 70, 2, 1, 64, torch.bfloat16, seed=75)
     odd = torch.zeros(dy.numel() + 3, device=DEV, dtype=dy.dtype)[3:].view_as(dy).copy_(dy)
