@@ -247,10 +247,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_dq(const rwkv_attn_
 //
 // With heads of 128 the two sums take half of a wave's 256 registers and the keys a quarter of the rest: the values are read from LDS.  There a workgroup has 8 waves
 // (256 keys; two waves a SIMD), or 4 where there are few workgroups (B2 T8192 H32 N128: with the values in registers and 4 waves 4.4 ms, so 2.5).
+//
+// The two halves of a tile go through one after the other; what a wave does not overlap others do.  With heads of 64 that leaves room for a third wave on a SIMD, except with
+// documents (8 to 22 registers spilled): B8 T4096 H32 N64 forward + backward, with the halves interleaved and two waves, and so: plain 2.96 / 2.81 ms, with slopes 3.08 / 2.97,
+// with a cap 4.16 / 3.97; with documents the same to 2 percent.
 template <class E, int D, int WAVES, bool CAP, bool BIAS, bool DOC>
-__global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void attn_dkv(const rwkv_attn_args p, const float* delta, const Range* key_ranges, const Range* ranges, const int* order, const int blocks_k, const int per_xcd, const int parts, float* part) {
+__global__ __launch_bounds__(64 * WAVES, D == 128 ? (WAVES == 4 ? 1 : 2) : DOC ? 2 : 3) void attn_dkv(const rwkv_attn_args p, const float* delta, const Range* key_ranges, const Range* ranges, const int* order, const int blocks_k, const int per_xcd, const int parts, float* part) {
     constexpr int KB = 32 * WAVES, PLANES = 4 * Plane<D>::BYTES, VALUES = D == 128 ? KB / TILE * Plane<D>::BYTES : 0;
-    constexpr int VALUS = 5 + (CAP ? 6 : 0) + (BIAS ? 2 : 0), TRANS = CAP ? 3 : 1;      // instructions of a pair
     // two planes of queries and of dY (below 64 KB: what M0 can name), lse, delta and documents of two tiles, the values of the block's keys
     __shared__ __align__(16) char smem[PLANES + 6 * 4 * TILE + VALUES];
     float *const row_lse = reinterpret_cast<float*>(smem + PLANES), *const row_delta = row_lse + 2 * TILE;
@@ -417,40 +420,18 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 && WAVES == 4 ? 1 : 2) void at
             const bool masked = part || shift + i0 < from_hi;
             u32x4 w[2], ds[2];
             const bool ahead = two_sided && shift + i0 < k0 + KB - 1;
-            if constexpr (D == 64) {
-                f32x16 s0, s1, p0, p1;
-                products(s0, p0, 0);
-                if (ahead) turn(sc, s0, i0);
-                __builtin_amdgcn_sched_barrier(0);
-                products(s1, p1, 1);
-                slopes(sc, s0, p0, i0, 0, par);
-                beside<2 * D / 16, D / 8 + 8, VALUS * 16, TRANS * 16>();
-                __builtin_amdgcn_sched_barrier(0);
-                if (masked) mask(s0, p0, i0, 0, par);
-                if (ahead) turn(sc, s1, i0 + 32);
-                w[0] = as_operand<E>(s0, 0), w[1] = as_operand<E>(s0, 1), ds[0] = as_operand<E>(p0, 0), ds[1] = as_operand<E>(p0, 1);
-                __builtin_amdgcn_sched_barrier(0);
-                add(w, ds, 0);
-                slopes(sc, s1, p1, i0, 1, par);
-                beside<2 * D / 16, D / 4 + 8, VALUS * 16, TRANS * 16>();
-                __builtin_amdgcn_sched_barrier(0);
-                if (masked) mask(s1, p1, i0, 1, par);
-                w[0] = as_operand<E>(s1, 0), w[1] = as_operand<E>(s1, 1), ds[0] = as_operand<E>(p1, 0), ds[1] = as_operand<E>(p1, 1);
-                add(w, ds, 1);
-            } else {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    f32x16 s, dp;
-                    products(s, dp, e);
-                    if (ahead) turn(sc, s, i0 + 32 * e);
-                    __builtin_amdgcn_sched_barrier(0);
-                    slopes(sc, s, dp, i0, e, par);
-                    if (masked) mask(s, dp, i0, e, par);
-                    w[0] = as_operand<E>(s, 0), w[1] = as_operand<E>(s, 1), ds[0] = as_operand<E>(dp, 0), ds[1] = as_operand<E>(dp, 1);
-                    __builtin_amdgcn_sched_barrier(0);
-                    add(w, ds, e);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+            for (int e = 0; e < 2; ++e) {
+                f32x16 s, dp;
+                products(s, dp, e);
+                if (ahead) turn(sc, s, i0 + 32 * e);
+                __builtin_amdgcn_sched_barrier(0);
+                slopes(sc, s, dp, i0, e, par);
+                if (masked) mask(s, dp, i0, e, par);
+                w[0] = as_operand<E>(s, 0), w[1] = as_operand<E>(s, 1), ds[0] = as_operand<E>(dp, 0), ds[1] = as_operand<E>(dp, 1);
+                __builtin_amdgcn_sched_barrier(0);
+                add(w, ds, e);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         rows.move(step);
