@@ -2,8 +2,8 @@
 // queries (dQ: three products a pair) and once by those that own keys (dK, dV: four), each sum in one wave's registers in a fixed order.
 //
 // Seven products where one kernel for all three would do with five: that one would have to add dQ from many workgroups, in an order that changes (atomics)
-// or through memory.  Bound by issue, as the forward.  bf16, causal: B2 T8192 H32 Hk8 N128 with a cap and prefixes dK dV 2.5 ms, dQ 1.95 ms; B8 T4096 H32 N64 with
-// slopes 1.55 ms (690 TFLOP/s) and 0.95 ms (860).
+// or through memory.  Bound by issue, as the forward.  bf16, causal: B2 T8192 H32 Hk8 N128 with a cap and prefixes dK dV 2.4 ms, dQ 1.9 ms; B8 T4096 H32 N64 with
+// slopes 1.25 ms (880 TFLOP/s) and 0.95 ms (870).
 #include "attn_tile.h"
 
 namespace rwkv {
@@ -79,7 +79,8 @@ template <class E, int D> __global__ __launch_bounds__(256) void attn_delta(cons
 }
 
 // dQ: 4 waves of 32 queries over the keys that any of them sees; S^T = K Q^T and dP^T = V dY^T, dQ^T += K^T dS^T
-// Three waves a SIMD with heads of 64, for 1 to 8 spilled registers where there is a bias (B8 T4096 H32 N64 with slopes, with the forward, 3.135 -> 3.086 ms).
+// Three waves a SIMD with heads of 64, for 1 to 8 spilled registers where there is a bias (B8 T4096 H32 N64 with slopes, forward + backward 3.135 -> 3.086 ms).  The halves of
+// a tile interleaved: one after the other, with four waves, is slower (2.77 -> 2.85 ms; heads of 128, two waves, dQ 1.91 -> 2.11).
 template <class E, int D, bool CAP, bool BIAS, bool DOC>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_dq(const rwkv_attn_args p, const float* delta, const Range* ranges, const int* order, const int blocks_q, const int per_xcd) {
     constexpr int QB = 128;
