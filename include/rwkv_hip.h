@@ -632,7 +632,7 @@ int rwkv_attn_backward(void* stream, const rwkv_attn_args* args);
 /* Attention of one new token a sequence over a cache in pages: sequence b has lens[b] tokens, the new one's position is lens[b] - 1, token t
  * is row t % page of page table[b][t / page].  Scores and key heads as above.  lens[b] <= 0: y = 0; more tokens than the table has
  * pages for are not seen; tokens of a page whose number is not in 0 .. P-1 are not seen.  k, v (may be NULL): the new token's key and value,
- * which are written to the cache at lens[b] - 1 and seen; a page that is written belongs to one sequence.  page is a power of two. */
+ * which are written to the cache at lens[b] - 1 and seen; a page that is written belongs to one sequence, in one place.  page is a power of two. */
 typedef struct rwkv_paged_args {
     int dtype;
     int B, H, Hk, N, P, page, M;

@@ -148,7 +148,8 @@ struct Place {
     DEVINL int there(const rwkv_grec_args& p) const { return n <= 0 ? 0 : p.T - t0 < S ? p.T - t0 : S; }      // the thread's tokens that there are (may be below zero)
 };
 // a thread's S tokens of [B,T,C]: the token's address is the same for the whole workgroup and the thread's part 32 bits, so that 24 accesses take one register of
-// addresses each array (with 64 bits a thread the backward spilled 28 registers and took 0.64 ms instead of 0.35 at B8 T4096 C4096, chained).  VEC promises that 32 bits do.
+// addresses each array (with 64 bits a thread, and pairs kept unpacked below, the backward
+// spilled 28 registers and took 0.64 ms instead of 0.35 at B8 T4096 C4096, chained).  VEC promises that 32 bits do.
 template <class E, bool VEC> struct Rows {
     char* base;
     int64_t step;

@@ -9,7 +9,8 @@ def RUN_CUDA(q, k_pages, v_pages, table, lens, k=None, v=None, slopes=None, cap=
 
     k_pages, v_pages [P,page,Hk,N]: page a power of two, N a multiple of 8 up to 128, the innermost dimension dense, the other strides
     multiples of 8.  Token t of sequence b is row t % page of page table[b, t // page] (int32 [B,M]).  With k and v [B,Hk,N] the new
-    token's key and value are written to the cache, at lens[b] - 1, and count from there; a page that is written must belong to one sequence.
+    token's key and value are written to the cache, at lens[b] - 1, and count from there; a page that is written must belong to one
+    sequence, in one place.
 
     A sequence with lens[b] <= 0 has y = 0.  Tokens beyond the table's pages, and tokens of pages that are not in 0 .. P-1, are left out
     (they are found on the GPU, where no error can be raised).  No gradients."""

@@ -135,3 +135,34 @@ def test_what_is_written_in_place_is_found_out_by_a_graph_that_saved_it(lib):
     PA.RUN_CUDA(z, kp, vp, table, lens, k=z, v=z)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.backward()
+
+
+def test_in_inference_mode(lib):
+    w, x, slopes = some(2, 20, torch.bfloat16, 51)
+    with torch.no_grad():
+        want = layers(w, x, None, slopes)
+    with torch.inference_mode():
+        got = layers(w, x, None, slopes)
+        z, h = G.RUN_CUDA(w[:, :-1], x[:, :-1])
+        kp, vp = (torch.zeros(4, 16, HK, N, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+        table = torch.tensor([[3, 1], [0, 2]], dtype=torch.int32, device=DEV)
+        for t in range(20):
+            last = G.STEP(w[:, -1], x[:, -1], h) if t == 19 else z[:, t]
+            q, k, v = (u.contiguous() for u in qkv(last))
+            y = PA.RUN_CUDA(q, kp, vp, table, torch.full((2,), t + 1, dtype=torch.int32, device=DEV), k=k, v=v, slopes=slopes, cap=20.0)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    within("y", y[:, None], tuple(t[:, -1:] for t in O.attention(*qkv(torch.cat([z, last[:, None]], 1)), slopes=slopes, cap=20.0)["y"]))
+
+
+def test_document_ids_at_their_ends(lib):
+    """The largest id, and one that follows it."""
+    B, T = 2, 140
+    w, x, slopes = some(B, T, torch.bfloat16, 61)
+    doc = torch.full((B, T), 2 ** 31 - 1, dtype=torch.int32)
+    doc[0, 30:90] = 0
+    doc[1, 100:] = -2 ** 31
+    doc = doc.to(DEV)
+    with torch.no_grad():
+        z, y = layers(w, x, doc, slopes)
+    within("z", z, O.gated_recurrence(w, x, doc=doc)["y"])
+    within("y", y, O.attention(*qkv(z), doc=doc, slopes=slopes, cap=20.0)["y"])
