@@ -14,9 +14,8 @@ bool multiples_of_8(std::initializer_list<int64_t> xs) {
     for (const int64_t x : xs) if (x % 8 != 0) return false;
     return true;
 }
-// a tile of 64 rows is addressed with 31 bits
 bool wide_rows(const rwkv_attn_args& p) {
-    for (const int64_t s : {p.q_st, p.k_st, p.v_st, static_cast<int64_t>(p.H) * p.N}) if (s < 0 || s >= 1 << 24) return true;
+    for (const int64_t s : {p.q_st, p.k_st, p.v_st, static_cast<int64_t>(p.H) * p.N}) if (s < 0 || s >= MAX_TOKEN_STRIDE) return true;
     return false;
 }
 }  // namespace

@@ -8,6 +8,8 @@
 // column a lane).
 #pragma once
 
+#include <climits>
+
 #include "common.h"
 #include "mixers.h"
 
@@ -110,9 +112,14 @@ DEVINL void here(float& x) { asm volatile("" : "+v"(x)); }
 // The way of a tile of 64 rows from memory straight to LDS: 16 bytes a lane, a wave's 1024 bytes in the order of its lanes, so that each lane fetches the piece whose
 // place it is.  Rows behind the last and channels behind N come as zeros (the buffer's bounds).  The compiler does not count these loads: arrived() before the barrier behind which they are read.  Of the waves of a
 // workgroup each brings every WAVES-th kilobyte.
+// The bounds are those of the tile's own rows, of all that are left: 31 bits hold no more than a tile.
+constexpr uint32_t NOWHERE = 0x7ffffff0u;                       // an offset beyond all bounds: such lanes bring zeros
+__host__ __device__ __forceinline__ constexpr uint32_t tile_bytes(const int rows, const int step, const int N) { return rows > 0 ? ((rows < TILE ? rows : TILE) - 1) * step + 2 * N : 0; }
+static_assert(tile_bytes(INT_MAX, 2 * (MAX_TOKEN_STRIDE - 1), 128) <= NOWHERE && tile_bytes(INT_MAX, 2 * (MAX_TOKEN_STRIDE - 1), 128) == 63u * 2 * (MAX_TOKEN_STRIDE - 1) + 256, "a tile in 31 bits");
+static_assert(tile_bytes(TILE, 256, 128) == TILE * 256 && tile_bytes(TILE + 1, 256, 128) == TILE * 256 && tile_bytes(TILE - 1, 256, 128) == (TILE - 1) * 256, "a tile's rows");
+static_assert(tile_bytes(1, 2 * (MAX_TOKEN_STRIDE - 1), 8) == 16 && tile_bytes(0, 256, 128) == 0 && tile_bytes(-1, 256, 128) == 0, "the last rows, and none");
 template <int D, int WAVES> struct Fetch {
     static constexpr int LANES = D / 8, ROWS = Plane<D>::ROWS, STEPS = TILE / (ROWS * WAVES);
-    static constexpr uint32_t NOWHERE = 0x7ffffff0u;             // beyond all bounds: such lanes bring zeros
     uint32_t row, off;
     DEVINL Fetch(const int tid, const int N) {
         const int lane = tid & 63;
@@ -120,9 +127,9 @@ template <int D, int WAVES> struct Fetch {
         const int piece = (lane % LANES) ^ Plane<D>::swap(row);
         off = 8 * piece < N ? 16 * piece : NOWHERE;
     }
-    // `rows` rows `step` bytes apart to the plane at `to`; of those only the ones whose bit is set
+    // the rows from `first` on, of which `rows` are left, `step` bytes apart, to the plane at `to`; of those only the ones whose bit is set
     template <bool SOME> DEVINL void operator()(const lds_t to, const void* first, const int rows, const int step, const int N, const uint64_t which) const {
-        const buf_t b = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(first), 0, rows > 0 ? (rows - 1) * step + 2 * N : 0, 0x00027000);
+        const buf_t b = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(first), 0, tile_bytes(rows, step, N), 0x00027000);
         const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         uint32_t first_off = off;
         asm volatile("" : "+v"(first_off));                     // (offsets are made anew: kept, they would be spilled, and a reload waits for all that is under way)
@@ -133,7 +140,7 @@ template <int D, int WAVES> struct Fetch {
             uint32_t o = first_off + (on ? i * ROWS * WAVES * step : 0);
             if (SOME) o = which >> (row + i * ROWS * WAVES) & 1 ? o : NOWHERE;
             // (M0 is read one wait state after it is written)
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(to + (i * WAVES + wave) * Plane<D>::STEP), "v"(o), "s"(b) : "memory");
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(to + (i * WAVES + wave) * Plane<D>::STEP), "v"(o), "s"(b) : "memory", "m0");
         }
     }
 };

@@ -20,6 +20,9 @@ template <class E> DEVINL E from_f(float x) {
 // What the scores' arithmetic holds for: the capped score is made as cap - 2 cap / (1 + e^z), which is off by 2^-23 cap, and e^z's argument must not overflow.
 inline bool scores_ok(const float scale, const float cap) { return scale > 0.f && scale <= 0x1p60f && (cap == 0.f || (cap >= 0x1p-20f && cap <= 4096.f)); }
 
+// Attention's tokens are less than this many elements apart: a tile of 64 rows is addressed with 31 bits.
+constexpr int MAX_TOKEN_STRIDE = 1 << 24;
+
 struct Range {
     int lo, hi;                                                 // of the tokens that are no padding; INT_MAX and -1 without one
     int whole;                                                  // 64 tokens, none of them padding

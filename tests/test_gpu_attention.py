@@ -218,3 +218,42 @@ def test_long_keys_and_tensors_beyond_2_31_elements(lib):
     got = A.RUN_CUDA(q.expand(2, -1, -1, -1).contiguous(), K, V)
     want = A.RUN_CUDA(q, k, v)
     assert torch.equal(got[:1], want) and torch.equal(got[1:], want)
+
+
+def far_rows(z, store, at):
+    """z [1,T,H,N] as a view of `store` [T,step], from column `at` on."""
+    view = store[:, at:at + z.shape[2] * z.shape[3]].unflatten(1, z.shape[2:])[None]
+    view.copy_(z)
+    return view
+
+
+def passes(q, k, v, dy, **how):
+    t = [z.detach().requires_grad_(True) for z in (q, k, v)]
+    y = A.RUN_CUDA(*t, **how)
+    return [y.detach()] + list(torch.autograd.grad([y], t, [dy]))
+
+
+@pytest.mark.parametrize("Tq,Tk,step,H,Hk,N,dtype", [(257, 257, 1 << 23, 4, 2, 40, "bf16"), (257, 257, 1 << 23, 2, 2, 128, "fp16"), (70, 131100, 16384, 4, 2, 64, "bf16"),
+                                                     (3, 350000, 6144, 2, 1, 96, "fp16")])
+def test_rows_that_span_more_than_4_gib(lib, Tq, Tk, step, H, Hk, N, dtype):
+    """Queries, keys and values a long way apart in one tensor, in which NaN stands between them: what the same rows side by side give."""
+    q, k, v, dy = inputs(1, Tq, Tk, H, Hk, N, DT[dtype], seed=21)
+    store = torch.full((Tk, step), float("nan"), device=DEV, dtype=DT[dtype])
+    assert store.numel() * 2 >= 1 << 32
+    far = [far_rows(z, store[Tk - z.shape[1]:], at) for z, at in ((q, 0), (k, 1024), (v, 2048))]
+    for n, a, b in zip(["y", "dq", "dk", "dv"], passes(*far, dy), passes(q, k, v, dy)):
+        assert torch.equal(a, b), n
+
+
+def test_padding_in_rows_that_span_more_than_2_gib(lib):
+    Tq, Tk, step, H, Hk, N = 70, 70001, 16384, 4, 2, 96
+    q, k, v, dy = inputs(1, Tq, Tk, H, Hk, N, torch.bfloat16, seed=25)
+    doc = torch.zeros(1, Tk, dtype=torch.int32, device=DEV)
+    doc[0, 100:190], doc[0, 50000:50007], doc[0, -9:-5] = -1, -2, -1
+    none = (doc < 0)[:, :, None, None]
+    q, k, v, dy = (z.masked_fill(none[:, -z.shape[1]:], 0.0) for z in (q, k, v, dy))
+    store = torch.full((Tk, step), float("nan"), device=DEV, dtype=torch.bfloat16)
+    assert store.numel() * 2 > 1 << 31
+    far = [far_rows(z.masked_fill(none[:, -z.shape[1]:], float("nan")), store[Tk - z.shape[1]:], at) for z, at in ((q, 0), (k, 1024), (v, 2048))]
+    for n, a, b in zip(["y", "dq", "dk", "dv"], passes(*far, dy.masked_fill(none[:, -Tq:], float("nan")), doc=doc), passes(q, k, v, dy, doc=doc)):
+        assert torch.equal(a, b), n
