@@ -616,7 +616,7 @@ typedef struct rwkv_attn_args {
     int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
     const float* slopes;              /* [H] or NULL */
     const int* doc;                   /* [B,Tk] or NULL */
-    const int* prefix;                /* [B] or NULL */
+    const int* prefix;                /* [B] or NULL; any numbers */
     void* y;                          /* [B,Tq,H,N], 16-byte aligned; forward: written, backward: read */
     void* y_rest;                     /* [B,Tq,H,N], 16-byte aligned */
     float* lse;                       /* [B,H,Tq]; forward: may be NULL */

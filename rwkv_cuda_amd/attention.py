@@ -5,7 +5,7 @@
 q [B,Tq,H,N], k, v [B,Tk,Hk,N] with H a multiple of Hk (head h reads key head h Hk / H) and N a multiple of 8 up to 128; the innermost
 dimension dense, the other strides multiples of 8 (views of one projection).  The queries are the last Tq of the Tk positions.
 
-Visible are all keys, or, with `causal`, those up to the query's own position and those before prefix[b] (int32 [B]).  `doc` [B,Tk] int32
+Visible are all keys, or, with `causal`, those up to the query's own position and those before prefix[b] (int32 [B]; below 0 is as 0).  `doc` [B,Tk] int32
 names the document of each token: a query sees its own document's keys only; a negative one is padding, which sees nothing (y = 0) and
 is not seen, whatever stands there.  (A NaN or an infinity in a real token may reach every row of its batch element and head, as in any
 product with weights of 0.)  Gradients of q, k and v."""

@@ -35,7 +35,7 @@ __global__ __launch_bounds__(1024) void attn_order(const rwkv_attn_args p, const
     const int blocks = items / p.B, lane = threadIdx.x & 63;
     for (int i = threadIdx.x >> 6; i < items; i += 16) {
         const int b = i / blocks, at = i % blocks * block, end = min(at + block, for_keys ? p.Tk : p.Tq);
-        const int reach = p.prefix ? min(p.prefix[b], p.Tk) : 0;
+        const int reach = reach_of(p, b);
         const Range* own = keys + wide(b) * tk;
         const Range* other = for_keys ? queries + wide(b) * tq : own;
         int lo = INT_MAX, hi = -1;
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_dq(const rwkv_attn_
     const E* kbase = static_cast<const E*>(p.k) + b * p.k_sb + hk * p.k_sh;
     const E* vbase = static_cast<const E*>(p.v) + b * p.v_sb + hk * p.v_sh;
     const int* doc = DOC ? p.doc + wide(b) * p.Tk : nullptr;
-    const int shift = p.Tk - p.Tq, reach = p.prefix ? min(p.prefix[b], p.Tk) - 1 : -1;
+    const int shift = p.Tk - p.Tq, reach = reach_of(p, b) - 1;
 
     const int i = q0 + wave * 32 + (lane & 31);
     const bool real = i < p.Tq;
@@ -272,7 +272,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? (WAVES == 4 ? 1 : 2) : DOC ?
     const lds_t lds = lds_of(smem);
     constexpr int BUF = 2 * Plane<D>::BYTES;
 
-    const int shift = p.Tk - p.Tq, reach = p.prefix ? min(p.prefix[b], p.Tk) : 0;
+    const int shift = p.Tk - p.Tq, reach = reach_of(p, b);
     const int* doc = DOC ? p.doc + wide(b) * p.Tk : nullptr;
     const int j = k0 + wave * 32 + (lane & 31);
     const bool real = j < p.Tk;

@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd(const rwkv_attn_args p, const
     const E* kbase = static_cast<const E*>(p.k) + b * p.k_sb + hk * p.k_sh;
     const E* vbase = static_cast<const E*>(p.v) + b * p.v_sb + hk * p.v_sh;
     const int* doc = DOC ? p.doc + wide(b) * p.Tk : nullptr;
-    const int shift = p.Tk - p.Tq, reach = p.prefix ? min(p.prefix[b], p.Tk) - 1 : -1;
+    const int shift = p.Tk - p.Tq, reach = reach_of(p, b) - 1;
 
     const int i = q0 + wave * 32 + (lane & 31);
     const bool real = i < p.Tq;

@@ -218,6 +218,8 @@ struct Scorer {
     }
 };
 
+// how many of the first keys are seen from everywhere; a prefix lies on the GPU and may be any number
+DEVINL int reach_of(const rwkv_attn_args& p, const int b) { return p.prefix ? max(0, min(p.prefix[b], p.Tk)) : 0; }
 // head (or group) c of n of an item whose blocks follow each other: neighbours to one XCD where that comes out even
 DEVINL int dealt(const int c, const int n) { return n % 8 == 0 ? (c & 7) * (n >> 3) + (c >> 3) : c; }
 __host__ __device__ __forceinline__ int64_t tiles_of(const int T) { return (wide(T) + TILE - 1) / TILE; }

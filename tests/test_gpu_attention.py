@@ -257,3 +257,15 @@ def test_padding_in_rows_that_span_more_than_2_gib(lib):
     far = [far_rows(z.masked_fill(none[:, -z.shape[1]:], float("nan")), store[Tk - z.shape[1]:], at) for z, at in ((q, 0), (k, 1024), (v, 2048))]
     for n, a, b in zip(["y", "dq", "dk", "dv"], passes(*far, dy.masked_fill(none[:, -Tq:], float("nan")), doc=doc), passes(q, k, v, dy, doc=doc)):
         assert torch.equal(a, b), n
+
+
+@pytest.mark.parametrize("doc", [None, "two", "padded"])
+def test_prefixes_below_zero_are_none(lib, doc):
+    B, T, H, Hk, N = 3, 200, 4, 2, 64
+    q, k, v, dy = inputs(B, T, T, H, Hk, N, torch.bfloat16, seed=121)
+    how = {} if doc is None else dict(doc=doc_ids(B, T, doc, seed=6).to(DEV))
+    at = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    want = passes(q, k, v, dy, prefix=at(0, 0, 0), **how)
+    for low in (at(-1, -64, -65), at(-2 ** 31, -2 ** 31 + 1, -2 ** 31 + 63)):
+        for n, a, b in zip(["y", "dq", "dk", "dv"], passes(q, k, v, dy, prefix=low, **how), want):
+            assert torch.equal(a, b), n
