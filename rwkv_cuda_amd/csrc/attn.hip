@@ -85,7 +85,7 @@ int attn_any(void* stream, const rwkv_attn_args* p, bool backward) {
 extern "C" {
 
 size_t rwkv_attn_workspace_bytes(int B, int Tq, int Tk, int H, int Hk, int N, int doc, int backward) {
-    if (B <= 0 || Tq <= 0 || Tk < Tq || H <= 0 || Hk <= 0 || H % Hk != 0 || N <= 0 || N > 128) return 0;
+    if (B <= 0 || Tq <= 0 || Tk < Tq || H <= 0 || Hk <= 0 || H % Hk != 0 || N <= 0 || N > 128 || B > 65535 || H > 65535) return 0;
     const rwkv::AttnPlan a = rwkv::attn_plan(B, Tq, Tk, H, Hk, N, doc != 0);
     return backward ? a.backward : a.forward;
 }

@@ -285,7 +285,7 @@ extern "C" {
 
 // a maximum, a sum and an output of each piece and head
 size_t rwkv_paged_workspace_bytes(int B, int H, int Hk, int N, int page, int M) {
-    if (B <= 0 || H <= 0 || Hk <= 0 || N <= 0 || page <= 0 || M <= 0) return 0;
+    if (B <= 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || N <= 0 || N > 128 || page <= 0 || M <= 0 || B > 65535 || H > 65535) return 0;
     const int pieces = rwkv::pieces_of(B, H, Hk, page, M);
     return pieces > 1 ? static_cast<size_t>(B) * H * pieces * (rwkv::width_of(N) + 4) * sizeof(float) : 0;
 }

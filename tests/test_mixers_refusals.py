@@ -172,3 +172,13 @@ def test_paged_refusals_on_the_device(lib):
             call()
     with pytest.raises(_lib.RwkvHipError):
         R(q, kp[:0], kp[:0], i32(2, 2), i32(2))
+
+
+def test_sizes_of_workspaces_for_heads_that_do_not_fit(lib):
+    """More key heads than heads, or heads that are no multiple of them: no size, as for any call that is refused."""
+    assert lib.rwkv_paged_workspace_bytes(1, 1, 2, 64, 16, 4096) == 0
+    assert lib.rwkv_paged_workspace_bytes(1, 3, 2, 64, 16, 4096) == 0
+    assert lib.rwkv_paged_workspace_bytes(1, 2, 1, 136, 16, 4096) == 0
+    assert lib.rwkv_attn_workspace_bytes(1, 4, 4, 1, 2, 64, 0, 1) == 0
+    many = 1 << 30                                                  # (as many workgroups are 0 modulo 2^64)
+    assert lib.rwkv_attn_workspace_bytes(many, 2048, 2048, many, many, 64, 0, 1) == 0 and lib.rwkv_paged_workspace_bytes(many, many, many, 64, 16, 4096) == 0
