@@ -97,8 +97,25 @@ def visible(Tq, Tk, doc=None, prefix=None, causal=True, device="cpu"):
     return on
 
 
-def _head(q, k, v, on, dist, slope, cap, scale, do, dt):
-    """One head: y, its bound, and with do the four pieces of the gradients with theirs."""
+def _least_operands(v, dy, doc, dt):
+    """Half of the smallest step of the scores' gradients and of the weights as operands of one batch element, fp16.  The former are taken times a power of two that brings
+    the largest |dy| |v| + |dy.y| (lengths of rows) of queries and keys that are no padding to 2^14 .. 2^15; |dy.y| is at most |dy| times the largest |v|, to the roundings of y.  The
+    latter are taken times 2^8."""
+    if dt != torch.float16:
+        return TINY[dt], TINY[dt]
+
+    def longest(z, doc):
+        n = z.detach().double().norm(dim=-1)
+        n = n if doc is None else n[doc >= 0]
+        n = n[torch.isfinite(n)]
+        return float(n.max()) if n.numel() else 0.0
+    most = 2.02 * longest(dy, None if doc is None else doc[-dy.shape[0]:]) * longest(v, doc)
+    return TINY[dt] * most * 2.0 ** -14, TINY[dt] * 2.0 ** -8
+
+
+def _head(q, k, v, on, dist, slope, cap, scale, do, dt, least=(0.0, 0.0)):
+    """One head: y, its bound, and with do the four pieces of the gradients with theirs.  `least`: what the gradients of the scores and the weights may be off by as
+    operands of the gradients' products, beside their relative rounding."""
     u, tiny, N = UNIT[dt], TINY[dt], q.shape[1]
     lost = 2.0 ** -126                                         # a weight below fp32's least normal number may be lost whole
     raw = (q @ k.T) * scale
@@ -134,11 +151,11 @@ def _head(q, k, v, on, dist, slope, cap, scale, do, dt):
     # 1 - t^2: off by twice the tanh's error
     eds = p * t1 * (edp + edelta) + ds.abs() * rel + (p * (dp - delta).abs() * 24 * U32 if cap else 0.0) + lost * seen * (1 + (dp - delta).abs())
 
-    def back(w, ew, on, z):                                    # w @ z with w rounded to the type before
-        return w @ z, (u * w.abs() + ew + tiny * on) @ z.abs()
-    dq, eq = back(ds, eds, seen, k)
-    dk, ek = back(ds.T, eds.T, seen.T, q)
-    dv, ev = back(p.T, (p * rel + lost * seen).T, seen.T, do)
+    def back(w, ew, on, z, least):                             # w @ z with w rounded to the type before
+        return w @ z, (u * w.abs() + ew + least * on) @ z.abs()
+    dq, eq = back(ds, eds, seen, k, least[0])
+    dk, ek = back(ds.T, eds.T, seen.T, q, least[0])
+    dv, ev = back(p.T, (p * rel + lost * seen).T, seen.T, do, least[1])
     more = 8 * U32 * math.sqrt(max(on.shape))                  # the fp32 sums of the three products
     eq, ek, ev = eq + more * (ds.abs() @ k.abs()), ek + more * (ds.T.abs() @ q.abs()), ev + more * (p.T @ do.abs())
     return y, ey, (scale * dq, scale * eq), (scale * dk, scale * ek), (dv, ev)
@@ -157,10 +174,11 @@ def attention(q, k, v, doc=None, prefix=None, slopes=None, cap=0.0, scale=None, 
     dist = (torch.arange(Tk - Tq, Tk, device=q.device)[:, None] - torch.arange(Tk, device=q.device)[None, :]).abs().double()
     for b in range(B):
         on = visible(Tq, Tk, None if doc is None else doc[b], None if prefix is None else int(prefix[b]), causal, q.device)
+        least = (0.0, 0.0) if dy is None else _least_operands(v[b], dy[b], None if doc is None else doc[b], dt)
         for h in range(H):
             g = h * Hk // H
             r = _head(Q[b, :, h], K[b, :, g], V[b, :, g], on, dist, None if slopes is None else float(slopes[h]), cap, scale,
-                      None if dy is None else dy[b, :, h].double(), dt)
+                      None if dy is None else dy[b, :, h].double(), dt, least)
             y[0][b, :, h], y[1][b, :, h] = r[0], r[1]
             if dy is None:
                 continue

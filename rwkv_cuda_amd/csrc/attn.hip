@@ -45,7 +45,11 @@ AttnPlan attn_plan(int B, int Tq, int Tk, int H, int Hk, int N, bool doc) {
     a.q_order = order(a.q_items);
     a.k_order = order(a.k_items);
     a.forward = a.ranges + a.q_order + (a.query_parts > 1 ? static_cast<size_t>(B) * H * Tq * a.query_parts * (width + 4) * sizeof(float) : 0);
-    a.backward = a.ranges + a.q_order + a.k_order + (doc ? static_cast<size_t>(B) * blocks(Tq, 64) * sizeof(Range) : 0) + (static_cast<size_t>(B) * Tq * H * sizeof(float) + 15) / 16 * 16 +
+    // enough workgroups to fill the card, and few enough for each of attn_dkv to look at what they leave
+    a.delta_blocks = static_cast<int>(std::min(blocks(static_cast<int64_t>(Tq) * H, 2048 / width), blocks(2048, B)));
+    a.delta = (static_cast<size_t>(B) * Tq * H * sizeof(float) + 15) / 16 * 16;
+    a.lengths = (static_cast<size_t>(B) * a.delta_blocks * 2 * sizeof(float) + static_cast<size_t>(B) * Hk * blocks(Tk, a.eight ? 256 : 128) * sizeof(float) + 15) / 16 * 16;
+    a.backward = a.ranges + a.q_order + a.k_order + (doc ? static_cast<size_t>(B) * blocks(Tq, 64) * sizeof(Range) : 0) + a.delta + a.lengths +
                  (a.key_parts > 1 ? 2 * static_cast<size_t>(a.key_parts) * B * Tk * Hk * N * sizeof(float) : 0);
     return a;
 }

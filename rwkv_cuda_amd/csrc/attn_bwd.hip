@@ -13,6 +13,32 @@ namespace {
 template <class E> constexpr float SHIFT = std::is_same_v<E, bf16_t> ? 0.f : 8.f;
 template <class E> constexpr float UNSHIFT = std::is_same_v<E, bf16_t> ? 1.f : 1.f / 256.f;
 
+// The gradients of the scores as fp16 operands: with thousands of keys and gradients of y as training has them most would be below fp16's normal numbers, and large
+// gradients of y would bring them above its largest.  |ds| is at most |dy| |v| + |delta|, lengths of rows: attn_delta leaves the largest |dy| and |delta| of a batch element,
+// attn_dkv finds the largest |v| of its keys and leaves it for attn_dq, and the operands are taken times the power of two that brings that bound to 2^14 .. 2^15: none
+// overflows, and down to 2^-29 of the bound they keep all their bits.  Padding and rows that are not finite do not count.  dQ of 128 queries on 16384 keys, dy of 1e-3, against 64
+// bits: off by 2.1e-2 of its size without, 1.3e-3 so, which its own rounding is; the times are the same (B8 T4096 H32 N64 fp16 backward 2.27 ms and 2.26).
+template <class E> constexpr bool LIFTED = !std::is_same_v<E, bf16_t>;
+DEVINL float lift_of(const float bound) {
+    const int e = 14 - (static_cast<int>(__float_as_uint(bound) >> 23) - 127);
+    return __uint_as_float(static_cast<uint32_t>(min(max(e, -40), 100) + 127) << 23);
+}
+DEVINL float inverse_of(const float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }       // of a power of two
+// the sum of squares of a lane's part of a row and its partner's
+template <class E, int D> DEVINL float squares(const u32x4 (&x)[D / 16]) {
+    float s = 0.f;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s = fmaf(unpack_lo<E>(x[c][i]), unpack_lo<E>(x[c][i]), fmaf(unpack_hi<E>(x[c][i]), unpack_hi<E>(x[c][i]), s));
+    return s + other_half(s);
+}
+DEVINL float wave_max(float x) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) x = fmaxf(x, __shfl_xor(x, m, 64));
+    return x;
+}
+
 // lo .. hi of the documents of each tile's real tokens, and whether all of them are real (4 us at T3001: a launch)
 __global__ __launch_bounds__(256) void attn_ranges(const int* doc, const int T, const int first, const int tiles, Range* out) {
     const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, b = blockIdx.y;
@@ -55,26 +81,41 @@ __global__ __launch_bounds__(1024) void attn_order(const rwkv_attn_args p, const
     }
 }
 
-// delta = sum over the channels of dy y, y as the forward had it before it was rounded; a row has D / 8 lanes.  Bound by memory: B8 T4096 H32 N64 0.073 ms, 405 MB, 5.5 TB/s.
-template <class E, int D> __global__ __launch_bounds__(256) void attn_delta(const rwkv_attn_args p, float* delta) {
-    constexpr int LANES = D / 8;
-    const int64_t row = (blockIdx.x * wide(256) + threadIdx.x) / LANES, rows = wide(p.B) * p.Tq * p.H;
-    const int d = threadIdx.x % LANES * 8;
-    float s = 0.f;
-    if (row < rows && d < p.N) {
-        const u32x4 a = *reinterpret_cast<const u32x4*>(static_cast<const E*>(p.dy) + row * p.N + d), y = *reinterpret_cast<const u32x4*>(static_cast<const E*>(p.y) + row * p.N + d),
-                    z = *reinterpret_cast<const u32x4*>(static_cast<const E*>(p.y_rest) + row * p.N + d);
+// delta = sum over the channels of dy y, y as the forward had it before it was rounded; a row has D / 8 lanes.  fp16: and the largest |dy|^2 and |delta| of a workgroup's rows,
+// of one batch element (blockIdx.y).  Bound by memory: B8 T4096 H32 N64 bf16 0.073 ms, 405 MB, 5.5 TB/s.
+template <class E, int D> __global__ __launch_bounds__(256) void attn_delta(const rwkv_attn_args p, float* delta, float2* most) {
+    constexpr int LANES = D / 8, ROWS = 256 / LANES;
+    __shared__ float2 of_wave[4];
+    const int b = blockIdx.y, d = threadIdx.x % LANES * 8;
+    const int64_t rows = wide(p.Tq) * p.H, first = b * rows;
+    float longest = 0.f, largest = 0.f;
+    for (int64_t at = blockIdx.x * wide(ROWS); at < rows; at += gridDim.x * wide(ROWS)) {
+        const int64_t row = at + threadIdx.x / LANES;
+        float s = 0.f, n = 0.f;
+        if (row < rows && d < p.N) {
+            const int64_t o = (first + row) * p.N + d;
+            const u32x4 a = *reinterpret_cast<const u32x4*>(static_cast<const E*>(p.dy) + o), y = *reinterpret_cast<const u32x4*>(static_cast<const E*>(p.y) + o),
+                        z = *reinterpret_cast<const u32x4*>(static_cast<const E*>(p.y_rest) + o);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            s = fmaf(unpack_lo<E>(a[i]), unpack_lo<E>(y[i]) + unpack_lo<E>(z[i]), s);
-            s = fmaf(unpack_hi<E>(a[i]), unpack_hi<E>(y[i]) + unpack_hi<E>(z[i]), s);
+            for (int i = 0; i < 4; ++i) {
+                s = fmaf(unpack_lo<E>(a[i]), unpack_lo<E>(y[i]) + unpack_lo<E>(z[i]), s);
+                s = fmaf(unpack_hi<E>(a[i]), unpack_hi<E>(y[i]) + unpack_hi<E>(z[i]), s);
+                if constexpr (LIFTED<E>) n = fmaf(unpack_lo<E>(a[i]), unpack_lo<E>(a[i]), fmaf(unpack_hi<E>(a[i]), unpack_hi<E>(a[i]), n));
+            }
         }
+        s = group_sum<LANES>(s);
+        if constexpr (LIFTED<E>) {
+            n = group_sum<LANES>(n);
+            if (row < rows && n < INFINITY && fabsf(s) < INFINITY && (p.doc == nullptr || p.doc[wide(b) * p.Tk + p.Tk - p.Tq + row / p.H] >= 0)) longest = fmaxf(longest, n), largest = fmaxf(largest, fabsf(s));
+        }
+        if (row < rows && d == 0) delta[(wide(b) * p.H + row % p.H) * p.Tq + row / p.H] = s;
     }
-    s = group_sum<LANES>(s);
-    if (row < rows && d == 0) {
-        const int h = row % p.H;
-        const int64_t bi = row / p.H;
-        delta[(bi / p.Tq * p.H + h) * p.Tq + bi % p.Tq] = s;
+    if constexpr (LIFTED<E>) {
+        longest = wave_max(longest), largest = wave_max(largest);
+        if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = make_float2(longest, largest);
+        __syncthreads();
+        if (threadIdx.x == 0)
+            most[wide(b) * gridDim.x + blockIdx.x] = make_float2(fmaxf(fmaxf(of_wave[0].x, of_wave[1].x), fmaxf(of_wave[2].x, of_wave[3].x)), fmaxf(fmaxf(of_wave[0].y, of_wave[1].y), fmaxf(of_wave[2].y, of_wave[3].y)));
     }
 }
 
@@ -82,7 +123,7 @@ template <class E, int D> __global__ __launch_bounds__(256) void attn_delta(cons
 // Three waves a SIMD with heads of 64, for 1 to 8 spilled registers where there is a bias (B8 T4096 H32 N64 with slopes, forward + backward 3.135 -> 3.086 ms).  The halves of
 // a tile interleaved: one after the other, with four waves, is slower (2.77 -> 2.85 ms; heads of 128, two waves, dQ 1.91 -> 2.11).
 template <class E, int D, bool CAP, bool BIAS, bool DOC>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_dq(const rwkv_attn_args p, const float* delta, const Range* ranges, const int* order, const int blocks_q, const int per_xcd) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_dq(const rwkv_attn_args p, const float* delta, const float* v_most, const int blocks_k, const Range* ranges, const int* order, const int blocks_q, const int per_xcd) {
     constexpr int QB = 128;
     constexpr int PLANES = 4 * Plane<D>::BYTES;
     constexpr int SLOPE_VALUS = 4 + (CAP ? 6 : 0) + (BIAS ? 2 : 0), SLOPE_TRANS = CAP ? 3 : 1;      // instructions of a pair
@@ -115,7 +156,14 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_dq(const rwkv_attn_
     const int lim = !real || qdoc < 0 ? -1 : (p.causal ? max(shift + i, reach) : p.Tk - 1);
     const float pos = static_cast<float>(shift + i);
     const int64_t stat = (wide(b) * p.H + h) * p.Tq + (real ? i : 0);
-    const float lse = lim >= 0 ? p.lse[stat] : INFINITY, dlt = lim >= 0 ? delta[stat] : 0.f;
+    const float lse = lim >= 0 ? p.lse[stat] : INFINITY;
+    float dlt = lim >= 0 ? delta[stat] : 0.f, lift = 1.f;       // fp16: of the lane's query; dlt times it
+    if constexpr (LIFTED<E>) {
+        float v = 0.f;
+        for (int x = lane; x < blocks_k; x += 64) v = fmaxf(v, v_most[(wide(b) * p.Hk + hk) * blocks_k + x]);
+        lift = lift_of(fmaf(__builtin_sqrtf(squares<E, D>(dy)), wave_max(v), fabsf(dlt)));
+        dlt *= lift;
+    }
     const int row_lo = q0 + __builtin_amdgcn_readfirstlane(wave) * 32;
     // the last key that all of the wave's queries see, and one that none behind sees
     const int lim_lo = __ballot(lim < 0) != 0ull ? -1 : (p.causal ? max(shift + row_lo, reach) : p.Tk - 1);
@@ -166,7 +214,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_dq(const rwkv_attn_
         for (int r = 0; r < 16; ++r) {
             const float x = s[r], sq = sc.squash<CAP>(x);
             const float t = LINE ? fmaf(x, sc.unit, fmaf(sc.slope, 8 * (r >> 2) + (r & 3), base)) : fmaf(sc.t<CAP, BIAS>(x, sq, dist - (8 * (r >> 2) + (r & 3))), mul, -lse);
-            float ds = __builtin_amdgcn_exp2f(t) * (dp[r] - dlt);
+            float ds = __builtin_amdgcn_exp2f(t) * (LIFTED<E> ? fmaf(dp[r], lift, -dlt) : dp[r] - dlt);
             if constexpr (CAP) ds *= 4.f * sq * (1.f - sq);
             s[r] = ds;
         }
@@ -240,7 +288,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_dq(const rwkv_attn_
         par ^= 1;
     }
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d) store32<E>(g[d], p.scale, static_cast<E*>(p.dq) + row, nullptr, 32 * d, p.N, real);
+    for (int d = 0; d < D / 32; ++d) store32<E>(g[d], LIFTED<E> ? p.scale * inverse_of(lift) : p.scale, static_cast<E*>(p.dq) + row, nullptr, 32 * d, p.N, real);
 }
 
 // dK, dV: 4 waves of 32 keys over the queries, of all heads that share them, that see any of them; S = Q K^T and dP = dY V^T,
@@ -253,10 +301,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_dq(const rwkv_attn_
 // documents (8 to 22 registers spilled): B8 T4096 H32 N64 forward + backward, with the halves interleaved and two waves, and so: plain 2.96 / 2.81 ms, with slopes 3.08 / 2.97,
 // with a cap 4.16 / 3.97; with documents the same to 2 percent.
 template <class E, int D, int WAVES, bool CAP, bool BIAS, bool DOC>
-__global__ __launch_bounds__(64 * WAVES, D == 128 ? (WAVES == 4 ? 1 : 2) : DOC ? 2 : 3) void attn_dkv(const rwkv_attn_args p, const float* delta, const Range* key_ranges, const Range* ranges, const int* order, const int blocks_k, const int per_xcd, const int parts, float* part) {
+__global__ __launch_bounds__(64 * WAVES, D == 128 ? (WAVES == 4 ? 1 : 2) : DOC ? 2 : 3) void attn_dkv(const rwkv_attn_args p, const float* delta, const float2* most, const int delta_blocks, float* v_most, const Range* key_ranges, const Range* ranges, const int* order, const int blocks_k, const int per_xcd, const int parts, float* part) {
     constexpr int KB = 32 * WAVES, PLANES = 4 * Plane<D>::BYTES, VALUES = D == 128 ? KB / TILE * Plane<D>::BYTES : 0;
-    // two planes of queries and of dY (below 64 KB: what M0 can name), lse, delta and documents of two tiles, the values of the block's keys
-    __shared__ __align__(16) char smem[PLANES + 6 * 4 * TILE + VALUES];
+    // two planes of queries and of dY (below 64 KB: what M0 can name), lse, delta and documents of two tiles, the values of the block's keys, three lengths of each wave
+    __shared__ __align__(16) char smem[PLANES + 6 * 4 * TILE + VALUES + (LIFTED<E> ? 3 * 4 * WAVES : 0)];
     float *const row_lse = reinterpret_cast<float*>(smem + PLANES), *const row_delta = row_lse + 2 * TILE;
     int* const row_doc = reinterpret_cast<int*>(row_delta + 2 * TILE);
     const int id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
@@ -309,6 +357,30 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? (WAVES == 4 ? 1 : 2) : DOC ?
     const lds_t values = lds + PLANES + 6 * 4 * TILE + wave / 2 * Plane<D>::BYTES;
     const RowReader<D> vrows(lane);
     const Fetch<D, WAVES> fetch(tid, p.N);
+    float lift = 1.f;                                            // fp16: of the block's keys
+    if constexpr (LIFTED<E>) {
+        float* const of_wave = reinterpret_cast<float*>(smem + PLANES + 6 * 4 * TILE + VALUES);
+        u32x4 x[D / 16];
+        if constexpr (D == 128) __syncthreads();
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) x[c] = D == 64 ? v[D == 64 ? c : 0] : vrows(values, wave & 1, c);
+        float n = squares<E, D>(x), longest = 0.f, largest = 0.f;
+        n = wave_max(real && kdoc >= 0 && n < INFINITY ? n : 0.f);
+        for (int i = tid; i < delta_blocks; i += 64 * WAVES) {
+            const float2 z = most[wide(b) * delta_blocks + i];
+            longest = fmaxf(longest, z.x), largest = fmaxf(largest, z.y);
+        }
+        longest = wave_max(longest), largest = wave_max(largest);
+        if (lane == 0) of_wave[3 * wave] = n, of_wave[3 * wave + 1] = longest, of_wave[3 * wave + 2] = largest;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) n = fmaxf(n, of_wave[3 * i]), longest = fmaxf(longest, of_wave[3 * i + 1]), largest = fmaxf(largest, of_wave[3 * i + 2]);
+        n = __builtin_sqrtf(n);
+        if (tid == 0 && mine == 0) v_most[(wide(b) * p.Hk + hk) * blocks_k + k0 / KB] = n;
+        lift = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(lift_of(fmaf(__builtin_sqrtf(longest), n, largest)))));
+    }
+    // 2^-SHIFT lift: to the gradients of the scores, from 2^SHIFT times the weights (by the exponent, in a scalar register)
+    const float down = __uint_as_float(__float_as_uint(lift) - (static_cast<uint32_t>(SHIFT<E>) << 23));
     f32x16 gk[D / 32], gv[D / 32];
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) gk[d] = gv[d] = f32x16{};
@@ -333,7 +405,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? (WAVES == 4 ? 1 : 2) : DOC ?
         if (tid < TILE) {
             const bool off = t * TILE + tid >= p.Tq || next_lse == -INFINITY;            // a row that is not there or sees nothing: weights of 0
             row_lse[slot * TILE + tid] = off ? INFINITY : (LINE ? fmaf(slope, tid, next_lse) : next_lse) - SHIFT<E>;      // with the query's part of the bias
-            row_delta[slot * TILE + tid] = off ? 0.f : next_delta * UNSHIFT<E>;
+            row_delta[slot * TILE + tid] = off ? 0.f : next_delta * down;
             if (DOC) row_doc[slot * TILE + tid] = next_doc;
         }
     };
@@ -361,7 +433,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? (WAVES == 4 ? 1 : 2) : DOC ?
                 const float x = s[at], sq = sc.squash<CAP>(x);
                 const float t = LINE ? fmaf(x, sc.unit, base - lse[r]) : fmaf(sc.t<CAP, BIAS>(x, sq, dist + (8 * n + r)), mul, -lse[r]);
                 const float w = __builtin_amdgcn_exp2f(t);
-                float ds = w * (SHIFT<E> == 0.f ? dp[at] - dlt[r] : fmaf(dp[at], UNSHIFT<E>, -dlt[r]));
+                float ds = w * (SHIFT<E> == 0.f ? dp[at] - dlt[r] : fmaf(dp[at], down, -dlt[r]));
                 if constexpr (CAP) ds *= 4.f * sq * (1.f - sq);
                 s[at] = w;
                 dp[at] = ds;
@@ -441,6 +513,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? (WAVES == 4 ? 1 : 2) : DOC ?
         par ^= 1;
     }
     const int64_t row = ((wide(b) * p.Tk + (real ? j : 0)) * p.Hk + hk) * p.N;
+    const float back = LIFTED<E> ? inverse_of(lift) : 1.f;
     if (parts > 1) {
         const int64_t size = wide(p.B) * p.Tk * p.Hk * p.N;
         float* to = part + 2 * mine * size + row;
@@ -450,14 +523,14 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? (WAVES == 4 ? 1 : 2) : DOC ?
             for (int n = 0; n < 4; ++n) {
                 const int c = 32 * d + 8 * n + 4 * hi;
                 if (!real || c >= p.N) continue;
-                *reinterpret_cast<float4*>(to + c) = make_float4(gk[d][4 * n], gk[d][4 * n + 1], gk[d][4 * n + 2], gk[d][4 * n + 3]);
+                *reinterpret_cast<float4*>(to + c) = make_float4(gk[d][4 * n] * back, gk[d][4 * n + 1] * back, gk[d][4 * n + 2] * back, gk[d][4 * n + 3] * back);
                 *reinterpret_cast<float4*>(to + size + c) = make_float4(gv[d][4 * n], gv[d][4 * n + 1], gv[d][4 * n + 2], gv[d][4 * n + 3]);
             }
         return;
     }
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) {
-        store32<E>(gk[d], p.scale, static_cast<E*>(p.dk) + row, nullptr, 32 * d, p.N, real);
+        store32<E>(gk[d], p.scale * back, static_cast<E*>(p.dk) + row, nullptr, 32 * d, p.N, real);
         store32<E>(gv[d], UNSHIFT<E>, static_cast<E*>(p.dv) + row, nullptr, 32 * d, p.N, real);
     }
 }
@@ -478,18 +551,20 @@ template <class E> __global__ __launch_bounds__(256) void attn_dkv_sum(const rwk
 }
 
 template <class E, int D> int run(hipStream_t st, const rwkv_attn_args& p) {
-    const int64_t rows = wide(p.B) * p.Tq * p.H, row_blocks = (rows * (D / 8) + 255) / 256;
     const AttnPlan plan = attn_plan(p.B, p.Tq, p.Tk, p.H, p.Hk, p.N, p.doc != nullptr);
+    const int64_t row_blocks = LIFTED<E> ? plan.delta_blocks : (wide(p.Tq) * p.H * (D / 8) + 255) / 256;
     const bool eight = plan.eight;
     const int blocks_q = (p.Tq + 127) / 128, blocks_k = eight ? (p.Tk + 255) / 256 : (p.Tk + 127) / 128;
     const int64_t per_q = (wide(blocks_q) * p.H * p.B + 7) / 8, per_k = (wide(blocks_k) * plan.key_parts * p.Hk * p.B + 7) / 8;
     const int64_t sums = (wide(p.B) * p.Tk * p.Hk * p.N / 8 + 255) / 256;
     if (row_blocks > INT_MAX || per_q * 8 > INT_MAX || per_k * 8 > INT_MAX || (plan.key_parts > 1 && sums > INT_MAX)) return RWKV_ERR_SHAPE;
-    // the documents of tiles of keys and of tiles of queries, the orders, delta, the sums of groups of heads
+    // the documents of tiles of keys and of tiles of queries, the orders, delta, the largest lengths, the sums of groups of heads
     Range *key_ranges = static_cast<Range*>(p.workspace), *ranges = key_ranges + (p.doc ? p.B * tiles_of(p.Tk) : 0);
     char* at = reinterpret_cast<char*>(ranges + (p.doc ? p.B * tiles_of(p.Tq) : 0));
     int *q_order = plan.q_items > 0 ? reinterpret_cast<int*>(at) : nullptr, *k_order = plan.k_items > 0 ? reinterpret_cast<int*>(at + plan.q_order) : nullptr;
     float* delta = reinterpret_cast<float*>(at + plan.q_order + plan.k_order);
+    float2* most = reinterpret_cast<float2*>(reinterpret_cast<char*>(delta) + plan.delta);
+    float* v_most = reinterpret_cast<float*>(most + wide(p.B) * plan.delta_blocks);
     float* part = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + plan.backward) - (plan.key_parts > 1 ? 2 * plan.key_parts * wide(p.B) * p.Tk * p.Hk * p.N : 0);
     if (p.doc) {
         launch_attn_ranges(st, p.doc, p.B, p.Tk, 0, key_ranges);
@@ -497,11 +572,11 @@ template <class E, int D> int run(hipStream_t st, const rwkv_attn_args& p) {
         else launch_attn_ranges(st, p.doc, p.B, p.Tk, p.Tk - p.Tq, ranges);
         if (q_order || k_order) launch_attn_order(st, p, key_ranges, ranges, plan, q_order, k_order);
     }
-    hipLaunchKernelGGL((attn_delta<E, D>), dim3(static_cast<unsigned>(row_blocks)), dim3(256), 0, st, p, delta);
+    hipLaunchKernelGGL((attn_delta<E, D>), dim3(static_cast<unsigned>(row_blocks), p.B), dim3(256), 0, st, p, delta, most);
     const auto go = [&](auto dq, auto dkv) {
-        hipLaunchKernelGGL(dkv, dim3(static_cast<unsigned>(per_k * 8)), dim3(eight ? 512 : 256), 0, st, p, delta, key_ranges, ranges, k_order, blocks_k, static_cast<int>(per_k), plan.key_parts, part);
+        hipLaunchKernelGGL(dkv, dim3(static_cast<unsigned>(per_k * 8)), dim3(eight ? 512 : 256), 0, st, p, delta, most, plan.delta_blocks, v_most, key_ranges, ranges, k_order, blocks_k, static_cast<int>(per_k), plan.key_parts, part);
         if (plan.key_parts > 1) hipLaunchKernelGGL((attn_dkv_sum<E>), dim3(static_cast<unsigned>(sums), 2), dim3(256), 0, st, p, plan.key_parts, part);
-        hipLaunchKernelGGL(dq, dim3(static_cast<unsigned>(per_q * 8)), dim3(256), 0, st, p, delta, key_ranges, q_order, blocks_q, static_cast<int>(per_q));
+        hipLaunchKernelGGL(dq, dim3(static_cast<unsigned>(per_q * 8)), dim3(256), 0, st, p, delta, v_most, blocks_k, key_ranges, q_order, blocks_q, static_cast<int>(per_q));
         return launch_status();
     };
     const auto masks = [&](auto cap, auto bias) {

@@ -34,7 +34,9 @@ struct AttnPlan {
     int query_parts, key_parts;
     bool eight;                                                 // heads of 128: 256 keys a workgroup of attn_dkv
     int q_items, k_items;                                       // blocks of queries, of keys, that are ordered by their work (0: they are not)
+    int delta_blocks;                                           // workgroups of attn_delta for a batch element, fp16, each of which leaves its largest lengths
     size_t ranges, q_order, k_order, forward, backward;         // bytes: documents of tiles; the orders; workspace of either direction
+    size_t delta, lengths;                                      // ... of delta; of the largest lengths of gradients and of values
 };
 constexpr int MAX_ORDER = 1024;
 AttnPlan attn_plan(int B, int Tq, int Tk, int H, int Hk, int N, bool doc);

@@ -269,3 +269,63 @@ def test_prefixes_below_zero_are_none(lib, doc):
     for low in (at(-1, -64, -65), at(-2 ** 31, -2 ** 31 + 1, -2 ** 31 + 63)):
         for n, a, b in zip(["y", "dq", "dk", "dv"], passes(q, k, v, dy, prefix=low, **how), want):
             assert torch.equal(a, b), n
+
+
+@pytest.mark.parametrize("Tq,Tk,H,Hk,N,how", [(200, 4096, 2, 1, 64, {}), (64, 16384, 2, 2, 64, {}), (130, 4096, 4, 1, 128, {}), (64, 16384, 2, 1, 96, dict(cap=30.0)), (4096, 4096, 1, 1, 64, {})])
+@pytest.mark.parametrize("up", [1e-2, 1e-3])
+def test_small_gradients_over_many_keys(lib, Tq, Tk, H, Hk, N, how, up):
+    """fp16: gradients of scores far below the type's normal numbers, for gradients of y as they are in training."""
+    q, k, v, dy = inputs(1, Tq, Tk, H, Hk, N, torch.float16, seed=101)
+    check(q, k, v, (dy.float() * up).half(), **how)
+
+
+@pytest.mark.parametrize("Tq,Tk,H,Hk,N", [(300, 300, 2, 1, 64), (150, 2000, 4, 2, 128), (64, 4096, 2, 2, 64)])
+def test_large_gradients(lib, Tq, Tk, H, Hk, N):
+    """fp16: gradients of scores beyond the type's largest number, where those of q, k and v are not.  (The first shape's reach 1.2e5 in 64 bits: from 65520 on, half a step
+    above 65504, a value rounds to infinity in fp16.)"""
+    q, k, v, dy = inputs(1, Tq, Tk, H, Hk, N, torch.float16, seed=105)
+    got = passes(q, k, v * 4, dy * 1e4)
+    want = O.attention(q, k, v * 4, dy=dy * 1e4)
+    for n, z in zip(["y", "dq", "dk", "dv"], got):
+        value, bound = want[n]
+        above, below = value.abs() - bound > 65520, value.abs() + bound < 65520
+        assert torch.equal(z[above].float(), torch.sign(value[above]).float() * torch.inf), n
+        within(n, z[below], (value[below], bound[below]))
+        assert below.float().mean() > 0.99
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), 65504.0])
+def test_padding_of_any_value_reaches_nothing_in_fp16(lib, value):
+    B, T, H, Hk, N = 2, 400, 4, 2, 128
+    q, k, v, dy = inputs(B, T, T, H, Hk, N, torch.float16, seed=109)
+    doc = doc_ids(B, T, "padded", seed=3).to(DEV)
+    doc[1, 60:], doc[1, 200:] = 4, -1
+    results = []
+    for x in (0.0, value):
+        t = [z.masked_fill((doc < 0)[:, :, None, None], x).requires_grad_(True) for z in (q, k, v)]
+        y = A.RUN_CUDA(*t, doc=doc)
+        results.append([y.detach()] + list(torch.autograd.grad([y], t, [(dy * 1e-3).masked_fill((doc < 0)[:, :, None, None], x)])))
+    for n, a, b in zip(["y", "dq", "dk", "dv"], *results):
+        assert torch.equal(a, b), n
+
+
+def test_fp16_rows_on_their_own_and_in_graphs(lib):
+    """Gradients of different sizes in the elements of a batch; the same bits every time, in a graph too."""
+    q, k, v, dy = inputs(3, 333, 333, 4, 2, 64, torch.float16, seed=113)
+    dy = dy * torch.tensor([1.0, 1e-4, 300.0], device=DEV).half().view(3, 1, 1, 1)
+    t = [z.detach().clone().requires_grad_(True) for z in (q, k, v)]
+
+    def once(q, k, v, dy):
+        y = A.RUN_CUDA(q, k, v)
+        return [y.detach()] + list(torch.autograd.grad([y], [q, k, v], [dy]))
+    graph, out = graph_of(lambda: once(*t, dy))
+    for i in range(4):
+        with torch.no_grad():
+            dy.mul_(0.5), t[2].copy_(randn(*v.shape, seed=120 + i, scale=2.0 ** i).half())
+        want = [z.clone() for z in once(*t, dy)]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, out)), i
+    for b in range(3):
+        alone = [z[b:b + 1].detach().requires_grad_(True) for z in t]
+        assert all(torch.equal(a[b:b + 1], c) for a, c in zip(want, once(*alone, dy[b:b + 1])))
