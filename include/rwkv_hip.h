@@ -574,6 +574,7 @@ enum { RWKV_GATE_SIGMOID = 0, RWKV_GATE_LOG = 1 };
  * a_t = sigmoid(w_t) or exp(w_t) (gate), u_t = (1 - a_t) x_t (tied) or x_t.  h_{-1} is h0, or 0 where that is NULL.
  * doc (may be NULL): a token with doc < 0 is padding, y is 0 there and the state passes by it; a real token whose predecessor has
  * another doc starts from a state of 0.  w, x, y (and dy, dw, dx) are of `dtype`, states are fp32; h0 and hT may be the same memory.
+ * Gates are multiplied over runs of tokens in fp32: a product beyond its largest number (log gates above 0) is an infinity to every state but 0.
  * The forward keeps in `saved` (may be NULL) what the backward needs beside w, x and doc; both may need a workspace. */
 typedef struct rwkv_grec_args {
     int dtype, gate, tied;

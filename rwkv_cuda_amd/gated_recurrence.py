@@ -3,7 +3,10 @@
     h_t = a_t h_{t-1} + u_t,  y_t = h_t        a = sigmoid(w) or exp(w),  u = (1 - a) x (tied) or x
 
 `doc` [B,T] int32 names the document of each token of a packed or padded batch, as for attention.RUN_CUDA: where it changes, a
-document starts from a state of zero; a negative one is padding, whose y is 0 and which the state passes by."""
+document starts from a state of zero; a negative one is padding, whose y is 0 and which the state passes by.
+
+Gates are multiplied over runs of up to T tokens in fp32.  With log gates above 0 such a product may exceed it, and is then an infinity to every
+state but one of exactly zero."""
 
 import torch
 

@@ -218,3 +218,19 @@ def test_a_tensor_of_more_than_2_31_elements(lib):
     y, hT = G.RUN_CUDA(w.contiguous(), x)
     want = G.RUN_CUDA(w[:, :, -64:].contiguous(), x[:, :, -64:])
     assert torch.equal(y[:, :, -64:], want[0]) and torch.equal(hT[:, -64:], want[1]) and not y[:, :, :64].any()
+
+
+@pytest.mark.parametrize("B,T,C", [(1, 129, 64), (2, 1300, 40), (9, 300, 3650), (1, 30, 66)])
+@pytest.mark.parametrize("tied", [False, True])
+def test_growth_of_nothing_is_nothing(lib, B, T, C, tied):
+    """Log gates above 0 over many tokens, on a state of zero and on gradients of zero: their product is beyond fp32, the results are not."""
+    w = torch.full((B, T, C), 1.0 if T > 60 else 20.0, device=DEV)
+    w[:, T // 2:T // 2 + 8] = 15.0
+    x = torch.zeros(B, T, C, device=DEV)
+    x[:, -3:] = randn(B, 3, C, seed=1).to(DEV)
+    dy = torch.zeros(B, T, C, device=DEV)
+    dy[:, :2] = randn(B, 2, C, seed=2).to(DEV)
+    check(w, x, torch.zeros(B, C, device=DEV), None, "log", tied, dy, None)
+    doc = torch.zeros(B, T, dtype=torch.int32, device=DEV)
+    doc[:, T // 3:], doc[:, T // 3 + 5:T // 3 + 9] = 1, -1
+    check(w, x, None, doc, "log", tied, dy, torch.zeros(B, C, device=DEV))
