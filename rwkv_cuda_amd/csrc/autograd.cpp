@@ -525,6 +525,10 @@ bool touch(const Tensor& a, const Tensor& b) {
     const auto s = span(a), t = span(b);
     return s.first < t.second && t.first < s.second;
 }
+// torch refuses to raise an inference tensor's version outside of inference mode: found out before the kernel writes it
+void check_writable(const Tensor& x, const char* n) {
+    require(!x.is_inference() || c10::InferenceMode::is_enabled(), std::string(n) + " is an inference tensor: it can be written in inference mode only");
+}
 // a tensor that a kernel writes: a graph that has saved it finds out
 void written(const Tensor& x) { x.unsafeGetTensorImpl()->bump_version(); }
 void once_only(const char* n) {
@@ -597,6 +601,7 @@ Tensor grec_step_op(const Tensor& w, const Tensor& x, const Tensor& h, const Ten
     check_rows({{&w, "w"}, {&x, "x"}}, w);
     check_side(h, "h", F32, w.sizes(), w);
     check_side(out, "out", F32, w.sizes(), w);
+    check_writable(out, "the new state");
     require(!touch(out, w) && !touch(out, x) && (out.data_ptr() == h.data_ptr() || !touch(out, h)), "out must be h, or share no memory with w, x and h");
     const Guard guard(w.device());
     rwkv_grec_args a = grec_args(w3, x3, gate, tied);
@@ -700,6 +705,7 @@ Tensor paged_op(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tenso
     require(k.defined() == v.defined(), "k and v go together");
     check_side(k, "k", q.scalar_type(), {B, Hk, N}, q);
     check_side(v, "v", q.scalar_type(), {B, Hk, N}, q);
+    if (k.defined()) check_writable(kp, "k_pages"), check_writable(vp, "v_pages");
     require(cap == 0.0 || (cap >= 0x1p-20 && cap <= 4096.0), "cap must be 0, or from 2^-20 to 4096");
     const Guard guard(q.device());
     rwkv_paged_args a{};

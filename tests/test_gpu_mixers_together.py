@@ -166,3 +166,21 @@ def test_document_ids_at_their_ends(lib):
         z, y = layers(w, x, doc, slopes)
     within("z", z, O.gated_recurrence(w, x, doc=doc)["y"])
     within("y", y, O.attention(*qkv(z), doc=doc, slopes=slopes, cap=20.0)["y"])
+
+
+def test_inference_tensors_are_not_written_outside_of_inference_mode(lib):
+    """torch refuses to write them there, and so do these; nothing has been written when they do."""
+    with torch.inference_mode():
+        h = torch.ones(2, C, device=DEV)
+        kp, vp = (torch.zeros(2, 16, HK, N, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    w, x, _ = some(2, 3, torch.float32, 71)
+    z = torch.ones(2, HK, N, device=DEV, dtype=torch.bfloat16)
+    table, lens = torch.tensor([[0], [1]], dtype=torch.int32, device=DEV), torch.ones(2, dtype=torch.int32, device=DEV)
+    with torch.no_grad():
+        for call in (lambda: G.STEP(w[:, 0], x[:, 0], h), lambda: G.STEP(w[:, 0], x[:, 0], torch.zeros(2, C, device=DEV), out=h),
+                     lambda: PA.RUN_CUDA(z, kp, vp, table, lens, k=z, v=z), lambda: PA.RUN_CUDA(z, kp.clone(), vp, table, lens, k=z, v=z)):
+            with pytest.raises(AssertionError, match="inference"):
+                call()
+        torch.cuda.synchronize()
+        assert bool((h == 1).all()) and not kp.any() and not vp.any()
+        PA.RUN_CUDA(z, kp, vp, table, lens)                          # reading is another matter
