@@ -607,7 +607,8 @@ int rwkv_grec_backward(void* stream, const rwkv_grec_args* args);
  * all of them, or with `causal` those with j <= p or j < prefix[b]; with doc only those of the query's own doc, and none where that is
  * negative.  A query that sees nothing has y = 0.  N is a multiple of 8 up to 128; q, k, v are bf16 or fp16, 16-byte aligned with strides
  * that are multiples of 8.  y_rest (may be NULL): what y lost when it was rounded, for the backward; lse: base-2 logarithm of the sum of
- * exp(s), [B,H,Tq].  No token's stride is 2^24 elements or more; cap is 0 or from 2^-20 to 4096; with slopes Tk is at most 2^24.
+ * exp(s), [B,H,Tq].  No token's stride is 2^24 elements or more; cap is 0 or from 2^-20 to 4096; scale is at most 2^60; with slopes scale is
+ * at least 2^-60 and Tk at most 2^24.
  * What stands in padding counts nowhere; a NaN or an infinity in a real token may reach any row of its batch element and head. */
 typedef struct rwkv_attn_args {
     int dtype, causal;

@@ -24,5 +24,5 @@ class ATTENTION(torch.autograd.Function):
 
 
 def RUN_CUDA(q, k, v, doc=None, prefix=None, slopes=None, cap=0.0, scale=None, causal=True):
-    """cap 0: scores are not capped, else from 2^-20 to 4096; scale None: 1 / sqrt(N)."""
+    """cap 0: scores are not capped, else from 2^-20 to 4096; scale None: 1 / sqrt(N), else above 0 up to 2^60 and, with slopes, from 2^-60."""
     return ATTENTION.apply(q, k, v, doc, prefix, slopes, cap, scale, causal)

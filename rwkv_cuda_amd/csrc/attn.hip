@@ -60,7 +60,7 @@ int check_attn(const rwkv_attn_args* p, bool backward) {
     if (p == nullptr) return RWKV_ERR_NULL;
     if ((p->dtype != RWKV_DTYPE_BF16 && p->dtype != RWKV_DTYPE_FP16) || p->B <= 0 || p->Tq <= 0 || p->Tk < p->Tq || p->H <= 0 || p->Hk <= 0 || p->H % p->Hk != 0 ||
         p->N <= 0 || p->N > 128 || p->N % 8 != 0 || p->B > 65535 || p->H > 65535 || wide_rows(*p) || !scores_ok(p->scale, p->cap) || p->Tk > INT_MAX - 65536 ||
-        (p->slopes != nullptr && p->Tk > 1 << 24) || (p->prefix != nullptr && !p->causal)) return RWKV_ERR_SHAPE;
+        (p->slopes != nullptr && (p->Tk > 1 << 24 || p->scale < 0x1p-60f)) || (p->prefix != nullptr && !p->causal)) return RWKV_ERR_SHAPE;
     if (!multiples_of_8({p->q_sb, p->q_st, p->q_sh, p->k_sb, p->k_st, p->k_sh, p->v_sb, p->v_st, p->v_sh})) return RWKV_ERR_ALIGN;
     if (const int rc = check_ptrs({p->q, p->k, p->v, p->y})) return rc;
     if (backward) {

@@ -683,6 +683,7 @@ Tensor attention_op(const Tensor& q, const Tensor& k, const Tensor& v, const May
     require(cap == 0.0 || (cap >= 0x1p-20 && cap <= 4096.0), "cap must be 0, or from 2^-20 to 4096");
     const float sc = scale_of(scale, N);
     require(sc > 0.f && std::isfinite(sc), "scale must be positive");
+    require(!slopes.has_value() || sc >= 0x1p-60f, "with slopes scale must be at least 2^-60");
     require(!slopes.has_value() || !wants_grad({&*slopes}), "slopes have no gradient");
     return Attn::apply(q, k, v, doc, prefix, slopes, cap, static_cast<double>(sc), causal, wants_grad({&q, &k, &v}));
 }

@@ -329,3 +329,16 @@ def test_fp16_rows_on_their_own_and_in_graphs(lib):
     for b in range(3):
         alone = [z[b:b + 1].detach().requires_grad_(True) for z in t]
         assert all(torch.equal(a[b:b + 1], c) for a, c in zip(want, once(*alone, dy[b:b + 1])))
+
+
+@pytest.mark.parametrize("how", [dict(causal=False), dict(prefix=True), dict(cap=3.0, causal=False)])
+def test_slopes_with_the_smallest_scale(lib, how):
+    """Scores of nothing but the bias, on both sides of a query; a smaller scale is refused where there are slopes."""
+    q, k, v, dy = inputs(2, 150, 150, 4, 2, 64, torch.bfloat16, seed=131)
+    slopes = torch.exp2(-torch.arange(1.0, 5.0)).to(DEV)
+    if "prefix" in how:
+        how = dict(prefix=torch.tensor([100, 7], dtype=torch.int32, device=DEV))
+    check(q, k, v, dy, slopes=slopes, scale=2.0 ** -60, **how)
+    with pytest.raises(AssertionError, match="scale"):
+        A.RUN_CUDA(q, k, v, slopes=slopes, scale=2.0 ** -61, **how)
+    check(q, k, v, dy, scale=2.0 ** -61, **how)

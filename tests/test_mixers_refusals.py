@@ -182,3 +182,10 @@ def test_sizes_of_workspaces_for_heads_that_do_not_fit(lib):
     assert lib.rwkv_attn_workspace_bytes(1, 4, 4, 1, 2, 64, 0, 1) == 0
     many = 1 << 30                                                  # (as many workgroups are 0 modulo 2^64)
     assert lib.rwkv_attn_workspace_bytes(many, 2048, 2048, many, many, 64, 0, 1) == 0 and lib.rwkv_paged_workspace_bytes(many, many, many, 64, 16, 4096) == 0
+
+
+def test_slopes_and_the_smallest_scale(lib):
+    """Biases are divided by the scale: below 2^-60 they would be infinities."""
+    for call in (lib.rwkv_attn_forward, lib.rwkv_attn_backward):
+        assert call(None, _attn(slopes=P, scale=2.0 ** -61)) == -1 and call(None, _attn(slopes=P, scale=1e-45)) == -1
+        assert call(None, _attn(slopes=P, scale=2.0 ** -60, q=None)) == -2 and call(None, _attn(scale=2.0 ** -61, q=None)) == -2
