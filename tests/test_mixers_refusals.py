@@ -189,3 +189,12 @@ def test_slopes_and_the_smallest_scale(lib):
     for call in (lib.rwkv_attn_forward, lib.rwkv_attn_backward):
         assert call(None, _attn(slopes=P, scale=2.0 ** -61)) == -1 and call(None, _attn(slopes=P, scale=1e-45)) == -1
         assert call(None, _attn(slopes=P, scale=2.0 ** -60, q=None)) == -2 and call(None, _attn(scale=2.0 ** -61, q=None)) == -2
+
+
+def test_calls_that_need_a_workspace_have_one(lib):
+    """The sizes for which a small or missing workspace is refused are sizes above 0, and short calls need none."""
+    n, m = lib.rwkv_grec_workspace_bytes(1, 1 << 16, 64), lib.rwkv_paged_workspace_bytes(1, 2, 1, 64, 16, 4096)
+    assert n > 0 and m > 0 and lib.rwkv_grec_workspace_bytes(2, 8, 4) == 0 and lib.rwkv_paged_workspace_bytes(1, 2, 1, 64, 16, 2) == 0
+    for ws in (dict(workspace=None), dict(workspace=P + 8)):
+        assert lib.rwkv_grec_forward(None, _grec(B=1, T=1 << 16, C=64, **ws)) == -4 and lib.rwkv_paged_attn(None, _paged(M=4096, **ws)) == -4
+    assert lib.rwkv_grec_forward(None, _grec(B=1, T=1 << 16, C=64, workspace_bytes=n - 1)) == -4 and lib.rwkv_paged_attn(None, _paged(M=4096, workspace_bytes=m - 1)) == -4
