@@ -50,7 +50,7 @@ SPILL_LIMIT = {"wkv6_local": 0, "wkv6_bwd_fused": 0, "wkv6_fwd_fused": 0, "wkv6_
                "wkv4_bwd_blkILb1ELi8E": 0, "wkv4_bwd_blkILb0ELi16E": 5, "wkv4_bwd_blkILb1ELi16E": 5, "timex_conv_h2": 0, "timex_gw_sum_h2": 0,
                "timex_conv_any": 0, "timex_gw_any": 0, "timex_gw_short": 0, "rwkv7c_fwd": 0, "rwkv7c_bwd": 0, "rwkv7c_local": 0, "rwkv7c_scan": 0,
                # attention's tiles are under way while its loops run: a reload waits for all of them
-               "attn_fwd": 0, "attn_dqI": 8, "attn_dkvI": 6, "paged_attn": 0, "grec_fwd": 0}
+               "attn_fwd": 0, "attn_dqI": 8, "attn_dkvI": 6, "paged_attn": 0, "grec_fwd": 0, "grec_bwdIf": 32, "grec_bwdINS": 1, "grec_bwdIDF16": 1}
 
 _lib = None
 
