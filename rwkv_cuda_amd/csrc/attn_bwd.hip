@@ -3,7 +3,7 @@
 //
 // Seven products where one kernel for all three would do with five: that one would have to add dQ from many workgroups, in an order that changes (atomics)
 // or through memory.  Bound by issue, as the forward.  bf16, causal: B2 T8192 H32 Hk8 N128 with a cap and prefixes dK dV 2.4 ms, dQ 1.9 ms; B8 T4096 H32 N64 with
-// slopes 1.25 ms (880 TFLOP/s) and 0.95 ms (870).
+// slopes 1.16 ms (950 TFLOP/s) and 0.88 ms (940).
 #include "attn_tile.h"
 
 namespace rwkv {

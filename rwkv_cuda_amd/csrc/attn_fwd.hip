@@ -4,7 +4,8 @@
 // Bound by issue: a half tile of 32 x 32 pairs takes the matrix unit 256 clocks with heads of 64 (512 with 128), its exponentials 128 and the
 // other vector instructions 300 and more of each SIMD.  So products and weights of neighbouring halves stand side by side in one stretch of code
 // (all_three), and tiles come to LDS past the registers.  128 queries a workgroup: 64 a wave spilled.  Two workgroups a CU with heads of 128, three or
-// four with 64.  bf16, causal: B1 T8192 H32 N128 985 TFLOP/s (775 with a cap), B8 T4096 H32 N64 735, with slopes 600; a library product of 8192^3 reaches 1266.
+// four with 64.  bf16, causal: B1 T8192 H32 N128 980 TFLOP/s (770 with a cap), B8 T4096 H32 N64 780, with slopes 740 (710 where
+// y_rest is written for a backward); a library product of 8192^3 reaches 1266.
 #include "attn_tile.h"
 
 namespace rwkv {

@@ -16,7 +16,7 @@ namespace {
 // Progress of the latter: a column's tiles are numbered by a ticket that a workgroup takes when it runs, a tile publishes its map before it
 // waits, and it waits for lower tickets of its column only: the lowest unfinished one waits for nothing.  (A counter a column: with one for
 // all a T3001 C1536 fp16 forward took 25 us instead of 17.)
-// Bound by memory.  bf16 B8 T4096 C4096: forward 0.19 ms (805 MB, 4.3 TB/s; a copy reaches 6.0), backward 0.29 ms (1342 MB, 4.6 TB/s).
+// Bound by memory.  bf16 B8 T4096 C4096: forward 0.195 ms (805 MB, 4.1 TB/s; a copy reaches 6.0), backward 0.29 ms (1342 MB, 4.6 TB/s).
 constexpr int S = 8, MAX_GROUPS = 16;
 
 inline int groups_of(int T) { const int g = (T + S - 1) / S; return g >= MAX_GROUPS ? MAX_GROUPS : (g + 1) / 2 * 2; }

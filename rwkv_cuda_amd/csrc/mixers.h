@@ -16,7 +16,6 @@ template <class E> DEVINL E from_f(float x) {
     else return static_cast<E>(x);
 }
 
-// The documents of a tile of 64 positions, made by a kernel of its own before the others.
 // What the scores' arithmetic holds for: the capped score is made as cap - 2 cap / (1 + e^z), which is off by 2^-23 cap, and e^z's argument must not overflow.
 // (attention's biases on keys behind a query are divided by the scale: check_attn.)
 inline bool scores_ok(const float scale, const float cap) { return scale > 0.f && scale <= 0x1p60f && (cap == 0.f || (cap >= 0x1p-20f && cap <= 4096.f)); }
@@ -24,6 +23,7 @@ inline bool scores_ok(const float scale, const float cap) { return scale > 0.f &
 // Attention's tokens are less than this many elements apart: a tile of 64 rows is addressed with 31 bits.
 constexpr int MAX_TOKEN_STRIDE = 1 << 24;
 
+// The documents of a tile of 64 positions, made by a kernel of its own before the others.
 struct Range {
     int lo, hi;                                                 // of the tokens that are no padding; INT_MAX and -1 without one
     int whole;                                                  // 64 tokens, none of them padding
