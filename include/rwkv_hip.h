@@ -653,6 +653,94 @@ typedef struct rwkv_paged_args {
 size_t rwkv_paged_workspace_bytes(int B, int H, int Hk, int N, int page, int M);
 int rwkv_paged_attn(void* stream, const rwkv_paged_args* args);
 
+/* Gated delta rule: a state of key by value channels for every head, decayed by one gate a token and head and corrected along the token's key:
+ *   S = e^g S;  u = beta (v - S^T k);  S += k u^T;  y = scale S^T q.
+ * q, k have Hk heads (head h reads head h Hk / H), v, y have H; N is a multiple of 8 up to 128.  The state before the first token is s0, or 0 where
+ * that is NULL; sT (may be s0's memory) is the one behind the last.  doc (may be NULL) as for the gated recurrence: padding (doc < 0) has y = 0 and
+ * leaves the state as it is, whatever stands there; a real token whose predecessor has another doc starts from a state of 0.  g is a log decay: below
+ * -104 it is e^g = 0 (as fp32 has it).  q, k, v, y and the gates are bf16 or fp16, states fp32; q, k, v are 16-byte aligned with strides that are multiples of 8.
+ * The forward keeps in `saved` (NULL: no backward follows) what the backward needs beside its inputs; both may need a workspace. */
+typedef struct rwkv_delta_args {
+    int dtype;
+    int B, T, H, Hk, N;
+    float scale;
+    const void *q, *k, *v;            /* [B,T,Hk,N], [B,T,Hk,N], [B,T,H,N] with strides */
+    int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+    const void *g, *beta;             /* [B,T,H] with strides */
+    int64_t g_sb, g_st, beta_sb, beta_st;
+    const float* s0;                  /* [B,H,N,N], key by value, 16-byte aligned, or NULL */
+    const int* doc;                   /* [B,T] or NULL */
+    void* y;                          /* forward: [B,T,H,N], 16-byte aligned */
+    float* sT;                        /* forward: [B,H,N,N], 16-byte aligned */
+    void* saved;                      /* 16-byte aligned */
+    size_t saved_bytes;
+    const void* dy;                   /* backward: [B,T,H,N], 16-byte aligned, or NULL (zeros) */
+    const float* dsT;                 /* backward: [B,H,N,N], 16-byte aligned, or NULL (zeros) */
+    void *dq, *dk, *dv;               /* backward: dense, 16-byte aligned */
+    void *dg, *dbeta;                 /* backward: [B,T,H] */
+    float* ds0;                       /* backward: [B,H,N,N], 16-byte aligned, or NULL */
+    void* workspace;                  /* 16-byte aligned */
+    size_t workspace_bytes;
+} rwkv_delta_args;
+size_t rwkv_delta_saved_bytes(int B, int T, int H, int Hk, int N);
+size_t rwkv_delta_workspace_bytes(int B, int T, int H, int Hk, int N, int backward);     /* backward: 0 or 1; 0: none is needed */
+int rwkv_delta_forward(void* stream, const rwkv_delta_args* args);
+int rwkv_delta_backward(void* stream, const rwkv_delta_args* args);
+
+/* A paged cache in 8 bits (e4m3: 4 bits of exponent, 3 of mantissa, largest 448): a value is its code times the scale of its page and head, a power of
+ * two.  rwkv_cache8_write puts n tokens into their slots (page number times page size plus the place in the page; a slot outside the cache: the
+ * token is left out).  New tokens of a page stand beside each other in the list, and none of its pages comes twice.  The scale is the least power of two, from 2^-100
+ * on, that holds the finite values; where a page holds tokens before the first new one its scale does not fall, and where it grows those are rounded again.  What is
+ * not finite becomes NaN.  N is a multiple of 16 up to 128, page a power of two; rows of the pages are 16-byte aligned. */
+typedef struct rwkv_cache8_args {
+    int dtype;
+    int n, Hk, N, P, page;
+    const void *k, *v;                /* [n,Hk,N] with strides that are multiples of 8, 16-byte aligned, bf16 or fp16 */
+    int64_t k_st, k_sh, v_st, v_sh;
+    void *k_pages, *v_pages;          /* [P,page,Hk,N] bytes with strides that are multiples of 16, 16-byte aligned */
+    int64_t kp_sp, kp_st, kp_sh, vp_sp, vp_st, vp_sh;
+    float *k_scales, *v_scales;       /* [P,Hk] */
+    const int* slots;                 /* [n] */
+} rwkv_cache8_args;
+int rwkv_cache8_write(void* stream, const rwkv_cache8_args* args);
+
+/* As rwkv_paged_attn, over such a cache; what is not seen may hold anything. */
+typedef struct rwkv_paged8_args {
+    int dtype;
+    int B, H, Hk, N, P, page, M;
+    float scale, cap;
+    const void* q;                    /* [B,H,N], 16-byte aligned, bf16 or fp16 */
+    const void *k_pages, *v_pages;    /* [P,page,Hk,N] bytes with strides that are multiples of 16, 16-byte aligned */
+    int64_t k_sp, k_st, k_sh, v_sp, v_st, v_sh;
+    const float *k_scales, *v_scales; /* [P,Hk] */
+    const int* table;                 /* [B,M] */
+    const int* lens;                  /* [B] */
+    const float* slopes;              /* [H] or NULL */
+    void* y;                          /* [B,H,N], 16-byte aligned */
+    void* workspace;                  /* 16-byte aligned */
+    size_t workspace_bytes;
+} rwkv_paged8_args;
+size_t rwkv_paged8_workspace_bytes(int B, int H, int Hk, int N, int page, int M);
+int rwkv_paged8_attn(void* stream, const rwkv_paged8_args* args);
+
+/* The page tables of a batch of requests that grow.  Row b holds lens[b] tokens (below 0: none) in its table's first pages; more[b] (below 0: none) are to
+ * come, of which those that M pages hold are taken in.  New pages are pool[taken], pool[taken + 1], ..., for row 0, then row 1, ...; they are written to the table.
+ * slots: of the new tokens, row after row, the place in the cache, page number times page size plus the place in the page; starts: where each row's begin, and the end
+ * of all (held at 2^31 - 1); held: lens[b] and what was taken in; taken_out: how many pages of the pool are given out then.  A page beyond the pool's F is -1 in the
+ * table; a token of a page below 0, or whose slot 31 bits do not hold, has slot -1, and so have slots behind the last token.  Tokens beyond n have no slot. */
+typedef struct rwkv_tables_args {
+    int B, M, F, page, n;
+    const int *lens, *more;           /* [B] */
+    int* table;                       /* [B,M] */
+    const int* pool;                  /* [F] */
+    const int* taken;                 /* [1] */
+    int* slots;                       /* [n] */
+    int* starts;                      /* [B + 1] */
+    int* held;                        /* [B] */
+    int* taken_out;                   /* [1] */
+} rwkv_tables_args;
+int rwkv_tables_extend(void* stream, const rwkv_tables_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,7 +18,7 @@ _INCLUDE = os.path.join(_ROOT, "include")
 LIB_PATH = os.path.join(_HERE, "librwkv_hip.so")
 HASH_PATH = LIB_PATH + ".srchash"        # digest of the sources the library was built from (content, not mtime)
 
-SOURCES = ["abi.hip", "wkv56.hip", "wkv6_fwd.hip", "wkv6_bwd_a.hip", "wkv6_bwd_b.hip", "wkv6_fwd_f.hip", "wkv6_bwd_f.hip", "wkv6_local.hip", "wkv4.hip", "timex.hip", "wkv5_f32.hip", "wkv5_bf.hip", "rwkv7.hip", "rwkv7_chunk.hip", "grec.hip", "attn.hip", "attn_fwd.hip", "attn_bwd.hip", "paged.hip"]
+SOURCES = ["abi.hip", "wkv56.hip", "wkv6_fwd.hip", "wkv6_bwd_a.hip", "wkv6_bwd_b.hip", "wkv6_fwd_f.hip", "wkv6_bwd_f.hip", "wkv6_local.hip", "wkv4.hip", "timex.hip", "wkv5_f32.hip", "wkv5_bf.hip", "rwkv7.hip", "rwkv7_chunk.hip", "grec.hip", "attn.hip", "attn_fwd.hip", "attn_bwd.hip", "paged.hip", "delta.hip", "cache8.hip", "paged8.hip", "tables.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
@@ -133,6 +133,13 @@ AttnArgs = _struct("AttnArgs", (_I, "dtype causal B Tq Tk H Hk N"), (_F, "scale 
                    (_P, "slopes doc prefix y y_rest lse dy dq dk dv workspace"), (_Z, "workspace_bytes"))
 PagedArgs = _struct("PagedArgs", (_I, "dtype B H Hk N P page M"), (_F, "scale cap"), (_P, "q k_pages v_pages"), (_L, "k_sp k_st k_sh v_sp v_st v_sh"),
                     (_P, "table lens slopes k v y workspace"), (_Z, "workspace_bytes"))
+DeltaArgs = _struct("DeltaArgs", (_I, "dtype B T H Hk N"), (_F, "scale"), (_P, "q k v"), (_L, "q_sb q_st q_sh k_sb k_st k_sh v_sb v_st v_sh"), (_P, "g beta"),
+                    (_L, "g_sb g_st beta_sb beta_st"), (_P, "s0 doc y sT saved"), (_Z, "saved_bytes"), (_P, "dy dsT dq dk dv dg dbeta ds0 workspace"), (_Z, "workspace_bytes"))
+Cache8Args = _struct("Cache8Args", (_I, "dtype n Hk N P page"), (_P, "k v"), (_L, "k_st k_sh v_st v_sh"), (_P, "k_pages v_pages"), (_L, "kp_sp kp_st kp_sh vp_sp vp_st vp_sh"),
+                     (_P, "k_scales v_scales slots"))
+Paged8Args = _struct("Paged8Args", (_I, "dtype B H Hk N P page M"), (_F, "scale cap"), (_P, "q k_pages v_pages"), (_L, "k_sp k_st k_sh v_sp v_st v_sh"),
+                     (_P, "k_scales v_scales table lens slopes y workspace"), (_Z, "workspace_bytes"))
+TablesArgs = _struct("TablesArgs", (_I, "B M F page n"), (_P, "lens more table pool taken slots starts held taken_out"))
 
 # name -> (restype, argtypes): one row per symbol in include/rwkv_hip.h
 SIGNATURES = {
@@ -237,6 +244,14 @@ SIGNATURES = {
     "rwkv_attn_backward": (_I, [_P, ctypes.POINTER(AttnArgs)]),
     "rwkv_paged_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I]),
     "rwkv_paged_attn": (_I, [_P, ctypes.POINTER(PagedArgs)]),
+    "rwkv_delta_saved_bytes": (_Z, [_I] * 5),
+    "rwkv_delta_workspace_bytes": (_Z, [_I] * 6),
+    "rwkv_delta_forward": (_I, [_P, ctypes.POINTER(DeltaArgs)]),
+    "rwkv_delta_backward": (_I, [_P, ctypes.POINTER(DeltaArgs)]),
+    "rwkv_cache8_write": (_I, [_P, ctypes.POINTER(Cache8Args)]),
+    "rwkv_paged8_workspace_bytes": (_Z, [_I] * 6),
+    "rwkv_paged8_attn": (_I, [_P, ctypes.POINTER(Paged8Args)]),
+    "rwkv_tables_extend": (_I, [_P, ctypes.POINTER(TablesArgs)]),
 }
 
 

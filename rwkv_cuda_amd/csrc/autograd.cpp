@@ -726,6 +726,205 @@ Tensor paged_op(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tenso
     return y;
 }
 
+// --------------------------------------------------------------------------------------------- gated delta rule
+rwkv_delta_args delta_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, double scale) {
+    rwkv_delta_args a{};
+    a.dtype = dtype_of(q, "q", false);
+    a.B = i32(v.size(0)); a.T = i32(v.size(1)); a.H = i32(v.size(2)); a.N = i32(v.size(3)); a.Hk = i32(k.size(2));
+    a.scale = static_cast<float>(scale);
+    a.q = q.data_ptr(); a.q_sb = stride_of(q, 0); a.q_st = stride_of(q, 1); a.q_sh = stride_of(q, 2);
+    a.k = k.data_ptr(); a.k_sb = stride_of(k, 0); a.k_st = stride_of(k, 1); a.k_sh = stride_of(k, 2);
+    a.v = v.data_ptr(); a.v_sb = stride_of(v, 0); a.v_st = stride_of(v, 1); a.v_sh = stride_of(v, 2);
+    a.g = g.data_ptr(); a.g_sb = stride_of(g, 0); a.g_st = stride_of(g, 1);
+    a.beta = beta.data_ptr(); a.beta_sb = stride_of(beta, 0); a.beta_st = stride_of(beta, 1);
+    return a;
+}
+// [B,T,heads,N] and [B,T,H]; returns the scale
+float check_delta(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, const c10::optional<double>& scale) {
+    check_rows({{&q, "q"}, {&k, "k"}, {&v, "v"}, {&g, "g"}, {&beta, "beta"}}, q);
+    const int64_t H = v.size(2), N = v.size(3);
+    require(k.sizes() == q.sizes() && k.size(0) == v.size(0) && k.size(1) == v.size(1) && k.size(3) == N, "q and k are [B,T,Hk,N], v is [B,T,H,N]");
+    require(k.size(2) > 0 && H % k.size(2) == 0, "H must be a multiple of Hk");
+    require(N >= 8 && N <= MAX_HEAD && N % 8 == 0, "the head size must be a multiple of 8 up to 128");
+    const std::vector<int64_t> gates = {v.size(0), v.size(1), H};
+    require(g.sizes() == gates && beta.sizes() == gates, "g and beta are [B,T,H]");
+    const float sc = scale_of(scale, N);
+    require(sc > 0.f && std::isfinite(sc), "scale must be positive");
+    return sc;
+}
+struct Delta : Function<Delta> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, const Maybe& s0_, const Maybe& doc_, double scale,
+                                 bool grad) {
+        const Tensor s0 = or_none(s0_), doc = or_none(doc_);
+        const int64_t B = v.size(0), T = v.size(1), H = v.size(2), N = v.size(3);
+        check_side(s0, "s0", F32, {B, H, N, N}, q);
+        check_side(doc, "doc", torch::kInt32, {B, T}, q);
+        const Guard guard(q.device());
+        rwkv_delta_args a = delta_args(q, k, v, g, beta, scale);
+        const Tensor start = s0.defined() ? on_16(s0) : Tensor();
+        Tensor y = at::empty({B, T, H, N}, q.options()), sT = at::empty({B, H, N, N}, q.options().dtype(F32)), saved;
+        a.s0 = P(start); a.doc = P(doc); a.y = P(y); a.sT = P(sT);
+        if (grad) {
+            a.saved_bytes = rwkv_delta_saved_bytes(a.B, a.T, a.H, a.Hk, a.N);
+            saved = bytes(q, a.saved_bytes);
+            a.saved = P(saved);
+        }
+        a.workspace_bytes = rwkv_delta_workspace_bytes(a.B, a.T, a.H, a.Hk, a.N, 0);
+        const Tensor ws = a.workspace_bytes > 0 ? bytes(q, a.workspace_bytes) : Tensor();
+        a.workspace = P(ws);
+        ok(rwkv_delta_forward(stream_of(q), &a));
+        if (grad) ctx->save_for_backward({q, k, v, g, beta, doc, saved});
+        ctx->saved_data["scale"] = scale;
+        put(ctx, {{"state", s0.defined()}});
+        ctx->set_materialize_grads(false);
+        return {y, sT};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        once_only("gated_delta");
+        const auto s = ctx->get_saved_variables();
+        const Tensor &q = s[0], &k = s[1], &v = s[2], &gate = s[3], &beta = s[4], &saved = s[6];
+        const Tensor dy = g[0].defined() ? on_16(g[0].contiguous()) : Tensor(), dsT = g[1].defined() ? on_16(g[1].contiguous()) : Tensor();
+        const Guard guard(q.device());
+        rwkv_delta_args a = delta_args(q, k, v, gate, beta, ctx->saved_data["scale"].toDouble());
+        Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
+        Tensor dg = at::empty(gate.sizes(), gate.options()), dbeta = at::empty(gate.sizes(), gate.options());
+        Tensor ds0 = get(ctx, "state") ? at::empty({a.B, a.H, a.N, a.N}, q.options().dtype(F32)) : Tensor();
+        a.doc = P(s[5]); a.saved = P(saved); a.saved_bytes = saved.numel();
+        a.dy = P(dy); a.dsT = P(dsT); a.dq = P(dq); a.dk = P(dk); a.dv = P(dv); a.dg = P(dg); a.dbeta = P(dbeta); a.ds0 = P(ds0);
+        a.workspace_bytes = rwkv_delta_workspace_bytes(a.B, a.T, a.H, a.Hk, a.N, 1);
+        const Tensor ws = a.workspace_bytes > 0 ? bytes(q, a.workspace_bytes) : Tensor();
+        a.workspace = P(ws);
+        ok(rwkv_delta_backward(stream_of(q), &a));
+        return {dq, dk, dv, dg, dbeta, ds0, NONE, NONE, NONE};
+    }
+};
+std::tuple<Tensor, Tensor> delta_op(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, const Maybe& s0, const Maybe& doc, c10::optional<double> scale) {
+    require(q.dim() == 4 && k.dim() == 4 && v.dim() == 4 && g.dim() == 3 && beta.dim() == 3, "q and k are [B,T,Hk,N], v is [B,T,H,N], g and beta are [B,T,H]");
+    const float sc = check_delta(q, k, v, g, beta, scale);
+    const Tensor s = or_none(s0);
+    variable_list o = Delta::apply(q, k, v, g, beta, s0, doc, static_cast<double>(sc), wants_grad({&q, &k, &v, &g, &beta}) || (s.defined() && wants_grad({&s})));
+    return {o[0], o[1]};
+}
+Tensor delta_step_op(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_, const Tensor& beta_, const Tensor& s, const Tensor& out, c10::optional<double> scale) {
+    require(!wants_grad({&q_, &k_, &v_, &g_, &beta_, &s, &out}), "STEP has no gradients: call it under torch.no_grad()");
+    require(q_.dim() == 3 && k_.dim() == 3 && v_.dim() == 3 && g_.dim() == 2 && beta_.dim() == 2, "q and k are [B,Hk,N], v is [B,H,N], g and beta are [B,H]");
+    const Tensor q = q_.unsqueeze(1), k = k_.unsqueeze(1), v = v_.unsqueeze(1), g = g_.unsqueeze(1), beta = beta_.unsqueeze(1);
+    const float sc = check_delta(q, k, v, g, beta, scale);
+    const int64_t B = v.size(0), H = v.size(2), N = v.size(3);
+    check_side(s, "s", F32, {B, H, N, N}, q);
+    check_side(out, "out", F32, {B, H, N, N}, q);
+    check_writable(out, "the new state");
+    for (const Tensor* x : {&q_, &k_, &v_, &g_, &beta_}) require(!touch(out, *x), "out must share no memory with q, k, v, g and beta");
+    require(out.data_ptr() == s.data_ptr() || !touch(out, s), "out must be s, or share no memory with it");
+    const Guard guard(q.device());
+    rwkv_delta_args a = delta_args(q, k, v, g, beta, sc);
+    Tensor y = at::empty({B, H, N}, q.options());
+    a.s0 = P(s); a.sT = P(out); a.y = P(y);
+    a.workspace_bytes = rwkv_delta_workspace_bytes(a.B, a.T, a.H, a.Hk, a.N, 0);
+    const Tensor ws = a.workspace_bytes > 0 ? bytes(q, a.workspace_bytes) : Tensor();
+    a.workspace = P(ws);
+    ok(rwkv_delta_forward(stream_of(q), &a));
+    written(out);
+    return y;
+}
+
+// --------------------------------------------------------------------------------------------- a paged cache in 8 bits
+constexpr auto F8 = torch::kFloat8_e4m3fn;
+// pages [P,page,Hk,N] in 8 bits and their scales [P,Hk], beside `first`
+void check_cache8(const Tensor& kp, const Tensor& vp, const Tensor& ks, const Tensor& vs, const Tensor& first, int64_t N) {
+    require(kp.dim() == 4 && vp.sizes() == kp.sizes(), "k_pages and v_pages are [P,page,Hk,N]");
+    const int64_t page = kp.size(1), Hk = kp.size(2);
+    for (const auto& t : std::initializer_list<std::pair<const Tensor*, const char*>>{{&kp, "k_pages"}, {&vp, "v_pages"}}) {
+        const std::string n = t.second;
+        require(t.first->is_cuda() && first.is_cuda(), "tensors must live on a HIP device: there is no CPU path");
+        require(t.first->device() == first.device(), n + " is on " + t.first->device().str() + ", expected " + first.device().str());
+        require(t.first->scalar_type() == F8, n + ".dtype must be torch.float8_e4m3fn, got " + str(t.first->scalar_type()));
+        require(t.first->stride(3) == 1, n + " must be dense in its last dimension");
+    }
+    require(kp.size(3) == N && Hk > 0, "the head size must be that of the pages");
+    require(N >= 16 && N <= MAX_HEAD && N % 16 == 0, "the head size must be a multiple of 16 up to 128");
+    require(page > 0 && (page & (page - 1)) == 0, "page must be a power of two");
+    check_side(ks, "k_scales", F32, {kp.size(0), Hk}, first);
+    check_side(vs, "v_scales", F32, {kp.size(0), Hk}, first);
+}
+void cache8_write_op(const Tensor& k, const Tensor& v, const Tensor& kp, const Tensor& vp, const Tensor& ks, const Tensor& vs, const Tensor& slots) {
+    require(!wants_grad({&k, &v}), "WRITE has no gradients: call it under torch.no_grad()");
+    require(k.dim() == 3 && v.sizes() == k.sizes(), "k and v are [n,Hk,N]");
+    check_rows({{&k, "k"}, {&v, "v"}}, k);
+    check_cache8(kp, vp, ks, vs, k, k.size(2));
+    require(kp.size(2) == k.size(1), "k, v and the pages have the same heads");
+    check_side(slots, "slots", torch::kInt32, {k.size(0)}, k);
+    check_writable(kp, "k_pages"), check_writable(vp, "v_pages"), check_writable(ks, "k_scales"), check_writable(vs, "v_scales");
+    rwkv_cache8_args a{};
+    a.dtype = dtype_of(k, "k", false);
+    if (k.size(0) == 0) return;
+    const Guard guard(k.device());
+    a.n = i32(k.size(0)); a.Hk = i32(k.size(1)); a.N = i32(k.size(2)); a.P = i32(kp.size(0)); a.page = i32(kp.size(1));
+    a.k = P(k); a.v = P(v); a.k_st = stride_of(k, 0); a.k_sh = stride_of(k, 1); a.v_st = stride_of(v, 0); a.v_sh = stride_of(v, 1);
+    a.k_pages = P(kp); a.v_pages = P(vp);
+    a.kp_sp = stride_of(kp, 0); a.kp_st = stride_of(kp, 1); a.kp_sh = stride_of(kp, 2);
+    a.vp_sp = stride_of(vp, 0); a.vp_st = stride_of(vp, 1); a.vp_sh = stride_of(vp, 2);
+    a.k_scales = P(ks); a.v_scales = P(vs); a.slots = P(slots);
+    ok(rwkv_cache8_write(stream_of(k), &a));
+    written(kp), written(vp), written(ks), written(vs);
+}
+Tensor paged8_op(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& ks, const Tensor& vs, const Tensor& table, const Tensor& lens, const Maybe& slopes_, double cap,
+                 c10::optional<double> scale) {
+    const Tensor slopes = or_none(slopes_);
+    require(!wants_grad({&q}), "paged_attention8 has no gradients: call it under torch.no_grad()");
+    require(q.dim() == 3, "q is [B,H,N]");
+    const int64_t B = q.size(0), H = q.size(1), N = q.size(2);
+    check({{&q, "q"}}, q.scalar_type(), q);
+    check_cache8(kp, vp, ks, vs, q, N);
+    const int64_t page = kp.size(1), Hk = kp.size(2);
+    require(H % Hk == 0, "H must be a multiple of Hk");
+    require(table.dim() == 2, "table is [B,M]");
+    check_side(table, "table", torch::kInt32, {B, table.size(1)}, q);
+    check_side(lens, "lens", torch::kInt32, {B}, q);
+    check_side(slopes, "slopes", F32, {H}, q);
+    require(cap == 0.0 || (cap >= 0x1p-20 && cap <= 4096.0), "cap must be 0, or from 2^-20 to 4096");
+    const Guard guard(q.device());
+    rwkv_paged8_args a{};
+    a.dtype = dtype_of(q, "q", false);
+    a.B = i32(B); a.H = i32(H); a.Hk = i32(Hk); a.N = i32(N); a.P = i32(kp.size(0)); a.page = i32(page); a.M = i32(table.size(1));
+    a.scale = scale_of(scale, N); a.cap = static_cast<float>(cap);
+    require(a.scale > 0.f && std::isfinite(a.scale), "scale must be positive");
+    a.k_sp = stride_of(kp, 0); a.k_st = stride_of(kp, 1); a.k_sh = stride_of(kp, 2);
+    a.v_sp = stride_of(vp, 0); a.v_st = stride_of(vp, 1); a.v_sh = stride_of(vp, 2);
+    const Tensor qq = on_16(q);
+    Tensor y = at::empty({B, H, N}, q.options());
+    a.q = P(qq); a.k_pages = P(kp); a.v_pages = P(vp); a.k_scales = P(ks); a.v_scales = P(vs); a.table = P(table); a.lens = P(lens); a.slopes = P(slopes); a.y = P(y);
+    a.workspace_bytes = rwkv_paged8_workspace_bytes(a.B, a.H, a.Hk, a.N, a.page, a.M);
+    const Tensor ws = a.workspace_bytes > 0 ? bytes(q, a.workspace_bytes) : Tensor();
+    a.workspace = P(ws);
+    ok(rwkv_paged8_attn(stream_of(q), &a));
+    return y;
+}
+
+// --------------------------------------------------------------------------------------------- page tables
+std::tuple<Tensor, Tensor, Tensor, Tensor> tables_op(const Tensor& lens, const Tensor& more, const Tensor& table, const Tensor& pool, const Tensor& taken, int64_t page, int64_t n) {
+    require(lens.dim() == 1 && table.dim() == 2 && pool.dim() == 1, "lens and more are [B], table is [B,M], pool is [F], taken is [1]");
+    constexpr auto I32 = torch::kInt32;
+    check({{&lens, "lens"}, {&table, "table"}, {&pool, "pool"}}, I32, lens);
+    const int64_t B = lens.size(0);
+    check_side(more, "more", I32, {B}, lens);
+    check_side(taken, "taken", I32, {1}, lens);
+    require(table.size(0) == B, "table is [B,M]");
+    require(page > 0 && page <= (1 << 30) && (page & (page - 1)) == 0, "page must be a power of two");
+    require(n >= 0 && n <= std::numeric_limits<int>::max(), "n must be from 0 to 2147483647");
+    check_writable(table, "table");
+    for (const Tensor* x : {&lens, &more, &pool, &taken}) require(!touch(table, *x), "table must share no memory with lens, more, pool and taken");
+    const Guard guard(lens.device());
+    rwkv_tables_args a{};
+    a.B = i32(B); a.M = i32(table.size(1)); a.F = i32(pool.size(0)); a.page = static_cast<int>(page); a.n = static_cast<int>(n);
+    Tensor slots = at::empty({n}, lens.options()), starts = at::empty({B + 1}, lens.options()), held = at::empty({B}, lens.options()), out = at::empty({1}, lens.options());
+    a.lens = P(lens); a.more = P(more); a.table = P(table); a.pool = P(pool); a.taken = P(taken);
+    a.slots = n > 0 ? slots.data_ptr<int>() : nullptr; a.starts = P(starts); a.held = P(held); a.taken_out = P(out);
+    ok(rwkv_tables_extend(stream_of(lens), &a));
+    written(table);
+    return {slots, starts, held, out};
+}
+
 }  // namespace
 
 void bind_autograd(py::module_& m) {
@@ -744,4 +943,9 @@ void bind_autograd(py::module_& m) {
     ops.def("gated_recurrence_step", &grec_step_op);
     ops.def("attention", &attention_op);
     ops.def("paged_attention", &paged_op);
+    ops.def("gated_delta", &delta_op);
+    ops.def("gated_delta_step", &delta_step_op);
+    ops.def("cache8_write", &cache8_write_op);
+    ops.def("paged_attention8", &paged8_op);
+    ops.def("tables_extend", &tables_op);
 }

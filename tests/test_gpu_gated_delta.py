@@ -1,0 +1,242 @@
+"""GPU: the gated delta rule against its 64-bit definition."""
+import pytest
+import torch
+
+from oracle import delta as O
+from rwkv_cuda_amd import gated_delta as G
+from _delta_util import inputs, near
+from _gpu_util import DEV
+from _mixers_util import DT, doc_ids, graph_of, randn
+
+pytestmark = pytest.mark.gpu
+NAMES = ("dq", "dk", "dv", "dg", "dbeta", "ds0")
+
+
+def check(t, s0, doc=None, dy=None, dsT=None, scale=None, steps=1.0):
+    """Both directions, or without dy and dsT the forward alone."""
+    want = O.gated_delta(*t, s0=s0, doc=doc, scale=scale, dy=dy, dsT=dsT)
+    grad = dy is not None or dsT is not None
+    leaves = [z.detach().requires_grad_(grad) for z in (*t, s0) if z is not None]
+    y, sT = G.RUN_CUDA(*leaves[:5], s0=leaves[5] if s0 is not None else None, doc=doc, scale=scale)
+    got = dict(y=y, sT=sT)
+    if grad:
+        out, d = zip(*[(o, g) for o, g in ((y, dy), (sT, dsT)) if g is not None])
+        got.update(zip(NAMES, torch.autograd.grad(out, leaves, d)))
+    torch.cuda.synchronize()
+    for n in got:
+        near(n, got[n], want[n], steps)
+    return got
+
+
+@pytest.mark.parametrize("T", [1, 2, 3, 9, 15, 16, 17, 63, 64, 65, 128, 129, 200])
+@pytest.mark.parametrize("H,Hk,N,dtype", [(2, 2, 64, "bf16"), (4, 2, 128, "fp16"), (3, 1, 24, "bf16")])
+def test_lengths(lib, T, H, Hk, N, dtype):
+    print(f"\nT={T} H={H} Hk={Hk} N={N} {dtype}", flush=True)
+    t, s0, dy, dsT = inputs(2, T, H, Hk, N, DT[dtype], seed=T)
+    check(t, s0, None, dy, dsT)
+    check(t, None)
+
+
+@pytest.mark.parametrize("B,T,H,Hk,N,dtype", [(1, 300, 1, 1, 8, "bf16"), (2, 130, 6, 2, 80, "fp16"), (3, 77, 8, 8, 96, "bf16"), (1, 700, 2, 1, 128, "bf16"), (2, 333, 4, 4, 64, "fp16"), (5, 66, 16, 2, 32, "bf16"),
+                                              (1, 70, 36, 36, 64, "bf16"), (9, 65, 40, 8, 112, "fp16"), (2, 64, 5, 5, 40, "fp16")])
+def test_heads(lib, B, T, H, Hk, N, dtype):
+    print(f"\nB={B} T={T} H={H} Hk={Hk} N={N} {dtype}", flush=True)
+    t, s0, dy, dsT = inputs(B, T, H, Hk, N, DT[dtype], seed=N)
+    check(t, s0, None, dy, dsT)
+
+
+@pytest.mark.parametrize("kind", ["two", "many", "padded", "one", "back"])
+@pytest.mark.parametrize("T,N,dtype", [(7, 64, "bf16"), (150, 64, "fp16"), (200, 128, "bf16"), (64, 40, "fp16")])
+def test_documents(lib, kind, T, N, dtype):
+    print(f"\n{kind} T={T} N={N} {dtype}", flush=True)
+    t, s0, dy, dsT = inputs(3, T, 4, 2, N, DT[dtype], seed=T)
+    doc = doc_ids(3, T, kind, seed=T).to(DEV)
+    check(t, s0, doc, dy, dsT)
+    check(t, None, doc, dy)
+
+
+def test_padding_counts_nowhere(lib):
+    """NaN and infinities in padding, before, between and behind; rows that are nothing else; dy there too."""
+    for N, T, value in ((64, 150, float("nan")), (128, 70, float("inf")), (64, 5, float("nan"))):
+        t, s0, dy, dsT = inputs(3, T, 2, 2, N, torch.bfloat16, seed=3)
+        doc = doc_ids(3, T, "padded", seed=T).to(DEV)
+        bad = doc < 0
+        want = check(t, s0, doc, torch.where(bad[:, :, None, None], 0, dy), dsT)
+        t2 = [torch.where(bad.view(3, T, *[1] * (z.dim() - 2)), value, z).to(z.dtype) for z in (*t, dy)]
+        leaves = [z.requires_grad_(True) for z in (*t2[:5], s0.clone())]
+        y, sT = G.RUN_CUDA(*leaves, doc)
+        got = [y, sT, *torch.autograd.grad([y, sT], leaves, [t2[5], dsT])]
+        for n, g in zip(("y", "sT") + NAMES, got):
+            assert torch.equal(g, want[n]), n
+            if n not in ("sT", "ds0"):
+                assert not g[bad].any(), n
+
+
+@pytest.mark.parametrize("T", [6, 140])
+def test_gates_at_their_ends(lib, T):
+    """Decays of nothing, of everything and beyond; beta of 0, 1 and between 1 and 2; the same key over and over."""
+    t, s0, dy, dsT = inputs(2, T, 3, 3, 64, torch.bfloat16, seed=5)
+    q, k, v, g, beta = t
+    g[:, ::5], g[:, 1::7], g[:, 3::11] = 0.0, -120.0, -float("inf")
+    g[0, T // 2:] = 0.0
+    beta[:, ::4], beta[:, 1::4] = 1.0, 0.0
+    beta[1, :, 2] = 1.5
+    k[0, :, 1] = k[0, :1, 1]
+    got = check(t, s0, None, dy, dsT, steps=2.0)                 # (sums of a hundred equal terms: errors of one sign)
+    assert all(torch.isfinite(z).all() for z in got.values()) and not got["dg"][g < -104].any()
+
+
+def test_strong_decays_beside_weak_ones(lib):
+    """Sums of log decays in the thousands, differences of which count to their last bits."""
+    t, s0, dy, dsT = inputs(1, 200, 2, 2, 64, torch.bfloat16, seed=6)
+    t[3][:, ::2] = -90.0
+    t[3][:, 1::2] = -0.01
+    t[3][:, 100:] = -0.003
+    check(t, s0, None, dy, dsT)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -30, 2.0 ** 20])
+def test_sizes_far_from_one(lib, size):
+    """Values, states and gradients of any size: bf16 has fp32's range."""
+    t, s0, dy, dsT = inputs(2, 100, 2, 2, 64, torch.bfloat16, seed=7)
+    t[2] = (t[2].float() * size).to(torch.bfloat16)
+    check(t, s0 * size, None, (dy.float() * size).to(torch.bfloat16), dsT * size)
+
+
+def test_small_gradients_in_fp16(lib):
+    """Gradients near the end of fp16 (its least step is 2^-24): as exact as their type."""
+    t, s0, dy, dsT = inputs(2, 100, 2, 2, 64, torch.float16, seed=8)
+    check(t, s0, None, (dy.float() * 2.0 ** -10).half(), dsT * 2.0 ** -10)
+    check([t[0], t[1], t[2] * 64, t[3], t[4]], s0 * 64, None, (dy.float() * 8).half(), dsT)
+
+
+def test_only_one_of_the_outputs_has_a_gradient(lib):
+    t, s0, dy, dsT = inputs(2, 90, 2, 2, 64, torch.bfloat16, seed=9)
+    check(t, s0, None, dy, None)
+    check(t, s0, None, None, dsT)
+    leaf = t[2].detach().requires_grad_(True)
+    y, _ = G.RUN_CUDA(t[0], t[1], leaf, t[3], t[4])
+    y.float().sum().backward()                                   # an upstream gradient with strides of zero
+    assert leaf.grad.shape == leaf.shape
+
+
+def test_views_and_broadcasts(lib):
+    """Views of one projection, tokens first in memory, gates at odd offsets; keys and values that all heads or tokens share."""
+    B, T, H, Hk, N = 2, 100, 4, 2, 64
+    t, s0, dy, dsT = inputs(B, T, H, Hk, N, torch.bfloat16, seed=10)
+    want = G.RUN_CUDA(*t, s0)
+    both = torch.cat([z.flatten(2) for z in t[:3]], 2)
+    q, k, v = (z.unflatten(2, (-1, N)) for z in both.split([Hk * N, Hk * N, H * N], 2))
+    gates = torch.cat([t[3], t[4], t[3]], 2)
+    views = [q, k, v, gates[..., 1:1 + H], gates[..., H:2 * H]]
+    assert all(torch.equal(a, b) for a, b in zip(G.RUN_CUDA(q, k, v, gates[..., :H], gates[..., H:2 * H], s0), want))
+    check(views, s0, None, dy, dsT)
+    turned = [z.transpose(0, 1).contiguous().transpose(0, 1) for z in t]
+    assert all(torch.equal(a, b) for a, b in zip(G.RUN_CUDA(*turned, s0), want))
+    one = [t[0], t[1][:, :, :1].expand(B, T, Hk, N), t[2][:, :1].expand(B, T, H, N), t[3], t[4]]
+    small = [one[0], t[1][:, :, :1].detach().requires_grad_(True), t[2][:, :1].detach().requires_grad_(True)]
+    y, _ = G.RUN_CUDA(one[0], small[1].expand(B, T, Hk, N), small[2].expand(B, T, H, N), t[3], t[4])
+    dk, dv = torch.autograd.grad(y, small[1:], dy)
+    ref = O.gated_delta(*one, dy=dy)
+    assert dk.shape == small[1].shape and dv.shape == small[2].shape
+    # (torch adds the heads' and tokens' gradients, rounded to 8 bits, in 32 bits and rounds once more)
+    assert float((dv.double() - ref["dv"].sum(1, keepdim=True)).norm() / ref["dv"].sum(1).norm()) < 2.0 ** -6
+    assert float((dk.double() - ref["dk"].sum(2, keepdim=True)).norm() / ref["dk"].sum(2).norm()) < 2.0 ** -6
+
+
+def test_two_calls_pass_the_state_on(lib):
+    t, s0, _, _ = inputs(2, 300, 4, 2, 128, torch.bfloat16, seed=11)
+    want = O.gated_delta(*t, s0=s0)
+    for cut in (1, 5, 64, 130, 299):
+        y0, s = G.RUN_CUDA(*(z[:, :cut] for z in t), s0)
+        y1, sT = G.RUN_CUDA(*(z[:, cut:] for z in t), s)
+        near("y", torch.cat([y0, y1], 1), want["y"])
+        near("sT", sT, want["sT"])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("B,H,Hk,N", [(1, 1, 1, 8), (3, 6, 2, 80), (32, 16, 16, 64), (5, 8, 4, 128)])
+def test_step(lib, dtype, B, H, Hk, N):
+    """A token at a time gives what whole sequences do, in place and into other memory."""
+    T = 5
+    t, s0, _, _ = inputs(B, T, H, Hk, N, DT[dtype], seed=12)
+    want = O.gated_delta(*t, s0=s0)
+    s, keep = s0.clone(), s0.clone()
+    other = torch.empty_like(s)
+    ys = []
+    for i in range(T):
+        now = [z[:, i] for z in t]
+        ys.append(G.STEP(*now, keep, out=other))
+        version = s._version
+        assert torch.equal(ys[-1], G.STEP(*now, s)) and torch.equal(s, other) and s._version > version
+        keep, other = other, keep
+    near("y", torch.stack(ys, 1), want["y"])
+    near("s", s, want["sT"])
+
+
+def test_the_same_bits_every_time_and_alone(lib):
+    t, s0, dy, dsT = inputs(3, 210, 4, 2, 64, torch.bfloat16, seed=13)
+
+    def once(t, s0, dy, dsT):
+        leaves = [z.detach().requires_grad_(True) for z in (*t, s0)]
+        y, sT = G.RUN_CUDA(*leaves)
+        return [y.detach(), sT.detach(), *torch.autograd.grad([y, sT], leaves, [dy, dsT])]
+    want = once(t, s0, dy, dsT)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(want, once(t, s0, dy, dsT)))
+
+
+def test_captured_and_replayed(lib):
+    """Forward and backward in a graph, replayed on changing inputs between eager calls; two graphs of the same leaves; the single token."""
+    t, s0, dy, dsT = inputs(2, 150, 4, 2, 64, torch.bfloat16, seed=14)
+    leaves = [z.detach().clone().requires_grad_(True) for z in (*t, s0)]
+
+    def once():
+        y, sT = G.RUN_CUDA(*leaves)
+        return [y.detach(), sT.detach(), *torch.autograd.grad([y, sT], leaves, [dy, dsT])]
+    (g1, o1), (g2, o2) = graph_of(once), graph_of(once)
+    now, s = [z[:, 0].clone() for z in t], s0.clone()
+    out = torch.empty_like(s)
+    g3, o3 = graph_of(lambda: G.STEP(*now, s, out=out))
+    for i in range(4):
+        with torch.no_grad():
+            leaves[2].copy_(randn(*t[2].shape, seed=100 + i).to(t[2].dtype))
+            now[2].copy_(leaves[2][:, 1])
+        want = [z.clone() for z in once()]
+        step = G.STEP(*now, s, out=out).clone()
+        after = out.clone()
+        out.zero_()
+        for g in (g1, g2, g3):
+            g.replay()
+        torch.cuda.synchronize()
+        for o in (o1, o2):
+            assert all(torch.equal(a, b) for a, b in zip(want, o)), i
+        assert torch.equal(step, o3) and torch.equal(after, out)
+
+
+def test_two_streams_at_once(lib):
+    cases = [inputs(2, 200, 4, 4, 64, torch.bfloat16, seed=s)[0] for s in (1, 2)]
+    want = [G.RUN_CUDA(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(4):
+        got = []
+        for c, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                got.append(G.RUN_CUDA(*c))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for m, n in zip(want, got) for a, b in zip(m, n))
+
+
+def test_tokens_far_apart_and_long_rows(lib):
+    """[T,B,...] in memory, offsets of a chunk beyond 32 bits; only some rows are looked at."""
+    T, B, H, N = 70, 32768, 16, 64
+    small = inputs(1, T, H, H, N, torch.bfloat16, seed=15)[0]
+    far = [z.transpose(0, 1).expand(T, B, *z.shape[2:]) for z in small]
+    v = far[2].contiguous().transpose(0, 1)
+    k = far[1].contiguous().transpose(0, 1)
+    assert v.stride(1) * 2 * (T - 1) > 1 << 32 and v.numel() > 1 << 31
+    one = lambda z: z.transpose(0, 1)
+    y, sT = G.RUN_CUDA(one(far[0]), k, v, one(far[3]).contiguous(), one(far[4]).contiguous())
+    want = G.RUN_CUDA(*small)
+    assert all(torch.equal(y[b], want[0][0]) and torch.equal(sT[b], want[1][0]) for b in (0, 1, 1000, B - 1))
