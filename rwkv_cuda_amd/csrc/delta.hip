@@ -11,11 +11,6 @@
 namespace rwkv {
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-
-DEVINL int64_t wide(int x) { return x; }
-
 template <class E, int ROWS>
 __global__ __launch_bounds__(256) void delta_steps(const rwkv_delta_args p, float* states) {
     __shared__ float sums[2][4][64 + 4];
@@ -239,7 +234,10 @@ template <class E> __global__ __launch_bounds__(256) void delta_sum(const rwkv_d
     }
 }
 
+// Few tokens go one by one: a chunk costs the same whatever it holds.
+constexpr int FEW = 8;
 template <class E> int run_fwd(hipStream_t st, const rwkv_delta_args& p) {
+    if (p.saved == nullptr && p.T > FEW) return launch_delta_fwd(st, p);
     const dim3 grid((p.N + 31) / 32, p.H, p.B);
     if (p.N <= 64) hipLaunchKernelGGL((delta_steps<E, 2>), grid, dim3(256), 0, st, p, static_cast<float*>(p.saved));
     else hipLaunchKernelGGL((delta_steps<E, 4>), grid, dim3(256), 0, st, p, static_cast<float*>(p.saved));
