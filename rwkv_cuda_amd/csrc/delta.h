@@ -33,8 +33,22 @@ DEVINL DeltaToken delta_token(const int* doc, const int64_t row, const int t, co
     return {d >= 0, d >= 0 && t > 0 && doc[row + t - 1] != d};
 }
 
-// delta_fwd.hip, delta_bwd.hip (arguments checked)
+// What the forward keeps for the backward, and the backward for its last kernel, of each head and chunk: the state that enters (whose gradient leaves) and the updates (their gradients), fp32, as
+// the waves hold them: tiles of 16 by 16, four neighbouring rows of a column a lane, 16 bytes.  States: [column tile][row tile], updates [column tile][token tile].
+struct DeltaTiles {
+    int tiles;                                                  // of 16 channels
+    int64_t chunks;                                             // all of them
+    __host__ __device__ explicit DeltaTiles(const rwkv_delta_args& p) : DeltaTiles(p.B, p.T, p.H, p.N) {}
+    __host__ __device__ DeltaTiles(int B, int T, int H, int N) : tiles((N + 15) / 16), chunks(static_cast<int64_t>(B) * H * ((T + DELTA_CHUNK - 1) / DELTA_CHUNK)) {}
+    __host__ __device__ size_t states() const { return static_cast<size_t>(chunks) * tiles * tiles * 256; }       // floats
+    __host__ __device__ size_t updates() const { return static_cast<size_t>(chunks) * tiles * 4 * 256; }
+    __host__ __device__ int64_t state(const int64_t chunk, const int column, const int row) const { return ((chunk * tiles + column) * tiles + row) * 256; }
+    __host__ __device__ int64_t update(const int64_t chunk, const int column, const int token) const { return ((chunk * tiles + column) * 4 + token) * 256; }
+};
+// delta_fwd.hip, delta_bwd.hip, delta_grads.hip (arguments checked)
 int launch_delta_fwd(hipStream_t st, const rwkv_delta_args& p);
+int launch_delta_bwd(hipStream_t st, const rwkv_delta_args& p, float* dS, float* dZ);
+int launch_delta_grads(hipStream_t st, const rwkv_delta_args& p, const float* dS, const float* dZ, float* dq, float* dk);
 
 namespace {
 
@@ -67,6 +81,7 @@ template <class E> DEVINL Two split(const f32x4 x) {
     }
     return o;
 }
+template <class E> DEVINL f32x4 four_of(const u32x2 v) { return f32x4{unpack_lo<E>(v[0]), unpack_hi<E>(v[0]), unpack_lo<E>(v[1]), unpack_hi<E>(v[1])}; }
 // a b + c of two such operands, bf16, over a single tile: both small products in one instruction, the large one beside zeros
 DEVINL f32x4 mma16(const Two& a, const Two& b, f32x4 c) {
     c = mma32<bf16_t>(join(a.h, a.l), join(b.l, b.h), c);
@@ -117,7 +132,7 @@ template <class E, int TILES> struct Beside {
 // The scalars of a chunk's 64 tokens, by token, fp32.  Log decays are summed in 64 bits, to base 2, and their sums kept as two numbers: differences count.  A cut, or a decay of nothing, is one
 // by 2^-(2^20): what crosses it is 0, and the others' differences stay exact to 2^-21.
 struct Scalars {
-    static constexpr lds_t SUM = 0, REST = 256, BETA = 512, ENTER = 768, LEAVE = 1024, TAIL = 1280, BYTES = 1536;      // TAIL: the decay up to the end of a token's block of 16
+    static constexpr lds_t SUM = 0, REST = 256, BETA = 512, ENTER = 768, LEAVE = 1024, TAIL = 1280, BYTES = 1536;      // TAIL: the decay up to the end of a token's block of 16, or (HEAD) since it began
 };
 constexpr double CUT = -0x1p20;
 
@@ -131,6 +146,8 @@ template <int D> struct Rows {
         lds_st(to, u32x2{x[0], x[1]});
         lds_st(to + 16, u32x2{x[2], x[3]});
     }
+    // four of a row's channels, 16 t + 4 g ..
+    static DEVINL u32x2 four(const lds_t base, const int row, const int t, const int g) { return lds_ld<u32x2>(base + row * PITCH + 64 * (t / 2) + 16 * g + 8 * (t % 2)); }
     // row 16 i + (lane & 15), channels of the 32 s-th: the contraction runs over channels
     static DEVINL u32x4 row(const lds_t base, const int lane, const int i, const int s) { return lds_ld<u32x4>(base + (16 * i + (lane & 15)) * PITCH + 64 * s + 16 * (lane >> 4)); }
     // channel 16 t + (lane & 15), rows of the 32 s-th: the contraction runs over rows
@@ -163,6 +180,25 @@ template <int FIRST> struct Lower {
         return {lds_ld<u32x4>(from), lds_ld<u32x4>(from + PLANE)};
     }
 };
+// Their transposes: rows 16 j + r, columns from block j (P) or j + 1 (A) on.
+template <int FIRST> struct Upper {
+    static constexpr int SHORT = 80, LONG = 144, PLANE = (16 * (2 * LONG + (2 - FIRST) * SHORT) + 511) / 512 * 512, BYTES = 2 * PLANE;
+    static DEVINL lds_t at(const lds_t base, const int j, const int r) { return base + (j < 2 ? (16 * j + r) * LONG : 32 * LONG + (16 * (j - 2) + r) * SHORT - 64); }
+    static DEVINL void put(const lds_t base, const int j, const int r, const int i, const int g, const Two& x) {
+        const lds_t to = at(base, j, r) + 64 * (i / 2) + 16 * g + 8 * (i % 2);
+        lds_st(to, x.h);
+        lds_st(to + PLANE, x.l);
+    }
+    // the lane's row of row block j: column block i, or blocks 2 s and 2 s + 1
+    static DEVINL Two one(const lds_t base, const int lane, const int j, const int i) {
+        const lds_t from = at(base, j, lane & 15) + 64 * (i / 2) + 16 * (lane >> 4) + 8 * (i % 2);
+        return {lds_ld<u32x2>(from), lds_ld<u32x2>(from + PLANE)};
+    }
+    static DEVINL Two32 two(const lds_t base, const int lane, const int j, const int s) {
+        const lds_t from = at(base, j, lane & 15) + 64 * s + 16 * (lane >> 4);
+        return {lds_ld<u32x4>(from), lds_ld<u32x4>(from + PLANE)};
+    }
+};
 // The inverses of the diagonal blocks of I + A, two planes each, rows of 32 bytes.
 struct Diagonal {
     static constexpr int PLANE = 512, BLOCK = 2 * PLANE, BYTES = 4 * BLOCK;
@@ -184,7 +220,7 @@ DEVINL double at_lane(const double x, const int lane) {
     return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
 // Scalars of a chunk (lane = token), by one wave.
-DEVINL void make_scalars(const lds_t to, const int lane, const DeltaToken token, const float gate, const float beta) {
+template <bool HEAD = false> DEVINL void make_scalars(const lds_t to, const int lane, const DeltaToken token, const float gate, const float beta) {
     double sum = token.cut || (token.real && gate < DELTA_NONE) ? CUT : (token.real ? static_cast<double>(gate) * 1.4426950408889634 : 0.0);
     sum += from_lane<0x111, 0xf>(sum);                          // row_shr 1, 2, 4, 8
     sum += from_lane<0x112, 0xf>(sum);
@@ -199,51 +235,63 @@ DEVINL void make_scalars(const lds_t to, const int lane, const DeltaToken token,
     lds_st(to + Scalars::BETA + 4 * lane, token.real ? beta : 0.f);
     lds_st(to + Scalars::ENTER + 4 * lane, __builtin_amdgcn_exp2f(h));
     lds_st(to + Scalars::LEAVE + 4 * lane, __builtin_amdgcn_exp2f(static_cast<float>(d - sum)));
-    lds_st(to + Scalars::TAIL + 4 * lane, __builtin_amdgcn_exp2f(static_cast<float>(end - sum)));
+    const double begin = lane < 16 ? 0.0 : (lane < 32 ? a : (lane < 48 ? b : c));
+    lds_st(to + Scalars::TAIL + 4 * lane, __builtin_amdgcn_exp2f(static_cast<float>(HEAD ? sum - begin : end - sum)));
 }
 
 // What HELPERS waves make of a chunk whose rows and scalars are there: -A, P and the inverses of the diagonal blocks.  Four have a block of 16 tokens on the diagonal each, four (the same, where there are no
 // more) the six blocks below, of A and P together: there D_ij = e^(G_i - G_end) e^(G_end - G_j) with `end` the last token of j's block, neither above 1 where no log decay is.
-template <class E, int D, int HELPERS> DEVINL void make_matrices(const lds_t K, const lds_t Q, const lds_t sc, const lds_t A, const lds_t P, const lds_t inv, const int wave, const int lane,
+// BACK: their transposes, and D_ij = e^(G_i - G_begin) e^(G_begin - G_j) with `begin` the token before i's block.
+template <class E, int D, int HELPERS, bool BACK> DEVINL void make_matrices(const lds_t K, const lds_t Q, const lds_t sc, const lds_t A, const lds_t P, const lds_t inv, const int wave, const int lane,
                                                                  const float scale) {
     const int col = lane & 15, grp = lane >> 4;
     if (HELPERS == 4 || wave >= 4) {
 #pragma unroll 1
         for (int n = wave & 3; n < 6; n += 4) {
-            const int i = n >= 3 ? 3 : (n >= 1 ? 2 : 1), j = n - i * (i - 1) / 2, token = 16 * i + col;
+            const int i = n >= 3 ? 3 : (n >= 1 ? 2 : 1), j = n - i * (i - 1) / 2, token = 16 * (BACK ? j : i) + col;
             f32x4 x = zero4(), y = zero4();
 #pragma unroll
             for (int s = 0; s < D / 32; ++s) {
-                const u32x4 k = Rows<D>::row(K, lane, j, s);
-                x = mma32<E>(k, Rows<D>::row(K, lane, i, s), x);
-                y = mma32<E>(k, Rows<D>::row(Q, lane, i, s), y);
+                const u32x4 k = Rows<D>::row(K, lane, j, s), ki = Rows<D>::row(K, lane, i, s), qi = Rows<D>::row(Q, lane, i, s);
+                x = BACK ? mma32<E>(ki, k, x) : mma32<E>(k, ki, x);
+                y = BACK ? mma32<E>(qi, k, y) : mma32<E>(k, qi, y);
             }
-            const lds_t end = sc + 4 * (16 * j + 15);
-            const float d = __builtin_amdgcn_exp2f((lds_ld<float>(sc + Scalars::SUM + 4 * token) - lds_ld<float>(end + Scalars::SUM)) + (lds_ld<float>(sc + Scalars::REST + 4 * token) - lds_ld<float>(end + Scalars::REST)));
-            const f32x4 tail = lds_ld<f32x4>(sc + Scalars::TAIL + 64 * j + 16 * grp);
-            const float beta = lds_ld<float>(sc + Scalars::BETA + 4 * token);
-            Lower<1>::put(A, i, col, j, grp, split<bf16_t>(x * (-beta * d) * tail));
-            Lower<0>::put(P, i, col, j, grp, split<bf16_t>(y * (scale * d) * tail));
+            const lds_t at = sc + 4 * token, ref = sc + 4 * (BACK ? 16 * i - 1 : 16 * j + 15);
+            const float up = (lds_ld<float>(at + Scalars::SUM) - lds_ld<float>(ref + Scalars::SUM)) + (lds_ld<float>(at + Scalars::REST) - lds_ld<float>(ref + Scalars::REST));
+            const float d = __builtin_amdgcn_exp2f(BACK ? -up : up);
+            const f32x4 tail = lds_ld<f32x4>(sc + Scalars::TAIL + 64 * (BACK ? i : j) + 16 * grp);
+            if constexpr (BACK) {
+                const f32x4 beta = lds_ld<f32x4>(sc + Scalars::BETA + 64 * i + 16 * grp);
+                Upper<1>::put(A, j, col, i, grp, split<bf16_t>(x * -d * tail * beta));
+                Upper<0>::put(P, j, col, i, grp, split<bf16_t>(y * (scale * d) * tail));
+            } else {
+                const float beta = lds_ld<float>(at + Scalars::BETA);
+                Lower<1>::put(A, i, col, j, grp, split<bf16_t>(x * (-beta * d) * tail));
+                Lower<0>::put(P, i, col, j, grp, split<bf16_t>(y * (scale * d) * tail));
+            }
         }
     }
     if (HELPERS == 4 || wave < 4) {
-        // A: rows 4 grp .. of the block, column lane & 15 (k_i.k_j is symmetric); P: row lane & 15, columns 4 grp ..
+        // A: rows 4 grp .. of the block, column lane & 15 (k_i.k_j is symmetric); P: row lane & 15, columns 4 grp ..; BACK: rows and columns the other way round
         f32x4 x = zero4(), y = zero4();
 #pragma unroll
         for (int s = 0; s < D / 32; ++s) {
-            const u32x4 k = Rows<D>::row(K, lane, wave, s);
+            const u32x4 k = Rows<D>::row(K, lane, wave, s), q = Rows<D>::row(Q, lane, wave, s);
             x = mma32<E>(k, k, x);
-            y = mma32<E>(k, Rows<D>::row(Q, lane, wave, s), y);
+            y = BACK ? mma32<E>(q, k, y) : mma32<E>(k, q, y);
         }
         const int token = 16 * wave + col;
         const float h = lds_ld<float>(sc + Scalars::SUM + 4 * token), l = lds_ld<float>(sc + Scalars::REST + 4 * token);
         const lds_t four = sc + 64 * wave + 16 * grp;
-        const f32x4 hj = lds_ld<f32x4>(four + Scalars::SUM) - h, lj = lds_ld<f32x4>(four + Scalars::REST) - l, beta = lds_ld<f32x4>(four + Scalars::BETA);
+        const f32x4 hj = lds_ld<f32x4>(four + Scalars::SUM) - h, lj = lds_ld<f32x4>(four + Scalars::REST) - l;
+        const f32x4 rows = lds_ld<f32x4>(four + Scalars::BETA);
+        const float row = lds_ld<float>(sc + Scalars::BETA + 4 * token);
         float m[16], z[16];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const float a = col < 4 * grp + r ? -beta[r] * __builtin_amdgcn_exp2f(hj[r] + lj[r]) * x[r] : 0.f;
-            y[r] = col >= 4 * grp + r ? scale * __builtin_amdgcn_exp2f(-hj[r] - lj[r]) * y[r] : 0.f;
+            const float down = __builtin_amdgcn_exp2f(hj[r] + lj[r]), up = __builtin_amdgcn_exp2f(-hj[r] - lj[r]);      // (one of them is used where it does not exceed 1)
+            const float a = BACK ? (col > 4 * grp + r ? -row * up * x[r] : 0.f) : (col < 4 * grp + r ? -rows[r] * down * x[r] : 0.f);
+            y[r] = BACK ? (col <= 4 * grp + r ? scale * down * y[r] : 0.f) : (col >= 4 * grp + r ? scale * up * y[r] : 0.f);
             // every group's rows to all groups
             const uint32_t u = __float_as_uint(a);
             const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
@@ -252,8 +300,9 @@ template <class E, int D, int HELPERS> DEVINL void make_matrices(const lds_t K, 
         }
 #pragma unroll
         for (int t = 0; t < 16; ++t) m[t] = t == col ? 1.f : 0.f;
-        solve_bc<true>(m, z);                                   // row lane & 15 of the inverse: m_s = -sum over t > s of m_t A_ts
-        Lower<0>::put(P, wave, col, wave, grp, split<bf16_t>(y));
+        solve_bc<!BACK>(m, z);                                  // row lane & 15 of the inverse: m_s = -sum over t > s of m_t A_ts; BACK: the column, m_s = -sum over t < s of A_st m_t
+        if constexpr (BACK) Upper<0>::put(P, wave, col, wave, grp, split<bf16_t>(y));
+        else Lower<0>::put(P, wave, col, wave, grp, split<bf16_t>(y));
         f32x4 o;
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[r] = grp == 0 ? m[r] : (grp == 1 ? m[4 + r] : (grp == 2 ? m[8 + r] : m[12 + r]));

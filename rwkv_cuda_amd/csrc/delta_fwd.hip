@@ -29,7 +29,9 @@ __global__ __launch_bounds__(64 * (SW + HELPERS)) void delta_fwd(const rwkv_delt
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, grp = lane >> 4;
 
     if (wave < SW) {
-        const int c0 = 16 * (piece * SW + wave);                 // its columns
+        const int ct = piece * SW + wave, c0 = 16 * ct;          // its columns
+        const DeltaTiles tiles(p);
+        float *states = static_cast<float*>(p.saved), *updates = states + tiles.states();
         const bool on = c0 + col < N;
         f32x4 S[D / 16];
         const float* s0 = p.s0 ? p.s0 + wide(hb) * N * N : nullptr;
@@ -45,6 +47,11 @@ __global__ __launch_bounds__(64 * (SW + HELPERS)) void delta_fwd(const rwkv_delt
             const lds_t rows = lds + (c & 1) * L::STAGE, mats = lds + L::MATRICES + (c & 1) * L::MATRIX_STAGE, sc = lds + L::SCALARS + c % 3 * Scalars::BYTES;
             const lds_t K = rows + L::K, Q = rows + L::Q, A = mats + L::A, P = mats + L::P, inv = mats + L::INV;
             typedef v4s __attribute__((address_space(3))) * ptr;
+            if (p.saved && c0 < N) {
+#pragma unroll
+                for (int t = 0; t < D / 16; ++t)
+                    if (t < tiles.tiles) *reinterpret_cast<f32x4*>(states + tiles.state(wide(hb) * chunks + c, ct, t) + 4 * lane) = S[t];
+            }
             // what a step reads from LDS is on its way a step earlier
             const Two inv0 = Diagonal::row(inv, lane, 0), a10 = Lower<1>::one(A, lane, 1, 0), inv1 = Diagonal::row(inv, lane, 1);
             f32x4 enter[4], beta[4], Z[4];
@@ -116,8 +123,7 @@ __global__ __launch_bounds__(64 * (SW + HELPERS)) void delta_fwd(const rwkv_delt
             queries(0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const f32x4 vf = {unpack_lo<E>(v[i][0]), unpack_hi<E>(v[i][0]), unpack_lo<E>(v[i][1]), unpack_hi<E>(v[i][1])};
-                Z[i] = beta[i] * (vf - enter[i] * s.back * Z[i]);
+                Z[i] = beta[i] * (four_of<E>(v[i]) - enter[i] * s.back * Z[i]);
             }
             U[0] = mma16(inv0, split<bf16_t>(Z[0]), zero4());
             outputs(0);
@@ -179,6 +185,10 @@ __global__ __launch_bounds__(64 * (SW + HELPERS)) void delta_fwd(const rwkv_delt
             Y[2] = mma16(u2, p22, Y[2]);
             u3 = split<bf16_t>(U[3]);
             Y[3] = mma32(join(u2, u3), p33, Y[3]);
+            if (p.saved && c0 < N) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) *reinterpret_cast<f32x4*>(updates + tiles.update(wide(hb) * chunks + c, ct, i) + 4 * lane) = U[i];
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int t = c * DELTA_CHUNK + 16 * i + col;
@@ -251,7 +261,7 @@ __global__ __launch_bounds__(64 * (SW + HELPERS)) void delta_fwd(const rwkv_delt
     };
     const auto matrices = [&](const int c) {
         const lds_t rows = lds + (c & 1) * L::STAGE, mats = lds + L::MATRICES + (c & 1) * L::MATRIX_STAGE;
-        make_matrices<E, D, HELPERS>(rows + L::K, rows + L::Q, lds + L::SCALARS + c % 3 * Scalars::BYTES, mats + L::A, mats + L::P, mats + L::INV, mine, lane, p.scale);
+        make_matrices<E, D, HELPERS, false>(rows + L::K, rows + L::Q, lds + L::SCALARS + c % 3 * Scalars::BYTES, mats + L::A, mats + L::P, mats + L::INV, mine, lane, p.scale);
     };
     load_scalars(0);
     load(0);

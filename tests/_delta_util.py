@@ -1,7 +1,7 @@
 """Helpers for the tests of the gated delta rule."""
 import torch
 
-from oracle.mixers import TINY, UNIT
+from oracle.mixers import LEAST, TINY, UNIT
 from _gpu_util import DEV
 from _mixers_util import randn
 
@@ -12,6 +12,8 @@ from _mixers_util import randn
 PAIRS = 2.0 ** -16
 # ... and for a single element up to 16 of these: it may be the sum of terms that are larger than itself, and the largest of some 10^6 errors is five of their root mean squares.
 SINGLE = 16
+# Decays below fp32's least normal number, 2^-126, are 0 to the hardware's exponential, so that 2^-126 of a state or gradient (here below 2^6 in magnitude), over up to 2^20 tokens, may be
+# lost: LEAST = 2^-100, as for the gated recurrence.
 
 
 def inputs(B, T, H, Hk, N, dt, seed=0, slow=3.0):
@@ -30,7 +32,7 @@ def near(name, got, want, steps=1.0):
     rms = float(want.square().mean().sqrt())
     u, tiny = UNIT[got.dtype], TINY[got.dtype]
     rounding = float((want.to(got.dtype).double() - want).square().mean().sqrt())
-    have, may = float(off.square().mean().sqrt()), rounding * 1.05 + steps * PAIRS * rms + tiny
-    single = (off / (u * want.abs() + tiny + SINGLE * steps * PAIRS * torch.maximum(want.abs(), torch.tensor(rms, device=want.device)) + 1e-30)).max() if off.numel() else 0.0
+    have, may = float(off.square().mean().sqrt()), rounding * 1.05 + steps * PAIRS * rms + tiny + LEAST
+    single = (off / (u * want.abs() + tiny + SINGLE * steps * PAIRS * torch.maximum(want.abs(), torch.tensor(rms, device=want.device)) + LEAST)).max() if off.numel() else 0.0
     print(f"  {name}: error {have:.3e} of {may:.3e}, an element at most {float(single):.3f} of its bound", flush=True)
     assert have <= may and float(single) <= 1.0, name
