@@ -239,77 +239,217 @@ template <bool HEAD = false> DEVINL void make_scalars(const lds_t to, const int 
     lds_st(to + Scalars::TAIL + 4 * lane, __builtin_amdgcn_exp2f(static_cast<float>(HEAD ? sum - begin : end - sum)));
 }
 
-// What HELPERS waves make of a chunk whose rows and scalars are there: -A, P and the inverses of the diagonal blocks.  Four have a block of 16 tokens on the diagonal each, four (the same, where there are no
-// more) the six blocks below, of A and P together: there D_ij = e^(G_i - G_end) e^(G_end - G_j) with `end` the last token of j's block, neither above 1 where no log decay is.
-// BACK: their transposes, and D_ij = e^(G_i - G_begin) e^(G_begin - G_j) with `begin` the token before i's block.
-template <class E, int D, int HELPERS, bool BACK> DEVINL void make_matrices(const lds_t K, const lds_t Q, const lds_t sc, const lds_t A, const lds_t P, const lds_t inv, const int wave, const int lane,
-                                                                 const float scale) {
+// Which of a chunk's matrices a helping wave makes, a rule on how many there are (8 waves a workgroup, of which 4, 2 or 1 walk: those come first, and the helpers with the least to do share their
+// SIMDs).  Bits 0 .. 5: the blocks below the diagonal, of A and P together, (1,0), (2,0), (2,1), (3,0), (3,1), (3,2); 6 .. 9: P's blocks on the diagonal; 10, 11: the inverses of blocks 0 and 1, of
+// 2 and 3; 12: the scalars.
+template <int HELPERS> DEVINL uint32_t tasks_of(const int wave) {
+    constexpr uint32_t INV0 = 1 << 10, INV1 = 1 << 11, SCALARS = 1 << 12;
+    if constexpr (HELPERS == 4) return wave == 0 ? INV0 | 0xc0 : (wave == 1 ? INV1 | 0x300 : (wave == 2 ? 0x07 | SCALARS : 0x38));
+    else if constexpr (HELPERS == 6) return wave == 0 ? INV0 : (wave == 1 ? INV1 : (wave == 2 ? 0x03 : (wave == 3 ? 0x04 | SCALARS : (wave == 4 ? 0x08 | 0xc0 : 0x30 | 0x300))));
+    else return wave == 0 ? INV0 : (wave == 1 ? INV1 : (wave == 2 ? 0x03 : (wave == 3 ? SCALARS : (wave == 4 ? 0x0c : (wave == 5 ? 0x10 | 0xc0 : 0x20 | 0x300)))));
+}
+
+// Those of a chunk whose rows and scalars are there.  Blocks below the diagonal: D_ij = e^(G_i - G_end) e^(G_end - G_j) with `end` the last token of j's block, neither above 1 where no log decay is.  Forward:
+// A without beta, and the inverses times beta (of their columns), so that the right side is V - e^G K S alone.  BACK: the transposes, and `end` is the token before i's block.
+template <class E, int D, bool BACK> DEVINL void make_matrices(const lds_t K, const lds_t Q, const lds_t sc, const lds_t A, const lds_t P, const lds_t inv, const uint32_t tasks, const int lane, const float scale) {
     const int col = lane & 15, grp = lane >> 4;
-    if (HELPERS == 4 || wave >= 4) {
+    const auto at = [&](const lds_t what, const int n) { return sc + what + 4 * n; };
 #pragma unroll 1
-        for (int n = wave & 3; n < 6; n += 4) {
-            const int i = n >= 3 ? 3 : (n >= 1 ? 2 : 1), j = n - i * (i - 1) / 2, token = 16 * (BACK ? j : i) + col;
-            f32x4 x = zero4(), y = zero4();
-#pragma unroll
-            for (int s = 0; s < D / 32; ++s) {
-                const u32x4 k = Rows<D>::row(K, lane, j, s), ki = Rows<D>::row(K, lane, i, s), qi = Rows<D>::row(Q, lane, i, s);
-                x = BACK ? mma32<E>(ki, k, x) : mma32<E>(k, ki, x);
-                y = BACK ? mma32<E>(qi, k, y) : mma32<E>(k, qi, y);
-            }
-            const lds_t at = sc + 4 * token, ref = sc + 4 * (BACK ? 16 * i - 1 : 16 * j + 15);
-            const float up = (lds_ld<float>(at + Scalars::SUM) - lds_ld<float>(ref + Scalars::SUM)) + (lds_ld<float>(at + Scalars::REST) - lds_ld<float>(ref + Scalars::REST));
-            const float d = __builtin_amdgcn_exp2f(BACK ? -up : up);
-            const f32x4 tail = lds_ld<f32x4>(sc + Scalars::TAIL + 64 * (BACK ? i : j) + 16 * grp);
-            if constexpr (BACK) {
-                const f32x4 beta = lds_ld<f32x4>(sc + Scalars::BETA + 64 * i + 16 * grp);
-                Upper<1>::put(A, j, col, i, grp, split<bf16_t>(x * -d * tail * beta));
-                Upper<0>::put(P, j, col, i, grp, split<bf16_t>(y * (scale * d) * tail));
-            } else {
-                const float beta = lds_ld<float>(at + Scalars::BETA);
-                Lower<1>::put(A, i, col, j, grp, split<bf16_t>(x * (-beta * d) * tail));
-                Lower<0>::put(P, i, col, j, grp, split<bf16_t>(y * (scale * d) * tail));
-            }
-        }
-    }
-    if (HELPERS == 4 || wave < 4) {
-        // A: rows 4 grp .. of the block, column lane & 15 (k_i.k_j is symmetric); P: row lane & 15, columns 4 grp ..; BACK: rows and columns the other way round
+    for (uint32_t left = tasks & 0x3f; left != 0; left &= left - 1) {
+        const int n = __builtin_ctz(left), i = n >= 3 ? 3 : (n >= 1 ? 2 : 1), j = n - i * (i - 1) / 2, token = 16 * (BACK ? j : i) + col;
         f32x4 x = zero4(), y = zero4();
 #pragma unroll
         for (int s = 0; s < D / 32; ++s) {
-            const u32x4 k = Rows<D>::row(K, lane, wave, s), q = Rows<D>::row(Q, lane, wave, s);
-            x = mma32<E>(k, k, x);
+            const u32x4 k = Rows<D>::row(K, lane, j, s), ki = Rows<D>::row(K, lane, i, s), qi = Rows<D>::row(Q, lane, i, s);
+            x = BACK ? mma32<E>(ki, k, x) : mma32<E>(k, ki, x);
+            y = BACK ? mma32<E>(qi, k, y) : mma32<E>(k, qi, y);
+        }
+        const int ref = BACK ? 16 * i - 1 : 16 * j + 15;
+        const float up = (lds_ld<float>(at(Scalars::SUM, token)) - lds_ld<float>(at(Scalars::SUM, ref))) + (lds_ld<float>(at(Scalars::REST, token)) - lds_ld<float>(at(Scalars::REST, ref)));
+        const float d = __builtin_amdgcn_exp2f(BACK ? -up : up);
+        const f32x4 tail = lds_ld<f32x4>(at(Scalars::TAIL, 16 * (BACK ? i : j) + 4 * grp)) * d;
+        if constexpr (BACK) {
+            Upper<1>::put(A, j, col, i, grp, split<bf16_t>(x * -tail * lds_ld<f32x4>(at(Scalars::BETA, 16 * i + 4 * grp))));
+            Upper<0>::put(P, j, col, i, grp, split<bf16_t>(y * scale * tail));
+        } else {
+            Lower<1>::put(A, i, col, j, grp, split<bf16_t>(x * -tail));
+            Lower<0>::put(P, i, col, j, grp, split<bf16_t>(y * scale * tail));
+        }
+    }
+#pragma unroll 1
+    for (uint32_t left = tasks >> 6 & 0xf; left != 0; left &= left - 1) {
+        const int w = __builtin_ctz(left);
+        f32x4 y = zero4();                                      // row lane & 15, columns 4 grp ..; BACK: the transpose's
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) {
+            const u32x4 k = Rows<D>::row(K, lane, w, s), q = Rows<D>::row(Q, lane, w, s);
             y = BACK ? mma32<E>(q, k, y) : mma32<E>(k, q, y);
         }
-        const int token = 16 * wave + col;
-        const float h = lds_ld<float>(sc + Scalars::SUM + 4 * token), l = lds_ld<float>(sc + Scalars::REST + 4 * token);
-        const lds_t four = sc + 64 * wave + 16 * grp;
-        const f32x4 hj = lds_ld<f32x4>(four + Scalars::SUM) - h, lj = lds_ld<f32x4>(four + Scalars::REST) - l;
-        const f32x4 rows = lds_ld<f32x4>(four + Scalars::BETA);
-        const float row = lds_ld<float>(sc + Scalars::BETA + 4 * token);
-        float m[16], z[16];
+        const float h = lds_ld<float>(at(Scalars::SUM, 16 * w + col)), l = lds_ld<float>(at(Scalars::REST, 16 * w + col));
+        const f32x4 hj = lds_ld<f32x4>(at(Scalars::SUM, 16 * w + 4 * grp)) - h, lj = lds_ld<f32x4>(at(Scalars::REST, 16 * w + 4 * grp)) - l;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const float down = __builtin_amdgcn_exp2f(hj[r] + lj[r]), up = __builtin_amdgcn_exp2f(-hj[r] - lj[r]);      // (one of them is used where it does not exceed 1)
-            const float a = BACK ? (col > 4 * grp + r ? -row * up * x[r] : 0.f) : (col < 4 * grp + r ? -rows[r] * down * x[r] : 0.f);
-            y[r] = BACK ? (col <= 4 * grp + r ? scale * down * y[r] : 0.f) : (col >= 4 * grp + r ? scale * up * y[r] : 0.f);
-            // every group's rows to all groups
-            const uint32_t u = __float_as_uint(a);
-            const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-            const auto even = __builtin_amdgcn_permlane32_swap(s[0], s[0], false, false), odd = __builtin_amdgcn_permlane32_swap(s[1], s[1], false, false);
-            z[r] = __uint_as_float(even[0]), z[8 + r] = __uint_as_float(even[1]), z[4 + r] = __uint_as_float(odd[0]), z[12 + r] = __uint_as_float(odd[1]);
+            const float d = __builtin_amdgcn_exp2f(BACK ? hj[r] + lj[r] : -hj[r] - lj[r]);
+            y[r] = (BACK ? col <= 4 * grp + r : col >= 4 * grp + r) ? scale * d * y[r] : 0.f;
+        }
+        if constexpr (BACK) Upper<0>::put(P, w, col, w, grp, split<bf16_t>(y));
+        else Lower<0>::put(P, w, col, w, grp, split<bf16_t>(y));
+    }
+    if (tasks >> 10 & 3) {                                       // blocks w and w + 1: at last one in the lanes' first half, one in the second
+        const int w = tasks >> 10 & 1 ? 0 : 2;
+        f32x4 a[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            f32x4 x = zero4();                                  // rows 4 grp .., column lane & 15 (k_i.k_j is symmetric); BACK: the other way round
+#pragma unroll
+            for (int s = 0; s < D / 32; ++s) {
+                const u32x4 k = Rows<D>::row(K, lane, w + e, s);
+                x = mma32<E>(k, k, x);
+            }
+            const int token = 16 * (w + e) + col, four = 16 * (w + e) + 4 * grp;
+            const float h = lds_ld<float>(at(Scalars::SUM, token)), l = lds_ld<float>(at(Scalars::REST, token));
+            const f32x4 hj = lds_ld<f32x4>(at(Scalars::SUM, four)) - h, lj = lds_ld<f32x4>(at(Scalars::REST, four)) - l, rows = lds_ld<f32x4>(at(Scalars::BETA, four));
+            const float row = lds_ld<float>(at(Scalars::BETA, token));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float d = __builtin_amdgcn_exp2f(BACK ? -hj[r] - lj[r] : hj[r] + lj[r]);
+                a[e][r] = (BACK ? col > 4 * grp + r : col < 4 * grp + r) ? -(BACK ? row : rows[r]) * d * x[r] : 0.f;
+            }
+        }
+        float m[16], z[16];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {                            // every group's rows to both groups of their block's half
+            const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(a[0][r]), __float_as_uint(a[1][r]), false, false);
+            const auto low = __builtin_amdgcn_permlane16_swap(s[0], s[0], false, false), high = __builtin_amdgcn_permlane16_swap(s[1], s[1], false, false);
+            z[r] = __uint_as_float(low[0]), z[4 + r] = __uint_as_float(low[1]), z[8 + r] = __uint_as_float(high[0]), z[12 + r] = __uint_as_float(high[1]);
         }
 #pragma unroll
         for (int t = 0; t < 16; ++t) m[t] = t == col ? 1.f : 0.f;
         solve_bc<!BACK>(m, z);                                  // row lane & 15 of the inverse: m_s = -sum over t > s of m_t A_ts; BACK: the column, m_s = -sum over t < s of A_st m_t
-        if constexpr (BACK) Upper<0>::put(P, wave, col, wave, grp, split<bf16_t>(y));
-        else Lower<0>::put(P, wave, col, wave, grp, split<bf16_t>(y));
-        f32x4 o;
+        const int block = w + (lane >> 5), half = grp & 1;       // of a row: the first or the last eight
+        const lds_t to = inv + block * Diagonal::BLOCK + col * 32 + 16 * half;
+        Two o[2];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = grp == 0 ? m[r] : (grp == 1 ? m[4 + r] : (grp == 2 ? m[8 + r] : m[12 + r]));
-        const Two w = split<bf16_t>(o);
-        lds_st(inv + wave * Diagonal::BLOCK + col * 32 + 8 * grp, w.h);
-        lds_st(inv + wave * Diagonal::BLOCK + Diagonal::PLANE + col * 32 + 8 * grp, w.l);
+        for (int e = 0; e < 2; ++e) {
+            f32x4 x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = half ? m[8 + 4 * e + r] : m[4 * e + r];
+            if constexpr (!BACK) x *= lds_ld<f32x4>(at(Scalars::BETA, 16 * block + 8 * half + 4 * e));
+            o[e] = split<bf16_t>(x);
+        }
+        lds_st(to, join(o[0].h, o[1].h));
+        lds_st(to + Diagonal::PLANE, join(o[0].l, o[1].l));
     }
+}
+
+// Where things are in a walking workgroup's LDS.  (Scalars are made a chunk earlier than what uses them.)
+template <int D, int SW, bool BACK> struct WalkPlace {
+    static constexpr int VPITCH = 32 * SW + 16;
+    static constexpr lds_t K = 0, Q = Rows<D>::BYTES, STAGE = 2 * Rows<D>::BYTES, V = 2 * STAGE, MATRICES = V + 64 * VPITCH, A = 0, P = BACK ? Upper<1>::BYTES : Lower<1>::BYTES,
+                           INV = P + (BACK ? Upper<0>::BYTES : Lower<0>::BYTES), MATRIX_STAGE = INV + Diagonal::BYTES, SCALARS = MATRICES + 2 * MATRIX_STAGE, BYTES = SCALARS + 3 * Scalars::BYTES;
+    static_assert(BYTES <= 160 * 1024);
+};
+
+// The helping waves of a walk: forward the chunks from the first on, with the values beside queries and keys; BACK from the last on, with the gradients of y.  Before the walkers' first barrier
+// a chunk's rows go to LDS, between it and the second the next chunk's matrices are made.
+template <class E, int D, int SW, int HELPERS, bool BACK> DEVINL void help(const rwkv_delta_args& p, const lds_t lds, const int b, const int h, const int hk, const int piece, const int mine, const int lane) {
+    using L = WalkPlace<D, SW, BACK>;
+    constexpr int LANES = 64 * HELPERS, RP = D / 8, KP = (64 * RP + LANES - 1) / LANES, VP = (64 * 2 * SW + LANES - 1) / LANES, KSTEP = LANES / RP, VSTEP = LANES / (2 * SW);       // 16 bytes a lane: pieces, rows between them
+    static_assert(LANES % RP == 0 && LANES % (2 * SW) == 0);
+    const int N = p.N, T = p.T, chunks = (T + DELTA_CHUNK - 1) / DELTA_CHUNK, tid = 64 * mine + lane;
+    const uint32_t tasks = tasks_of<HELPERS>(mine);
+    const int krow = tid / RP, kd = 8 * (tid % RP), vrow = tid / (2 * SW), vd = 16 * SW * piece + 8 * (tid % (2 * SW));
+    const bool kin = kd < N, vin = vd < N && (!BACK || p.dy);
+    const int64_t v_st = BACK ? wide(p.H) * N : p.v_st;
+    const auto first = [&](const int c) { return (BACK ? chunks - 1 - c : c) * DELTA_CHUNK; };
+    const E *k = static_cast<const E*>(p.k) + b * p.k_sb + hk * p.k_sh + (kin ? kd : 0), *q = static_cast<const E*>(p.q) + b * p.q_sb + hk * p.q_sh + (kin ? kd : 0);
+    const E* v = BACK ? static_cast<const E*>(p.dy) + (wide(b) * T * p.H + h) * N : static_cast<const E*>(p.v) + b * p.v_sb + h * p.v_sh;
+    if (BACK && !p.dy) v = q - (kin ? kd : 0);                   // (read, not used)
+    v += vin ? vd : 0;
+    const int64_t vs = BACK && !p.dy ? 0 : v_st;
+    u32x4 kr[KP], qr[KP], vr[VP];
+    const auto load = [&](const int c) {
+        const int t0 = first(c), most = T - 1 - t0;              // rows behind the last are read as it
+        const E *kc = k + wide(t0) * p.k_st, *qc = q + wide(t0) * p.q_st, *vc = v + wide(t0) * vs;
+#pragma unroll
+        for (int i = 0; i < KP; ++i) {
+            const int row = min(krow + KSTEP * i, min(most, 63));
+            kr[i] = *reinterpret_cast<const u32x4*>(kc + row * p.k_st);
+            qr[i] = *reinterpret_cast<const u32x4*>(qc + row * p.q_st);
+        }
+#pragma unroll
+        for (int i = 0; i < VP; ++i) vr[i] = *reinterpret_cast<const u32x4*>(vc + min(vrow + VSTEP * i, min(most, 63)) * vs);
+    };
+    const E *g = static_cast<const E*>(p.g) + b * p.g_sb + h, *beta = static_cast<const E*>(p.beta) + b * p.beta_sb + h;
+    E gate, bt;                                                  // (as they come: what is made of them here would wait for them)
+    int doc = 0, before = 0;
+    const auto load_scalars = [&](const int c) {
+        const int t = min(first(c) + lane, T - 1);
+        if (tasks >> 12) gate = g[t * p.g_st], bt = beta[t * p.beta_st];
+        if (p.doc) doc = p.doc[wide(b) * T + t], before = p.doc[wide(b) * T + max(t - 1, 0)];
+    };
+    uint64_t real;
+    const auto scalars = [&](const int c) {
+        const int t = first(c) + lane;
+        const bool is = t < T && doc >= 0;
+        real = __ballot(is);
+        if (tasks >> 12) make_scalars<BACK>(lds + L::SCALARS + c % 3 * Scalars::BYTES, lane, {is, is && t > 0 && doc != before}, to_f(gate), to_f(bt));
+    };
+    const auto mask_of = [&](const int row) { return 0u - static_cast<uint32_t>(real >> (row & 63) & 1); };      // all bits of a real token's, none of others
+    const auto put = [&](const int c) {
+        const lds_t to = lds + (c & 1) * L::STAGE;
+#pragma unroll
+        for (int i = 0; i < KP; ++i) {
+            const int row = krow + KSTEP * i;
+            if (64 * RP % LANES != 0 && i == KP - 1 && row >= 64) continue;
+            const uint32_t keep = kin ? mask_of(row) : 0;
+            Rows<D>::put(to + L::K, row, kd / 8, kr[i] & keep);
+            Rows<D>::put(to + L::Q, row, kd / 8, qr[i] & keep);
+        }
+    };
+    const auto put_values = [&] {
+#pragma unroll
+        for (int i = 0; i < VP; ++i) {
+            const int row = vrow + VSTEP * i;
+            if (64 * 2 * SW % LANES != 0 && i == VP - 1 && row >= 64) continue;
+            lds_st(lds + L::V + row * L::VPITCH + 16 * (tid % (2 * SW)), vr[i] & (vin ? mask_of(row) : 0));
+        }
+    };
+    const auto matrices = [&](const int c) {
+        const lds_t rows = lds + (c & 1) * L::STAGE, mats = lds + L::MATRICES + (c & 1) * L::MATRIX_STAGE;
+        make_matrices<E, D, BACK>(rows + L::K, rows + L::Q, lds + L::SCALARS + c % 3 * Scalars::BYTES, mats + L::A, mats + L::P, mats + L::INV, tasks, lane, p.scale);
+    };
+    load_scalars(0);
+    load(0);
+    scalars(0);
+    if (chunks > 1) load_scalars(1);
+    put(0);
+    put_values();
+    if (chunks > 1) load(1), scalars(1);
+    if (chunks > 2) load_scalars(2);
+    __syncthreads();
+    matrices(0);
+    __syncthreads();
+    for (int c = 0; c < chunks; ++c) {
+        const bool more = c + 1 < chunks;
+        if (more) put(c + 1);
+        __syncthreads();
+        if (more) {
+            put_values();                                        // (the walkers have read this chunk's)
+            if (c + 2 < chunks) load(c + 2);
+            matrices(c + 1);
+            if (c + 2 < chunks) scalars(c + 2);
+            if (c + 3 < chunks) load_scalars(c + 3);
+        }
+        __syncthreads();
+    }
+}
+// Columns a walking workgroup has, in tiles of 16: as many as leave a workgroup for every CU, so that matrices are made as seldom as may be.
+template <class Run> int walk_width(const rwkv_delta_args& p, Run run) {
+    const int64_t heads = static_cast<int64_t>(p.B) * p.H, tiles = (p.N + 15) / 16;
+    const auto enough = [&](int sw) { return heads * ((tiles + sw - 1) / sw) >= 256; };
+    if (enough(4)) return run(std::integral_constant<int, 4>{});
+    return enough(2) ? run(std::integral_constant<int, 2>{}) : run(std::integral_constant<int, 1>{});
 }
 
 }  // namespace

@@ -9,13 +9,6 @@
 namespace rwkv {
 namespace {
 
-template <int D, int SW> struct Place {
-    static constexpr int VPITCH = 32 * SW + 16;
-    static constexpr lds_t ROWS = 0, K = 0, Q = Rows<D>::BYTES, STAGE = 2 * Rows<D>::BYTES, V = 2 * STAGE, MATRICES = V + 64 * VPITCH, A = 0, P = Upper<1>::BYTES, INV = P + Upper<0>::BYTES,
-                           MATRIX_STAGE = INV + Diagonal::BYTES, SCALARS = MATRICES + 2 * MATRIX_STAGE, BYTES = SCALARS + 3 * Scalars::BYTES;
-    static_assert(BYTES <= 160 * 1024);
-};
-
 // a b + c with b the gradients of four tokens as they came: one number of bf16, or of fp16 made two
 template <class E> struct Gradients {
     Two x;
@@ -36,8 +29,8 @@ template <class E> DEVINL f32x4 gradients32(const Two32& a, const Gradients<E>& 
 }
 
 template <class E, int D, int SW, int HELPERS>
-__global__ __launch_bounds__(64 * (SW + HELPERS)) void delta_bwd(const rwkv_delta_args p, const int pieces, float* states, float* updates) {
-    using L = Place<D, SW>;
+__global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_delta_args p, const int pieces, float* states, float* updates) {
+    using L = WalkPlace<D, SW, true>;
     __shared__ __align__(16) char smem[L::BYTES];
     const lds_t lds = lds_of(smem);
     const int slot = blockIdx.x >> 3, piece = slot % pieces, hb = slot / pieces * 8 + (blockIdx.x & 7);
@@ -170,113 +163,25 @@ __global__ __launch_bounds__(64 * (SW + HELPERS)) void delta_bwd(const rwkv_delt
         return;
     }
 
-    // the helpers
-    const int tid = threadIdx.x - 64 * SW, mine = wave - SW;
-    constexpr int LANES = 64 * HELPERS, KP = (64 * D / 8 + LANES - 1) / LANES, VP = (64 * 2 * SW + LANES - 1) / LANES;       // pieces of 16 bytes a lane
-    const E *q = static_cast<const E*>(p.q) + b * p.q_sb + hk * p.q_sh, *k = static_cast<const E*>(p.k) + b * p.k_sb + hk * p.k_sh, *v = static_cast<const E*>(p.dy) + (wide(b) * T * p.H + h) * N;
-    const int64_t v_st = p.dy ? wide(p.H) * N : 0;
-    const E *g = static_cast<const E*>(p.g) + b * p.g_sb + h, *beta = static_cast<const E*>(p.beta) + b * p.beta_sb + h;
-    u32x4 kr[KP], qr[KP], vr[VP];
-    const auto load = [&](const int c) {
-        const int t0 = (chunks - 1 - c) * DELTA_CHUNK;
-#pragma unroll
-        for (int i = 0; i < KP; ++i) {
-            const int x = tid + LANES * i, row = x / (D / 8), d = 8 * (x % (D / 8));
-            const bool ok = t0 + row < T && d < N;
-            kr[i] = ok ? *reinterpret_cast<const u32x4*>(k + wide(t0 + row) * p.k_st + d) : u32x4{0, 0, 0, 0};
-            qr[i] = ok ? *reinterpret_cast<const u32x4*>(q + wide(t0 + row) * p.q_st + d) : u32x4{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int i = 0; i < VP; ++i) {
-            const int x = tid + LANES * i, row = x / (2 * SW), d = 16 * SW * piece + 8 * (x % (2 * SW));
-            vr[i] = p.dy && row < 64 && t0 + row < T && d < N ? *reinterpret_cast<const u32x4*>(v + wide(t0 + row) * v_st + d) : u32x4{0, 0, 0, 0};
-        }
-    };
-    E gate, bt;                                                  // (as they come: what is made of them here would wait for them)
-    int doc, before;
-    const auto load_scalars = [&](const int c) {
-        const int t = min((chunks - 1 - c) * DELTA_CHUNK + lane, T - 1);
-        gate = g[t * p.g_st];
-        bt = beta[t * p.beta_st];
-        if (p.doc) doc = p.doc[wide(b) * T + t], before = p.doc[wide(b) * T + max(t - 1, 0)];
-    };
-    uint64_t real;
-    const auto scalars = [&](const int c) {
-        const int t = (chunks - 1 - c) * DELTA_CHUNK + lane;
-        const bool is = t < T && (!p.doc || doc >= 0);
-        real = __ballot(is);
-        if (mine == HELPERS - 1) make_scalars<true>(lds + L::SCALARS + c % 3 * Scalars::BYTES, lane, {is, is && p.doc && t > 0 && doc != before}, to_f(gate), to_f(bt));   // (the wave with the fewest blocks)
-    };
-    static_assert(64 * D / 8 % LANES == 0);
-    const auto put = [&](const int c) {
-        const lds_t rows = lds + (c & 1) * L::STAGE;
-#pragma unroll
-        for (int i = 0; i < KP; ++i) {
-            const int x = tid + LANES * i, row = x / (D / 8), d = x % (D / 8);
-            const bool ok = real >> row & 1;
-            Rows<D>::put(rows + L::K, row, d, ok ? kr[i] : u32x4{0, 0, 0, 0});
-            Rows<D>::put(rows + L::Q, row, d, ok ? qr[i] : u32x4{0, 0, 0, 0});
-        }
-    };
-    const auto put_values = [&] {
-#pragma unroll
-        for (int i = 0; i < VP; ++i) {
-            const int x = tid + LANES * i, row = x / (2 * SW), d = x % (2 * SW);
-            if (row < 64) lds_st(lds + L::V + row * L::VPITCH + 16 * d, real >> row & 1 ? vr[i] : u32x4{0, 0, 0, 0});
-        }
-    };
-    const auto matrices = [&](const int c) {
-        const lds_t rows = lds + (c & 1) * L::STAGE, mats = lds + L::MATRICES + (c & 1) * L::MATRIX_STAGE;
-        make_matrices<E, D, HELPERS, true>(rows + L::K, rows + L::Q, lds + L::SCALARS + c % 3 * Scalars::BYTES, mats + L::A, mats + L::P, mats + L::INV, mine, lane, p.scale);
-    };
-    load_scalars(0);
-    load(0);
-    scalars(0);
-    if (chunks > 1) load_scalars(1);
-    put(0);
-    put_values();
-    if (chunks > 1) load(1), scalars(1);
-    if (chunks > 2) load_scalars(2);
-    __syncthreads();
-    matrices(0);
-    __syncthreads();
-    for (int c = 0; c < chunks; ++c) {
-        const bool more = c + 1 < chunks;
-        if (more) put(c + 1);
-        __syncthreads();
-        if (more) {
-            put_values();                                        // (the others have read this chunk's)
-            if (c + 2 < chunks) load(c + 2);
-            matrices(c + 1);
-            if (c + 2 < chunks) scalars(c + 2);
-            if (c + 3 < chunks) load_scalars(c + 3);
-        }
-        __syncthreads();
-    }
+    help<E, D, SW, HELPERS, true>(p, lds, b, h, hk, piece, wave - SW, lane);
 }
 
-template <class E, int D, int SW, int HELPERS> int run(hipStream_t st, const rwkv_delta_args& p, float* dS, float* dZ) {
-    const int pieces = (p.N + 16 * SW - 1) / (16 * SW);
-    const int64_t blocks = (static_cast<int64_t>(p.B) * p.H + 7) / 8 * 8 * pieces;
-    if (blocks > INT_MAX) return RWKV_ERR_SHAPE;
-    hipLaunchKernelGGL((delta_bwd<E, D, SW, HELPERS>), dim3(static_cast<unsigned>(blocks)), dim3(64 * (SW + HELPERS)), 0, st, p, pieces, dS, dZ);
-    return launch_status();
-}
-// Columns a workgroup has: as many as leave a workgroup for every CU, so that matrices are made as seldom as may be.
-template <class E, int D> int run_any(hipStream_t st, const rwkv_delta_args& p, float* dS, float* dZ) {
-    const int64_t heads = static_cast<int64_t>(p.B) * p.H, tiles = (p.N + 15) / 16;
-    const auto enough = [&](int sw) { return heads * ((tiles + sw - 1) / sw) >= 256; };
-    constexpr int HELPERS = D == 64 ? 8 : 4;
-    if (enough(4)) return run<E, D, 4, HELPERS>(st, p, dS, dZ);
-    if (enough(2)) return run<E, D, 2, HELPERS>(st, p, dS, dZ);
-    return run<E, D, 1, HELPERS>(st, p, dS, dZ);
+template <class E, int D> int run(hipStream_t st, const rwkv_delta_args& p, float* dS, float* dZ) {
+    return walk_width(p, [&](auto sw) {
+        constexpr int SW = decltype(sw)::value;
+        const int pieces = (p.N + 16 * SW - 1) / (16 * SW);
+        const int64_t blocks = (static_cast<int64_t>(p.B) * p.H + 7) / 8 * 8 * pieces;
+        if (blocks > INT_MAX) return static_cast<int>(RWKV_ERR_SHAPE);
+        hipLaunchKernelGGL((delta_bwd<E, D, SW, 8 - SW>), dim3(static_cast<unsigned>(blocks)), dim3(512), 0, st, p, pieces, dS, dZ);
+        return launch_status();
+    });
 }
 
 }  // namespace
 
 int launch_delta_bwd(hipStream_t st, const rwkv_delta_args& p, float* dS, float* dZ) {
-    if (p.dtype == RWKV_DTYPE_BF16) return p.N <= 64 ? run_any<bf16_t, 64>(st, p, dS, dZ) : run_any<bf16_t, 128>(st, p, dS, dZ);
-    return p.N <= 64 ? run_any<half_t, 64>(st, p, dS, dZ) : run_any<half_t, 128>(st, p, dS, dZ);
+    if (p.dtype == RWKV_DTYPE_BF16) return p.N <= 64 ? run<bf16_t, 64>(st, p, dS, dZ) : run<bf16_t, 128>(st, p, dS, dZ);
+    return p.N <= 64 ? run<half_t, 64>(st, p, dS, dZ) : run<half_t, 128>(st, p, dS, dZ);
 }
 
 }  // namespace rwkv

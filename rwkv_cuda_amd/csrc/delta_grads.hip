@@ -102,7 +102,7 @@ template <class E, int D> struct Place {
 };
 
 template <class E, int D>
-__global__ __launch_bounds__(4 * D) void delta_grads(const rwkv_delta_args p, const float* dS, const float* dZ, float* dq_of, float* dk_of) {
+__global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p, const float* dS, const float* dZ, float* dq_of, float* dk_of) {
     using L = Place<E, D>;
     constexpr int WAVES = L::WAVES, LANES = 64 * WAVES, OWN = (10 + WAVES - 1) / WAVES, PARTS = 8 / WAVES, PLANES = Input<E>::PLANES;
     __shared__ __align__(16) char smem[L::BYTES];
@@ -122,20 +122,6 @@ __global__ __launch_bounds__(4 * D) void delta_grads(const rwkv_delta_args p, co
     const DeltaToken token = delta_token(p.doc, wide(b) * T, t0 + lane, T);
     const uint64_t real = __ballot(token.real);
     const lds_t sc = lds + L::SCALARS;
-    if (wave == 0) make_scalars(sc, lane, token, gate, beta_t);
-#pragma unroll
-    for (int i = 0; i < 64 * D / 8 / LANES; ++i) {
-        const int x = tid + LANES * i, row = x / (D / 8), c = x % (D / 8);
-        const bool ok = (real >> row & 1) && 8 * c < N;
-        u32x4 o[PLANES];
-        planes_of<E>(ok ? *reinterpret_cast<const u32x4*>(k + wide(t0 + row) * p.k_st + 8 * c) : u32x4{0, 0, 0, 0}, o);
-#pragma unroll
-        for (int n = 0; n < PLANES; ++n) Rows<D>::put(lds + L::K + n * Rows<D>::BYTES, row, c, o[n]);
-        planes_of<E>(ok ? *reinterpret_cast<const u32x4*>(q + wide(t0 + row) * p.q_st + 8 * c) : u32x4{0, 0, 0, 0}, o);
-#pragma unroll
-        for (int n = 0; n < PLANES; ++n) Rows<D>::put(lds + L::Q + n * Rows<D>::BYTES, row, c, o[n]);
-    }
-
     // the contractions over value channels, 32 at a time
     f32x4 sr[2], dr[2], ur[PARTS], zr[PARTS];
     u32x4 yr[2];                                                 // (of y's gradients and of the values; one of them where there are lanes enough)
@@ -171,7 +157,28 @@ __global__ __launch_bounds__(4 * D) void delta_grads(const rwkv_delta_args p, co
     // block n of the lower triangle
     const auto row_of = [](const int n) { return n >= 6 ? 3 : (n >= 3 ? 2 : (n >= 1 ? 1 : 0)); };
     const auto column_of = [&](const int n) { return n - row_of(n) * (row_of(n) + 1) / 2; };
+    constexpr int PIECES = 64 * D / 8 / LANES;
+    u32x4 kr[PIECES], qr[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int x = tid + LANES * i, row = x / (D / 8), c = x % (D / 8);
+        const bool ok = (real >> row & 1) && 8 * c < N;
+        kr[i] = ok ? *reinterpret_cast<const u32x4*>(k + wide(t0 + row) * p.k_st + 8 * c) : u32x4{0, 0, 0, 0};
+        qr[i] = ok ? *reinterpret_cast<const u32x4*>(q + wide(t0 + row) * p.q_st + 8 * c) : u32x4{0, 0, 0, 0};
+    }
     load(0);
+    if (wave == 0) make_scalars(sc, lane, token, gate, beta_t);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int x = tid + LANES * i, row = x / (D / 8), c = x % (D / 8);
+        u32x4 o[PLANES];
+        planes_of<E>(kr[i], o);
+#pragma unroll
+        for (int n = 0; n < PLANES; ++n) Rows<D>::put(lds + L::K + n * Rows<D>::BYTES, row, c, o[n]);
+        planes_of<E>(qr[i], o);
+#pragma unroll
+        for (int n = 0; n < PLANES; ++n) Rows<D>::put(lds + L::Q + n * Rows<D>::BYTES, row, c, o[n]);
+    }
     for (int step = 0; step < steps; ++step) {
         __syncthreads();                                         // (the step before has been read)
 #pragma unroll
