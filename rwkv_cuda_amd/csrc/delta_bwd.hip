@@ -61,97 +61,112 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_d
                 for (int t = 0; t < D / 16; ++t)
                     if (t < tiles.tiles) *reinterpret_cast<f32x4*>(states + tiles.state(chunk, ct, t) + 4 * lane) = S[t];
             }
+            // what a step reads from LDS is on its way a step earlier
             u32x2 v[4];
             Beside<E, D / 16> s;
-            u32x4 x[4];
-            f32x4 X[4];
+            u32x4 kx[D / 32][4], kc[D / 16];
+            f32x4 X[4], Z[4], z[4], leave[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(vread + 16 * i * L::VPITCH)));
-                x[i] = Rows<D>::row(K, lane, i, 0);
-            }
+            for (int i = 0; i < 4; ++i) v[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(vread + 16 * i * L::VPITCH)));
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) kx[k][i] = Rows<D>::row(K, lane, i, k);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) leave[i] = lds_ld<f32x4>(sc + Scalars::LEAVE + 64 * i + 16 * grp);
             in_order();
             s.take(S);
             __syncthreads();                                     // (the gradients of y have been read)
+            const Two inv3 = Diagonal::row(inv, lane, 3), p33 = Upper<0>::one(P, lane, 3, 3);
+            const Two32 p2 = Upper<0>::two(P, lane, 2, 1);
+            const float whole = lds_ld<float>(sc + Scalars::ENTER + 4 * 63);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) X[i] = mma32<E>(x[i], s.lo(0), zero4());
+            for (int i = 0; i < 4; ++i) X[i] = mma32<E>(kx[0][i], s.lo(0), zero4());
 #pragma unroll
             for (int k = 0; k < D / 32; ++k) {
-                u32x4 next[4];
-                if (k + 1 < D / 32)
+                if (k > 0)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) next[i] = Rows<D>::row(K, lane, i, k + 1);
+                    for (int i = 0; i < 4; ++i) X[i] = mma32<E>(kx[k][i], s.lo(k), X[i]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) X[i] = mma32<E>(x[i], s.hi(k), X[i]);
-                if (k + 1 < D / 32)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] = next[i], X[i] = mma32<E>(x[i], s.lo(k + 1), X[i]);
-                in_order();
+                for (int i = 0; i < 4; ++i) X[i] = mma32<E>(kx[k][i], s.hi(k), X[i]);
             }
-            const Gradients<E> d0(v[0]), d1(v[1]), d2(v[2]), d3(v[3]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) X[i] *= lds_ld<f32x4>(sc + Scalars::LEAVE + 64 * i + 16 * grp) * s.back;
-            X[3] = gradients16(Upper<0>::one(P, lane, 3, 3), d3, X[3]);
-            X[2] = gradients32(Upper<0>::two(P, lane, 2, 1), d2, d3, X[2]);
+            in_order();
             // the triangular system; dS: what the queries leave, then what the keys take
-            f32x4 z[4];
-            const float whole = lds_ld<float>(sc + Scalars::ENTER + 4 * 63);
+            const Gradients<E> d0(v[0]), d1(v[1]), d2(v[2]), d3(v[3]);
             const auto factors = [&](const int i) { return lds_ld<f32x4>(sc + Scalars::ENTER + 64 * i + 16 * grp); };
-            const auto of_y = [&](const int i) { return four_of<E>(v[i]) * factors(i) * p.scale; };
-            const auto of_z = [&](const int i, const f32x4 dz) { return dz * factors(i) * -lds_ld<f32x4>(sc + Scalars::BETA + 64 * i + 16 * grp); };
-            const auto advance = [&](const lds_t from, const Beside<E, 2>& u, const int k, const float by) {
+            const auto betas = [&](const int i) { return lds_ld<f32x4>(sc + Scalars::BETA + 64 * i + 16 * grp); };
+            const auto columns = [&](const lds_t from, const int k) {
+#pragma unroll
+                for (int t = 0; t < D / 16; ++t) kc[t] = Rows<D>::col(from, lane, t, k);
+            };
+            const auto advance = [&](const Beside<E, 2>& u, const float by) {
 #pragma unroll
                 for (int t = 0; t < D / 16; t += 4) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = Rows<D>::col(from, lane, t + e, k);
+                    for (int e = 0; e < 4; ++e) z[e] = mma32<E>(kc[t + e], u.lo(0), zero4());
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) z[e] = mma32<E>(x[e], u.lo(0), zero4());
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) z[e] = mma32<E>(x[e], u.hi(0), z[e]);
+                    for (int e = 0; e < 4; ++e) z[e] = mma32<E>(kc[t + e], u.hi(0), z[e]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) S[t + e] = by * S[t + e] + z[e] * u.back;
                 }
             };
-            const auto leave = [&](const int i, const f32x4 dz) {
-                if (c0 < N) *reinterpret_cast<f32x4*>(updates + tiles.update(chunk, ct, i) + 4 * lane) = dz;
+            const auto keep = [&](const int i) {
+                if (c0 < N) *reinterpret_cast<f32x4*>(updates + tiles.update(chunk, ct, i) + 4 * lane) = Z[i];
             };
-            f32x4 Z[4];
             Beside<E, 2> w;
-            Z[3] = mma16(Diagonal::row(inv, lane, 3), split<bf16_t>(X[3]), zero4());
-            X[1] = gradients16(Upper<0>::one(P, lane, 1, 1), d1, X[1]);
-            X[1] = gradients32(Upper<0>::two(P, lane, 1, 1), d2, d3, X[1]);
-            w.take({of_y(2), of_y(3)});
-            advance(Q, w, 1, whole);
+            const Two p11 = Upper<0>::one(P, lane, 1, 1), a23 = Upper<1>::one(A, lane, 2, 3), inv2 = Diagonal::row(inv, lane, 2);
+            const Two32 p1 = Upper<0>::two(P, lane, 1, 1);
+            f32x4 fa = factors(2), fb = factors(3);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) X[i] *= leave[i] * s.back;
+            X[3] = gradients16(p33, d3, X[3]);
+            X[2] = gradients32(p2, d2, d3, X[2]);
+            Z[3] = mma16(inv3, split<bf16_t>(X[3]), zero4());
+            w.take({four_of<E>(v[2]) * fa * p.scale, four_of<E>(v[3]) * fb * p.scale});
             in_order();
+            columns(Q, 1);
+            const Two32 a1 = Upper<1>::two(A, lane, 1, 1), a0 = Upper<1>::two(A, lane, 0, 1);
             const Two z3 = split<bf16_t>(Z[3]);
-            X[2] = mma16(Upper<1>::one(A, lane, 2, 3), z3, X[2]);
-            X[0] = gradients32(Upper<0>::two(P, lane, 0, 0), d0, d1, X[0]);
-            X[0] = gradients32(Upper<0>::two(P, lane, 0, 1), d2, d3, X[0]);
+            X[2] = mma16(a23, z3, X[2]);
+            X[1] = gradients16(p11, d1, X[1]);
+            X[1] = gradients32(p1, d2, d3, X[1]);
             in_order();
-            Z[2] = mma16(Diagonal::row(inv, lane, 2), split<bf16_t>(X[2]), zero4());
-            w.take({of_y(0), of_y(1)});
-            advance(Q, w, 0, 1.f);
+            const Two32 p0 = Upper<0>::two(P, lane, 0, 0), p02 = Upper<0>::two(P, lane, 0, 1);
+            const Two inv1 = Diagonal::row(inv, lane, 1);
+            Z[2] = mma16(inv2, split<bf16_t>(X[2]), zero4());
+            advance(w, whole);
             in_order();
+            fa = factors(0), fb = factors(1);
+            columns(Q, 0);
             const Two z2 = split<bf16_t>(Z[2]);
             const Two32 z23 = join(z2, z3);
-            X[1] = mma32(Upper<1>::two(A, lane, 1, 1), z23, X[1]);
-            X[0] = mma32(Upper<1>::two(A, lane, 0, 1), z23, X[0]);
-            leave(3, Z[3]);
+            X[1] = mma32(a1, z23, X[1]);
+            X[0] = mma32(a0, z23, X[0]);
+            X[0] = gradients32(p0, d0, d1, X[0]);
+            X[0] = gradients32(p02, d2, d3, X[0]);
+            w.take({four_of<E>(v[0]) * fa * p.scale, four_of<E>(v[1]) * fb * p.scale});
+            keep(3);
             in_order();
-            Z[1] = mma16(Diagonal::row(inv, lane, 1), split<bf16_t>(X[1]), zero4());
-            leave(2, Z[2]);
-            w.take({of_z(2, Z[2]), of_z(3, Z[3])});
-            advance(K, w, 1, 1.f);
+            const Two a01 = Upper<1>::one(A, lane, 0, 1), inv0 = Diagonal::row(inv, lane, 0);
+            f32x4 ba = betas(2) * factors(2), bb = betas(3) * factors(3);
+            Z[1] = mma16(inv1, split<bf16_t>(X[1]), zero4());
+            advance(w, 1.f);
+            keep(2);
             in_order();
+            columns(K, 1);
             const Two z1 = split<bf16_t>(Z[1]);
-            X[0] = mma16(Upper<1>::one(A, lane, 0, 1), z1, X[0]);
-            leave(1, Z[1]);
+            X[0] = mma16(a01, z1, X[0]);
+            w.take({Z[2] * -ba, Z[3] * -bb});
             in_order();
-            Z[0] = mma16(Diagonal::row(inv, lane, 0), split<bf16_t>(X[0]), zero4());
+            ba = betas(0) * factors(0), bb = betas(1) * factors(1);
+            Z[0] = mma16(inv0, split<bf16_t>(X[0]), zero4());
+            advance(w, 1.f);
+            keep(1);
             in_order();
-            w.take({of_z(0, Z[0]), of_z(1, Z[1])});
-            advance(K, w, 0, 1.f);
-            leave(0, Z[0]);
+            columns(K, 0);
+            w.take({Z[0] * -ba, Z[1] * -bb});
+            advance(w, 1.f);
+            keep(0);
             __syncthreads();
         }
         if (on && p.ds0)
