@@ -33,8 +33,10 @@ DEVINL DeltaToken delta_token(const int* doc, const int64_t row, const int t, co
     return {d >= 0, d >= 0 && t > 0 && doc[row + t - 1] != d};
 }
 
-// What the forward keeps for the backward, and the backward for its last kernel, of each head and chunk: the state that enters (whose gradient leaves) and the updates (their gradients), fp32, as
-// the waves hold them: tiles of 16 by 16, four neighbouring rows of a column a lane, 16 bytes.  States: [column tile][row tile], updates [column tile][token tile].
+// What the forward keeps for the backward, and the backward for its last kernel, of each head and chunk, as the waves hold them: tiles of 16 by 16, four neighbouring rows of a column a lane, 16
+// bytes.  The state that enters (whose gradient leaves), fp32, [column tile][row tile], stored at a chunk's start, where its wave waits; and the updates (their gradients), [column tile][token tile],
+// as the two numbers that they were operands as, four first ones, then four second ones.  (fp16 alone, 11 bits, would halve the traffic, but states and updates cancel within a chunk wherever new
+// values replace old ones, and where these are the larger its error would be seen.)
 struct DeltaTiles {
     int tiles;                                                  // of 16 channels
     int64_t chunks;                                             // all of them
@@ -103,6 +105,7 @@ DEVINL float wave_max(float x) {
     const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
 }
+DEVINL void keep(float* to, const Two& x) { *reinterpret_cast<u32x4*>(to) = join(x.h, x.l); }
 // Tiles as operands beside an input of type E: bf16 as they are, fp16 times a power of two, whose inverse is what the product is to be multiplied with.
 template <class E, int TILES> struct Beside {
     Two x[TILES];

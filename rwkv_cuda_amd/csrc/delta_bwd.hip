@@ -110,9 +110,6 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_d
                     for (int e = 0; e < 4; ++e) S[t + e] = by * S[t + e] + z[e] * u.back;
                 }
             };
-            const auto keep = [&](const int i) {
-                if (c0 < N) *reinterpret_cast<f32x4*>(updates + tiles.update(chunk, ct, i) + 4 * lane) = Z[i];
-            };
             Beside<E, 2> w;
             const Two p11 = Upper<0>::one(P, lane, 1, 1), a23 = Upper<1>::one(A, lane, 2, 3), inv2 = Diagonal::row(inv, lane, 2);
             const Two32 p1 = Upper<0>::two(P, lane, 1, 1);
@@ -145,13 +142,11 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_d
             X[0] = gradients32(p0, d0, d1, X[0]);
             X[0] = gradients32(p02, d2, d3, X[0]);
             w.take({four_of<E>(v[0]) * fa * p.scale, four_of<E>(v[1]) * fb * p.scale});
-            keep(3);
             in_order();
             const Two a01 = Upper<1>::one(A, lane, 0, 1), inv0 = Diagonal::row(inv, lane, 0);
             f32x4 ba = betas(2) * factors(2), bb = betas(3) * factors(3);
             Z[1] = mma16(inv1, split<bf16_t>(X[1]), zero4());
             advance(w, 1.f);
-            keep(2);
             in_order();
             columns(K, 1);
             const Two z1 = split<bf16_t>(Z[1]);
@@ -161,12 +156,14 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_d
             ba = betas(0) * factors(0), bb = betas(1) * factors(1);
             Z[0] = mma16(inv0, split<bf16_t>(X[0]), zero4());
             advance(w, 1.f);
-            keep(1);
             in_order();
             columns(K, 0);
             w.take({Z[0] * -ba, Z[1] * -bb});
             advance(w, 1.f);
-            keep(0);
+            if (c0 < N) {
+                float* to = updates + tiles.update(chunk, ct, 0) + 4 * lane;
+                keep(to, split<bf16_t>(Z[0])), keep(to + 256, z1), keep(to + 512, z2), keep(to + 768, z3);
+            }
             __syncthreads();
         }
         if (on && p.ds0)

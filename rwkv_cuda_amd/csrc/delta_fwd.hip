@@ -172,8 +172,8 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_d
             u3 = split<bf16_t>(U[3]);
             Y[3] = mma32(join(u2, u3), p33, Y[3]);
             if (p.saved && c0 < N) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) *reinterpret_cast<f32x4*>(updates + tiles.update(wide(hb) * chunks + c, ct, i) + 4 * lane) = U[i];
+                float* to = updates + tiles.update(wide(hb) * chunks + c, ct, 0) + 4 * lane;
+                keep(to, u0), keep(to + 256, u1), keep(to + 512, u2), keep(to + 768, u3);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {

@@ -64,24 +64,42 @@ template <class E> DEVINL f32x4 mma_in(const Input<E>& a, const Input<E>& b, f32
     return mma32<bf16_t>(a.x[0], b.x[0], c);
 }
 
-// 32 value channels by WIDTH tokens or key channels in LDS, two planes
+// 32 value channels by WIDTH tokens or key channels in LDS, two planes.  Tiles of a row, and their halves, are exchanged with the row's number, so that neither the writes (16 rows, 16 bytes) nor the
+// reads (8 rows, 32 bytes) of half a wave meet in a bank.
 template <int WIDTH> struct Slice {
-    static constexpr int PITCH = 2 * WIDTH + 16, PLANE = 32 * PITCH, BYTES = 2 * PLANE;
-    static DEVINL void put(const lds_t base, const int lane, const int half, const int tile, const f32x4 x) {
-        const Two w = split<bf16_t>(x);
-        const lds_t to = base + (16 * half + (lane & 15)) * PITCH + 32 * tile + 8 * (lane >> 4);
-        lds_st(to, w.h);
-        lds_st(to + PLANE, w.l);
+    static constexpr int PITCH = 2 * WIDTH, PLANE = 32 * PITCH, BYTES = 2 * PLANE;
+    static DEVINL lds_t at(const lds_t base, const int row, const int tile, const int byte) {
+        return base + row * PITCH + 32 * (tile ^ (WIDTH == 64 ? row >> 1 & 3 : row & 7)) + (byte ^ (row >> 3 & 1) * 16);
     }
-    static DEVINL u32x4 plane(const lds_t base, const int lane, const int tile) {
+    static DEVINL void put(const lds_t base, const int lane, const int half, const int tile, const u32x4 x) {
+        const lds_t to = at(base, lane & 15, tile, 8 * (lane >> 4)) + 16 * half * PITCH;
+        lds_st(to, u32x2{x[0], x[1]});
+        lds_st(to + PLANE, u32x2{x[2], x[3]});
+    }
+    static DEVINL Two32 get(const lds_t base, const int lane, const int tile) {
         typedef v4s __attribute__((address_space(3))) * ptr;
-        const int l = lane & 15;
-        const lds_t at = base + (4 * (lane >> 4) + (l >> 2)) * PITCH + 32 * tile + 8 * (l & 3);
-        const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(at)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(at + 16 * PITCH));
-        return join(__builtin_bit_cast(u32x2, a), __builtin_bit_cast(u32x2, b));
+        const lds_t from = at(base, 4 * (lane >> 4) + (lane >> 2 & 3), tile, 8 * (lane & 3));
+        u32x2 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(from + (i & 1) * 16 * PITCH + (i >> 1) * PLANE)));
+        return {join(x[0], x[1]), join(x[2], x[3])};
     }
-    static DEVINL Two32 get(const lds_t base, const int lane, const int tile) { return {plane(base, lane, tile), plane(base + PLANE, lane, tile)}; }
 };
+// a lane's part of a kept state
+DEVINL u32x4 kept_state(const u32x4 x) {
+    const Two w = split<bf16_t>(__builtin_bit_cast(f32x4, x));
+    return join(w.h, w.l);
+}
+// the sum of products of two kept tiles' numbers
+DEVINL float dot(const uint32_t a, const uint32_t b, const float c) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, a), __builtin_bit_cast(bf16x2, b), c, false);
+}
+DEVINL float dot(const u32x4 a, const u32x4 b, float c) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) c = dot(a[i], b[i], dot(a[i], b[i + 2], dot(a[i + 2], b[i], c)));
+    return c;
+}
 // column block j, rows of blocks 2 s and 2 s + 1, of a Lower: the lane's column, the contraction over rows
 DEVINL u32x4 lower_column(const lds_t base, const int lane, const int j, const int s) {
     typedef v4s __attribute__((address_space(3))) * ptr;
@@ -94,17 +112,17 @@ DEVINL Two32 lower_columns(const lds_t base, const int lane, const int j, const 
 
 template <class E, int D> struct Place {
     static constexpr int PLANES = Input<E>::PLANES, WAVES = D / 16;
-    static constexpr lds_t K = 0, Q = K + PLANES * Rows<D>::BYTES, SLICES = Q + PLANES * Rows<D>::BYTES, DY = SLICES, V = DY + PLANES * Rows<32>::BYTES, U = V + PLANES * Rows<32>::BYTES, Z = U + Slice<64>::BYTES,
+    static constexpr lds_t K = 0, Q = K + PLANES * Rows<D>::BYTES, SLICES = Q + PLANES * Rows<D>::BYTES, DY = SLICES, U = DY + PLANES * Rows<32>::BYTES, Z = U + Slice<64>::BYTES,
                            S = Z + Slice<64>::BYTES, DS = S + Slice<D>::BYTES, SLICES_END = DS + Slice<D>::BYTES, P = SLICES, A = P + Lower<0>::BYTES, MATRICES_END = A + Lower<0>::BYTES,
-                           SCALARS = SLICES_END > MATRICES_END ? SLICES_END : MATRICES_END, ROW = SCALARS + Scalars::BYTES, COLUMN = ROW + 1024, BETA = COLUMN + 1024, VALUES = BETA + 1024, QUERIES = VALUES + 256,
-                           KEYS = QUERIES + 256 * WAVES, READS = KEYS + 256 * WAVES, STATES = READS + 256 * WAVES, BYTES = STATES + 64;
+                           SCALARS = SLICES_END > MATRICES_END ? SLICES_END : MATRICES_END, ROW = SCALARS + Scalars::BYTES, COLUMN = ROW + 1024, BETA = COLUMN + 1024, VALUES = BETA + 1024,
+                           QUERIES = VALUES + 512, KEYS = QUERIES + 256 * WAVES, READS = KEYS + 256 * WAVES, STATES = READS + 256 * WAVES, BYTES = STATES + 64;
     static_assert(BYTES <= 160 * 1024);
 };
 
 template <class E, int D>
 __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p, const float* dS, const float* dZ, float* dq_of, float* dk_of) {
     using L = Place<E, D>;
-    constexpr int WAVES = L::WAVES, LANES = 64 * WAVES, OWN = (10 + WAVES - 1) / WAVES, PARTS = 8 / WAVES, PLANES = Input<E>::PLANES;
+    constexpr int WAVES = L::WAVES, LANES = 64 * WAVES, OWN = 16 / WAVES, PARTS = 8 / WAVES, PLANES = Input<E>::PLANES;
     __shared__ __align__(16) char smem[L::BYTES];
     const lds_t lds = lds_of(smem);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, grp = lane >> 4;
@@ -113,120 +131,145 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
     const int hb = static_cast<int>(chunk / chunks), t0 = static_cast<int>(chunk % chunks) * DELTA_CHUNK, b = hb / p.H, h = hb % p.H, hk = h / (p.H / p.Hk);
     const DeltaTiles tiles(p);
     const float *states = static_cast<const float*>(p.saved), *updates = states + tiles.states();
-    const E *q = static_cast<const E*>(p.q) + b * p.q_sb + hk * p.q_sh, *k = static_cast<const E*>(p.k) + b * p.k_sb + hk * p.k_sh, *v = static_cast<const E*>(p.v) + b * p.v_sb + h * p.v_sh;
-    const E* dy = p.dy ? static_cast<const E*>(p.dy) + (wide(b) * T * p.H + h) * N : nullptr;
 
     // lane = token
     const int t = min(t0 + lane, T - 1);
     const float gate = to_f(static_cast<const E*>(p.g)[b * p.g_sb + t * p.g_st + h]), beta_t = to_f(static_cast<const E*>(p.beta)[b * p.beta_sb + t * p.beta_st + h]);
     const DeltaToken token = delta_token(p.doc, wide(b) * T, t0 + lane, T);
     const uint64_t real = __ballot(token.real);
+    const auto mask_of = [&](const int row) { return 0u - static_cast<uint32_t>(real >> (row & 63) & 1); };
     const lds_t sc = lds + L::SCALARS;
-    // the contractions over value channels, 32 at a time
-    f32x4 sr[2], dr[2], ur[PARTS], zr[PARTS];
-    u32x4 yr[2];                                                 // (of y's gradients and of the values; one of them where there are lanes enough)
-    const auto load = [&](const int step) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int ct = 2 * step + e;
-            const bool is = ct < tiles.tiles && wave < tiles.tiles;
-            sr[e] = is ? *reinterpret_cast<const f32x4*>(states + tiles.state(chunk, ct, wave) + 4 * lane) : zero4();
-            dr[e] = is ? *reinterpret_cast<const f32x4*>(dS + tiles.state(chunk, ct, wave) + 4 * lane) : zero4();
-        }
-#pragma unroll
-        for (int m = 0; m < PARTS; ++m) {
-            const int n = wave + WAVES * m, ct = 2 * step + n / 4;
-            ur[m] = ct < tiles.tiles ? *reinterpret_cast<const f32x4*>(updates + tiles.update(chunk, ct, n % 4) + 4 * lane) : zero4();
-            zr[m] = ct < tiles.tiles ? *reinterpret_cast<const f32x4*>(dZ + tiles.update(chunk, ct, n % 4) + 4 * lane) : zero4();
-        }
-#pragma unroll
-        for (int m = 0; m < (WAVES == 4 ? 2 : 1); ++m) {
-            const int x = tid & 255, row = x / 4, c = 32 * step + 8 * (x % 4);
-            const bool values = WAVES == 4 ? m == 1 : tid >= 256, ok = (real >> row & 1) && c < N && (values || dy);
-            const E* from = values ? v + wide(t0 + row) * p.v_st + c : dy + wide(t0 + row) * p.H * N + c;
-            yr[m] = ok ? *reinterpret_cast<const u32x4*>(from) : u32x4{0, 0, 0, 0};
-        }
-    };
-    const int steps = (tiles.tiles + 1) / 2;
-    f32x4 dQ[4], dK[4], R[4], dP[OWN], dA[OWN], vz = zero4();
-    float both = 0.f;                                            // of <dS', S>
-#pragma unroll
-    for (int i = 0; i < 4; ++i) dQ[i] = dK[i] = R[i] = zero4();
-#pragma unroll
-    for (int m = 0; m < OWN; ++m) dP[m] = dA[m] = zero4();
-    // block n of the lower triangle
-    const auto row_of = [](const int n) { return n >= 6 ? 3 : (n >= 3 ? 2 : (n >= 1 ? 1 : 0)); };
-    const auto column_of = [&](const int n) { return n - row_of(n) * (row_of(n) + 1) / 2; };
-    constexpr int PIECES = 64 * D / 8 / LANES;
+
+    // rows of inputs, 16 bytes a lane, BELOW rows from piece to piece; of rows behind the last and channels that are not there others are read, and masked
+    constexpr int PIECES = 64 * D / 8 / LANES, BELOW = LANES / (D / 8);
+    const int row0 = tid / (D / 8), d0 = 8 * (tid % (D / 8)), most = T - 1 - t0;
+    const bool in = d0 < N;
     u32x4 kr[PIECES], qr[PIECES];
+    {
+        const E *k = static_cast<const E*>(p.k) + b * p.k_sb + hk * p.k_sh + wide(t0) * p.k_st + (in ? d0 : 0), *q = static_cast<const E*>(p.q) + b * p.q_sb + hk * p.q_sh + wide(t0) * p.q_st + (in ? d0 : 0);
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-        const int x = tid + LANES * i, row = x / (D / 8), c = x % (D / 8);
-        const bool ok = (real >> row & 1) && 8 * c < N;
-        kr[i] = ok ? *reinterpret_cast<const u32x4*>(k + wide(t0 + row) * p.k_st + 8 * c) : u32x4{0, 0, 0, 0};
-        qr[i] = ok ? *reinterpret_cast<const u32x4*>(q + wide(t0 + row) * p.q_st + 8 * c) : u32x4{0, 0, 0, 0};
+        for (int i = 0; i < PIECES; ++i) {
+            const int row = min(row0 + BELOW * i, most);
+            kr[i] = *reinterpret_cast<const u32x4*>(k + row * p.k_st);
+            qr[i] = *reinterpret_cast<const u32x4*>(q + row * p.q_st);
+        }
     }
-    load(0);
-    if (wave == 0) make_scalars(sc, lane, token, gate, beta_t);
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-        const int x = tid + LANES * i, row = x / (D / 8), c = x % (D / 8);
-        u32x4 o[PLANES];
-        planes_of<E>(kr[i], o);
-#pragma unroll
-        for (int n = 0; n < PLANES; ++n) Rows<D>::put(lds + L::K + n * Rows<D>::BYTES, row, c, o[n]);
-        planes_of<E>(qr[i], o);
-#pragma unroll
-        for (int n = 0; n < PLANES; ++n) Rows<D>::put(lds + L::Q + n * Rows<D>::BYTES, row, c, o[n]);
-    }
-    for (int step = 0; step < steps; ++step) {
-        __syncthreads();                                         // (the step before has been read)
+    // the contractions over value channels, 32 at a time: a wave brings a tile of 32 of either state, and PARTS tiles of updates and of their gradients
+    u32x4 sr[2], dr[2], ur[PARTS], zr[PARTS], yr;
+    // ... and has 16 tokens of the values and of their gradients, all 8 or 4 value channels of the 32 in a lane
+    constexpr int OWNS = WAVES == 4 ? 2 : 1;
+    const int own = 16 * (wave & 3) + col, part = wave >> 2;
+    u32x2 vr[OWNS];
+    const E* v = static_cast<const E*>(p.v) + b * p.v_sb + h * p.v_sh + (t0 + min(own, most)) * p.v_st;
+    const E* dy = p.dy ? static_cast<const E*>(p.dy) + ((wide(b) * T + t0 + min((tid & 255) / 4, most)) * p.H + h) * N : v;      // (without one the values are read, and not used)
+    E* dv = static_cast<E*>(p.dv) + ((wide(b) * T + t0 + own) * p.H + h) * N;
+    const auto load = [&](const int step) {
+        const int row = min(wave, tiles.tiles - 1);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            Slice<D>::put(lds + L::S, lane, e, wave, sr[e]);
-            Slice<D>::put(lds + L::DS, lane, e, wave, dr[e]);
-            both += sum4(sr[e] * dr[e]);
+            const int64_t from = tiles.state(chunk, min(2 * step + e, tiles.tiles - 1), row) + 4 * lane;
+            sr[e] = *reinterpret_cast<const u32x4*>(states + from);
+            dr[e] = *reinterpret_cast<const u32x4*>(dS + from);
         }
 #pragma unroll
         for (int m = 0; m < PARTS; ++m) {
             const int n = wave + WAVES * m;
-            Slice<64>::put(lds + L::U, lane, n / 4, n % 4, ur[m]);
-            Slice<64>::put(lds + L::Z, lane, n / 4, n % 4, zr[m]);
+            const int64_t from = tiles.update(chunk, min(2 * step + n / 4, tiles.tiles - 1), n % 4) + 4 * lane;
+            ur[m] = *reinterpret_cast<const u32x4*>(updates + from);
+            zr[m] = *reinterpret_cast<const u32x4*>(dZ + from);
+        }
+        if (tid < 256) {
+            const int c = 32 * step + 8 * (tid % 4);
+            yr = *reinterpret_cast<const u32x4*>(dy + (c < N ? c : 0));
         }
 #pragma unroll
-        for (int m = 0; m < (WAVES == 4 ? 2 : 1); ++m) {
-            const int x = tid & 255;
-            const bool values = WAVES == 4 ? m == 1 : tid >= 256;
+        for (int e = 0; e < OWNS; ++e) {
+            const int c = 32 * step + 16 * (part + e) + 4 * grp;
+            vr[e] = *reinterpret_cast<const u32x2*>(v + (c < N ? c : 0));
+        }
+    };
+    load(0);
+    if (wave == 0) make_scalars(sc, lane, token, gate, beta_t);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int row = row0 + BELOW * i;
+        const uint32_t mask = in ? mask_of(row) : 0;
+        u32x4 o[PLANES];
+        planes_of<E>(kr[i] & mask, o);
+#pragma unroll
+        for (int n = 0; n < PLANES; ++n) Rows<D>::put(lds + L::K + n * Rows<D>::BYTES, row, d0 / 8, o[n]);
+        planes_of<E>(qr[i] & mask, o);
+#pragma unroll
+        for (int n = 0; n < PLANES; ++n) Rows<D>::put(lds + L::Q + n * Rows<D>::BYTES, row, d0 / 8, o[n]);
+    }
+    const uint32_t y_mask = p.dy ? mask_of((tid & 255) / 4) : 0, v_mask = mask_of(own);
+    f32x4 dQ[4], dK[4], R[4], dP[OWN], dA[OWN];
+    float both = 0.f, vz = 0.f;                                  // of <dS', S>; of dZ V^T the diagonal
+    // The pairs' blocks of row block `pi`: column blocks pj(0), pj(1) .. up to it
+    const int pi = wave & 3;
+    const auto pj = [&](const int m) { return WAVES == 4 ? m : 2 * m + part; };
+#pragma unroll
+    for (int step = 0; step < D / 32; ++step) {
+        if (32 * step >= N) continue;
+        const auto add = [&](const f32x4& c) { return step ? c : zero4(); };
+        __syncthreads();                                         // (the step before has been read)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint32_t mask = 2 * step + e < tiles.tiles && wave < tiles.tiles ? ~0u : 0;
+            const u32x4 x = kept_state(sr[e] & mask), y = kept_state(dr[e] & mask);
+            Slice<D>::put(lds + L::S, lane, e, wave, x);
+            Slice<D>::put(lds + L::DS, lane, e, wave, y);
+            both = dot(x, y, both);
+        }
+#pragma unroll
+        for (int m = 0; m < PARTS; ++m) {
+            const int n = wave + WAVES * m;
+            const uint32_t mask = 2 * step + n / 4 < tiles.tiles ? ~0u : 0;
+            Slice<64>::put(lds + L::U, lane, n / 4, n % 4, ur[m] & mask);
+            Slice<64>::put(lds + L::Z, lane, n / 4, n % 4, zr[m] & mask);
+        }
+        if (tid < 256) {
             u32x4 o[PLANES];
-            planes_of<E>(yr[m], o);
+            planes_of<E>(yr & (32 * step + 8 * (tid % 4) < N ? y_mask : 0), o);
 #pragma unroll
-            for (int n = 0; n < PLANES; ++n) Rows<32>::put(lds + (values ? L::V : L::DY) + n * Rows<32>::BYTES, x / 4, x % 4, o[n]);
+            for (int n = 0; n < PLANES; ++n) Rows<32>::put(lds + L::DY + n * Rows<32>::BYTES, tid / 4, tid % 4, o[n]);
         }
+        f32x4 values[OWNS];
+#pragma unroll
+        for (int e = 0; e < OWNS; ++e) values[e] = four_of<E>(vr[e] & (32 * step + 16 * (part + e) + 4 * grp < N ? v_mask : 0));
         __syncthreads();
-        if (step + 1 < steps) load(step + 1);
+        if (32 * (step + 1) < N) load(step + 1);
         const Two32 s = Slice<D>::get(lds + L::S, lane, wave), ds = Slice<D>::get(lds + L::DS, lane, wave);
+        const auto gradient = [&](const int i) {
+            Input<E> y;
+            y.read(Rows<32>::BYTES, lds + L::DY, [&](const lds_t at) { return Rows<32>::row(at, lane, i, 0); });
+            return y;
+        };
+        Two32 u[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            Input<E> y;
-            y.read(Rows<32>::BYTES, lds + L::DY, [&](const lds_t at) { return Rows<32>::row(at, lane, i, 0); });
-            dQ[i] = mma_in<E>(s, y, dQ[i]);
-            dK[i] = mma32(ds, Slice<64>::get(lds + L::U, lane, i), dK[i]);
-            R[i] = mma32(s, Slice<64>::get(lds + L::Z, lane, i), R[i]);
+            u[i] = Slice<64>::get(lds + L::U, lane, i);
+            dQ[i] = mma_in<E>(s, gradient(i), add(dQ[i]));
+            dK[i] = mma32(ds, u[i], add(dK[i]));
+            R[i] = mma32(s, Slice<64>::get(lds + L::Z, lane, i), add(R[i]));
         }
+        const Input<E> y = gradient(pi);
+        const Two32 z = Slice<64>::get(lds + L::Z, lane, pi);
 #pragma unroll
         for (int m = 0; m < OWN; ++m) {
-            const int n = wave + WAVES * m, i = row_of(n), j = column_of(n);
-            if (n >= 10) continue;
-            const Two32 u = Slice<64>::get(lds + L::U, lane, j);
-            Input<E> y;
-            y.read(Rows<32>::BYTES, lds + L::DY, [&](const lds_t at) { return Rows<32>::row(at, lane, i, 0); });
-            dP[m] = mma_in<E>(u, y, dP[m]);
-            dA[m] = mma32(u, Slice<64>::get(lds + L::Z, lane, i), dA[m]);
+            if (pj(m) > pi) continue;
+            const Two32 uj = WAVES == 4 ? u[m] : (part ? u[2 * m + 1] : u[2 * m]);
+            dP[m] = mma_in<E>(uj, y, add(dP[m]));
+            dA[m] = mma32(uj, z, add(dA[m]));
         }
-        if (wave < 4) {                                          // of dZ V^T the diagonal counts
-            Input<E> y;
-            y.read(Rows<32>::BYTES, lds + L::V, [&](const lds_t at) { return Rows<32>::row(at, lane, wave, 0); });
-            vz = mma_in<E>(y, Slice<64>::get(lds + L::Z, lane, wave), vz);
+        const float beta = lds_ld<float>(sc + Scalars::BETA + 4 * own);
+#pragma unroll
+        for (int e = 0; e < OWNS; ++e) {
+            const int w = WAVES == 4 ? e : part, c = 32 * step + 16 * w + 4 * grp;
+            const u32x2 zh = w ? u32x2{z.h[2], z.h[3]} : u32x2{z.h[0], z.h[1]}, zl = w ? u32x2{z.l[2], z.l[3]} : u32x2{z.l[0], z.l[1]};
+            const f32x4 x = four_of<bf16_t>(zh) + four_of<bf16_t>(zl);
+            vz += sum4(x * values[e]);
+            if (c < N && own <= most) *reinterpret_cast<u32x2*>(dv + c) = u32x2{pack2<E>(beta * x[0], beta * x[1]), pack2<E>(beta * x[2], beta * x[3])};
         }
     }
     __syncthreads();
@@ -235,8 +278,8 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
     const auto at = [&](const lds_t what, const int n) { return sc + what + 4 * n; };
 #pragma unroll
     for (int m = 0; m < OWN; ++m) {
-        const int n = wave + WAVES * m, i = row_of(n), j = column_of(n), ti = 16 * i + col, tj = 16 * j + 4 * grp;
-        if (n >= 10) continue;
+        const int i = pi, j = pj(m), ti = 16 * i + col, tj = 16 * j + 4 * grp;
+        if (j > i) continue;
         f32x4 kk = zero4(), qk = zero4();
 #pragma unroll
         for (int s = 0; s < D / 32; ++s) {
@@ -283,10 +326,8 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
         Lower<0>::put(lds + L::P, 2 * wave, col, 2 * wave + 1, grp, none);
         Lower<0>::put(lds + L::A, 2 * wave, col, 2 * wave + 1, grp, none);
     }
-    if (wave < 4 && col >> 2 == grp) {
-        const float x = (col & 3) == 0 ? vz[0] : ((col & 3) == 1 ? vz[1] : ((col & 3) == 2 ? vz[2] : vz[3]));
-        lds_st(lds + L::VALUES + 4 * (16 * wave + col), x);
-    }
+    vz = group_sum4(vz);
+    if (grp == 0) lds_st(lds + L::VALUES + 256 * part + 4 * own, vz);
     const float all = group_sum4(row_sum(both));
     if (lane == 0) lds_st(lds + L::STATES + 4 * wave, all);
     __syncthreads();
@@ -341,20 +382,9 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
             *reinterpret_cast<u32x2*>(static_cast<E*>(p.dk) + to) = u32x2{pack2<E>(dK[i][0], dK[i][1]), pack2<E>(dK[i][2], dK[i][3])};
         }
     }
-    // dv: 16 value channels a wave, as the updates lie
-    for (int ct = wave; ct < tiles.tiles; ct += WAVES)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const f32x4 z = *reinterpret_cast<const f32x4*>(dZ + tiles.update(chunk, ct, i) + 4 * lane) * lds_ld<f32x4>(at(Scalars::BETA, 16 * i + 4 * grp));
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int tt = t0 + 16 * i + 4 * grp + r;
-                if (tt < T && 16 * ct + col < N) static_cast<E*>(p.dv)[((wide(b) * T + tt) * p.H + h) * N + 16 * ct + col] = from_f<E>(z[r]);
-            }
-        }
     __syncthreads();
     if (wave != 0 || t0 + lane >= T) return;
-    float after = 0.f, before = 0.f, reads = 0.f, db = lds_ld<float>(lds + L::VALUES + 4 * lane), ends = 0.f;
+    float after = 0.f, before = 0.f, reads = 0.f, db = lds_ld<float>(lds + L::VALUES + 4 * lane) + (WAVES == 8 ? lds_ld<float>(lds + L::VALUES + 256 + 4 * lane) : 0.f), ends = 0.f;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
         after += lds_ld<float>(lds + L::QUERIES + 256 * w + 4 * lane);
