@@ -9,6 +9,17 @@
 namespace rwkv {
 namespace {
 
+DEVINL u32x4 join(const u32x2 a, const u32x2 b) { return u32x4{a[0], a[1], b[0], b[1]}; }
+template <int HOW> DEVINL float other_lane(const float x) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), HOW, 0xf, 0xf, true)); }
+// over 16 lanes: rotations by 8, 4, 2 and 1
+DEVINL float row_max(float x) {
+    x = fmaxf(x, other_lane<0x128>(x)), x = fmaxf(x, other_lane<0x124>(x)), x = fmaxf(x, other_lane<0x122>(x));
+    return fmaxf(x, other_lane<0x121>(x));
+}
+DEVINL float row_add(float x) {
+    x += other_lane<0x128>(x), x += other_lane<0x124>(x), x += other_lane<0x122>(x);
+    return x + other_lane<0x121>(x);
+}
 // codes 4 x .. 4 x + 3 of a register as two registers of E
 template <class E> DEVINL u32x2 widen(const uint32_t x) {
     if constexpr (std::is_same_v<E, bf16_t>)
@@ -196,9 +207,249 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged8_attn(const rwkv_paged8_a
     }
 }
 
-// Heads are dealt out as over 16 bits (group_of in paged.hip), with rows of half the bytes.
+// The same for at most 8 query heads of a key head, 64 tokens a step.  There a product of 16 keys and 16 heads would have empty columns, and the softmax, which costs most of the instructions, would
+// run over them; so the heads' side of the product has the heads once for each of TILES tiles of 16 tokens, in rows of their own, zero elsewhere, and TILES products add up to scores that fill the
+// lanes: 4 tiles of one or two heads (a lane has a token, and R heads), or 2 tiles of up to 8 (R = 4).  A lane has its own token's scales.  The weights go to the other product through LDS, 128 bytes a head.
+template <class E, int D, int TILES, int R>
+__global__ __launch_bounds__(64 * WAVES, 2) void paged8_few(const rwkv_paged8_args p, const int shift, const int pieces, const int group, const int shares, float* part) {
+    constexpr int PER = 16 / TILES, SETS = 4 / TILES, TOKENS = 64, ROWS = 64 / (D / 16), VSTEPS = TOKENS / ROWS, WPITCH = 2 * TOKENS + 16;
+    __shared__ __align__(16) char smem[WAVES * STEP * 2 * D];
+    __shared__ __align__(16) char weights[WAVES][PER * WPITCH];
+    __shared__ float top_of[WAVES][PER], sum_of[WAVES][PER];
+    const int slot = group > 1 ? blockIdx.x >> 3 : blockIdx.x, share = group > 1 ? slot / group * 8 + (blockIdx.x & 7) : slot;
+    if (share >= shares) return;
+    const int of_piece = p.Hk / max(group, 1);
+    const int hk = group == 0 ? share / pieces % p.Hk : share % of_piece * group + slot % group, piece = group == 0 ? share % pieces : share / of_piece % pieces;
+    const int b = share / of_piece / pieces, G = p.H / p.Hk;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, grp = lane >> 4;
+    const int all = p.lens[b], n = tokens_of(p, b, shift), size = piece_of(n, pieces);
+    const int64_t begin = wide(piece) * size;
+    const int end = static_cast<int>(min(begin + size, wide(n)));
+    const bool alone = pieces == 1;
+    if (begin >= n && !alone) return;
+    const int* table = p.table + wide(b) * p.M;
+    const uint8_t *kpages = static_cast<const uint8_t*>(p.k_pages) + hk * p.k_sh, *vpages = static_cast<const uint8_t*>(p.v_pages) + hk * p.v_sh;
+    const float *kscales = p.k_scales + hk, *vscales = p.v_scales + hk;
+
+    u32x4 q[TILES][D / 32];
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+        const int d = 64 * (s / 2) + 16 * grp + 8 * (s % 2), head = col % PER;
+        const u32x4 x = head < G && d < p.N ? *reinterpret_cast<const u32x4*>(static_cast<const E*>(p.q) + (wide(b) * p.H + hk * G + head) * p.N + d) : u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) q[t][s] = x & (col / PER == t ? ~0u : 0u);
+    }
+    const float unit = p.scale * LOG2E, in = p.cap > 0.f ? 2.f * unit / p.cap : 0.f, out = p.cap * LOG2E;
+    float slope[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) slope[r] = p.slopes ? p.slopes[hk * G + min((4 * grp + r) % PER, G - 1)] * LOG2E : 0.f;
+    const lds_t plane = lds_of(smem) + wave * STEP * 2 * D, weight = lds_of(weights[wave]);
+    lds_t vread[2];
+    vread[0] = value_at<D>(4 * grp + (col >> 2), (col & 3) >> 1) + 8 * (col & 1);
+    vread[1] = value_at<D>(16 + 4 * grp + (col >> 2), (col & 3) >> 1) + 8 * (col & 1);
+    const lds_t wread = weight + min(col % PER, (R - 1) | (PER - 4)) * WPITCH + 8 * grp;
+
+    const int own = 16 * (grp * TILES / 4) + col;                    // a lane's token, of each set of 16 TILES
+    const int kd = 16 * grp, vd = 16 * (lane % (D / 16));
+    u32x4 kr[4][D / 64], vr[VSTEPS];
+    float kscale[SETS], vscale[SETS];
+    bool on[SETS];
+    int page[SETS], ahead[SETS];                                     // ahead: of the step after the next, so that nothing waits for a page's number
+    const auto load_pages = [&](const int j0) {
+#pragma unroll
+        for (int a = 0; a < SETS; ++a) ahead[a] = table[min(j0 + 16 * TILES * a + own, end - 1) >> shift];
+    };
+    const auto page_of = [&](const int tile, const int row) { return static_cast<uint32_t>(__shfl(page[tile / TILES], 64 / TILES * (tile % TILES) + row, 64)); };
+    const auto load_keys = [&](const int j0) {
+#pragma unroll
+        for (int a = 0; a < SETS; ++a) {
+            on[a] = j0 + 16 * TILES * a + own < end && static_cast<unsigned>(ahead[a]) < static_cast<unsigned>(p.P);
+            page[a] = on[a] ? ahead[a] : 0;                          // (a page that there is; what is read of it does not count)
+            const float k = kscales[wide(page[a]) * p.Hk], v = vscales[wide(page[a]) * p.Hk];
+            kscale[a] = k, vscale[a] = on[a] ? v : 1.f;
+        }
+        if (j0 + WAVES * TOKENS < end) load_pages(j0 + WAVES * TOKENS);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const uint8_t* row = kpages + page_of(t, col) * p.k_sp + ((j0 + 16 * t + col) & (p.page - 1)) * p.k_st;
+#pragma unroll
+            for (int s = 0; s < D / 64; ++s) kr[t][s] = *reinterpret_cast<const u32x4*>(row + (64 * s + kd < p.N ? 64 * s + kd : 0));
+        }
+    };
+    const auto load_values = [&](const int j0) {
+#pragma unroll
+        for (int i = 0; i < VSTEPS; ++i) {
+            const int r = i * ROWS + lane / (D / 16);
+            const uint8_t* row = vpages + page_of(i * ROWS / 16, r & 15) * p.v_sp + ((j0 + r) & (p.page - 1)) * p.v_st;
+            vr[i] = *reinterpret_cast<const u32x4*>(row + (vd < p.N ? vd : 0));
+        }
+    };
+
+    f32x4_t o[D / 16];
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) o[d] = f32x4_t{};
+    float m[R], l[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) m[r] = -INFINITY, l[r] = 0.f;
+    int j0 = static_cast<int>(begin) + wave * TOKENS;
+    if (j0 < end) load_pages(j0), load_keys(j0), load_values(j0);
+    for (; j0 < end; j0 += WAVES * TOKENS) {
+        // what belongs to no token that counts, or stands behind a row's end, is zero: a weight of 0 would leave values that are no numbers, and keys' meet in the sums of the tiles' products
+        bool whole = p.N == D;
+        uint64_t counts[SETS];
+#pragma unroll
+        for (int a = 0; a < SETS; ++a) {
+            counts[a] = __ballot(on[a]);
+            whole &= counts[a] == ~0ull;
+        }
+        if (!whole) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const uint32_t keep = counts[t / TILES] >> (64 / TILES * (t % TILES) + col) & 1 ? ~0u : 0u;
+#pragma unroll
+                for (int s = 0; s < D / 64; ++s) kr[t][s] &= 64 * s + kd < p.N ? keep : 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < VSTEPS; ++i) {
+                const int tile = i * ROWS / 16, r = (i * ROWS + lane / (D / 16)) & 15;
+                vr[i] &= vd < p.N && counts[tile / TILES] >> (64 / TILES * (tile % TILES) + r) & 1 ? ~0u : 0u;
+            }
+        }
+        f32x4_t s[SETS];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            f32x4_t& to = s[t / TILES];
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+                to = mma16<E>(q[t % TILES][2 * c], widen8<E>(kr[t][c][0], kr[t][c][1]), c == 0 && t % TILES == 0 ? f32x4_t{} : to);
+                to = mma16<E>(q[t % TILES][2 * c + 1], widen8<E>(kr[t][c][2], kr[t][c][3]), to);
+            }
+        }
+        float ks[SETS], lv[SETS], iv[SETS];
+        bool is[SETS];
+#pragma unroll
+        for (int a = 0; a < SETS; ++a) ks[a] = kscale[a], lv[a] = __builtin_amdgcn_logf(vscale[a]), iv[a] = __builtin_amdgcn_rcpf(vscale[a]), is[a] = on[a];
+        const int next = j0 + WAVES * TOKENS;
+        if (next < end) load_keys(next);
+        float x[SETS][R], top[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) top[r] = -INFINITY;
+#pragma unroll
+        for (int a = 0; a < SETS; ++a) {
+            const float ago = static_cast<float>(all - 1 - j0 - 16 * TILES * a - own);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float dot = s[a][r] * ks[a];
+                float y = dot * unit;
+                if (p.cap > 0.f) y = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(dot * in)), -2.f * out, out);
+                y = fmaf(ago, -slope[r], y) + lv[a];
+                x[a][r] = is[a] ? y : -INFINITY;
+                top[r] = fmaxf(top[r], x[a][r]);
+            }
+        }
+        bool rises = false;
+#pragma unroll
+        for (int r = 0; r < R; ++r) rises |= top[r] > m[r];
+        if (__ballot(rises) != 0ull) {
+            float f[R], mine = 1.f;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float to = row_max(top[r]);
+                if constexpr (TILES == 4) to = fmaxf(to, __shfl_xor(to, 16, 64));
+                to = fmaxf(fmaxf(to, __shfl_xor(to, 32, 64)), m[r]);
+                f[r] = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - to);
+                m[r] = to;
+                l[r] *= f[r];
+                const float other = PER == 4 ? f[r] : __shfl(f[r], col % PER / 4 * 16, 64);
+                mine = R == 1 || (col & 3) == r ? other : mine;
+            }
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[d][r] *= mine;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float base = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+            for (int a = 0; a < SETS; ++a) {
+                const float w = __builtin_amdgcn_exp2f(x[a][r] - base);
+                l[r] = fmaf(w, iv[a], l[r]);
+                lds_st(weight + (4 * grp + r) % PER * WPITCH + 2 * (16 * TILES * a + own), __builtin_bit_cast(uint16_t, from_f<E>(w)));
+            }
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int i = 0; i < VSTEPS / 2; ++i) {
+                const int r = i * ROWS + lane / (D / 16), c = 2 * (lane % (D / 16));
+                const u32x4 y = vr[half * VSTEPS / 2 + i];
+                lds_st(plane + value_at<D>(r, c), widen8<E>(y[0], y[1]));
+                lds_st(plane + value_at<D>(r, c + 1), widen8<E>(y[2], y[3]));
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the wave's own writes above
+            if (half == 1 && next < end) load_values(next);
+            const u32x4 w = join(lds_ld<u32x2>(wread + 64 * half), lds_ld<u32x2>(wread + 64 * half + 32));
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+                typedef v4s __attribute__((address_space(3))) * ptr;
+                const lds_t at = 32 * d;                             // two pieces on: the swaps leave the lowest bit and are taken against it
+                const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(plane + (vread[0] ^ at))), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(plane + (vread[1] ^ at)));
+                const u32x2 y = __builtin_bit_cast(u32x2, lo), z = __builtin_bit_cast(u32x2, hi);
+                o[d] = mma16<E>(u32x4{y[0], y[1], z[0], z[1]}, w, o[d]);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        l[r] = row_add(l[r]);
+        if constexpr (TILES == 4) l[r] += __shfl_xor(l[r], 16, 64);
+        l[r] += __shfl_xor(l[r], 32, 64);
+    }
+    __syncthreads();
+    float* sums = reinterpret_cast<float*>(smem);                    // [wave][head][D], pieces of four channels of a head turned by the head
+    if (col == 0 && grp < PER / 4)
+#pragma unroll
+        for (int r = 0; r < R; ++r) top_of[wave][4 * grp + r] = m[r], sum_of[wave][4 * grp + r] = l[r];
+    if (col < PER)
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4_t*>(sums + (wave * PER + col) * D + 4 * ((4 * d + grp) ^ col)) = o[d];
+    __syncthreads();
+    for (int i = tid; i < G * D / 4; i += 64 * WAVES) {
+        const int h = i / (D / 4), c = i % (D / 4);
+        if (4 * c >= p.N) continue;
+        float top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < WAVES; ++k) top = fmaxf(top, top_of[k][h]);
+        const float base = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+        f32x4_t y = f32x4_t{};
+#pragma unroll
+        for (int k = 0; k < WAVES; ++k) {
+            const float f = __builtin_amdgcn_exp2f(top_of[k][h] - base);
+            sum = fmaf(sum_of[k][h], f, sum);
+            y += *reinterpret_cast<const f32x4_t*>(sums + (k * PER + h) * D + 4 * (c ^ h)) * f;
+        }
+        const int64_t row = wide(b) * p.H + hk * G + h;
+        if (alone) {
+            const float f = sum == 0.f ? 0.f : 1.f / sum;
+            *reinterpret_cast<u32x2*>(static_cast<E*>(p.y) + row * p.N + 4 * c) = u32x2{pack2<E>(y[0] * f, y[1] * f), pack2<E>(y[2] * f, y[3] * f)};
+        } else {
+            float* to = part + (row * pieces + piece) * (D + 4);
+            *reinterpret_cast<f32x4_t*>(to + 4 + 4 * c) = y;
+            if (c == 0) to[0] = top, to[1] = sum;
+        }
+    }
+}
+
+// Rows of 64 bytes: sixteen or eight neighbouring heads on one XCD, whose L2 reads lines of 128 bytes.  B64, up to 4096 tokens, H32 Hk32 N64: 196 us one by one, 158 in twos, 142 in eights, 133 in
+// sixteens; B64 H32 Hk8 N64 54, 45, 45.  Rows of 128 bytes gain nothing: there the heads of a piece come one after the other, or where pieces are many the pieces of a head: B16, up to 8192 tokens,
+// H32 Hk8 N128, 16 pieces, 54 us and 58 (in eights 58); B4, up to 131072, H64 Hk8 N128, 64 pieces, 181 and 171 (in eights 177).
 inline int group_of(int N, int heads, int pieces, int64_t blocks) {
-    if (heads % 8 == 0 && blocks >= 64 * 8) return 8;
+    if (N <= 64 && blocks >= 64 * 8)
+        for (const int group : {16, 8})
+            if (heads % group == 0) return group;
     return pieces >= 32 ? 0 : 1;
 }
 
@@ -209,7 +460,18 @@ template <class E, int D> int run(hipStream_t st, const rwkv_paged8_args& p) {
     const int group = group_of(p.N, p.Hk * chunks, pieces, blocks);
     const int64_t shares = blocks / std::max(group, 1), grid = group > 1 ? (shares + 7) / 8 * 8 * group : blocks;
     if (grid > INT_MAX) return RWKV_ERR_SHAPE;
-    hipLaunchKernelGGL((paged8_attn<E, D>), dim3(static_cast<unsigned>(grid)), dim3(64 * WAVES), 0, st, p, shift, pieces, chunks, group, static_cast<int>(shares), part);
+    const auto few = [&](auto tiles, auto heads) {
+        hipLaunchKernelGGL((paged8_few<E, D, decltype(tiles)::value, decltype(heads)::value>), dim3(static_cast<unsigned>(grid)), dim3(64 * WAVES), 0, st, p, shift, pieces, group, static_cast<int>(shares), part);
+    };
+    using std::integral_constant;
+    // us, B16, up to 8192 tokens, heads of 64 (16 keys' heads) and of 128 (8); paged8_few with 4 tiles, with 2, paged8_attn:
+    //   1 query head a key head 35.5 40.4 43.2, 42.9 46.4 45.0;   2: 36.8 41.2 43.8, 47.2 45.9 44.1;   4: 45.1 42.1 45.1, 54.0 46.0 45.2;   8: - 42.9 45.4, - 47.2 45.1
+    // but B4, up to 131072 tokens, 8 heads of 128: 171 and 180.  (Four copies of the queries take 64 registers where heads have 128 channels.)
+    const int G = p.H / p.Hk;
+    if (G == 1) few(integral_constant<int, 4>(), integral_constant<int, 1>());
+    else if (D == 64 && G == 2) few(integral_constant<int, 4>(), integral_constant<int, D == 64 ? 2 : 1>());
+    else if (G <= 8 && (D == 64 || G > 4)) few(integral_constant<int, 2>(), integral_constant<int, 4>());
+    else hipLaunchKernelGGL((paged8_attn<E, D>), dim3(static_cast<unsigned>(grid)), dim3(64 * WAVES), 0, st, p, shift, pieces, chunks, group, static_cast<int>(shares), part);
     if (pieces > 1) hipLaunchKernelGGL((paged_join<rwkv_paged8_args, E, D>), dim3(p.H, p.B), dim3(256), 0, st, p, shift, pieces, part);
     return launch_status();
 }

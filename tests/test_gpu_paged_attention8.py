@@ -191,6 +191,17 @@ def test_many_heads(lib, H, Hk, N, B):
     check(*cache(lens, H, Hk, N, 16, torch.bfloat16, seed=61))
 
 
+@pytest.mark.parametrize("G", [1, 2, 3, 4, 5, 7, 8, 9, 16, 17])
+@pytest.mark.parametrize("N,page,dtype", [(64, 16, "bf16"), (128, 8, "fp16"), (48, 2, "fp16"), (112, 128, "bf16")])
+def test_query_heads_of_a_key_head(lib, G, N, page, dtype):
+    """Each way to lay heads and tokens over the lanes, with caps and biases, over several rounds of the waves; pages missing in the middle of a tile."""
+    q, kv, table, lens = cache([1500, 3, 260, 0, 63], 3 * G, 3, N, page, DT[dtype], seed=G)
+    for i in range(3, 1500 // page, 5):
+        table[0, i] = -1
+    check(q, kv, table, lens, cap=20.0, slopes=torch.exp2(-torch.arange(1.0, 3 * G + 1) / G).to(DEV))
+    check(q, kv, table, lens)
+
+
 @pytest.mark.parametrize("how", ["cap", "bias", "both", "scale"])
 def test_caps_and_biases(lib, how):
     H = 8
