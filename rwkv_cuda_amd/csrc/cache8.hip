@@ -1,7 +1,7 @@
 // A paged cache in 8 bits: writing it (the arguments are explained in rwkv_hip.h).
 //
 // A scale belongs to a page and head, so the tokens that go into one page are one wave's, for one head and for keys or values: a pass for the
-// largest magnitude, the scale, a pass that rounds (its reads hit the cache), and, where the page held tokens and its scale grew, those once more.  Scales are powers
+// largest magnitude, the scale, a pass that rounds (the first HOLD rows of the wave stay in registers and are on their way at once, others are read again), and, where the page held tokens and its scale grew, those once more.  Scales are powers
 // of two: a token's own rounding is all that is lost until its page's scale grows, and a second one is the first one's number where no bits fall off.
 #include <climits>
 
@@ -26,6 +26,21 @@ template <class E> DEVINL void values8(const u32x4 x, float (&f)[8]) {
         }
     }
 }
+// Magnitudes of 16-bit numbers are ordered as their bits without the sign.
+DEVINL uint32_t larger(const uint32_t a, const uint32_t b) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+template <class E> DEVINL uint32_t largest(const u32x4 x, const uint32_t than) {
+    return larger(larger(than, x[0] & 0x7fff7fffu), larger(larger(x[1] & 0x7fff7fffu, x[2] & 0x7fff7fffu), x[3] & 0x7fff7fffu));
+}
+// ... infinities and NaN as zeros
+template <class E> DEVINL u32x4 finite_ones(u32x4 x) {
+    constexpr uint32_t TOP = std::is_same_v<E, bf16_t> ? 0x7f80 : 0x7c00;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] &= ((x[i] & TOP) == TOP ? 0u : 0xffffu) | ((x[i] >> 16 & TOP) == TOP ? 0u : 0xffff0000u);
+    return x;
+}
 // four values as codes, to nearest even; none is above 448
 DEVINL uint32_t codes4(const float a, const float b, const float c, const float d) {
     int x = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
@@ -44,7 +59,7 @@ DEVINL int exponent_for(const float top) {
 }
 DEVINL float power(const int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }     // -126 .. 127
 
-template <class E>
+template <class E, int HOLD>
 __global__ __launch_bounds__(64 * WAVES) void cache8_write(const rwkv_cache8_args p, const int shift, const int window, const int windows) {
     const int lane = threadIdx.x & 63, pieces = p.N / 8;        // of 8 values; a lane has one of them, in every 64 / width-th token
     const int width = p.N <= 64 ? 8 : 16, piece = lane & (width - 1), row = lane / width, rows = 64 / width;
@@ -54,7 +69,7 @@ __global__ __launch_bounds__(64 * WAVES) void cache8_write(const rwkv_cache8_arg
     const int64_t at = work / p.Hk / 2;
     if (at >= windows) return;
     const int w0 = static_cast<int>(at) * window;
-    const E* x = static_cast<const E*>(kv ? p.v : p.k) + head * (kv ? p.v_sh : p.k_sh) + 8 * piece;
+    const E* x = static_cast<const E*>(kv ? p.v : p.k) + head * (kv ? p.v_sh : p.k_sh) + (on ? 8 * piece : 0);
     const int64_t xt = kv ? p.v_st : p.k_st, sp = kv ? p.vp_sp : p.kp_sp, st = kv ? p.vp_st : p.kp_st;
     uint8_t* pages = static_cast<uint8_t*>(kv ? p.v_pages : p.k_pages) + head * (kv ? p.vp_sh : p.kp_sh) + 8 * piece;
     float* scales = (kv ? p.v_scales : p.k_scales) + head;
@@ -70,38 +85,59 @@ __global__ __launch_bounds__(64 * WAVES) void cache8_write(const rwkv_cache8_arg
         starts &= starts - 1;
         const int begin = w0 + s, page = __shfl(mine, s, 64);
         // up to the next token of another page, and the first place that is written
-        int end = begin + 1, first = INT_MAX;
+        int end = begin + 1, first = INT_MAX, place = 0;        // place: of token begin + lane
         for (int i = begin;; i += 64) {
             const bool same = page_of(i + lane) == page;
             const uint64_t other = ~__ballot(same);
             const int n = other == 0ull ? 64 : __builtin_ctzll(other);
-            if (lane < n) first = min(first, p.slots[i + lane] & mask);
+            if (lane < n) {
+                const int z = p.slots[i + lane] & mask;
+                first = min(first, z), place = i == begin ? z : place;
+            }
             end = i + n;
             if (n < 64) break;
         }
+        u32x4 held[HOLD];
+#pragma unroll
+        for (int u = 0; u < HOLD; ++u)
+            if (begin + rows * u < end) held[u] = *reinterpret_cast<const u32x4*>(x + min(begin + row + rows * u, end - 1) * xt);
 #pragma unroll
         for (int m = 32; m >= 1; m >>= 1) first = min(first, __shfl_xor(first, m, 64));
-        float top = 0.f;
-        for (int i = begin + row; i < end; i += rows) {
-            if (!on) continue;
-            float f[8];
-            values8<E>(*reinterpret_cast<const u32x4*>(x + i * xt), f);
+        const float old = scales[static_cast<int64_t>(page) * p.Hk];
+        const auto top_of = [&](auto only) {                    // (where rows end inside of the last access it is the last token's once more)
+            uint32_t top = 0;
+            const auto take = [&](const u32x4 v) { top = largest<E>(only ? finite_ones<E>(v) : v, top); };
 #pragma unroll
-            for (int e = 0; e < 8; ++e) top = fmaxf(top, finite_bits(__float_as_uint(f[e])) ? fabsf(f[e]) : 0.f);
-        }
+            for (int u = 0; u < HOLD; ++u)
+                if (begin + rows * u < end) take(held[u]);
+            for (int i = begin + row + rows * HOLD; i < end; i += rows) take(*reinterpret_cast<const u32x4*>(x + i * xt));
+            top = on ? max(top & 0xffff, top >> 16) : 0;
 #pragma unroll
-        for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-        const float need = power(exponent_for(top)), old = scales[static_cast<int64_t>(page) * p.Hk], scale = first > 0 ? fmaxf(need, old) : need;
+            for (int m = 32; m >= 1; m >>= 1) top = max(top, __shfl_xor(top, m, 64));
+            return top;
+        };
+        uint32_t top = top_of(std::false_type());
+        const bool odd = top >= (std::is_same_v<E, bf16_t> ? 0x7f80 : 0x7c00);      // infinities or NaN: a second look, without them
+        if (odd) top = top_of(std::true_type());
+        const float need = power(exponent_for(to_f(__builtin_bit_cast(E, static_cast<uint16_t>(top))))), scale = first > 0 ? fmaxf(need, old) : need;
         const float by = 1.f / scale;
         uint8_t* to = pages + page * sp;
-        for (int i = begin + row; i < end; i += rows) {
-            if (!on) continue;
+        const auto put = [&](const u32x4 v, const int z) {
             float f[8];
-            values8<E>(*reinterpret_cast<const u32x4*>(x + i * xt), f);
+            values8<E>(v, f);
+            if (odd)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = finite_bits(__float_as_uint(f[e])) ? f[e] * by : NAN;
-            *reinterpret_cast<u32x2*>(to + (p.slots[i] & mask) * st) = u32x2{codes4(f[0], f[1], f[2], f[3]), codes4(f[4], f[5], f[6], f[7])};
-        }
+                for (int e = 0; e < 8; ++e) f[e] = finite_bits(__float_as_uint(f[e])) ? f[e] : NAN;
+            *reinterpret_cast<u32x2*>(to + z * st) = u32x2{codes4(f[0] * by, f[1] * by, f[2] * by, f[3] * by), codes4(f[4] * by, f[5] * by, f[6] * by, f[7] * by)};
+        };
+#pragma unroll
+        for (int u = 0; u < HOLD; ++u)
+            if (begin + rows * u < end) {
+                const int n = row + rows * u, z = n < 64 ? __shfl(place, n & 63, 64) : p.slots[min(begin + n, end - 1)] & mask;
+                if (on && begin + n < end) put(held[u], z);
+            }
+        for (int i = begin + row + rows * HOLD; i < end; i += rows)
+            if (on) put(*reinterpret_cast<const u32x4*>(x + i * xt), p.slots[i] & mask);
         if (first > 0 && scale > old) {
             const float fit = old / scale;
             for (int i = row; i < first; i += rows) {
@@ -116,7 +152,10 @@ __global__ __launch_bounds__(64 * WAVES) void cache8_write(const rwkv_cache8_arg
 }
 
 // How many tokens a wave looks through for pages that begin: one while waves are few (a token of each of many sequences: a page each), more as there are more of them (a
-// prompt's tokens fill pages, and most begin none), up to a page or the lanes of a wave.
+// prompt's tokens fill pages, and most begin none), up to a page or the lanes of a wave.  And how many rows it keeps: 16 where it looks through more than 8 tokens, 4 below, where most runs are of
+// one token and the longer code and the registers only cost.  us, 8 heads of 128, with 4096, 8192, 32768 waves (4 rows up to 4 tokens), and 8192 waves with 4 rows up to 8:
+//   64 sequences of one token 4.5 4.2 4.5 4.7;   1024 of one 9.4 10.0 11.6 10.1;   4096 of one 72 59 30 27;   256 of 8 8.9 8.4 22 8.3;   one prompt of 1000 11.4 12.7 12.8 12.7;   4 of 1000
+//   (pages of 16) 10.0 10.2 25 7.7;   4 of 2000 13.9 14.3 35 14.4;   16 of 2000 41.6 41.6 39.2 41.7, which is 202 MB at 4.8 TB/s
 constexpr int BUSY = 8192;
 int window_of(const rwkv_cache8_args& p) {
     const int64_t waves = 2ll * p.n * p.Hk;
@@ -128,7 +167,8 @@ template <class E> int run(hipStream_t st, const rwkv_cache8_args& p) {
     const int window = window_of(p), windows = static_cast<int>((static_cast<int64_t>(p.n) + window - 1) / window);
     const int64_t blocks = (2ll * windows * p.Hk + WAVES - 1) / WAVES;
     if (blocks > INT_MAX) return RWKV_ERR_SHAPE;
-    hipLaunchKernelGGL(cache8_write<E>, dim3(static_cast<unsigned>(blocks)), dim3(64 * WAVES), 0, st, p, __builtin_ctz(p.page), window, windows);
+    const auto kernel = window > 8 ? cache8_write<E, 16> : cache8_write<E, 4>;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * WAVES), 0, st, p, __builtin_ctz(p.page), window, windows);
     return launch_status();
 }
 
