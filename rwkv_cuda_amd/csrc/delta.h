@@ -139,25 +139,36 @@ struct Scalars {
 };
 constexpr double CUT = -0x1p20;
 
-// 64 rows of D inputs in LDS, 16 bytes more than their size apart (16 rows at one place touch all banks).  Of every 32 channels number 16 e + 4 g + r is at place 8 g + 4 e + r: 16 bytes
+// LDS is read 256 bytes a cycle: of 16 bytes a lane by lanes 0-3, 12-15 and 20-27, then 4-11, 16-19 and 28-31, and likewise from 32 on; of 8 by half a wave; it is written 128 bytes a cycle, by 8 or
+// 16 neighbours.  (Found with the counters of conflicts.)  A row of 64 bytes or more is cut into blocks of 64, these into pieces of 16, and rows exchange both among themselves, so that 16 rows'
+// pieces, one a row, fall on all banks once in each of those groups; where columns are read, 8 bytes of a piece, two rows meet.
+DEVINL int piece_swap(const int row) { return -(row >> 2) & 3; }
+template <int BYTES> DEVINL int block_swap(const int row) { return BYTES == 256 ? row & 3 : (BYTES == 128 ? row >> 1 & 1 : 0); }
+template <int BYTES> DEVINL lds_t place(const int row, const int block, const int piece) { return row * BYTES + 64 * (block ^ block_swap<BYTES>(row)) + 16 * (piece ^ piece_swap(row)); }
+
+// Which of eight rows the lanes' n-th is where rows are written, and which 16 bytes of it a lane has: 16 neighbours have 128 bytes (64) of two rows (four), which then meet nowhere.
+template <int D> DEVINL int written_row(const int n) { return D == 32 ? (n & ~7) | (n & 1) | (n << 1 & 4) | (n >> 1 & 2) : (n & ~7) | (n << 2 & 4) | (n >> 1 & 3); }
+template <int D> DEVINL int written_order(const int lane) { return D == 128 ? (lane >> 4 & ~1) | (lane >> 3 & 1) : lane / (D / 8); }
+template <int D> DEVINL int written_piece(const int lane) { return D == 128 ? (lane & 7) | (lane >> 1 & 8) : lane % (D / 8); }
+// 64 rows of D inputs in LDS.  Of every 32 channels number 16 e + 4 g + r is at place 8 g + 4 e + r: 16 bytes
 // are what a lane of group g needs.
 template <int D> struct Rows {
-    static constexpr int PITCH = 2 * D + 16, BYTES = 64 * PITCH;
+    static constexpr int PITCH = 2 * D, BYTES = 64 * PITCH;
     // channels 8 c .. 8 c + 7 of a row
     static DEVINL void put(const lds_t base, const int row, const int c, const u32x4 x) {
-        const lds_t to = base + row * PITCH + 64 * (c / 4) + 32 * (c % 2) + 8 * (c / 2 % 2);
-        lds_st(to, u32x2{x[0], x[1]});
-        lds_st(to + 16, u32x2{x[2], x[3]});
+        const lds_t to = place<PITCH>(row, c / 4, 2 * (c % 2)) + 8 * (c / 2 % 2);
+        lds_st(base + to, u32x2{x[0], x[1]});
+        lds_st(base + (to ^ 16), u32x2{x[2], x[3]});
     }
     // four of a row's channels, 16 t + 4 g ..
-    static DEVINL u32x2 four(const lds_t base, const int row, const int t, const int g) { return lds_ld<u32x2>(base + row * PITCH + 64 * (t / 2) + 16 * g + 8 * (t % 2)); }
+    static DEVINL u32x2 four(const lds_t base, const int row, const int t, const int g) { return lds_ld<u32x2>(base + place<PITCH>(row, t / 2, g) + 8 * (t % 2)); }
     // row 16 i + (lane & 15), channels of the 32 s-th: the contraction runs over channels
-    static DEVINL u32x4 row(const lds_t base, const int lane, const int i, const int s) { return lds_ld<u32x4>(base + (16 * i + (lane & 15)) * PITCH + 64 * s + 16 * (lane >> 4)); }
+    static DEVINL u32x4 row(const lds_t base, const int lane, const int i, const int s) { return lds_ld<u32x4>(base + 16 * i * PITCH + place<PITCH>(lane & 15, s, lane >> 4)); }
     // channel 16 t + (lane & 15), rows of the 32 s-th: the contraction runs over rows
     static DEVINL u32x4 col(const lds_t base, const int lane, const int t, const int s) {
         typedef v4s __attribute__((address_space(3))) * ptr;
         const int l = lane & 15;
-        const lds_t at = base + (32 * s + 4 * (lane >> 4) + (l >> 2)) * PITCH + 64 * (t / 2) + 16 * (l & 3) + 8 * (t % 2);
+        const lds_t at = base + 32 * s * PITCH + place<PITCH>(4 * (lane >> 4) + (l >> 2), t / 2, l & 3) + 8 * (t % 2);
         const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(at)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(at + 16 * PITCH));
         return join(__builtin_bit_cast(u32x2, a), __builtin_bit_cast(u32x2, b));
     }
@@ -165,48 +176,53 @@ template <int D> struct Rows {
 
 // A lower triangle of 64 by 64, by blocks of 16, as two planes of bf16, columns in the order of Rows: P, or (FIRST = 1) A without the blocks of its diagonal, whose first row block is 1.
 template <int FIRST> struct Lower {
-    static constexpr int SHORT = 80, LONG = 144, PLANE = (16 * (2 * SHORT + (2 - FIRST) * LONG) + 511) / 512 * 512, BYTES = 2 * PLANE;
-    static DEVINL lds_t at(const lds_t base, const int i, const int r) { return base + (i - FIRST < 2 ? (16 * (i - FIRST) + r) * SHORT : 32 * SHORT + (16 * (i - FIRST - 2) + r) * LONG); }
+    static constexpr int SHORT = 64, LONG = 128, PLANE = 16 * (2 * SHORT + (2 - FIRST) * LONG), BYTES = 2 * PLANE;
+    // a piece of row 16 i + r: columns 16 (2 s) + 4 g .. and 16 (2 s + 1) + 4 g ..
+    static DEVINL lds_t at(const lds_t base, const int i, const int r, const int s, const int g) {
+        return base + (i - FIRST < 2 ? 16 * (i - FIRST) * SHORT + place<SHORT>(r, s, g) : 32 * SHORT + 16 * (i - FIRST - 2) * LONG + place<LONG>(r, s, g));
+    }
     // rows 16 i + r; columns 16 j + 4 g ..
     static DEVINL void put(const lds_t base, const int i, const int r, const int j, const int g, const Two& x) {
-        const lds_t to = at(base, i, r) + 64 * (j / 2) + 16 * g + 8 * (j % 2);
+        const lds_t to = at(base, i, r, j / 2, g) + 8 * (j % 2);
         lds_st(to, x.h);
         lds_st(to + PLANE, x.l);
     }
     // the lane's row of row block i: block 2 s of its columns, or blocks 2 s and 2 s + 1
     static DEVINL Two one(const lds_t base, const int lane, const int i, const int s) {
-        const lds_t from = at(base, i, lane & 15) + 64 * s + 16 * (lane >> 4);
-        return {lds_ld<u32x2>(from), lds_ld<u32x2>(from + PLANE)};
+        const Two32 x = two(base, lane, i, s);                  // (half a piece would take as long)
+        return {u32x2{x.h[0], x.h[1]}, u32x2{x.l[0], x.l[1]}};
     }
     static DEVINL Two32 two(const lds_t base, const int lane, const int i, const int s) {
-        const lds_t from = at(base, i, lane & 15) + 64 * s + 16 * (lane >> 4);
+        const lds_t from = at(base, i, lane & 15, s, lane >> 4);
         return {lds_ld<u32x4>(from), lds_ld<u32x4>(from + PLANE)};
     }
 };
 // Their transposes: rows 16 j + r, columns from block j (P) or j + 1 (A) on.
 template <int FIRST> struct Upper {
-    static constexpr int SHORT = 80, LONG = 144, PLANE = (16 * (2 * LONG + (2 - FIRST) * SHORT) + 511) / 512 * 512, BYTES = 2 * PLANE;
-    static DEVINL lds_t at(const lds_t base, const int j, const int r) { return base + (j < 2 ? (16 * j + r) * LONG : 32 * LONG + (16 * (j - 2) + r) * SHORT - 64); }
+    static constexpr int SHORT = 64, LONG = 128, PLANE = 16 * (2 * LONG + (2 - FIRST) * SHORT), BYTES = 2 * PLANE;
+    static DEVINL lds_t at(const lds_t base, const int j, const int r, const int s, const int g) {
+        return base + (j < 2 ? 16 * j * LONG + place<LONG>(r, s, g) : 32 * LONG + 16 * (j - 2) * SHORT + place<SHORT>(r, s - 1, g));
+    }
     static DEVINL void put(const lds_t base, const int j, const int r, const int i, const int g, const Two& x) {
-        const lds_t to = at(base, j, r) + 64 * (i / 2) + 16 * g + 8 * (i % 2);
+        const lds_t to = at(base, j, r, i / 2, g) + 8 * (i % 2);
         lds_st(to, x.h);
         lds_st(to + PLANE, x.l);
     }
     // the lane's row of row block j: column block i, or blocks 2 s and 2 s + 1
     static DEVINL Two one(const lds_t base, const int lane, const int j, const int i) {
-        const lds_t from = at(base, j, lane & 15) + 64 * (i / 2) + 16 * (lane >> 4) + 8 * (i % 2);
-        return {lds_ld<u32x2>(from), lds_ld<u32x2>(from + PLANE)};
+        const Two32 x = two(base, lane, j, i / 2);
+        return i % 2 ? Two{u32x2{x.h[2], x.h[3]}, u32x2{x.l[2], x.l[3]}} : Two{u32x2{x.h[0], x.h[1]}, u32x2{x.l[0], x.l[1]}};
     }
     static DEVINL Two32 two(const lds_t base, const int lane, const int j, const int s) {
-        const lds_t from = at(base, j, lane & 15) + 64 * s + 16 * (lane >> 4);
+        const lds_t from = at(base, j, lane & 15, s, lane >> 4);
         return {lds_ld<u32x4>(from), lds_ld<u32x4>(from + PLANE)};
     }
 };
-// The inverses of the diagonal blocks of I + A, two planes each, rows of 32 bytes.
+// The inverses of the diagonal blocks of I + A, two planes each, rows of 32 bytes, whose halves the second eight rows exchange.
 struct Diagonal {
     static constexpr int PLANE = 512, BLOCK = 2 * PLANE, BYTES = 4 * BLOCK;
     static DEVINL Two row(const lds_t base, const int lane, const int i) {
-        const lds_t from = base + i * BLOCK + (lane & 15) * 32 + 8 * (lane >> 4);
+        const lds_t from = base + i * BLOCK + (lane & 15) * 32 + (8 * (lane >> 4) ^ 2 * (lane & 8));
         return {lds_ld<u32x2>(from), lds_ld<u32x2>(from + PLANE)};
     }
 };
@@ -330,7 +346,7 @@ template <class E, int D, bool BACK> DEVINL void make_matrices(const lds_t K, co
         for (int t = 0; t < 16; ++t) m[t] = t == col ? 1.f : 0.f;
         solve_bc<!BACK>(m, z);                                  // row lane & 15 of the inverse: m_s = -sum over t > s of m_t A_ts; BACK: the column, m_s = -sum over t < s of A_st m_t
         const int block = w + (lane >> 5), half = grp & 1;       // of a row: the first or the last eight
-        const lds_t to = inv + block * Diagonal::BLOCK + col * 32 + 16 * half;
+        const lds_t to = inv + block * Diagonal::BLOCK + col * 32 + (16 * half ^ 2 * (col & 8));
         Two o[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -361,7 +377,7 @@ template <class E, int D, int SW, int HELPERS, bool BACK> DEVINL void help(const
     static_assert(LANES % RP == 0 && LANES % (2 * SW) == 0);
     const int N = p.N, T = p.T, chunks = (T + DELTA_CHUNK - 1) / DELTA_CHUNK, tid = 64 * mine + lane;
     const uint32_t tasks = tasks_of<HELPERS>(mine);
-    const int krow = tid / RP, kd = 8 * (tid % RP), vrow = tid / (2 * SW), vd = 16 * SW * piece + 8 * (tid % (2 * SW));
+    const int krow = written_order<D>(tid), kd = 8 * written_piece<D>(tid), vrow = tid / (2 * SW), vd = 16 * SW * piece + 8 * (tid % (2 * SW));
     const bool kin = kd < N, vin = vd < N && (!BACK || p.dy);
     const int64_t v_st = BACK ? wide(p.H) * N : p.v_st;
     const auto first = [&](const int c) { return (BACK ? chunks - 1 - c : c) * DELTA_CHUNK; };
@@ -376,7 +392,7 @@ template <class E, int D, int SW, int HELPERS, bool BACK> DEVINL void help(const
         const E *kc = k + wide(t0) * p.k_st, *qc = q + wide(t0) * p.q_st, *vc = v + wide(t0) * vs;
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
-            const int row = min(krow + KSTEP * i, min(most, 63));
+            const int row = min(written_row<D>(krow + KSTEP * i), min(most, 63));
             kr[i] = *reinterpret_cast<const u32x4*>(kc + row * p.k_st);
             qr[i] = *reinterpret_cast<const u32x4*>(qc + row * p.q_st);
         }
@@ -403,7 +419,7 @@ template <class E, int D, int SW, int HELPERS, bool BACK> DEVINL void help(const
         const lds_t to = lds + (c & 1) * L::STAGE;
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
-            const int row = krow + KSTEP * i;
+            const int row = written_row<D>(krow + KSTEP * i);
             if (64 * RP % LANES != 0 && i == KP - 1 && row >= 64) continue;
             const uint32_t keep = kin ? mask_of(row) : 0;
             Rows<D>::put(to + L::K, row, kd / 8, kr[i] & keep);

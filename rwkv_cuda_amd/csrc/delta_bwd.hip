@@ -99,7 +99,14 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_d
 #pragma unroll
                 for (int t = 0; t < D / 16; ++t) kc[t] = Rows<D>::col(from, lane, t, k);
             };
-            const auto advance = [&](const Beside<E, 2>& u, const float by) {
+            constexpr std::integral_constant<int, 1> one;
+            const auto advance = [&](const Beside<E, 2>& u, const auto by) {
+                if constexpr (std::is_same_v<E, bf16_t>) {
+#pragma unroll
+                    for (int t = 0; t < D / 16; ++t) S[t] = mma32<E>(kc[t], u.lo(0), std::is_same_v<decltype(by), const std::integral_constant<int, 1>> ? S[t] : S[t] * static_cast<float>(by));
+#pragma unroll
+                    for (int t = 0; t < D / 16; ++t) S[t] = mma32<E>(kc[t], u.hi(0), S[t]);
+                } else
 #pragma unroll
                 for (int t = 0; t < D / 16; t += 4) {
 #pragma unroll
@@ -107,7 +114,7 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_d
 #pragma unroll
                     for (int e = 0; e < 4; ++e) z[e] = mma32<E>(kc[t + e], u.hi(0), z[e]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) S[t + e] = by * S[t + e] + z[e] * u.back;
+                    for (int e = 0; e < 4; ++e) S[t + e] = static_cast<float>(by) * S[t + e] + z[e] * u.back;
                 }
             };
             Beside<E, 2> w;
@@ -146,7 +153,7 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_d
             const Two a01 = Upper<1>::one(A, lane, 0, 1), inv0 = Diagonal::row(inv, lane, 0);
             f32x4 ba = betas(2) * factors(2), bb = betas(3) * factors(3);
             Z[1] = mma16(inv1, split<bf16_t>(X[1]), zero4());
-            advance(w, 1.f);
+            advance(w, one);
             in_order();
             columns(K, 1);
             const Two z1 = split<bf16_t>(Z[1]);
@@ -155,11 +162,11 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_d
             in_order();
             ba = betas(0) * factors(0), bb = betas(1) * factors(1);
             Z[0] = mma16(inv0, split<bf16_t>(X[0]), zero4());
-            advance(w, 1.f);
+            advance(w, one);
             in_order();
             columns(K, 0);
             w.take({Z[0] * -ba, Z[1] * -bb});
-            advance(w, 1.f);
+            advance(w, one);
             if (c0 < N) {
                 float* to = updates + tiles.update(chunk, ct, 0) + 4 * lane;
                 keep(to, split<bf16_t>(Z[0])), keep(to + 256, z1), keep(to + 512, z2), keep(to + 768, z3);

@@ -33,7 +33,10 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_d
 #pragma unroll
             for (int r = 0; r < 4; ++r) S[t][r] = s0 && on && 16 * t + 4 * grp + r < N ? s0[(16 * t + 4 * grp + r) * N + c0 + col] : 0.f;
         const lds_t vread = L::V + lds + (4 * grp + (col >> 2)) * L::VPITCH + 32 * wave + 8 * (col & 3);
-        E* y = static_cast<E*>(p.y) + (wide(b) * T * p.H + h) * N + c0 + 4 * grp;
+        // outputs: a chunk's place, and a lane's in it
+        const int row_bytes = p.H * N * 2;
+        char* const yc = reinterpret_cast<char*>(static_cast<E*>(p.y) + (wide(b) * T * p.H + h) * N + c0);
+        const uint32_t y_lane = static_cast<uint32_t>(col) * row_bytes + 8 * grp;
         __syncthreads();
         __syncthreads();
         for (int c = 0; c < chunks; ++c) {
@@ -74,7 +77,7 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_d
             }
             in_order();
             // the triangular system, and beside it the outputs
-            f32x4 Y[4], U[4], z[4], leave;
+            f32x4 Y[4], U[4], z[4];
             float enters;
             const float whole = lds_ld<float>(sc + Scalars::ENTER + 4 * 63);
             Two u0, u1, u2, u3;
@@ -99,7 +102,14 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_d
 #pragma unroll
                 for (int t = 0; t < D / 16; ++t) kc[t] = Rows<D>::col(K, lane, t, k);
             };
-            const auto advance = [&](const Beside<E, 2>& u, const float by) {
+            constexpr std::integral_constant<int, 1> one;
+            const auto advance = [&](const Beside<E, 2>& u, const auto by) {
+                if constexpr (std::is_same_v<E, bf16_t>) {
+#pragma unroll
+                    for (int t = 0; t < D / 16; ++t) S[t] = mma32<E>(kc[t], u.lo(0), std::is_same_v<decltype(by), const std::integral_constant<int, 1>> ? S[t] : S[t] * static_cast<float>(by));
+#pragma unroll
+                    for (int t = 0; t < D / 16; ++t) S[t] = mma32<E>(kc[t], u.hi(0), S[t]);
+                } else
 #pragma unroll
                 for (int t = 0; t < D / 16; t += 4) {
 #pragma unroll
@@ -107,7 +117,7 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_d
 #pragma unroll
                     for (int e = 0; e < 4; ++e) z[e] = mma32<E>(kc[t + e], u.hi(0), z[e]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) S[t + e] = by * S[t + e] + z[e] * u.back;
+                    for (int e = 0; e < 4; ++e) S[t + e] = static_cast<float>(by) * S[t + e] + z[e] * u.back;
                 }
             };
             queries(0);
@@ -165,7 +175,7 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_d
             Y[3] = mma32(u01, p3, Y[3]);
             in_order();
             x23.take({l2 * U[2], l3 * U[3]});
-            advance(x23, 1.f);
+            advance(x23, one);
             const Two32 p33 = Lower<0>::two(P, lane, 3, 1);
             in_order();
             Y[2] = mma16(u2, p22, Y[2]);
@@ -175,11 +185,15 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_d
                 float* to = updates + tiles.update(wide(hb) * chunks + c, ct, 0) + 4 * lane;
                 keep(to, u0), keep(to + 256, u1), keep(to + 512, u2), keep(to + 768, u3);
             }
+            char* const to = yc + wide(c) * DELTA_CHUNK * row_bytes;
+            const auto out = [&](const int i) { *reinterpret_cast<u32x2*>(to + wide(16 * i) * row_bytes + y_lane) = u32x2{pack2<E>(Y[i][0], Y[i][1]), pack2<E>(Y[i][2], Y[i][3])}; };
+            if ((c + 1) * DELTA_CHUNK <= T && c0 + 16 <= N)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = c * DELTA_CHUNK + 16 * i + col;
-                if (t < T && c0 + 4 * grp < N) *reinterpret_cast<u32x2*>(y + wide(t) * p.H * N) = u32x2{pack2<E>(Y[i][0], Y[i][1]), pack2<E>(Y[i][2], Y[i][3])};
-            }
+                for (int i = 0; i < 4; ++i) out(i);
+            else
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (c * DELTA_CHUNK + 16 * i + col < T && c0 + 4 * grp < N) out(i);
             __syncthreads();
         }
         if (on)

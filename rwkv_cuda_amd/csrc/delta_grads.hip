@@ -104,7 +104,7 @@ DEVINL float dot(const u32x4 a, const u32x4 b, float c) {
 DEVINL u32x4 lower_column(const lds_t base, const int lane, const int j, const int s) {
     typedef v4s __attribute__((address_space(3))) * ptr;
     const int l = lane & 15;
-    const lds_t at = Lower<0>::at(base, 2 * s, 4 * (lane >> 4) + (l >> 2)) + 64 * (j / 2) + 16 * (l & 3) + 8 * (j % 2);
+    const lds_t at = Lower<0>::at(base, 2 * s, 4 * (lane >> 4) + (l >> 2), j / 2, l & 3) + 8 * (j % 2);
     const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(at)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(at + 16 * (s ? Lower<0>::LONG : Lower<0>::SHORT)));
     return join(__builtin_bit_cast(u32x2, a), __builtin_bit_cast(u32x2, b));
 }
@@ -142,7 +142,8 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
 
     // rows of inputs, 16 bytes a lane, BELOW rows from piece to piece; of rows behind the last and channels that are not there others are read, and masked
     constexpr int PIECES = 64 * D / 8 / LANES, BELOW = LANES / (D / 8);
-    const int row0 = tid / (D / 8), d0 = 8 * (tid % (D / 8)), most = T - 1 - t0;
+    const int row0 = written_row<D>(written_order<D>(tid)), d0 = 8 * written_piece<D>(tid), most = T - 1 - t0, yrow = written_row<32>(written_order<32>(tid & 255));
+    static_assert(BELOW % 8 == 0);
     const bool in = d0 < N;
     u32x4 kr[PIECES], qr[PIECES];
     {
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
     const int own = 16 * (wave & 3) + col, part = wave >> 2;
     u32x2 vr[OWNS];
     const E* v = static_cast<const E*>(p.v) + b * p.v_sb + h * p.v_sh + (t0 + min(own, most)) * p.v_st;
-    const E* dy = p.dy ? static_cast<const E*>(p.dy) + ((wide(b) * T + t0 + min((tid & 255) / 4, most)) * p.H + h) * N : v;      // (without one the values are read, and not used)
+    const E* dy = p.dy ? static_cast<const E*>(p.dy) + ((wide(b) * T + t0 + min(yrow, most)) * p.H + h) * N : v;      // (without one the values are read, and not used)
     E* dv = static_cast<E*>(p.dv) + ((wide(b) * T + t0 + own) * p.H + h) * N;
     const auto load = [&](const int step) {
         const int row = min(wave, tiles.tiles - 1);
@@ -202,7 +203,7 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
 #pragma unroll
         for (int n = 0; n < PLANES; ++n) Rows<D>::put(lds + L::Q + n * Rows<D>::BYTES, row, d0 / 8, o[n]);
     }
-    const uint32_t y_mask = p.dy ? mask_of((tid & 255) / 4) : 0, v_mask = mask_of(own);
+    const uint32_t y_mask = p.dy ? mask_of(yrow) : 0, v_mask = mask_of(own);
     f32x4 dQ[4], dK[4], R[4], dP[OWN], dA[OWN];
     float both = 0.f, vz = 0.f;                                  // of <dS', S>; of dZ V^T the diagonal
     // The pairs' blocks of row block `pi`: column blocks pj(0), pj(1) .. up to it
@@ -232,7 +233,7 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
             u32x4 o[PLANES];
             planes_of<E>(yr & (32 * step + 8 * (tid % 4) < N ? y_mask : 0), o);
 #pragma unroll
-            for (int n = 0; n < PLANES; ++n) Rows<32>::put(lds + L::DY + n * Rows<32>::BYTES, tid / 4, tid % 4, o[n]);
+            for (int n = 0; n < PLANES; ++n) Rows<32>::put(lds + L::DY + n * Rows<32>::BYTES, yrow, tid % 4, o[n]);
         }
         f32x4 values[OWNS];
 #pragma unroll
