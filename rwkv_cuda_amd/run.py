@@ -2,7 +2,7 @@
 
     python -m rwkv_cuda_amd.run OP [check|benchmark] [--B n --T n --H n]
 
-    OP: wkv  depthwise_conv1d  wkv5  wkv5_bf16  wkv5a  wkv6  wkv6_state  rwkv7  rwkv7_fp32  gated_recurrence  attention
+    OP: wkv  depthwise_conv1d  wkv5  wkv5_bf16  wkv5a  wkv6  wkv6_state  rwkv7  rwkv7_fp32  gated_recurrence  gated_delta  attention
 
 `check` runs the HIP op forward and backward (through the "strange loss" of the reference's checks,
 wkv6_state/run.py:171-172) beside a plain torch formula of the same op evaluated in fp32 on the same
@@ -104,6 +104,19 @@ def formula_recurrence(w, x, h0):
     return torch.stack(ys, 1), h
 
 
+def formula_delta(q, k, v, g, beta, s0):
+    """gated_delta with the scale 1 / sqrt(N): S = e^g S + k beta (v - (e^g S)^T k)^T, y = scale S^T q; q, k [B,T,Hk,N], v [B,T,H,N], s0 [B,H,N,N]."""
+    G = v.shape[2] // k.shape[2]
+    q, k = (z.repeat_interleave(G, 2) for z in (q, k))
+    S, ys = s0, []
+    for t in range(q.shape[1]):
+        S = S * torch.exp(g[:, t])[..., None, None]
+        u = beta[:, t, :, None] * (v[:, t] - (k[:, t, :, :, None] * S).sum(2))
+        S = S + k[:, t, :, :, None] * u[:, :, None]
+        ys.append((q[:, t, :, :, None] * S).sum(2) * q.shape[-1] ** -0.5)
+    return torch.stack(ys, 1), S
+
+
 def formula_attention(q, k, v, slopes, cap):
     """attention, causal, with capped scores and a distance bias; q [B,T,H,N], k, v [B,T,Hk,N]."""
     T, G = q.shape[1], q.shape[2] // k.shape[2]
@@ -126,7 +139,7 @@ def case(op, dev, B, T, H, bench=False):
     the op's dtype).  Outputs are tuples; every output enters the loss.  With bench=True the wkv6 decays are the
     per-channel uniform(-8, 1) of the reference's speed runs (wkv6_state/run.py:188,284) instead of the low-rank form,
     whose spread grows with C until every decay is 0 or 1."""
-    from . import attention, depthwise_conv1d, gated_recurrence, rwkv7_fast_fused, wkv, wkv5, wkv5_bf16, wkv5a, wkv6, wkv6_state
+    from . import attention, depthwise_conv1d, gated_delta, gated_recurrence, rwkv7_fast_fused, wkv, wkv5, wkv5_bf16, wkv5a, wkv6, wkv6_state
     C = H * N
     bf = torch.bfloat16
     U = lambda lo, hi, *s: _uniform(dev, lo, hi, *s)
@@ -189,6 +202,12 @@ def case(op, dev, B, T, H, bench=False):
     if op == "gated_recurrence":
         names, t = ["w", "x", "h0"], [rb(U(0, 4, B, T, C)), rb(U(-1, 1, B, T, C)), U(-1, 1, B, C)]
         return names, t, formula_recurrence, lambda w, x, h0: gated_recurrence.RUN_CUDA(w, x, h0.float()), bf
+    if op == "gated_delta":                          # two heads to a key head where H is even; q and k of length 1
+        Hk = H // 2 if H % 2 == 0 else H
+        unit = lambda z: rb(z / z.norm(dim=-1, keepdim=True))
+        names, t = ["q", "k", "v", "g", "beta", "s0"], [unit(U(-1, 1, B, T, Hk, N)), unit(U(-1, 1, B, T, Hk, N)), rb(U(-1, 1, B, T, H, N)), rb(-torch.exp(U(-4, 0, B, T, H))), rb(U(0, 1, B, T, H)),
+                                                        rb(U(-1, 1, B, H, N, N) * 0.1)]
+        return names, t, formula_delta, lambda q, k, v, g, beta, s0: gated_delta.RUN_CUDA(q, k, v, g, beta, s0.float()), bf
     if op == "attention":                            # two query heads to a key head where H is even
         Hk = H // 2 if H % 2 == 0 else H
         names, t = ["q", "k", "v"], [rb(U(-2, 2, B, T, H, N)), rb(U(-2, 2, B, T, Hk, N)), rb(U(-1, 1, B, T, Hk, N))]
@@ -198,7 +217,7 @@ def case(op, dev, B, T, H, bench=False):
     raise SystemExit(f"unknown op {op!r}")
 
 
-OPS = ["wkv", "depthwise_conv1d", "wkv5", "wkv5_bf16", "wkv5a", "wkv6", "wkv6_state", "rwkv7", "rwkv7_fp32", "gated_recurrence", "attention"]
+OPS = ["wkv", "depthwise_conv1d", "wkv5", "wkv5_bf16", "wkv5a", "wkv6", "wkv6_state", "rwkv7", "rwkv7_fp32", "gated_recurrence", "gated_delta", "attention"]
 # err-ratio bars of `check`: bf16 outputs carry 2^-9 relative rounding; fp32 paths sum in a different order only
 BAR = {torch.bfloat16: 2e-2, torch.float32: 2e-4}
 
@@ -231,7 +250,7 @@ def check(op, dev, B, T, H, out=print):
 # the reference's benchmark shapes: (B, T, H); its wkv6 shape or the like for what it does not have
 BENCH_SHAPE = {"wkv": (4, 512, 12), "depthwise_conv1d": (32, 768, 12), "wkv5": (8, 4096, 64), "wkv5_bf16": (8, 4096, 32),
                "wkv5a": (8, 4096, 64), "wkv6": (8, 4096, 32), "wkv6_state": (8, 4096, 32), "rwkv7": (8, 1024, 64),
-               "rwkv7_fp32": (8, 1024, 64), "gated_recurrence": (8, 4096, 64), "attention": (8, 4096, 32)}
+               "rwkv7_fp32": (8, 1024, 64), "gated_recurrence": (8, 4096, 64), "gated_delta": (8, 4096, 32), "attention": (8, 4096, 32)}
 
 
 def benchmark(op, dev, B, T, H, out=print):
