@@ -127,8 +127,8 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
     const lds_t lds = lds_of(smem);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, grp = lane >> 4;
     const int N = p.N, T = p.T, chunks = (T + DELTA_CHUNK - 1) / DELTA_CHUNK;
-    const int64_t chunk = blockIdx.x;
-    const int hb = static_cast<int>(chunk / chunks), t0 = static_cast<int>(chunk % chunks) * DELTA_CHUNK, b = hb / p.H, h = hb % p.H, hk = h / (p.H / p.Hk);
+    const int t0 = blockIdx.x * DELTA_CHUNK, h = blockIdx.y, b = blockIdx.z, hk = h / (p.H / p.Hk);
+    const int64_t chunk = (wide(b) * p.H + h) * chunks + blockIdx.x;
     const DeltaTiles tiles(p);
     const float *states = static_cast<const float*>(p.saved), *updates = states + tiles.states();
 
@@ -349,6 +349,11 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
         }
         return o;
     };
+    // where a wave's part of the chunk begins, what 16 tokens take there, and a lane's place: bytes
+    const bool own_channels = 16 * wave + 4 * grp < N;
+    const int size = dq_of ? 4 : 2, heads = dq_of ? p.H : p.Hk;
+    const int64_t to = (((wide(b) * T + t0) * heads + (dq_of ? h : hk)) * N + 16 * wave) * size, step = wide(16) * heads * N * size;
+    const uint32_t at_lane = (static_cast<uint32_t>(col) * heads * N + 4 * grp) * size;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int ti = 16 * i + col;
@@ -371,16 +376,13 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
                 dK[i] = mma_in<E>(kc[s], lower_columns(lds + L::A, lane, i, s), dK[i]);
             }
         }
-        const int tt = t0 + ti, c = 16 * wave + 4 * grp;
-        if (tt >= T || c >= N) continue;
+        if (t0 + ti >= T || !own_channels) continue;
         if (dq_of) {
-            const int64_t to = ((wide(b) * T + tt) * p.H + h) * N + c;
-            *reinterpret_cast<f32x4*>(dq_of + to) = dQ[i];
-            *reinterpret_cast<f32x4*>(dk_of + to) = dK[i];
+            *reinterpret_cast<f32x4*>(reinterpret_cast<char*>(dq_of) + to + i * step + at_lane) = dQ[i];
+            *reinterpret_cast<f32x4*>(reinterpret_cast<char*>(dk_of) + to + i * step + at_lane) = dK[i];
         } else {
-            const int64_t to = ((wide(b) * T + tt) * p.Hk + hk) * N + c;
-            *reinterpret_cast<u32x2*>(static_cast<E*>(p.dq) + to) = u32x2{pack2<E>(dQ[i][0], dQ[i][1]), pack2<E>(dQ[i][2], dQ[i][3])};
-            *reinterpret_cast<u32x2*>(static_cast<E*>(p.dk) + to) = u32x2{pack2<E>(dK[i][0], dK[i][1]), pack2<E>(dK[i][2], dK[i][3])};
+            *reinterpret_cast<u32x2*>(static_cast<char*>(p.dq) + to + i * step + at_lane) = u32x2{pack2<E>(dQ[i][0], dQ[i][1]), pack2<E>(dQ[i][2], dQ[i][3])};
+            *reinterpret_cast<u32x2*>(static_cast<char*>(p.dk) + to + i * step + at_lane) = u32x2{pack2<E>(dK[i][0], dK[i][1]), pack2<E>(dK[i][2], dK[i][3])};
         }
     }
     __syncthreads();
@@ -409,15 +411,15 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
         if (lane >= x) prefix += c;
     }
     const bool counts = token.real && !token.cut && !(gate < DELTA_NONE);
-    const int64_t to = (wide(b) * T + t0 + lane) * p.H + h;
-    static_cast<E*>(p.dg)[to] = from_f<E>(counts ? suffix + (prefix - before) + ends * lds_ld<float>(at(Scalars::ENTER, 63)) : 0.f);
-    static_cast<E*>(p.dbeta)[to] = from_f<E>(db);
+    const int64_t token_at = (wide(b) * T + t0 + lane) * p.H + h;
+    static_cast<E*>(p.dg)[token_at] = from_f<E>(counts ? suffix + (prefix - before) + ends * lds_ld<float>(at(Scalars::ENTER, 63)) : 0.f);
+    static_cast<E*>(p.dbeta)[token_at] = from_f<E>(db);
 }
 
 template <class E, int D> int run(hipStream_t st, const rwkv_delta_args& p, const float* dS, const float* dZ, float* dq, float* dk) {
     const int64_t blocks = DeltaTiles(p).chunks;
     if (blocks > INT_MAX) return RWKV_ERR_SHAPE;
-    hipLaunchKernelGGL((delta_grads<E, D>), dim3(static_cast<unsigned>(blocks)), dim3(4 * D), 0, st, p, dS, dZ, dq, dk);
+    hipLaunchKernelGGL((delta_grads<E, D>), dim3(static_cast<unsigned>(blocks / p.B / p.H), p.H, p.B), dim3(4 * D), 0, st, p, dS, dZ, dq, dk);
     return launch_status();
 }
 
