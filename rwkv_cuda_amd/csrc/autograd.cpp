@@ -855,9 +855,14 @@ void cache8_write_op(const Tensor& k, const Tensor& v, const Tensor& kp, const T
     require(kp.size(2) == k.size(1), "k, v and the pages have the same heads");
     check_side(slots, "slots", torch::kInt32, {k.size(0)}, k);
     check_writable(kp, "k_pages"), check_writable(vp, "v_pages"), check_writable(ks, "k_scales"), check_writable(vs, "v_scales");
+    for (const Tensor* x : {&kp, &vp})
+        for (int64_t d = 0; d < 3; ++d) require(x->size(d) <= 1 || x->stride(d) != 0, "pages are written: no place of theirs may stand for several (as in an expanded tensor)");
     rwkv_cache8_args a{};
     a.dtype = dtype_of(k, "k", false);
     if (k.size(0) == 0) return;
+    require(kp.numel() == 0 || (kp.data_ptr() != vp.data_ptr() && !touch(ks, vs)), "keys and values need pages and scales of their own");
+    for (const Tensor* x : {&kp, &vp, &ks, &vs})
+        for (const Tensor* y : {&k, &v, &slots}) require(!touch(*x, *y), "pages and scales must share no memory with k, v and slots");
     const Guard guard(k.device());
     a.n = i32(k.size(0)); a.Hk = i32(k.size(1)); a.N = i32(k.size(2)); a.P = i32(kp.size(0)); a.page = i32(kp.size(1));
     a.k = P(k); a.v = P(v); a.k_st = stride_of(k, 0); a.k_sh = stride_of(k, 1); a.v_st = stride_of(v, 0); a.v_sh = stride_of(v, 1);

@@ -4,7 +4,8 @@
 
 q, k [B,T,Hk,N], v [B,T,H,N] with H a multiple of Hk (head h reads head h Hk / H) and N a multiple of 8 up to 128; the innermost dimension
 dense, the other strides multiples of 8 (views of one projection).  g (a log decay) and beta [B,T,H].  Keys are taken as they are: with lengths above
-1 and beta above 1 the state may grow without bounds.  Below -104 a log decay is a decay of 0, as exp gives it in fp32.
+1 and beta above 1 the state may grow without bounds.  Below -104 a log decay is a decay of 0, as exp gives it in fp32; above 0 it lets the state
+grow, and e to the sum of 64 of them in a row must be an fp32 number.
 
 `doc` [B,T] int32 names the document of each token of a packed or padded batch, as for gated_recurrence.RUN_CUDA: where it changes, a
 document starts from a state of zero; a negative one is padding, whose y is 0 and which leaves the state as it is, whatever stands there."""

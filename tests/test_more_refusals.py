@@ -142,9 +142,19 @@ def test_cache_refusals_on_the_device(lib):
                  lambda: R(q.clone().requires_grad_(True), pages, pages, sc, sc, i32(2, 2), i32(2)), lambda: R(q, pages, pages, sc, sc, i32(2, 2), i32(2), slopes=z(3, dt=torch.float32))):
         with pytest.raises(AssertionError):
             call()
-    for call in (lambda: W(k, k, pages[:0], pages[:0], sc[:0], sc[:0], i32(5)), lambda: R(q, pages, pages, sc, sc, i32(2, 0), i32(2)), lambda: W(z(5, 2, 68)[..., 4:], k, pages, pages, sc, sc, i32(5))):
+    for call in (lambda: W(k, k, pages[:0], pages[:0], sc[:0], sc[:0], i32(5)), lambda: R(q, pages, pages, sc, sc, i32(2, 0), i32(2)), lambda: W(z(5, 2, 68)[..., 4:], k, pages, pages.clone(), sc, sc.clone(), i32(5))):
         with pytest.raises(_lib.RwkvHipError):
             call()
+    # what two waves would write at once, or one while another reads it
+    vp, vs = pages.clone(), sc.clone()
+    W(k, k, pages, vp, sc, vs, i32(5))
+    wide, whole = pages[:1].expand(3, 16, 2, 64), z(3, 2, 16, 2, 64, dt=torch.uint8).view(torch.float8_e4m3fn)
+    for call, what in ((lambda: W(k, k, pages, pages, sc, vs, i32(5)), "of their own"), (lambda: W(k, k, pages, vp, sc, sc, i32(5)), "of their own"), (lambda: W(k, k, wide, vp, sc, vs, i32(5)), "expanded"),
+                       (lambda: W(k, k, pages, vp[:, :1].expand(3, 16, 2, 64), sc, vs, i32(5)), "expanded"), (lambda: W(k, k, pages, vp, sc, vs, sc.view(torch.int32).flatten()[:5]), "share no memory"),
+                       (lambda: W(pages.view(torch.bfloat16).flatten()[:640].view(5, 2, 64), k, pages, vp, sc, vs, i32(5)), "share no memory")):
+        with pytest.raises(AssertionError, match=what):
+            call()
+    W(k, k, whole[:, 0], whole[:, 1], sc, vs, i32(5))            # (side by side they may lie)
 
 
 @gpu
