@@ -32,12 +32,12 @@ template <class E> DEVINL u32x4 widen8(const uint32_t x, const uint32_t y) {
     return u32x4{a[0], a[1], b[0], b[1]};
 }
 
-template <class E, int D>
-__global__ __launch_bounds__(64 * WAVES, 2) void paged8_attn(const rwkv_paged8_args p, const int shift, const int pieces, const int chunks, const int group, const int shares, float* part) {
+template <class E, int D, int W>
+__global__ __launch_bounds__(64 * W, 2) void paged8_attn(const rwkv_paged8_args p, const int shift, const int pieces, const int chunks, const int group, const int shares, float* part) {
     constexpr int ROWS = 64 / (D / 16), VSTEPS = STEP / ROWS;       // rows of an access of a wave, accesses of 32 rows
-    __shared__ __align__(16) char smem[WAVES * STEP * 2 * D];
-    __shared__ __align__(16) float scale_of_key[WAVES][STEP], log_of_value[WAVES][STEP], inverse_of_value[WAVES][STEP];
-    __shared__ float top_of[WAVES][HEADS], sum_of[WAVES][HEADS];
+    __shared__ __align__(16) char smem[W * STEP * 2 * D];
+    __shared__ __align__(16) float scale_of_key[W][STEP], log_of_value[W][STEP], inverse_of_value[W][STEP];
+    __shared__ float top_of[W][HEADS], sum_of[W][HEADS];
     // `group` neighbouring heads (with their chunks) are a share, and an XCD has whole shares; 0: the pieces of a head one after the other
     const int slot = group > 1 ? blockIdx.x >> 3 : blockIdx.x, share = group > 1 ? slot / group * 8 + (blockIdx.x & 7) : slot;
     if (share >= shares) return;
@@ -101,7 +101,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged8_attn(const rwkv_paged8_a
     float m = -INFINITY, l = 0.f;
     int j0 = static_cast<int>(begin) + wave * STEP;
     if (j0 < end) load(j0);
-    for (; j0 < end; j0 += WAVES * STEP) {
+    for (; j0 < end; j0 += W * STEP) {
         f32x4_t s[2] = {f32x4_t{}, f32x4_t{}};
 #pragma unroll
         for (int e = 0; e < 2; ++e)
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged8_attn(const rwkv_paged8_a
         }
         const uint32_t on = static_cast<uint32_t>(__ballot(on_of));  // which of the 32 tokens count (twice)
         const int now = j0;
-        if (j0 + WAVES * STEP < end) load(j0 + WAVES * STEP);
+        if (j0 + W * STEP < end) load(j0 + W * STEP);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // the wave's own writes above
         float top = -INFINITY;
 #pragma unroll
@@ -180,17 +180,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged8_attn(const rwkv_paged8_a
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4_t*>(sums + (wave * HEADS + col) * D + 4 * ((4 * d + grp) ^ col)) = o[d];
     __syncthreads();
-    for (int i = tid; i < HEADS * D / 4; i += 64 * WAVES) {
+    for (int i = tid; i < HEADS * D / 4; i += 64 * W) {
         const int x = i / (D / 4), c = i % (D / 4), hd = chunk * HEADS + x;
         if (hd >= G || 4 * c >= p.N) continue;
         float top = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < WAVES; ++k) top = fmaxf(top, top_of[k][x]);
+        for (int k = 0; k < W; ++k) top = fmaxf(top, top_of[k][x]);
         const float base = top == -INFINITY ? 0.f : top;
         float sum = 0.f;
         f32x4_t y = f32x4_t{};
 #pragma unroll
-        for (int k = 0; k < WAVES; ++k) {
+        for (int k = 0; k < W; ++k) {
             const float f = __builtin_amdgcn_exp2f(top_of[k][x] - base);
             sum = fmaf(sum_of[k][x], f, sum);
             y += *reinterpret_cast<const f32x4_t*>(sums + (k * HEADS + x) * D + 4 * (c ^ x)) * f;
@@ -210,12 +210,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged8_attn(const rwkv_paged8_a
 // The same for at most 8 query heads of a key head, 64 tokens a step.  There a product of 16 keys and 16 heads would have empty columns, and the softmax, which costs most of the instructions, would
 // run over them; so the heads' side of the product has the heads once for each of TILES tiles of 16 tokens, in rows of their own, zero elsewhere, and TILES products add up to scores that fill the
 // lanes: 4 tiles of one or two heads (a lane has a token, and R heads), or 2 tiles of up to 8 (R = 4).  A lane has its own token's scales.  The weights go to the other product through LDS, 128 bytes a head.
-template <class E, int D, int TILES, int R>
-__global__ __launch_bounds__(64 * WAVES, 2) void paged8_few(const rwkv_paged8_args p, const int shift, const int pieces, const int group, const int shares, float* part) {
+template <class E, int D, int TILES, int R, int W>
+__global__ __launch_bounds__(64 * W, 2) void paged8_few(const rwkv_paged8_args p, const int shift, const int pieces, const int group, const int shares, float* part) {
     constexpr int PER = 16 / TILES, SETS = 4 / TILES, TOKENS = 64, ROWS = 64 / (D / 16), VSTEPS = TOKENS / ROWS, WPITCH = 2 * TOKENS + 16;
-    __shared__ __align__(16) char smem[WAVES * STEP * 2 * D];
-    __shared__ __align__(16) char weights[WAVES][PER * WPITCH];
-    __shared__ float top_of[WAVES][PER], sum_of[WAVES][PER];
+    __shared__ __align__(16) char smem[W * STEP * 2 * D];
+    __shared__ __align__(16) char weights[W][PER * WPITCH];
+    __shared__ float top_of[W][PER], sum_of[W][PER];
     const int slot = group > 1 ? blockIdx.x >> 3 : blockIdx.x, share = group > 1 ? slot / group * 8 + (blockIdx.x & 7) : slot;
     if (share >= shares) return;
     const int of_piece = p.Hk / max(group, 1);
@@ -268,7 +268,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged8_few(const rwkv_paged8_ar
             const float k = kscales[wide(page[a]) * p.Hk], v = vscales[wide(page[a]) * p.Hk];
             kscale[a] = k, vscale[a] = on[a] ? v : 1.f;
         }
-        if (j0 + WAVES * TOKENS < end) load_pages(j0 + WAVES * TOKENS);
+        if (j0 + W * TOKENS < end) load_pages(j0 + W * TOKENS);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             const uint8_t* row = kpages + page_of(t, col) * p.k_sp + ((j0 + 16 * t + col) & (p.page - 1)) * p.k_st;
@@ -293,7 +293,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged8_few(const rwkv_paged8_ar
     for (int r = 0; r < R; ++r) m[r] = -INFINITY, l[r] = 0.f;
     int j0 = static_cast<int>(begin) + wave * TOKENS;
     if (j0 < end) load_pages(j0), load_keys(j0), load_values(j0);
-    for (; j0 < end; j0 += WAVES * TOKENS) {
+    for (; j0 < end; j0 += W * TOKENS) {
         // what belongs to no token that counts, or stands behind a row's end, is zero: a weight of 0 would leave values that are no numbers, and keys' meet in the sums of the tiles' products
         bool whole = p.N == D;
         uint64_t counts[SETS];
@@ -329,7 +329,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged8_few(const rwkv_paged8_ar
         bool is[SETS];
 #pragma unroll
         for (int a = 0; a < SETS; ++a) ks[a] = kscale[a], lv[a] = __builtin_amdgcn_logf(vscale[a]), iv[a] = __builtin_amdgcn_rcpf(vscale[a]), is[a] = on[a];
-        const int next = j0 + WAVES * TOKENS;
+        const int next = j0 + W * TOKENS;
         if (next < end) load_keys(next);
         float x[SETS][R], top[R];
 #pragma unroll
@@ -416,17 +416,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged8_few(const rwkv_paged8_ar
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4_t*>(sums + (wave * PER + col) * D + 4 * ((4 * d + grp) ^ col)) = o[d];
     __syncthreads();
-    for (int i = tid; i < G * D / 4; i += 64 * WAVES) {
+    for (int i = tid; i < G * D / 4; i += 64 * W) {
         const int h = i / (D / 4), c = i % (D / 4);
         if (4 * c >= p.N) continue;
         float top = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < WAVES; ++k) top = fmaxf(top, top_of[k][h]);
+        for (int k = 0; k < W; ++k) top = fmaxf(top, top_of[k][h]);
         const float base = top == -INFINITY ? 0.f : top;
         float sum = 0.f;
         f32x4_t y = f32x4_t{};
 #pragma unroll
-        for (int k = 0; k < WAVES; ++k) {
+        for (int k = 0; k < W; ++k) {
             const float f = __builtin_amdgcn_exp2f(top_of[k][h] - base);
             sum = fmaf(sum_of[k][h], f, sum);
             y += *reinterpret_cast<const f32x4_t*>(sums + (k * PER + h) * D + 4 * (c ^ h)) * f;
@@ -443,6 +443,16 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged8_few(const rwkv_paged8_ar
     }
 }
 
+// How many pieces a sequence is cut into; 0: it stays whole, a workgroup of eight waves each, and is not joined: where two rounds of those are enough, or where there are so many sequences and heads that pieces
+// would be small.  us, in pieces and whole: heads of 128, 8 keys' heads, 4 query heads each, room for 500 tokens, 1 row 9.3 9.6, 8 rows 10.2 9.8, 32 rows 16.4 10.0, 64 rows 28 19;  for 1000 tokens (four
+// rounds) 9.0 14.1, 10.6 14.2, 25.0 15.2, 34 27;  for 2000, 32 rows 33 25.5, 64 rows 46 42.5;   heads of 64, 32 keys' heads, one query head, 500 tokens 8.4 6.1, 11.7 6.2, 1000 tokens 8.5 7.7, 15.2 11.5;
+// 8 keys' heads, 4 query heads, 1000 tokens, 32 rows 21.0 10.8.  (32 keys' heads and 64 rows are 2048 workgroups that stay whole with four waves: with eight 45 us instead of 30.)
+inline int plan_of(int B, int H, int Hk, int N, int page, int M) {
+    const int64_t blocks = static_cast<int64_t>(B) * Hk * chunks_of(H, Hk), round = N <= 64 && H / Hk <= 8 ? 512 : 256, rounds = (static_cast<int64_t>(M) * page + round - 1) / round;
+    const int pieces = pieces_of(B, H, Hk, page, M);
+    return pieces > 1 && (rounds <= 2 || (blocks >= 128 && rounds <= 8)) ? 0 : pieces;
+}
+
 // Rows of 64 bytes: sixteen or eight neighbouring heads on one XCD, whose L2 reads lines of 128 bytes.  B64, up to 4096 tokens, H32 Hk32 N64: 196 us one by one, 158 in twos, 142 in eights, 133 in
 // sixteens; B64 H32 Hk8 N64 54, 45, 45.  Rows of 128 bytes gain nothing: there the heads of a piece come one after the other, or where pieces are many the pieces of a head: B16, up to 8192 tokens,
 // H32 Hk8 N128, 16 pieces, 54 us and 58 (in eights 58); B4, up to 131072, H64 Hk8 N128, 64 pieces, 181 and 171 (in eights 177).
@@ -453,15 +463,16 @@ inline int group_of(int N, int heads, int pieces, int64_t blocks) {
     return pieces >= 32 ? 0 : 1;
 }
 
-template <class E, int D> int run(hipStream_t st, const rwkv_paged8_args& p) {
-    const int shift = __builtin_ctz(p.page), pieces = pieces_of(p.B, p.H, p.Hk, p.page, p.M), chunks = chunks_of(p.H, p.Hk);
+// W waves a workgroup
+template <class E, int D, int W> int run(hipStream_t st, const rwkv_paged8_args& p, const int pieces) {
+    const int shift = __builtin_ctz(p.page), chunks = chunks_of(p.H, p.Hk);
     float* part = static_cast<float*>(p.workspace);
     const int64_t blocks = static_cast<int64_t>(pieces) * p.Hk * chunks * p.B;
     const int group = group_of(p.N, p.Hk * chunks, pieces, blocks);
     const int64_t shares = blocks / std::max(group, 1), grid = group > 1 ? (shares + 7) / 8 * 8 * group : blocks;
     if (grid > INT_MAX) return RWKV_ERR_SHAPE;
     const auto few = [&](auto tiles, auto heads) {
-        hipLaunchKernelGGL((paged8_few<E, D, decltype(tiles)::value, decltype(heads)::value>), dim3(static_cast<unsigned>(grid)), dim3(64 * WAVES), 0, st, p, shift, pieces, group, static_cast<int>(shares), part);
+        hipLaunchKernelGGL((paged8_few<E, D, decltype(tiles)::value, decltype(heads)::value, W>), dim3(static_cast<unsigned>(grid)), dim3(64 * W), 0, st, p, shift, pieces, group, static_cast<int>(shares), part);
     };
     using std::integral_constant;
     // us, B16, up to 8192 tokens, heads of 64 (16 keys' heads) and of 128 (8); paged8_few with 4 tiles, with 2, paged8_attn:
@@ -471,11 +482,15 @@ template <class E, int D> int run(hipStream_t st, const rwkv_paged8_args& p) {
     if (G == 1) few(integral_constant<int, 4>(), integral_constant<int, 1>());
     else if (D == 64 && G == 2) few(integral_constant<int, 4>(), integral_constant<int, D == 64 ? 2 : 1>());
     else if (G <= 8 && (D == 64 || G > 4)) few(integral_constant<int, 2>(), integral_constant<int, 4>());
-    else hipLaunchKernelGGL((paged8_attn<E, D>), dim3(static_cast<unsigned>(grid)), dim3(64 * WAVES), 0, st, p, shift, pieces, chunks, group, static_cast<int>(shares), part);
+    else hipLaunchKernelGGL((paged8_attn<E, D, W>), dim3(static_cast<unsigned>(grid)), dim3(64 * W), 0, st, p, shift, pieces, chunks, group, static_cast<int>(shares), part);
     if (pieces > 1) hipLaunchKernelGGL((paged_join<rwkv_paged8_args, E, D>), dim3(p.H, p.B), dim3(256), 0, st, p, shift, pieces, part);
     return launch_status();
 }
-template <class E> int run_any(hipStream_t st, const rwkv_paged8_args& p) { return p.N <= 64 ? run<E, 64>(st, p) : run<E, 128>(st, p); }
+template <class E> int run_any(hipStream_t st, const rwkv_paged8_args& p) {
+    const int pieces = plan_of(p.B, p.H, p.Hk, p.N, p.page, p.M);
+    if (pieces == 0) return p.N <= 64 ? run<E, 64, 8>(st, p, 1) : run<E, 128, 8>(st, p, 1);
+    return p.N <= 64 ? run<E, 64, WAVES>(st, p, pieces) : run<E, 128, WAVES>(st, p, pieces);
+}
 
 int check_paged8(const rwkv_paged8_args* p) {
     if (p == nullptr) return RWKV_ERR_NULL;
@@ -499,7 +514,7 @@ extern "C" {
 // a maximum, a sum and an output of each piece and head
 size_t rwkv_paged8_workspace_bytes(int B, int H, int Hk, int N, int page, int M) {
     if (B <= 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || N <= 0 || N > 128 || page <= 0 || M <= 0 || B > 65535 || H > 65535) return 0;
-    const int pieces = rwkv::pieces_of(B, H, Hk, page, M);
+    const int pieces = rwkv::plan_of(B, H, Hk, N, page, M);
     return pieces > 1 ? static_cast<size_t>(B) * H * pieces * (rwkv::width_of(N) + 4) * sizeof(float) : 0;
 }
 
