@@ -463,13 +463,14 @@ template <class E, int D, int SW, int HELPERS, bool BACK> DEVINL void help(const
         __syncthreads();
     }
 }
-// Columns a walking workgroup has, in tiles of 16: as many as leave a workgroup for every CU, so that matrices are made as seldom as may be.  us of the forward, 2048 tokens, bf16, with one, two and
-// four tiles:  heads of 64: 64 of them 65 73 89;  128: 124 76 90;  256: 250 143 98;   heads of 128: 32 of them 81 88 115;  64: 155 94 116;  128: 309 176 131;  256: 619 350 256
+// Columns a walking workgroup has, in tiles of 16.  A CU holds one workgroup, and one with more tiles takes longer, by the costs below, but makes its matrices for more of them: the width whose rounds
+// over 256 CUs take the least.  us of the forward, 2048 tokens, bf16, with one, two and four tiles:  heads of 64: 64 of them 65 73 89;  128: 124 76 90;  256: 250 143 98;   heads of 128: 32 of them
+// 81 88 115;  64: 155 94 116;  128: 309 176 131;  256: 619 350 256
 template <class Run> int walk_width(const rwkv_delta_args& p, Run run) {
     const int64_t heads = static_cast<int64_t>(p.B) * p.H, tiles = (p.N + 15) / 16;
-    const auto enough = [&](int sw) { return heads * ((tiles + sw - 1) / sw) >= 256; };
-    if (enough(4)) return run(std::integral_constant<int, 4>{});
-    return enough(2) ? run(std::integral_constant<int, 2>{}) : run(std::integral_constant<int, 1>{});
+    const auto cost = [&](const int sw) { return (heads * ((tiles + sw - 1) / sw) + 255) / 256 * (sw == 1 ? 8 : (sw == 2 ? 9 : 12)); };
+    if (cost(1) <= cost(2) && cost(1) <= cost(4)) return run(std::integral_constant<int, 1>{});
+    return cost(2) <= cost(4) ? run(std::integral_constant<int, 2>{}) : run(std::integral_constant<int, 4>{});
 }
 
 }  // namespace
