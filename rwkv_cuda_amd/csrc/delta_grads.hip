@@ -115,7 +115,7 @@ template <class E, int D> struct Place {
     static constexpr lds_t K = 0, Q = K + PLANES * Rows<D>::BYTES, SLICES = Q + PLANES * Rows<D>::BYTES, DY = SLICES, U = DY + PLANES * Rows<32>::BYTES, Z = U + Slice<64>::BYTES,
                            S = Z + Slice<64>::BYTES, DS = S + Slice<D>::BYTES, SLICES_END = DS + Slice<D>::BYTES, P = SLICES, A = P + Lower<0>::BYTES, MATRICES_END = A + Lower<0>::BYTES,
                            SCALARS = SLICES_END > MATRICES_END ? SLICES_END : MATRICES_END, ROW = SCALARS + Scalars::BYTES, COLUMN = ROW + 1024, BETA = COLUMN + 1024, VALUES = BETA + 1024,
-                           QUERIES = VALUES + 512, KEYS = QUERIES + 256 * WAVES, READS = KEYS + 256 * WAVES, STATES = READS + 256 * WAVES, BYTES = STATES + 64;
+                           QUERIES = VALUES + 64 * WAVES, KEYS = QUERIES + 256 * WAVES, READS = KEYS + 256 * WAVES, STATES = READS + 256 * WAVES, BYTES = STATES + 64;
     static_assert(BYTES <= 160 * 1024);
 };
 
