@@ -45,6 +45,15 @@ def test_heads(lib, B, T, H, Hk, N, dtype):
     check(t, s0, None, dy, dsT)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("B,H,Hk,N", [(2, 40, 40, 64), (4, 40, 20, 64), (2, 24, 24, 128), (2, 48, 16, 128), (3, 30, 30, 112), (5, 24, 8, 40)])
+def test_every_width_of_the_walks(lib, B, H, Hk, N, dtype):
+    """Heads for two and for four column tiles a workgroup, some of them beyond the last channel."""
+    T = 140
+    t, s0, dy, dsT = inputs(B, T, H, Hk, N, DT[dtype], seed=H)
+    check(t, s0, doc_ids(B, T, "many", seed=N).to(DEV), dy, dsT)
+
+
 @pytest.mark.parametrize("kind", ["two", "many", "padded", "one", "back"])
 @pytest.mark.parametrize("T,N,dtype", [(7, 64, "bf16"), (150, 64, "fp16"), (200, 128, "bf16"), (64, 40, "fp16")])
 def test_documents(lib, kind, T, N, dtype):
@@ -240,3 +249,22 @@ def test_tokens_far_apart_and_long_rows(lib):
     y, sT = G.RUN_CUDA(one(far[0]), k, v, one(far[3]).contiguous(), one(far[4]).contiguous())
     want = G.RUN_CUDA(*small)
     assert all(torch.equal(y[b], want[0][0]) and torch.equal(sT[b], want[1][0]) for b in (0, 1, 1000, B - 1))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("N,kind", [(64, None), (128, "many"), (24, "padded"), (80, "one")])
+def test_what_memory_held_before_counts_nowhere(lib, N, kind, dtype):
+    """The same bits whatever the outputs' and the workspaces' memory held: zeros, NaN, large numbers; and again, twenty times."""
+    t, s0, dy, dsT = inputs(3, 200, 4, 2, N, DT[dtype], seed=N)
+    doc = None if kind is None else doc_ids(3, 200, kind, seed=N).to(DEV)
+    first = None
+    for value in [0.0, float("nan"), 1e4] + 20 * [None]:
+        if value is not None:
+            held = [torch.full((n,), value, device=DEV) for n in (1 << 8, 1 << 12, 1 << 16, 1 << 18, 1 << 20) for _ in range(12)]
+            torch.cuda.synchronize()
+            del held
+        leaves = [z.detach().requires_grad_(True) for z in (*t, s0)]
+        y, sT = G.RUN_CUDA(*leaves[:5], s0=leaves[5], doc=doc)
+        got = [y.detach(), sT.detach(), *torch.autograd.grad((y, sT), leaves, (dy, dsT))]
+        first = got if first is None else first
+        assert all(torch.equal(a, b) for a, b in zip(first, got)), value

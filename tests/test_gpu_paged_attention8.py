@@ -312,3 +312,16 @@ def test_versions_and_streams(lib):
             got.append(P8.RUN_CUDA(q, *c, table, lens))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(want, got)) and all(z._version > b for z, b in zip(caches[0], before))
+
+
+@pytest.mark.parametrize("H,Hk,N,lens", [(4, 4, 64, [3000, 0, 70]), (8, 2, 128, [2500, 1]), (16, 2, 64, [4000]), (32, 2, 128, [1300, 77])])
+def test_what_memory_held_before_counts_nowhere(lib, H, Hk, N, lens):
+    """The same bits whatever the output's and the workspace's memory held, and again."""
+    q, kv, table, lens = cache(lens, H, Hk, N, 16, torch.bfloat16, seed=21)
+    want = check(q, kv, table, lens)
+    for value in [0.0, float("nan"), 1e4] + 10 * [None]:
+        if value is not None:
+            held = [torch.full((n,), value, device=DEV) for n in (1 << 8, 1 << 12, 1 << 16, 1 << 18, 1 << 20) for _ in range(12)]
+            torch.cuda.synchronize()
+            del held
+        assert torch.equal(P8.RUN_CUDA(q, *kv, table, lens), want), value
