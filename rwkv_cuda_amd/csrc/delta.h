@@ -381,23 +381,34 @@ template <class E, int D, int SW, int HELPERS, bool BACK> DEVINL void help(const
     const bool kin = kd < N, vin = vd < N && (!BACK || p.dy);
     const int64_t v_st = BACK ? wide(p.H) * N : p.v_st;
     const auto first = [&](const int c) { return (BACK ? chunks - 1 - c : c) * DELTA_CHUNK; };
-    const E *k = static_cast<const E*>(p.k) + b * p.k_sb + hk * p.k_sh + (kin ? kd : 0), *q = static_cast<const E*>(p.q) + b * p.q_sb + hk * p.q_sh + (kin ? kd : 0);
-    const E* v = BACK ? static_cast<const E*>(p.dy) + (wide(b) * T * p.H + h) * N : static_cast<const E*>(p.v) + b * p.v_sb + h * p.v_sh;
-    if (BACK && !p.dy) v = q - (kin ? kd : 0);                   // (read, not used)
-    v += vin ? vd : 0;
-    const int64_t vs = BACK && !p.dy ? 0 : v_st;
+    const char *k = reinterpret_cast<const char*>(static_cast<const E*>(p.k) + b * p.k_sb + hk * p.k_sh), *q = reinterpret_cast<const char*>(static_cast<const E*>(p.q) + b * p.q_sb + hk * p.q_sh);
+    const char* v = reinterpret_cast<const char*>(BACK ? static_cast<const E*>(p.dy) + (wide(b) * T * p.H + h) * N : static_cast<const E*>(p.v) + b * p.v_sb + h * p.v_sh);
+    if (BACK && !p.dy) v = q;                                    // (read, not used)
+    const int64_t ks = 2 * p.k_st, qs = 2 * p.q_st, vs = BACK && !p.dy ? 0 : 2 * v_st;
     u32x4 kr[KP], qr[KP], vr[VP];
+    // a lane's places in a chunk, bytes, made again only where a chunk has other rows than the one before: rows behind the last are read as it
+    int64_t ko[KP], qo[KP], vo[VP];
+    int rows = -1;
     const auto load = [&](const int c) {
-        const int t0 = first(c), most = T - 1 - t0;              // rows behind the last are read as it
-        const E *kc = k + wide(t0) * p.k_st, *qc = q + wide(t0) * p.q_st, *vc = v + wide(t0) * vs;
+        const int t0 = first(c), last = min(T - 1 - t0, 63);
+        if (last != rows) {
+            rows = last;
+#pragma unroll
+            for (int i = 0; i < KP; ++i) {
+                const int row = min(written_row<D>(krow + KSTEP * i), last), d = 2 * (kin ? kd : 0);
+                ko[i] = row * ks + d, qo[i] = row * qs + d;
+            }
+#pragma unroll
+            for (int i = 0; i < VP; ++i) vo[i] = min(vrow + VSTEP * i, last) * vs + 2 * (vin ? vd : 0);
+        }
+        const char *kc = k + t0 * ks, *qc = q + t0 * qs, *vc = v + t0 * vs;
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
-            const int row = min(written_row<D>(krow + KSTEP * i), min(most, 63));
-            kr[i] = *reinterpret_cast<const u32x4*>(kc + row * p.k_st);
-            qr[i] = *reinterpret_cast<const u32x4*>(qc + row * p.q_st);
+            kr[i] = *reinterpret_cast<const u32x4*>(kc + ko[i]);
+            qr[i] = *reinterpret_cast<const u32x4*>(qc + qo[i]);
         }
 #pragma unroll
-        for (int i = 0; i < VP; ++i) vr[i] = *reinterpret_cast<const u32x4*>(vc + min(vrow + VSTEP * i, min(most, 63)) * vs);
+        for (int i = 0; i < VP; ++i) vr[i] = *reinterpret_cast<const u32x4*>(vc + vo[i]);
     };
     const E *g = static_cast<const E*>(p.g) + b * p.g_sb + h, *beta = static_cast<const E*>(p.beta) + b * p.beta_sb + h;
     E gate, bt;                                                  // (as they come: what is made of them here would wait for them)
