@@ -426,16 +426,26 @@ template <class E, int D, int SW, int HELPERS, bool BACK> DEVINL void help(const
         if (tasks >> 12) make_scalars<BACK>(lds + L::SCALARS + c % 3 * Scalars::BYTES, lane, {is, is && t > 0 && doc != before}, to_f(gate), to_f(bt));
     };
     const auto mask_of = [&](const int row) { return 0u - static_cast<uint32_t>(real >> (row & 63) & 1); };      // all bits of a real token's, none of others
-    const auto put = [&](const int c) {
+    // (with a whole chunk of real tokens and all channels there is nothing to mask)
+    const auto put_rows = [&](const int c, auto whole) {
         const lds_t to = lds + (c & 1) * L::STAGE;
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
             const int row = written_row<D>(krow + KSTEP * i);
             if (64 * RP % LANES != 0 && i == KP - 1 && row >= 64) continue;
-            const uint32_t keep = kin ? mask_of(row) : 0;
-            Rows<D>::put(to + L::K, row, kd / 8, kr[i] & keep);
-            Rows<D>::put(to + L::Q, row, kd / 8, qr[i] & keep);
+            if constexpr (decltype(whole)::value) {
+                Rows<D>::put(to + L::K, row, kd / 8, kr[i]);
+                Rows<D>::put(to + L::Q, row, kd / 8, qr[i]);
+            } else {
+                const uint32_t keep = kin ? mask_of(row) : 0;
+                Rows<D>::put(to + L::K, row, kd / 8, kr[i] & keep);
+                Rows<D>::put(to + L::Q, row, kd / 8, qr[i] & keep);
+            }
         }
+    };
+    const auto put = [&](const int c) {
+        if (real == ~0ull && N == D) put_rows(c, std::true_type());
+        else put_rows(c, std::false_type());
     };
     const auto put_values = [&] {
 #pragma unroll
