@@ -386,29 +386,44 @@ template <class E, int D, int SW, int HELPERS, bool BACK> DEVINL void help(const
     if (BACK && !p.dy) v = q;                                    // (read, not used)
     const int64_t ks = 2 * p.k_st, qs = 2 * p.q_st, vs = BACK && !p.dy ? 0 : 2 * v_st;
     u32x4 kr[KP], qr[KP], vr[VP];
-    // a lane's places in a chunk, bytes, made again only where a chunk has other rows than the one before: rows behind the last are read as it
+    // A lane's places in a chunk, bytes; rows behind the last are read as it.  Heads of 64 keep them from chunk to chunk (32768 tokens of 32 heads: 945 us instead, with them 884), with heads of 128 loads that
+    // follow each other at once cost more than the instructions between them (1148 us, and 1200).
+    constexpr bool KEPT = D == 64;
+    const int kc0 = 2 * (kin ? kd : 0), vc0 = 2 * (vin ? vd : 0);
     int64_t ko[KP], qo[KP], vo[VP];
     int rows = -1;
     const auto load = [&](const int c) {
         const int t0 = first(c), last = min(T - 1 - t0, 63);
-        if (last != rows) {
-            rows = last;
+        const char *kc = k + t0 * ks, *qc = q + t0 * qs, *vc = v + t0 * vs;
+        if constexpr (KEPT) {
+            if (last != rows) {
+                rows = last;
 #pragma unroll
-            for (int i = 0; i < KP; ++i) {
-                const int row = min(written_row<D>(krow + KSTEP * i), last), d = 2 * (kin ? kd : 0);
-                ko[i] = row * ks + d, qo[i] = row * qs + d;
+                for (int i = 0; i < KP; ++i) {
+                    const int row = min(written_row<D>(krow + KSTEP * i), last);
+                    ko[i] = row * ks + kc0, qo[i] = row * qs + kc0;
+                }
+#pragma unroll
+                for (int i = 0; i < VP; ++i) vo[i] = min(vrow + VSTEP * i, last) * vs + vc0;
             }
 #pragma unroll
-            for (int i = 0; i < VP; ++i) vo[i] = min(vrow + VSTEP * i, last) * vs + 2 * (vin ? vd : 0);
-        }
-        const char *kc = k + t0 * ks, *qc = q + t0 * qs, *vc = v + t0 * vs;
+            for (int i = 0; i < KP; ++i) {
+                kr[i] = *reinterpret_cast<const u32x4*>(kc + ko[i]);
+                qr[i] = *reinterpret_cast<const u32x4*>(qc + qo[i]);
+            }
 #pragma unroll
-        for (int i = 0; i < KP; ++i) {
-            kr[i] = *reinterpret_cast<const u32x4*>(kc + ko[i]);
-            qr[i] = *reinterpret_cast<const u32x4*>(qc + qo[i]);
-        }
+            for (int i = 0; i < VP; ++i) vr[i] = *reinterpret_cast<const u32x4*>(vc + vo[i]);
+        } else {
+            kc += kc0, qc += kc0, vc += vc0;
 #pragma unroll
-        for (int i = 0; i < VP; ++i) vr[i] = *reinterpret_cast<const u32x4*>(vc + vo[i]);
+            for (int i = 0; i < KP; ++i) {
+                const int row = min(written_row<D>(krow + KSTEP * i), last);
+                kr[i] = *reinterpret_cast<const u32x4*>(kc + row * ks);
+                qr[i] = *reinterpret_cast<const u32x4*>(qc + row * qs);
+            }
+#pragma unroll
+            for (int i = 0; i < VP; ++i) vr[i] = *reinterpret_cast<const u32x4*>(vc + min(vrow + VSTEP * i, last) * vs);
+        }
     };
     const E *g = static_cast<const E*>(p.g) + b * p.g_sb + h, *beta = static_cast<const E*>(p.beta) + b * p.beta_sb + h;
     E gate, bt;                                                  // (as they come: what is made of them here would wait for them)
