@@ -3,6 +3,8 @@
 // A workgroup has 16 SW of a head's value channels and walks through the sequence, a chunk of 64 tokens after the other.  SW waves keep 16 columns of the state each and do what
 // depends on it; the others bring the next chunk's inputs and make its matrices meanwhile: -A, P and the inverses of the blocks of I + A on the diagonal, with which the triangular system is
 // four steps of products.  Two barriers a chunk: before the first the next chunk's rows go to LDS, behind it they are read.
+// A chunk takes what its walking wave's instructions take, some 560 (heads of 64) or 780 (of 128) at 5 to 6 cycles, 80 to 130 of them products; where a workgroup has four tiles, its SIMDs' issue.  bf16: 32768 tokens
+// of 32 heads of 128 1150 us, 2.25 a chunk; B8 T4096 H32 N64 190 to 200 us, with states and updates kept 230 to 245.
 #include <algorithm>
 
 #include "delta.h"

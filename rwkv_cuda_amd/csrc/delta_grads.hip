@@ -8,6 +8,7 @@
 //   dg_t: all that passes token t, i.e. e^G_64 <dS', S>, the keys' part through dS' of the tokens before, the queries' and keys' parts through S of t and those behind, and the pairs around it.
 // The contractions over value channels go 32 at a time: what the state's waves left as four rows a lane goes to LDS as columns and comes back as rows (ds_read_b64_tr_b16).  A wave has 16 of the
 // key channels, all tokens, and some of the pairs' blocks.  All sums are in a fixed order.
+// Bound by memory: of B8 T4096 H32 N64 bf16 120 KB a chunk and head (64 of them kept by the walks), 2.0 GB in 500 us; two workgroups a CU, whose phases cover each other.
 #include <algorithm>
 
 #include "delta.h"
