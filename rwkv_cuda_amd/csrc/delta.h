@@ -16,6 +16,8 @@
 // bf16 operands they were 2^-9, as large as an output's own rounding, and an fp32 state that is passed on would lose 15 of its 24 bits.
 #pragma once
 
+#include <climits>
+
 #include "attn_tile.h"
 
 namespace rwkv {
@@ -369,18 +371,19 @@ template <int D, int SW, bool BACK> struct WalkPlace {
     static_assert(BYTES <= 160 * 1024);
 };
 
-// The helping waves of a walk: forward the chunks from the first on, with the values beside queries and keys; BACK from the last on, with the gradients of y.  Before the walkers' first barrier
+// The helping waves of a walk over `chunks` chunks from `start` on: forward, with the values beside queries and keys; BACK, downwards, with the gradients of y.  Before the walkers' first barrier
 // a chunk's rows go to LDS, between it and the second the next chunk's matrices are made.
-template <class E, int D, int SW, int HELPERS, bool BACK> DEVINL void help(const rwkv_delta_args& p, const lds_t lds, const int b, const int h, const int hk, const int piece, const int mine, const int lane) {
+template <class E, int D, int SW, int HELPERS, bool BACK> DEVINL void help(const rwkv_delta_args& p, const lds_t lds, const int b, const int h, const int hk, const int piece, const int mine, const int lane, const int start,
+                                                                                      const int chunks) {
     using L = WalkPlace<D, SW, BACK>;
     constexpr int LANES = 64 * HELPERS, RP = D / 8, KP = (64 * RP + LANES - 1) / LANES, VP = (64 * 2 * SW + LANES - 1) / LANES, KSTEP = LANES / RP, VSTEP = LANES / (2 * SW);       // 16 bytes a lane: pieces, rows between them
     static_assert(LANES % RP == 0 && LANES % (2 * SW) == 0);
-    const int N = p.N, T = p.T, chunks = (T + DELTA_CHUNK - 1) / DELTA_CHUNK, tid = 64 * mine + lane;
+    const int N = p.N, T = p.T, tid = 64 * mine + lane;
     const uint32_t tasks = tasks_of<HELPERS>(mine);
     const int krow = written_order<D>(tid), kd = 8 * written_piece<D>(tid), vrow = tid / (2 * SW), vd = 16 * SW * piece + 8 * (tid % (2 * SW));
     const bool kin = kd < N, vin = vd < N && (!BACK || p.dy);
     const int64_t v_st = BACK ? wide(p.H) * N : p.v_st;
-    const auto first = [&](const int c) { return (BACK ? chunks - 1 - c : c) * DELTA_CHUNK; };
+    const auto first = [&](const int c) { return (BACK ? start - c : start + c) * DELTA_CHUNK; };
     const char *k = reinterpret_cast<const char*>(static_cast<const E*>(p.k) + b * p.k_sb + hk * p.k_sh), *q = reinterpret_cast<const char*>(static_cast<const E*>(p.q) + b * p.q_sb + hk * p.q_sh);
     const char* v = reinterpret_cast<const char*>(BACK ? static_cast<const E*>(p.dy) + (wide(b) * T * p.H + h) * N : static_cast<const E*>(p.v) + b * p.v_sb + h * p.v_sh);
     if (BACK && !p.dy) v = q;                                    // (read, not used)
@@ -499,14 +502,39 @@ template <class E, int D, int SW, int HELPERS, bool BACK> DEVINL void help(const
         __syncthreads();
     }
 }
+// Where a row of documents is walked by two workgroups.  Behind a cut nothing counts of what stood before, so that the second of them may begin with a chunk that has one, from a state of zero: what it has at
+// that chunk's end is right, while the chunk itself is the first one's.  (Backward the other way round: the first part's gradient begins with that chunk, which is the second one's.)  The chunk with a cut
+// that is nearest the middle; -1 without one.  By all threads.
+DEVINL int split_at(const int* doc, const int T, const int chunks, int* best) {
+    if (threadIdx.x == 0) *best = INT_MAX;
+    __syncthreads();
+    for (int t = 1 + threadIdx.x; t < T; t += blockDim.x) {
+        const int d = doc[t];
+        if (d < 0 || doc[t - 1] == d) continue;
+        const int off = 2 * (t / DELTA_CHUNK) + 1 - chunks;
+        atomicMin(best, off < 0 ? -2 * off : 2 * off + 1);
+    }
+    __syncthreads();
+    const int key = *best;
+    return key == INT_MAX ? -1 : (chunks - 1 + (key & 1 ? key >> 1 : -(key >> 1))) / 2;
+}
 // Columns a walking workgroup has, in tiles of 16.  A CU holds one workgroup, and one with more tiles takes longer, by the costs below, but makes its matrices for more of them: the width whose rounds
 // over 256 CUs take the least.  us of the forward, 2048 tokens, bf16, with one, two and four tiles:  heads of 64: 64 of them 65 73 89;  128: 124 76 90;  256: 250 143 98;   heads of 128: 32 of them
 // 81 88 115;  64: 155 94 116;  128: 309 176 131;  256: 619 350 256
+// With documents two workgroups may share a row: a walk of three quarters of it is reckoned with, and taken where it costs less (one document then costs an eighth more: split in two a workgroup
+// has two tiles where it had one).
 template <class Run> int walk_width(const rwkv_delta_args& p, Run run) {
-    const int64_t heads = static_cast<int64_t>(p.B) * p.H, tiles = (p.N + 15) / 16;
-    const auto cost = [&](const int sw) { return (heads * ((tiles + sw - 1) / sw) + 255) / 256 * (sw == 1 ? 8 : (sw == 2 ? 9 : 12)); };
-    if (cost(1) <= cost(2) && cost(1) <= cost(4)) return run(std::integral_constant<int, 1>{});
-    return cost(2) <= cost(4) ? run(std::integral_constant<int, 2>{}) : run(std::integral_constant<int, 4>{});
+    using std::integral_constant;
+    const int64_t heads = static_cast<int64_t>(p.B) * p.H, tiles = (p.N + 15) / 16, chunks = (p.T + DELTA_CHUNK - 1) / DELTA_CHUNK;
+    const auto cost = [&](const int sw, const int segments) {
+        return (heads * segments * ((tiles + sw - 1) / sw) + 255) / 256 * (sw == 1 ? 8 : (sw == 2 ? 9 : 12)) * (segments == 1 ? 4 * chunks : 3 * chunks + 4);
+    };
+    int best = 1, segments = 1;
+    for (const int n : {1, 2})
+        for (const int sw : {1, 2, 4})
+            if ((n == 1 || (p.doc && chunks >= 8)) && cost(sw, n) < cost(best, segments)) best = sw, segments = n;
+    if (best == 1) return run(integral_constant<int, 1>{}, segments);
+    return best == 2 ? run(integral_constant<int, 2>{}, segments) : run(integral_constant<int, 4>{}, segments);
 }
 
 }  // namespace

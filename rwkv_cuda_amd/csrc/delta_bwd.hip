@@ -30,21 +30,33 @@ template <class E> DEVINL f32x4 gradients32(const Two32& a, const Gradients<E>& 
 }
 
 template <class E, int D, int SW, int HELPERS>
-__global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_delta_args p, const int pieces, float* states, float* updates) {
+__global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_delta_args p, const int pieces, const int segments, float* states, float* updates) {
     using L = WalkPlace<D, SW, true>;
     __shared__ __align__(16) char smem[L::BYTES];
     const lds_t lds = lds_of(smem);
-    const int slot = blockIdx.x >> 3, piece = slot % pieces, hb = slot / pieces * 8 + (blockIdx.x & 7);
+    const int slot = blockIdx.x >> 3, piece = slot % pieces, segment = slot / pieces % segments, hb = slot / pieces / segments * 8 + (blockIdx.x & 7);
     if (hb >= p.B * p.H) return;
     const int b = hb / p.H, h = hb % p.H, hk = h / (p.H / p.Hk), N = p.N, T = p.T, chunks = (T + DELTA_CHUNK - 1) / DELTA_CHUNK;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, grp = lane >> 4;
+
+    // the chunks of this workgroup, downwards, and whether the first of them is its own
+    int start = chunks - 1, count = chunks;
+    bool first_own = true;
+    if (segments == 2) {
+        __shared__ int best;
+        const int at = split_at(p.doc + wide(b) * T, T, chunks, &best);
+        if (at <= 0) {
+            if (segment == 1) return;
+        } else if (segment == 1) count = chunks - at;
+        else start = at, count = at + 1, first_own = false;
+    }
 
     if (wave < SW) {
         const int ct = piece * SW + wave, c0 = 16 * ct;
         const bool on = c0 + col < N;
         const DeltaTiles tiles(p);
         f32x4 S[D / 16];                                         // dS
-        const float* end = p.dsT ? p.dsT + wide(hb) * N * N : nullptr;
+        const float* end = p.dsT && first_own ? p.dsT + wide(hb) * N * N : nullptr;
 #pragma unroll
         for (int t = 0; t < D / 16; ++t)
 #pragma unroll
@@ -52,12 +64,13 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_d
         const lds_t vread = L::V + lds + (4 * grp + (col >> 2)) * L::VPITCH + 32 * wave + 8 * (col & 3);
         __syncthreads();
         __syncthreads();
-        for (int c = 0; c < chunks; ++c) {
+        for (int c = 0; c < count; ++c) {
+            const bool own = first_own || c > 0;
             const lds_t rows = lds + (c & 1) * L::STAGE, mats = lds + L::MATRICES + (c & 1) * L::MATRIX_STAGE, sc = lds + L::SCALARS + c % 3 * Scalars::BYTES;
             const lds_t K = rows + L::K, Q = rows + L::Q, A = mats + L::A, P = mats + L::P, inv = mats + L::INV;
-            const int64_t chunk = wide(hb) * chunks + chunks - 1 - c;
+            const int64_t chunk = wide(hb) * chunks + start - c;
             typedef v4s __attribute__((address_space(3))) * ptr;
-            if (c0 < N) {
+            if (c0 < N && own) {
 #pragma unroll
                 for (int t = 0; t < D / 16; ++t)
                     if (t < tiles.tiles) *reinterpret_cast<f32x4*>(states + tiles.state(chunk, ct, t) + 4 * lane) = S[t];
@@ -168,13 +181,13 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_d
             columns(K, 0);
             w.take({Z[0] * -ba, Z[1] * -bb});
             advance(w, one);
-            if (c0 < N) {
+            if (c0 < N && own) {
                 float* to = updates + tiles.update(chunk, ct, 0) + 4 * lane;
                 keep(to, split<bf16_t>(Z[0])), keep(to + 256, z1), keep(to + 512, z2), keep(to + 768, z3);
             }
             __syncthreads();
         }
-        if (on && p.ds0)
+        if (on && p.ds0 && start + 1 == count)
 #pragma unroll
             for (int t = 0; t < D / 16; ++t)
 #pragma unroll
@@ -183,16 +196,16 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_d
         return;
     }
 
-    help<E, D, SW, HELPERS, true>(p, lds, b, h, hk, piece, wave - SW, lane);
+    help<E, D, SW, HELPERS, true>(p, lds, b, h, hk, piece, wave - SW, lane, start, count);
 }
 
 template <class E, int D> int run(hipStream_t st, const rwkv_delta_args& p, float* dS, float* dZ) {
-    return walk_width(p, [&](auto sw) {
+    return walk_width(p, [&](auto sw, const int segments) {
         constexpr int SW = decltype(sw)::value;
         const int pieces = (p.N + 16 * SW - 1) / (16 * SW);
-        const int64_t blocks = (static_cast<int64_t>(p.B) * p.H + 7) / 8 * 8 * pieces;
+        const int64_t blocks = (static_cast<int64_t>(p.B) * p.H + 7) / 8 * 8 * pieces * segments;
         if (blocks > INT_MAX) return static_cast<int>(RWKV_ERR_SHAPE);
-        hipLaunchKernelGGL((delta_bwd<E, D, SW, 8 - SW>), dim3(static_cast<unsigned>(blocks)), dim3(512), 0, st, p, pieces, dS, dZ);
+        hipLaunchKernelGGL((delta_bwd<E, D, SW, 8 - SW>), dim3(static_cast<unsigned>(blocks)), dim3(512), 0, st, p, pieces, segments, dS, dZ);
         return launch_status();
     });
 }

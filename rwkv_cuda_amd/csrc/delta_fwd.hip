@@ -13,15 +13,27 @@ namespace rwkv {
 namespace {
 
 template <class E, int D, int SW, int HELPERS>
-__global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_delta_args p, const int pieces) {
+__global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_delta_args p, const int pieces, const int segments) {
     using L = WalkPlace<D, SW, false>;
     __shared__ __align__(16) char smem[L::BYTES];
     const lds_t lds = lds_of(smem);
     // the pieces of a head are neighbours on one XCD: they read the same keys and queries
-    const int slot = blockIdx.x >> 3, piece = slot % pieces, hb = slot / pieces * 8 + (blockIdx.x & 7);
+    const int slot = blockIdx.x >> 3, piece = slot % pieces, segment = slot / pieces % segments, hb = slot / pieces / segments * 8 + (blockIdx.x & 7);
     if (hb >= p.B * p.H) return;
     const int b = hb / p.H, h = hb % p.H, hk = h / (p.H / p.Hk), N = p.N, T = p.T, chunks = (T + DELTA_CHUNK - 1) / DELTA_CHUNK;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, grp = lane >> 4;
+
+    // the chunks of this workgroup, and whether the first of them is its own
+    int start = 0, count = chunks;
+    bool first_own = true;
+    if (segments == 2) {
+        __shared__ int best;
+        const int at = split_at(p.doc + wide(b) * T, T, chunks, &best);
+        if (at < 0 || at == chunks - 1) {
+            if (segment == 1) return;
+        } else if (segment == 0) count = at + 1;
+        else start = at, count = chunks - at, first_own = false;
+    }
 
     if (wave < SW) {
         const int ct = piece * SW + wave, c0 = 16 * ct;          // its columns
@@ -29,7 +41,7 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_d
         float *states = static_cast<float*>(p.saved), *updates = states + tiles.states();
         const bool on = c0 + col < N;
         f32x4 S[D / 16];
-        const float* s0 = p.s0 ? p.s0 + wide(hb) * N * N : nullptr;
+        const float* s0 = p.s0 && first_own ? p.s0 + wide(hb) * N * N : nullptr;
 #pragma unroll
         for (int t = 0; t < D / 16; ++t)
 #pragma unroll
@@ -41,14 +53,16 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_d
         const uint32_t y_lane = static_cast<uint32_t>(col) * row_bytes + 8 * grp;
         __syncthreads();
         __syncthreads();
-        for (int c = 0; c < chunks; ++c) {
+        for (int c = 0; c < count; ++c) {
+            const int at = start + c;
+            const bool own = first_own || c > 0;
             const lds_t rows = lds + (c & 1) * L::STAGE, mats = lds + L::MATRICES + (c & 1) * L::MATRIX_STAGE, sc = lds + L::SCALARS + c % 3 * Scalars::BYTES;
             const lds_t K = rows + L::K, Q = rows + L::Q, A = mats + L::A, P = mats + L::P, inv = mats + L::INV;
             typedef v4s __attribute__((address_space(3))) * ptr;
-            if (p.saved && c0 < N) {
+            if (p.saved && c0 < N && own) {
 #pragma unroll
                 for (int t = 0; t < D / 16; ++t)
-                    if (t < tiles.tiles) *reinterpret_cast<f32x4*>(states + tiles.state(wide(hb) * chunks + c, ct, t) + 4 * lane) = S[t];
+                    if (t < tiles.tiles) *reinterpret_cast<f32x4*>(states + tiles.state(wide(hb) * chunks + at, ct, t) + 4 * lane) = S[t];
             }
             // what a step reads from LDS is on its way a step earlier
             const Two inv0 = Diagonal::row(inv, lane, 0), a10 = Lower<1>::one(A, lane, 1, 0), inv1 = Diagonal::row(inv, lane, 1);
@@ -183,22 +197,22 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_d
             Y[2] = mma16(u2, p22, Y[2]);
             u3 = split<bf16_t>(U[3]);
             Y[3] = mma32(join(u2, u3), p33, Y[3]);
-            if (p.saved && c0 < N) {
-                float* to = updates + tiles.update(wide(hb) * chunks + c, ct, 0) + 4 * lane;
+            if (p.saved && c0 < N && own) {
+                float* to = updates + tiles.update(wide(hb) * chunks + at, ct, 0) + 4 * lane;
                 keep(to, u0), keep(to + 256, u1), keep(to + 512, u2), keep(to + 768, u3);
             }
-            char* const to = yc + wide(c) * DELTA_CHUNK * row_bytes;
+            char* const to = yc + wide(at) * DELTA_CHUNK * row_bytes;
             const auto out = [&](const int i) { *reinterpret_cast<u32x2*>(to + wide(16 * i) * row_bytes + y_lane) = u32x2{pack2<E>(Y[i][0], Y[i][1]), pack2<E>(Y[i][2], Y[i][3])}; };
-            if ((c + 1) * DELTA_CHUNK <= T && c0 + 16 <= N)
+            if (own && (at + 1) * DELTA_CHUNK <= T && c0 + 16 <= N)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) out(i);
-            else
+            else if (own)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (c * DELTA_CHUNK + 16 * i + col < T && c0 + 4 * grp < N) out(i);
+                    if (at * DELTA_CHUNK + 16 * i + col < T && c0 + 4 * grp < N) out(i);
             __syncthreads();
         }
-        if (on)
+        if (on && start + count == chunks)
 #pragma unroll
             for (int t = 0; t < D / 16; ++t)
 #pragma unroll
@@ -207,16 +221,16 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_d
         return;
     }
 
-    help<E, D, SW, HELPERS, false>(p, lds, b, h, hk, piece, wave - SW, lane);
+    help<E, D, SW, HELPERS, false>(p, lds, b, h, hk, piece, wave - SW, lane, start, count);
 }
 
 template <class E, int D> int run(hipStream_t st, const rwkv_delta_args& p) {
-    return walk_width(p, [&](auto sw) {
+    return walk_width(p, [&](auto sw, const int segments) {
         constexpr int SW = decltype(sw)::value;
         const int pieces = (p.N + 16 * SW - 1) / (16 * SW);
-        const int64_t blocks = (static_cast<int64_t>(p.B) * p.H + 7) / 8 * 8 * pieces;
+        const int64_t blocks = (static_cast<int64_t>(p.B) * p.H + 7) / 8 * 8 * pieces * segments;
         if (blocks > INT_MAX) return static_cast<int>(RWKV_ERR_SHAPE);
-        hipLaunchKernelGGL((delta_fwd<E, D, SW, 8 - SW>), dim3(static_cast<unsigned>(blocks)), dim3(512), 0, st, p, pieces);
+        hipLaunchKernelGGL((delta_fwd<E, D, SW, 8 - SW>), dim3(static_cast<unsigned>(blocks)), dim3(512), 0, st, p, pieces, segments);
         return launch_status();
     });
 }

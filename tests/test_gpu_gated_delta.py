@@ -64,6 +64,23 @@ def test_documents(lib, kind, T, N, dtype):
     check(t, None, doc, dy)
 
 
+@pytest.mark.parametrize("cuts", [[], [1], [300], [320], [384], [511, 513], [63, 700], [704], [767], [100, 101, 102, 400, 640], list(range(1, 768))])
+@pytest.mark.parametrize("N,dtype", [(64, "bf16"), (128, "fp16"), (40, "fp16")])
+def test_rows_walked_by_two_workgroups(lib, N, dtype, cuts):
+    """Twelve chunks: documents that begin nowhere, in the first and last chunk only, at chunks' edges, several in a chunk, everywhere; another row without any, and padding around cuts."""
+    T = 768
+    t, s0, dy, dsT = inputs(3, T, 4, 2, N, DT[dtype], seed=len(cuts) + N)
+    doc = torch.zeros(3, T, dtype=torch.int32)
+    for c in cuts:
+        doc[0, c:] += 1
+    doc[2] = doc[0]
+    for c in cuts[:3]:
+        doc[2, max(0, c - 5):c] = -1
+    doc[2, -70:] = -1
+    check(t, s0, doc.to(DEV), dy, dsT)
+    check(t, None, doc.to(DEV), dy)
+
+
 def test_padding_counts_nowhere(lib):
     """NaN and infinities in padding, before, between and behind; rows that are nothing else; dy there too."""
     for N, T, value in ((64, 150, float("nan")), (128, 70, float("inf")), (64, 5, float("nan"))):
