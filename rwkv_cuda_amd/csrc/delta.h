@@ -521,8 +521,8 @@ DEVINL int split_at(const int* doc, const int T, const int chunks, int* best) {
 // Columns a walking workgroup has, in tiles of 16.  A CU holds one workgroup, and one with more tiles takes longer, by the costs below, but makes its matrices for more of them: the width whose rounds
 // over 256 CUs take the least.  us of the forward, 2048 tokens, bf16, with one, two and four tiles:  heads of 64: 64 of them 65 73 89;  128: 124 76 90;  256: 250 143 98;   heads of 128: 32 of them
 // 81 88 115;  64: 155 94 116;  128: 309 176 131;  256: 619 350 256
-// With documents two workgroups may share a row: a walk of three quarters of it is reckoned with, and taken where it costs less (one document then costs an eighth more: split in two a workgroup
-// has two tiles where it had one).
+// With documents two workgroups may share a row: a walk of three quarters of it is reckoned with, and taken where it costs less.  us of the forward, bf16, a row of 3001 tokens, 32 heads of 128, no documents,
+// one, two halves, five: 122 135 76 86;  32 heads of 64 95 100 58 66;  8192 tokens of 8 heads of 64 246 257 135 160;  4 rows of 2048, 16 heads of 64, 69 77 46 53
 template <class Run> int walk_width(const rwkv_delta_args& p, Run run) {
     using std::integral_constant;
     const int64_t heads = static_cast<int64_t>(p.B) * p.H, tiles = (p.N + 15) / 16, chunks = (p.T + DELTA_CHUNK - 1) / DELTA_CHUNK;

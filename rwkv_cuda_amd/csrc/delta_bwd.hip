@@ -2,7 +2,7 @@
 //
 // As delta_fwd.hip, from the last chunk to the first: a workgroup has 16 SW value channels of a head's state gradient dS.  Of each chunk it leaves dS as it leaves the chunk and dZ, the gradient
 // of the triangular system's right side, in memory; the gradients of the inputs, whose sums run over all value channels, are delta_grads.hip's.  Bound as the forward: B8 T4096 H32 N64 bf16 220 to 235 us,
-// 3001 tokens of 32 heads of 128 fp16 165 us, 3.5 a chunk.
+// 3001 tokens of 32 heads of 128 fp16 165 us, 3.5 a chunk, in five documents 108.
 #include <algorithm>
 
 #include "delta.h"
