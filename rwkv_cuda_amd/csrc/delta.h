@@ -533,8 +533,11 @@ template <class Run> int walk_width(const rwkv_delta_args& p, Run run) {
     for (const int n : {1, 2})
         for (const int sw : {1, 2, 4})
             if ((n == 1 || (p.doc && chunks >= 8)) && cost(sw, n) < cost(best, segments)) best = sw, segments = n;
-    if (best == 1) return run(integral_constant<int, 1>{}, segments);
-    return best == 2 ? run(integral_constant<int, 2>{}, segments) : run(integral_constant<int, 4>{}, segments);
+    const auto with = [&](auto parts) {
+        if (best == 1) return run(integral_constant<int, 1>{}, parts);
+        return best == 2 ? run(integral_constant<int, 2>{}, parts) : run(integral_constant<int, 4>{}, parts);
+    };
+    return segments == 2 ? with(std::true_type()) : with(std::false_type());
 }
 
 }  // namespace

@@ -29,12 +29,12 @@ template <class E> DEVINL f32x4 gradients32(const Two32& a, const Gradients<E>& 
     } else return mma32(a, join(b.x, d.x), c);
 }
 
-template <class E, int D, int SW, int HELPERS>
-__global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_delta_args p, const int pieces, const int segments, float* states, float* updates) {
+template <class E, int D, int SW, int HELPERS, bool PARTS>
+__global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_delta_args p, const int pieces, float* states, float* updates) {
     using L = WalkPlace<D, SW, true>;
     __shared__ __align__(16) char smem[L::BYTES];
     const lds_t lds = lds_of(smem);
-    const int slot = blockIdx.x >> 3, piece = slot % pieces, segment = slot / pieces % segments, hb = slot / pieces / segments * 8 + (blockIdx.x & 7);
+    const int slot = blockIdx.x >> 3, piece = slot % pieces, segment = PARTS ? slot / pieces % 2 : 0, hb = slot / pieces / (PARTS ? 2 : 1) * 8 + (blockIdx.x & 7);
     if (hb >= p.B * p.H) return;
     const int b = hb / p.H, h = hb % p.H, hk = h / (p.H / p.Hk), N = p.N, T = p.T, chunks = (T + DELTA_CHUNK - 1) / DELTA_CHUNK;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, grp = lane >> 4;
@@ -42,7 +42,7 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_d
     // the chunks of this workgroup, downwards, and whether the first of them is its own
     int start = chunks - 1, count = chunks;
     bool first_own = true;
-    if (segments == 2) {
+    if constexpr (PARTS) {
         __shared__ int best;
         const int at = split_at(p.doc + wide(b) * T, T, chunks, &best);
         if (at <= 0) {
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_d
         __syncthreads();
         __syncthreads();
         for (int c = 0; c < count; ++c) {
-            const bool own = first_own || c > 0;
+            const bool own = !PARTS || first_own || c > 0;
             const lds_t rows = lds + (c & 1) * L::STAGE, mats = lds + L::MATRICES + (c & 1) * L::MATRIX_STAGE, sc = lds + L::SCALARS + c % 3 * Scalars::BYTES;
             const lds_t K = rows + L::K, Q = rows + L::Q, A = mats + L::A, P = mats + L::P, inv = mats + L::INV;
             const int64_t chunk = wide(hb) * chunks + start - c;
@@ -200,12 +200,13 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_d
 }
 
 template <class E, int D> int run(hipStream_t st, const rwkv_delta_args& p, float* dS, float* dZ) {
-    return walk_width(p, [&](auto sw, const int segments) {
+    return walk_width(p, [&](auto sw, auto parts) {
         constexpr int SW = decltype(sw)::value;
+        constexpr bool PARTS = decltype(parts)::value;
         const int pieces = (p.N + 16 * SW - 1) / (16 * SW);
-        const int64_t blocks = (static_cast<int64_t>(p.B) * p.H + 7) / 8 * 8 * pieces * segments;
+        const int64_t blocks = (static_cast<int64_t>(p.B) * p.H + 7) / 8 * 8 * pieces * (PARTS ? 2 : 1);
         if (blocks > INT_MAX) return static_cast<int>(RWKV_ERR_SHAPE);
-        hipLaunchKernelGGL((delta_bwd<E, D, SW, 8 - SW>), dim3(static_cast<unsigned>(blocks)), dim3(512), 0, st, p, pieces, segments, dS, dZ);
+        hipLaunchKernelGGL((delta_bwd<E, D, SW, 8 - SW, PARTS>), dim3(static_cast<unsigned>(blocks)), dim3(512), 0, st, p, pieces, dS, dZ);
         return launch_status();
     });
 }

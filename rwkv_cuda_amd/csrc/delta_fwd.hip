@@ -12,13 +12,13 @@
 namespace rwkv {
 namespace {
 
-template <class E, int D, int SW, int HELPERS>
-__global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_delta_args p, const int pieces, const int segments) {
+template <class E, int D, int SW, int HELPERS, bool PARTS>
+__global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_delta_args p, const int pieces) {
     using L = WalkPlace<D, SW, false>;
     __shared__ __align__(16) char smem[L::BYTES];
     const lds_t lds = lds_of(smem);
     // the pieces of a head are neighbours on one XCD: they read the same keys and queries
-    const int slot = blockIdx.x >> 3, piece = slot % pieces, segment = slot / pieces % segments, hb = slot / pieces / segments * 8 + (blockIdx.x & 7);
+    const int slot = blockIdx.x >> 3, piece = slot % pieces, segment = PARTS ? slot / pieces % 2 : 0, hb = slot / pieces / (PARTS ? 2 : 1) * 8 + (blockIdx.x & 7);
     if (hb >= p.B * p.H) return;
     const int b = hb / p.H, h = hb % p.H, hk = h / (p.H / p.Hk), N = p.N, T = p.T, chunks = (T + DELTA_CHUNK - 1) / DELTA_CHUNK;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, grp = lane >> 4;
@@ -26,7 +26,7 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_d
     // the chunks of this workgroup, and whether the first of them is its own
     int start = 0, count = chunks;
     bool first_own = true;
-    if (segments == 2) {
+    if constexpr (PARTS) {
         __shared__ int best;
         const int at = split_at(p.doc + wide(b) * T, T, chunks, &best);
         if (at < 0 || at == chunks - 1) {
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_d
         __syncthreads();
         for (int c = 0; c < count; ++c) {
             const int at = start + c;
-            const bool own = first_own || c > 0;
+            const bool own = !PARTS || first_own || c > 0;
             const lds_t rows = lds + (c & 1) * L::STAGE, mats = lds + L::MATRICES + (c & 1) * L::MATRIX_STAGE, sc = lds + L::SCALARS + c % 3 * Scalars::BYTES;
             const lds_t K = rows + L::K, Q = rows + L::Q, A = mats + L::A, P = mats + L::P, inv = mats + L::INV;
             typedef v4s __attribute__((address_space(3))) * ptr;
@@ -225,12 +225,13 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_d
 }
 
 template <class E, int D> int run(hipStream_t st, const rwkv_delta_args& p) {
-    return walk_width(p, [&](auto sw, const int segments) {
+    return walk_width(p, [&](auto sw, auto parts) {
         constexpr int SW = decltype(sw)::value;
+        constexpr bool PARTS = decltype(parts)::value;
         const int pieces = (p.N + 16 * SW - 1) / (16 * SW);
-        const int64_t blocks = (static_cast<int64_t>(p.B) * p.H + 7) / 8 * 8 * pieces * segments;
+        const int64_t blocks = (static_cast<int64_t>(p.B) * p.H + 7) / 8 * 8 * pieces * (PARTS ? 2 : 1);
         if (blocks > INT_MAX) return static_cast<int>(RWKV_ERR_SHAPE);
-        hipLaunchKernelGGL((delta_fwd<E, D, SW, 8 - SW>), dim3(static_cast<unsigned>(blocks)), dim3(512), 0, st, p, pieces, segments);
+        hipLaunchKernelGGL((delta_fwd<E, D, SW, 8 - SW, PARTS>), dim3(static_cast<unsigned>(blocks)), dim3(512), 0, st, p, pieces);
         return launch_status();
     });
 }
