@@ -137,7 +137,7 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
     const int t = min(t0 + lane, T - 1);
     const float gate = to_f(static_cast<const E*>(p.g)[b * p.g_sb + t * p.g_st + h]), beta_t = to_f(static_cast<const E*>(p.beta)[b * p.beta_sb + t * p.beta_st + h]);
     const DeltaToken token = delta_token(p.doc, wide(b) * T, t0 + lane, T);
-    const uint64_t real = __ballot(token.real);
+    const uint64_t real = __ballot(token.real), cuts = __ballot(token.cut || (token.real && gate < DELTA_NONE));
     const auto mask_of = [&](const int row) { return 0u - static_cast<uint32_t>(real >> (row & 63) & 1); };
     const lds_t sc = lds + L::SCALARS;
 
@@ -404,14 +404,16 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
         if (n <= lane >> 4) after += lds_ld<float>(lds + L::ROW + 256 * n + 4 * lane), db += lds_ld<float>(lds + L::BETA + 256 * n + 4 * lane);
         if (n >= lane >> 4) after -= lds_ld<float>(lds + L::COLUMN + 256 * n + 4 * lane);
     }
+    // (what passes token t ends at the next cut, and began behind the last: added up across them, others' sums would cancel but to their rounding)
     float suffix = after, prefix = before;
+    const int until = cuts >> lane >> 1 ? lane + 1 + __builtin_ctzll(cuts >> lane >> 1) : min(64, T - t0), since = 63 - __builtin_clzll((cuts & (2ull << lane) - 1) | 1);
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) {
         const float a = __shfl_down(suffix, x, 64), c = __shfl_up(prefix, x, 64);
-        if (lane + x < min(64, T - t0)) suffix += a;
-        if (lane >= x) prefix += c;
+        if (lane + x < until) suffix += a;
+        if (lane - x >= since) prefix += c;
     }
-    const bool counts = token.real && !token.cut && !(gate < DELTA_NONE);
+    const bool counts = token.real && !(cuts >> lane & 1);
     const int64_t token_at = (wide(b) * T + t0 + lane) * p.H + h;
     static_cast<E*>(p.dg)[token_at] = from_f<E>(counts ? suffix + (prefix - before) + ends * lds_ld<float>(at(Scalars::ENTER, 63)) : 0.f);
     static_cast<E*>(p.dbeta)[token_at] = from_f<E>(db);

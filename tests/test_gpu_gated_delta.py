@@ -285,3 +285,37 @@ def test_what_memory_held_before_counts_nowhere(lib, N, kind, dtype):
         got = [y.detach(), sT.detach(), *torch.autograd.grad((y, sT), leaves, (dy, dsT))]
         first = got if first is None else first
         assert all(torch.equal(a, b) for a, b in zip(first, got)), value
+
+
+def rows_of(lengths, T, pad=None):
+    """[1,T] of documents of these lengths, `pad` (begin, end) of it padding."""
+    doc = torch.cat([torch.full((n,), i, dtype=torch.int32) for i, n in enumerate(lengths)])
+    assert doc.numel() == T
+    if pad:
+        doc[pad[0]:pad[1]] = -1
+    return doc[None]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_gate_gradients_of_documents_beside_each_other(lib, dtype):
+    """What a document's gradients are does not depend on the others of its 64 tokens: none where it has no dy, however large theirs are, and as exact as alone where they are a millionth."""
+    lengths = [20, 12, 17, 15, 40, 30]
+    T = sum(lengths)
+    doc = rows_of(lengths, T).to(DEV)
+    t, _, dy, _ = inputs(1, T, 3, 3, 64, DT[dtype], seed=17)
+    t[3][:, 25] = -110.0                                         # (a decay of nothing is where a document might begin)
+    dy[:, 32:49] = 0
+    dy[:, 64:104] *= 2.0 ** -10
+    dy[:, :20] *= 2.0 ** 6
+    leaves = [z.requires_grad_(True) for z in t]
+    y, _ = G.RUN_CUDA(*leaves, doc=doc)
+    got = dict(zip(NAMES, torch.autograd.grad(y, leaves, dy)))
+    want = O.gated_delta(*t, doc=doc, dy=dy)
+    at = 0
+    for n in lengths:
+        print(f"\n{n} tokens from {at} on", flush=True)
+        for name in got:
+            if not dy[:, at:at + n].any():
+                assert not got[name][:, at:at + n].any(), name
+            near(name, got[name][:, at:at + n], want[name][:, at:at + n], steps=2.0)
+        at += n
