@@ -187,6 +187,8 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_d
             }
             __syncthreads();
         }
+        if (c0 < N && __ballot(!finite(S[0][0])) != 0ull &&         // something that is no number is in all of its column by now
+            walk_by_token<E, D, true>((DeltaArguments*)__builtin_amdgcn_kernarg_segment_ptr(), hb, start, count, c0, !PARTS || first_own, states, updates)) return;
         if (on && p.ds0 && start + 1 == count)
 #pragma unroll
             for (int t = 0; t < D / 16; ++t)

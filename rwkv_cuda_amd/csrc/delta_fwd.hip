@@ -212,6 +212,8 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_d
                     if (at * DELTA_CHUNK + 16 * i + col < T && c0 + 4 * grp < N) out(i);
             __syncthreads();
         }
+        if (c0 < N && __ballot(!finite(S[0][0])) != 0ull &&         // something that is no number is in all of its column by now
+            walk_by_token<E, D, false>((DeltaArguments*)__builtin_amdgcn_kernarg_segment_ptr(), hb, start, count, c0, !PARTS || first_own, static_cast<float*>(p.saved), updates)) return;
         if (on && start + count == chunks)
 #pragma unroll
             for (int t = 0; t < D / 16; ++t)

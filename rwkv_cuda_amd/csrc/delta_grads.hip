@@ -22,13 +22,6 @@ DEVINL float row_sum(float x) {                                 // over 16 lanes
     x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x122, 0xf, 0xf, true));
     return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x121, 0xf, 0xf, true));
 }
-DEVINL float group_sum4(const float x) {                        // over the four lanes with the same lane & 15
-    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    const float y = __uint_as_float(s[0]) + __uint_as_float(s[1]);
-    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
-    return __uint_as_float(t[0]) + __uint_as_float(t[1]);
-}
-DEVINL float sum4(const f32x4 x) { return (x[0] + x[1]) + (x[2] + x[3]); }
 
 // Inputs as operands: one number of bf16, or two for fp16 (8 and 3 of its 11 bits)
 template <class E> struct Input {
@@ -63,6 +56,13 @@ template <class E> DEVINL f32x4 mma_in(const Input<E>& a, const Input<E>& b, f32
         c = mma32<bf16_t>(a.x[1], b.x[0], c);
     }
     return mma32<bf16_t>(a.x[0], b.x[0], c);
+}
+
+// infinities and NaN of bf16 as zeros
+DEVINL u32x4 finite_ones(u32x4 x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] &= ((x[i] & 0x7f80) == 0x7f80 ? 0u : 0xffffu) | ((x[i] >> 16 & 0x7f80) == 0x7f80 ? 0u : 0xffff0000u);
+    return x;
 }
 
 // 32 value channels by WIDTH tokens or key channels in LDS, two planes.  Tiles of a row, and their halves, are exchanged with the row's number, so that neither the writes (16 rows, 16 bytes) nor the
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
     const int t = min(t0 + lane, T - 1);
     const float gate = to_f(static_cast<const E*>(p.g)[b * p.g_sb + t * p.g_st + h]), beta_t = to_f(static_cast<const E*>(p.beta)[b * p.beta_sb + t * p.beta_st + h]);
     const DeltaToken token = delta_token(p.doc, wide(b) * T, t0 + lane, T);
-    const uint64_t real = __ballot(token.real), cuts = __ballot(token.cut || (token.real && gate < DELTA_NONE));
+    const uint64_t real = __ballot(token.real);
     const auto mask_of = [&](const int row) { return 0u - static_cast<uint32_t>(real >> (row & 63) & 1); };
     const lds_t sc = lds + L::SCALARS;
 
@@ -191,7 +191,16 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
         }
     };
     load(0);
-    if (wave == 0) make_scalars(sc, lane, token, gate, beta_t);
+    // Documents do not see each other, whatever stands in them: pairs across a cut, and states beyond one, are left out (a 0 would not do beside an infinity), and where there is a cut or padding, queries, keys and
+    // gates that are no numbers become zeros: their document's states, updates and gradients are no numbers already, and the sums over tokens hold the others' too.
+    const uint64_t cuts = __ballot(token.cut || (token.real && gate < DELTA_NONE));                // (not before the loads above are on their way)
+    const bool apart = cuts != 0ull || __ballot(t0 + lane < T && !token.real) != 0ull;
+    const auto upto = [](const int n) { return (2ull << n) - 1; };                                 // bits 0 .. n
+    const auto pairs_of = [&](const int n) {                                                       // tokens up to n that n sees
+        const uint64_t here = upto(n), cut = cuts & here;
+        return real >> n & 1 ? real & here & (cut ? ~0ull << (63 - __builtin_clzll(cut)) : ~0ull) : 0ull;
+    };
+    if (wave == 0) make_scalars(sc, lane, token, apart && !finite(gate) && !(gate < DELTA_NONE) ? 0.f : gate, beta_t);
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
         const int row = row0 + BELOW * i;
@@ -275,6 +284,10 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
         }
     }
     __syncthreads();
+    if (apart) {
+        for (lds_t x = lds + L::K + 16 * tid; x < lds + L::SLICES; x += 16 * LANES) lds_st(x, finite_ones(lds_ld<u32x4>(x)));
+        __syncthreads();
+    }
 
     // the pairs: rows j of a block and its column i in the lanes
     const auto at = [&](const lds_t what, const int n) { return sc + what + 4 * n; };
@@ -282,6 +295,7 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
     for (int m = 0; m < OWN; ++m) {
         const int i = pi, j = pj(m), ti = 16 * i + col, tj = 16 * j + 4 * grp;
         if (j > i) continue;
+        const uint32_t seen = static_cast<uint32_t>(pairs_of(ti) >> tj);                           // bit r: token tj + r
         f32x4 kk = zero4(), qk = zero4();
 #pragma unroll
         for (int s = 0; s < D / 32; ++s) {
@@ -297,7 +311,7 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
         if (i == j) {
             const f32x4 hj = lds_ld<f32x4>(at(Scalars::SUM, tj)), lj = lds_ld<f32x4>(at(Scalars::REST, tj));
 #pragma unroll
-            for (int r = 0; r < 4; ++r) d[r] = ti >= tj + r ? __builtin_amdgcn_exp2f((h - hj[r]) + (l - lj[r])) : 0.f;
+            for (int r = 0; r < 4; ++r) d[r] = seen >> r & 1 ? __builtin_amdgcn_exp2f((h - hj[r]) + (l - lj[r])) : 0.f;
         } else {
             const int end = 16 * j + 15;
             d = lds_ld<f32x4>(at(Scalars::TAIL, tj)) * __builtin_amdgcn_exp2f((h - lds_ld<float>(at(Scalars::SUM, end))) + (l - lds_ld<float>(at(Scalars::REST, end))));
@@ -306,10 +320,10 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
         float db = 0.f;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const bool below = ti > tj + r;
-            dp[r] = ti >= tj + r ? p.scale * d[r] * dP[m][r] : 0.f;
+            const bool sees = seen >> r & 1, below = sees && ti > tj + r;
+            dp[r] = sees ? p.scale * d[r] * dP[m][r] : 0.f;
             const float da = below ? -d[r] * dA[m][r] : 0.f;
-            ab[r] = beta * da;
+            ab[r] = below ? beta * da : 0.f;
             db = fmaf(da, kk[r], db);
             pair[r] = below ? dp[r] * qk[r] + ab[r] * kk[r] : 0.f;
         }
@@ -360,9 +374,10 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
         const int ti = 16 * i + col;
         const float enter = lds_ld<float>(at(Scalars::ENTER, ti)), leave = lds_ld<float>(at(Scalars::LEAVE, ti)), beta = lds_ld<float>(at(Scalars::BETA, ti));
         const f32x4 q4 = four(lds + L::Q, ti), k4 = four(lds + L::K, ti);
-        dQ[i] *= p.scale * enter;
-        dK[i] *= leave;
-        R[i] *= enter;
+        const bool is = real >> ti & 1, enters = is && !(cuts & upto(ti)), leaves = is && !(cuts >> ti >> 1);
+        dQ[i] = enters ? dQ[i] * (p.scale * enter) : zero4();
+        dK[i] = leaves ? dK[i] * leave : zero4();
+        R[i] = enters ? R[i] * enter : zero4();
         const float queries = group_sum4(sum4(q4 * dQ[i])), keys = group_sum4(sum4(k4 * dK[i])), reads = group_sum4(sum4(k4 * R[i]));
         if (grp == 0) lds_st(lds + L::QUERIES + 256 * wave + 4 * ti, queries), lds_st(lds + L::KEYS + 256 * wave + 4 * ti, keys), lds_st(lds + L::READS + 256 * wave + 4 * ti, reads);
         dK[i] -= beta * R[i];
@@ -415,7 +430,7 @@ __global__ __launch_bounds__(4 * D, 2) void delta_grads(const rwkv_delta_args p,
     }
     const bool counts = token.real && !(cuts >> lane & 1);
     const int64_t token_at = (wide(b) * T + t0 + lane) * p.H + h;
-    static_cast<E*>(p.dg)[token_at] = from_f<E>(counts ? suffix + (prefix - before) + ends * lds_ld<float>(at(Scalars::ENTER, 63)) : 0.f);
+    static_cast<E*>(p.dg)[token_at] = from_f<E>(counts ? suffix + (prefix - before) + (cuts ? 0.f : ends * lds_ld<float>(at(Scalars::ENTER, 63))) : 0.f);
     static_cast<E*>(p.dbeta)[token_at] = from_f<E>(db);
 }
 

@@ -8,7 +8,9 @@ dense, the other strides multiples of 8 (views of one projection).  g (a log dec
 grow, and e to the sum of 64 of them in a row must be an fp32 number.
 
 `doc` [B,T] int32 names the document of each token of a packed or padded batch, as for gated_recurrence.RUN_CUDA: where it changes, a
-document starts from a state of zero; a negative one is padding, whose y is 0 and which leaves the state as it is, whatever stands there."""
+document starts from a state of zero; a negative one is padding, whose y is 0 and which leaves the state as it is, whatever stands there.  Not even an
+infinity or NaN passes from one document to another, in either direction, nor a decay of nothing; within its document it may reach up to 63 tokens before it
+(behind it, in the gradients).  Rows with such values are done again token by token where they have documents, padding or decays of nothing: some 2 us a token."""
 
 import torch
 

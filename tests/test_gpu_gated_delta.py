@@ -319,3 +319,73 @@ def test_gate_gradients_of_documents_beside_each_other(lib, dtype):
                 assert not got[name][:, at:at + n].any(), name
             near(name, got[name][:, at:at + n], want[name][:, at:at + n], steps=2.0)
         at += n
+
+
+@pytest.mark.parametrize("H,N,dtype", [(2, 64, "bf16"), (4, 128, "fp16"), (3, 40, "bf16")])
+@pytest.mark.parametrize("lengths,pad", [([2, 2], None), ([4, 5, 3], (7, 9)), ([64, 64, 64], None), ([10, 54, 36, 50], (140, 150)), ([30, 9, 9, 9, 73], None), ([300, 100, 240, 128], (380, 410))])
+def test_what_is_no_number_stays_in_its_document(lib, lengths, pad, H, N, dtype):
+    """An infinity, a NaN or a state that overflows in one document, whatever it comes from: the others' outputs and gradients are those without it, padding has none."""
+    T, dt = sum(lengths), DT[dtype]
+    doc = rows_of(lengths, T, pad).to(DEV)
+    t, s0, dy, dsT = inputs(1, T, H, 1 if H == 3 else 2, N, dt, seed=T)
+    want = O.gated_delta(*t, s0=s0, doc=doc, dy=dy, dsT=dsT)
+    begins = [sum(lengths[:i]) for i in range(len(lengths))]
+    for bad in range(len(lengths)):
+        real = [i for i in range(begins[bad], begins[bad] + lengths[bad]) if int(doc[0, i]) >= 0]
+        at, last = real[len(real) // 2], real[-1]
+        for what in ("q", "k", "v", "g", "grows", "beta", "dy", "s0", "dsT"):
+            if (what == "s0" and bad > 0) or (what == "dsT" and bad + 1 < len(lengths)) or (what == "grows" and len(real) < 12):
+                continue
+            print(f"\n{lengths} H={H} N={N} {dtype}: document {bad}, {what}", flush=True)
+            x = dict(zip(("q", "k", "v", "g", "beta", "s0", "dy", "dsT"), [z.clone() for z in (*t, s0, dy, dsT)]))
+            if what == "grows":
+                x["k"][0, real[0]:last + 1] *= 1e15 if dt == torch.bfloat16 else 1e3
+            elif what in ("s0", "dsT"):
+                x[what][0, 0, 1, 3] = float("inf")
+            elif what in ("g", "beta"):
+                x[what][0, at, 0] = float("nan") if what == "beta" else float("inf")
+            else:
+                x[what][0, at, 0, 1] = float("nan") if what == "k" else float("inf")
+            leaves = [x[n].requires_grad_(True) for n in ("q", "k", "v", "g", "beta", "s0")]
+            y, sT = G.RUN_CUDA(*leaves, doc)
+            got = dict(zip(("y", "sT") + NAMES, (y, sT, *torch.autograd.grad([y, sT], leaves, [x["dy"], x["dsT"]]))))
+            y0, s1 = G.RUN_CUDA(*[z.detach() for z in leaves], doc)      # (another way for a few tokens)
+            torch.cuda.synchronize()
+            others = torch.zeros(1, T, dtype=torch.bool, device=DEV)
+            others[0, [i for i in range(T) if int(doc[0, i]) >= 0 and not begins[bad] <= i < begins[bad] + lengths[bad]]] = True
+            for n in got:
+                if n in ("sT", "ds0"):
+                    if bad != (len(lengths) - 1 if n == "sT" else 0):
+                        near(n, got[n], want[n])
+                else:
+                    near(n, got[n][others], want[n][others])
+                    assert not got[n][doc < 0].any(), n
+            near("y", y0[others], want["y"][others])
+            assert not y0[doc < 0].any()
+            if bad + 1 < len(lengths):
+                near("sT", s1, want["sT"])
+            if what not in ("q", "dy", "dsT"):                   # ... and is seen there
+                assert not torch.isfinite(y[0, last]).all() and not torch.isfinite(y0[0, last]).all()
+            assert not all(torch.isfinite(got[n][0, begins[bad]:last + 1]).all() for n in ("y", "dq", "dk", "dv", "dg", "dbeta"))
+
+
+@pytest.mark.parametrize("T,at", [(4, 2), (60, 30), (200, 64), (200, 101)])
+@pytest.mark.parametrize("N,dtype", [(64, "fp16"), (128, "bf16")])
+def test_a_decay_of_nothing_lets_no_infinity_through(lib, T, at, N, dtype):
+    t, s0, dy, dsT = inputs(2, T, 2, 2, N, DT[dtype], seed=19)
+    t[3][:, at] = -float("inf")
+    want = O.gated_delta(*t, s0=s0, dy=dy, dsT=dsT)
+    for before in (True, False):
+        x = [z.clone() for z in (*t, s0, dy, dsT)]
+        if before:
+            x[2][:, at - 2], x[5][0, 1, 2, 3] = float("inf"), float("nan")
+        else:
+            x[6][:, at + 1], x[7][0, 1, 2, 3] = -float("inf"), float("nan")
+        leaves = [z.requires_grad_(True) for z in x[:6]]
+        y, sT = G.RUN_CUDA(*leaves)
+        got = dict(zip(("y", "sT") + NAMES, (y, sT, *torch.autograd.grad([y, sT], leaves, x[6:]))))
+        rest = slice(at, None) if before else slice(None, at)
+        for n in got:
+            if n not in ("sT", "ds0"):
+                near(n, got[n][:, rest], want[n][:, rest])
+        near("sT", sT, want["sT"]) if before else near("ds0", got["ds0"], want["ds0"])
