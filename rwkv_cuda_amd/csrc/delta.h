@@ -122,7 +122,12 @@ DEVINL void keep_token(float* updates, const int token, const int col, const flo
     const bf16_t h = from_f<bf16_t>(x);
     to[0] = __builtin_bit_cast(uint16_t, h), to[4] = __builtin_bit_cast(uint16_t, from_f<bf16_t>(x - to_f(h)));
 }
-// Tiles as operands beside an input of type E: bf16 as they are, fp16 times a power of two, whose inverse is what the product is to be multiplied with.
+// Tiles as operands beside an input of type E: bf16 as they are, fp16 times a power of two, whose inverse is what the product is to be multiplied with.  (A value 2^-k of the wave's
+// largest keeps 35 - k bits, 22 at most.  NaN do not count as large; infinities would, so that what comes from outside is made no_infinity: a column with one is NaN after its first product in any case.)
+template <class E, class V> DEVINL V no_infinity(const V x) {
+    if constexpr (std::is_same_v<E, bf16_t>) return x;
+    else return __builtin_elementwise_fma(x, V(0.f), x);
+}
 template <class E, int TILES> struct Beside {
     Two x[TILES];
     float back;

@@ -60,7 +60,7 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_d
 #pragma unroll
         for (int t = 0; t < D / 16; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) S[t][r] = end && on && 16 * t + 4 * grp + r < N ? end[(16 * t + 4 * grp + r) * N + c0 + col] : 0.f;
+            for (int r = 0; r < 4; ++r) S[t][r] = end && on && 16 * t + 4 * grp + r < N ? no_infinity<E>(end[(16 * t + 4 * grp + r) * N + c0 + col]) : 0.f;
         const lds_t vread = L::V + lds + (4 * grp + (col >> 2)) * L::VPITCH + 32 * wave + 8 * (col & 3);
         __syncthreads();
         __syncthreads();
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_d
             X[3] = gradients16(p33, d3, X[3]);
             X[2] = gradients32(p2, d2, d3, X[2]);
             Z[3] = mma16(inv3, split<bf16_t>(X[3]), zero4());
-            w.take({four_of<E>(v[2]) * fa * p.scale, four_of<E>(v[3]) * fb * p.scale});
+            w.take({no_infinity<E>(four_of<E>(v[2])) * fa * p.scale, no_infinity<E>(four_of<E>(v[3])) * fb * p.scale});
             in_order();
             columns(Q, 1);
             const Two32 a1 = Upper<1>::two(A, lane, 1, 1), a0 = Upper<1>::two(A, lane, 0, 1);
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_bwd(const rwkv_d
             X[0] = mma32(a0, z23, X[0]);
             X[0] = gradients32(p0, d0, d1, X[0]);
             X[0] = gradients32(p02, d2, d3, X[0]);
-            w.take({four_of<E>(v[0]) * fa * p.scale, four_of<E>(v[1]) * fb * p.scale});
+            w.take({no_infinity<E>(four_of<E>(v[0])) * fa * p.scale, no_infinity<E>(four_of<E>(v[1])) * fb * p.scale});
             in_order();
             const Two a01 = Upper<1>::one(A, lane, 0, 1), inv0 = Diagonal::row(inv, lane, 0);
             f32x4 ba = betas(2) * factors(2), bb = betas(3) * factors(3);

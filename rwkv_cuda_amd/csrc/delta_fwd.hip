@@ -45,7 +45,7 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_d
 #pragma unroll
         for (int t = 0; t < D / 16; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) S[t][r] = s0 && on && 16 * t + 4 * grp + r < N ? s0[(16 * t + 4 * grp + r) * N + c0 + col] : 0.f;
+            for (int r = 0; r < 4; ++r) S[t][r] = s0 && on && 16 * t + 4 * grp + r < N ? no_infinity<E>(s0[(16 * t + 4 * grp + r) * N + c0 + col]) : 0.f;
         const lds_t vread = L::V + lds + (4 * grp + (col >> 2)) * L::VPITCH + 32 * wave + 8 * (col & 3);
         // outputs: a chunk's place, and a lane's in it
         const int row_bytes = p.H * N * 2;

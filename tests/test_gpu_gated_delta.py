@@ -389,3 +389,27 @@ def test_a_decay_of_nothing_lets_no_infinity_through(lib, T, at, N, dtype):
             if n not in ("sT", "ds0"):
                 near(n, got[n][:, rest], want[n][:, rest])
         near("sT", sT, want["sT"]) if before else near("ds0", got["ds0"], want["ds0"])
+
+
+def test_infinities_in_one_value_channel_of_fp16(lib):
+    """Value channels do not depend on each other: the others' outputs, states and gradients are those without the infinity."""
+    t, s0, dy, dsT = inputs(2, 200, 3, 3, 64, torch.float16, seed=18)
+    want = O.gated_delta(*t, s0=s0, dy=dy, dsT=dsT)
+    rest = [c for c in range(64) if c != 5]
+    for name in ("v", "s0", "dy", "dsT"):
+        x = dict(v=t[2].clone(), s0=s0.clone(), dy=dy.clone(), dsT=dsT.clone())
+        if name in ("v", "dy"):
+            x[name][:, 100, :, 5] = float("inf")
+        else:
+            x[name][:, :, 7, 5] = -float("inf")
+        leaves = [t[0], t[1], x["v"], t[3], t[4], x["s0"]]
+        for z in leaves:
+            z.requires_grad_(True)
+        y, sT = G.RUN_CUDA(*leaves)
+        dv, ds0 = torch.autograd.grad([y, sT], [leaves[2], leaves[5]], [x["dy"], x["dsT"]])
+        print(f"\n{name}", flush=True)
+        near("y", y[..., rest], want["y"][..., rest])
+        near("sT", sT[..., rest], want["sT"][..., rest])
+        near("dv", dv[..., rest], want["dv"][..., rest])
+        near("ds0", ds0[..., rest], want["ds0"][..., rest])
+        assert not all(torch.isfinite(z[..., 5]).all() for z in (y, sT, dv, ds0))
