@@ -656,7 +656,7 @@ int rwkv_paged_attn(void* stream, const rwkv_paged_args* args);
 /* Gated delta rule: a state of key by value channels for every head, decayed by one gate a token and head and corrected along the token's key:
  *   S = e^g S;  u = beta (v - S^T k);  S += k u^T;  y = scale S^T q.
  * q, k have Hk heads (head h reads head h Hk / H), v, y have H; N is a multiple of 8 up to 128.  The state before the first token is s0, or 0 where
- * that is NULL; sT (may be s0's memory) is the one behind the last.  doc (may be NULL) as for the gated recurrence: padding (doc < 0) has y = 0 and
+ * that is NULL; sT (may be s0's memory, as ds0 may be dsT's) is the one behind the last.  doc (may be NULL) as for the gated recurrence: padding (doc < 0) has y = 0 and
  * leaves the state as it is, whatever stands there; a real token whose predecessor has another doc starts from a state of 0: not even an infinity or NaN of
  * the document before passes (nor, backward, one behind), though within its document it may reach up to 63 tokens on the other side too.  g is a log decay: below
  * -104 it is e^g = 0, which lets nothing pass either.  q, k, v, y and the gates are bf16 or fp16, states fp32; q, k, v are 16-byte aligned with strides that are multiples of 8.

@@ -635,16 +635,19 @@ DEVINL int split_at(const int* doc, const int T, const int chunks, int* best) {
 // 81 88 115;  64: 155 94 116;  128: 309 176 131;  256: 619 350 256
 // With documents two workgroups may share a row: a walk of three quarters of it is reckoned with, and taken where it costs less.  us of the forward, bf16, a row of 3001 tokens, 32 heads of 128, no documents,
 // one, two halves, five: 122 135 76 86;  32 heads of 64 95 100 58 66;  8192 tokens of 8 heads of 64 246 257 135 160;  4 rows of 2048, 16 heads of 64, 69 77 46 53
-template <class Run> int walk_width(const rwkv_delta_args& p, Run run) {
+// `in`, `out`: the states that a walk reads first and writes last; where they share memory a row stays with one workgroup, as two do not wait for each other.
+template <class Run> int walk_width(const rwkv_delta_args& p, const float* in, const float* out, Run run) {
     using std::integral_constant;
     const int64_t heads = static_cast<int64_t>(p.B) * p.H, tiles = (p.N + 15) / 16, chunks = (p.T + DELTA_CHUNK - 1) / DELTA_CHUNK;
     const auto cost = [&](const int sw, const int segments) {
         return (heads * segments * ((tiles + sw - 1) / sw) + 255) / 256 * (sw == 1 ? 8 : (sw == 2 ? 9 : 12)) * (segments == 1 ? 4 * chunks : 3 * chunks + 4);
     };
+    const uintptr_t from = reinterpret_cast<uintptr_t>(in), to = reinterpret_cast<uintptr_t>(out), size = static_cast<uintptr_t>(heads) * p.N * p.N * sizeof(float);
+    const bool parts = p.doc && chunks >= 8 && !(in && out && from < to + size && to < from + size);
     int best = 1, segments = 1;
     for (const int n : {1, 2})
         for (const int sw : {1, 2, 4})
-            if ((n == 1 || (p.doc && chunks >= 8)) && cost(sw, n) < cost(best, segments)) best = sw, segments = n;
+            if ((n == 1 || parts) && cost(sw, n) < cost(best, segments)) best = sw, segments = n;
     const auto with = [&](auto parts) {
         if (best == 1) return run(integral_constant<int, 1>{}, parts);
         return best == 2 ? run(integral_constant<int, 2>{}, parts) : run(integral_constant<int, 4>{}, parts);

@@ -227,7 +227,7 @@ __global__ __launch_bounds__(64 * (SW + HELPERS), 1) void delta_fwd(const rwkv_d
 }
 
 template <class E, int D> int run(hipStream_t st, const rwkv_delta_args& p) {
-    return walk_width(p, [&](auto sw, auto parts) {
+    return walk_width(p, p.s0, p.sT, [&](auto sw, auto parts) {
         constexpr int SW = decltype(sw)::value;
         constexpr bool PARTS = decltype(parts)::value;
         const int pieces = (p.N + 16 * SW - 1) / (16 * SW);

@@ -1,9 +1,11 @@
 """GPU: the gated delta rule against its 64-bit definition."""
+import ctypes
+
 import pytest
 import torch
 
 from oracle import delta as O
-from rwkv_cuda_amd import gated_delta as G
+from rwkv_cuda_amd import _lib, gated_delta as G
 from _delta_util import inputs, near
 from _gpu_util import DEV
 from _mixers_util import DT, doc_ids, graph_of, randn
@@ -413,3 +415,37 @@ def test_infinities_in_one_value_channel_of_fp16(lib):
         near("dv", dv[..., rest], want["dv"][..., rest])
         near("ds0", ds0[..., rest], want["ds0"][..., rest])
         assert not all(torch.isfinite(z[..., 5]).all() for z in (y, sT, dv, ds0))
+
+
+@pytest.mark.parametrize("cuts", [[], [300], [384, 500]])
+@pytest.mark.parametrize("B,T,H,N,dtype", [(1, 768, 4, 64, "bf16"), (1, 1024, 32, 128, "fp16"), (2, 3, 2, 64, "bf16")])
+def test_states_in_place(lib, B, T, H, N, dtype, cuts):
+    """By the C ABI, sT in the memory of s0 and ds0 in that of dsT: the bits of separate tensors, also in rows of documents that two workgroups would walk."""
+    dt = DT[dtype]
+    t, s0, dy, dsT = inputs(B, T, H, H, N, dt, seed=20)
+    doc = torch.zeros(B, T, dtype=torch.int32)
+    for c in cuts:
+        doc[:, c:] += 1
+    doc = doc.to(DEV)
+    q, k, v, g, beta = t
+    wide, gate = (T * H * N, H * N, N), (T * H, H)
+    at = lambda z: None if z is None else z.data_ptr()
+    res = []
+    for place in (False, True):
+        a, b = s0.clone(), dsT.clone()
+        sT, ds0 = (a, b) if place else (torch.full_like(s0, float("nan")), torch.full_like(s0, float("nan")))
+        new = lambda *s: torch.empty(*s, dtype=dt, device=DEV)
+        y, d, dgates = new(B, T, H, N), [new(B, T, H, N) for _ in range(3)], [new(B, T, H) for _ in range(2)]
+        saved = torch.empty(lib.rwkv_delta_saved_bytes(B, T, H, H, N), dtype=torch.uint8, device=DEV)
+        ws = torch.empty(max(16, lib.rwkv_delta_workspace_bytes(B, T, H, H, N, 1)), dtype=torch.uint8, device=DEV)
+        args = _lib.DeltaArgs(dtype=0 if dt == torch.bfloat16 else 1, B=B, T=T, H=H, Hk=H, N=N, scale=0.125, q=at(q), k=at(k), v=at(v), g=at(g), beta=at(beta), s0=at(a), doc=at(doc), y=at(y), sT=at(sT),
+                              saved=at(saved), saved_bytes=saved.numel(), dy=at(dy), dsT=at(b), dq=at(d[0]), dk=at(d[1]), dv=at(d[2]), dg=at(dgates[0]), dbeta=at(dgates[1]), ds0=at(ds0), workspace=at(ws),
+                              workspace_bytes=ws.numel(), **{f"{n}_{s}": x for n in "qkv" for s, x in zip(("sb", "st", "sh"), wide)}, **{f"{n}_{s}": x for n in ("g", "beta") for s, x in zip(("sb", "st"), gate)})
+        stream = torch.cuda.current_stream().cuda_stream
+        assert lib.rwkv_delta_forward(stream, ctypes.byref(args)) == 0 and lib.rwkv_delta_backward(stream, ctypes.byref(args)) == 0
+        torch.cuda.synchronize()
+        res.append([y, sT, *d, *dgates, ds0])
+    want = O.gated_delta(*t, s0=s0, doc=doc, scale=0.125, dy=dy, dsT=dsT)
+    for n, x, z in zip(("y", "sT") + NAMES, *res):
+        assert torch.equal(x, z), n
+        near(n, z, want[n])
