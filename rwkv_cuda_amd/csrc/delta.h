@@ -646,13 +646,12 @@ template <class Run> int walk_width(const rwkv_delta_args& p, const float* in, c
     const bool parts = p.doc && chunks >= 8 && !(in && out && from < to + size && to < from + size);
     int best = 1, segments = 1;
     for (const int n : {1, 2})
-        for (const int sw : {1, 2, 4})
-            if ((n == 1 || parts) && cost(sw, n) < cost(best, segments)) best = sw, segments = n;
-    const auto with = [&](auto parts) {
-        if (best == 1) return run(integral_constant<int, 1>{}, parts);
-        return best == 2 ? run(integral_constant<int, 2>{}, parts) : run(integral_constant<int, 4>{}, parts);
-    };
-    return segments == 2 ? with(std::true_type()) : with(std::false_type());
+        for (const int sw : {1, 2, 4})                           // (four tiles and two workgroups a row never win: two tiles and one take no more rounds, of 9 times 4 chunks against 12 times 3 and more)
+            if ((n == 1 || (parts && sw < 4)) && cost(sw, n) < cost(best, segments)) best = sw, segments = n;
+    using std::true_type, std::false_type;
+    if (segments == 2) return best == 1 ? run(integral_constant<int, 1>{}, true_type()) : run(integral_constant<int, 2>{}, true_type());
+    if (best == 1) return run(integral_constant<int, 1>{}, false_type());
+    return best == 2 ? run(integral_constant<int, 2>{}, false_type()) : run(integral_constant<int, 4>{}, false_type());
 }
 
 }  // namespace

@@ -449,3 +449,16 @@ def test_states_in_place(lib, B, T, H, N, dtype, cuts):
     for n, x, z in zip(("y", "sT") + NAMES, *res):
         assert torch.equal(x, z), n
         near(n, z, want[n])
+
+
+@pytest.mark.parametrize("cuts", [[1], [300, 384], [448], [100, 101, 102, 400, 640], [767]])
+@pytest.mark.parametrize("B,H,Hk,N,dtype", [(1, 32, 16, 128, "bf16"), (1, 32, 32, 120, "fp16"), (2, 32, 8, 64, "fp16"), (1, 64, 64, 40, "bf16")])
+def test_rows_walked_by_two_workgroups_of_two_column_tiles(lib, B, H, Hk, N, dtype, cuts):
+    """As above with as many heads as make workgroups of two tiles the fewest rounds, some of whose channels are behind the last."""
+    T = 768
+    t, s0, dy, dsT = inputs(B, T, H, Hk, N, DT[dtype], seed=N)
+    doc = torch.zeros(B, T, dtype=torch.int32)
+    for c in cuts:
+        doc[:, c:] += 1
+    doc[-1, cuts[0] - 1:cuts[0]] = -1
+    check(t, s0, doc.to(DEV), dy, dsT)
