@@ -2,7 +2,9 @@
 //
 // As paged.hip, with half the bytes: the codes of e4m3 are numbers of bf16 and of fp16 as they stand, so they are widened in registers (two a v_cvt_scalef32_pk) and
 // multiplied on v_mfma_f32_16x16x32.  A key's scale multiplies its score.  A value's scale goes into the weight's exponent, w_j = 2^(s_j + log2 scale_j - m) with m the running
-// maximum of that sum, so that weights stay within 1 in 16 bits whatever the scales, and O = sum w_j code_j; the sum of the softmax is sum w_j / scale_j, in 32 bits.
+// maximum of that sum, so that weights stay within 1 in 16 bits whatever the scales, and O = sum w_j code_j.  The sum of the softmax is the sum of 2^(s_j - r), in 32 bits, with an r of its own: scales may lie 2^220 apart,
+// and w_j / scale_j would be nothing where a page of zeros stands beside large ones.  Y = O 2^(m - r) / sum.  (What a small scale's values lose to 16-bit weights, 2^-24 of the largest in fp16, is less than the
+// large scale's own codes round off.)
 // A lane reads 16 codes of a key at once: of every 64 channels a group of 16 lanes has 16 neighbouring ones, eight for either of two products, and so has the query.
 // Bound by memory where there is work: B64, up to 4096 tokens, H32 Hk32 N64 bf16, 554 MB in 125 to 130 us; B4, up to 131072, H64 Hk8 N128 fp16, 752 MB in 150 to 160 us.
 #include "paged_tile.h"
@@ -33,12 +35,20 @@ template <class E> DEVINL u32x4 widen8(const uint32_t x, const uint32_t y) {
     return u32x4{a[0], a[1], b[0], b[1]};
 }
 
+// A sum of 2^(s - ref) whose ref follows the largest s: far behind, as long as 32 bits hold it (2^31 terms of 2^FAR).
+constexpr float FAR = 64.f;
+DEVINL void raise(float& ref, float& sum, const float most) {
+    const float to = fmaxf(ref, most);
+    sum = to == -INFINITY ? 0.f : sum * __builtin_amdgcn_exp2f(ref - to);
+    ref = to;
+}
+
 template <class E, int D, int W>
 __global__ __launch_bounds__(64 * W, 2) void paged8_attn(const rwkv_paged8_args p, const int shift, const int pieces, const int chunks, const int group, const int shares, float* part) {
     constexpr int ROWS = 64 / (D / 16), VSTEPS = STEP / ROWS;       // rows of an access of a wave, accesses of 32 rows
     __shared__ __align__(16) char smem[W * STEP * 2 * D];
-    __shared__ __align__(16) float scale_of_key[W][STEP], log_of_value[W][STEP], inverse_of_value[W][STEP];
-    __shared__ float top_of[W][HEADS], sum_of[W][HEADS];
+    __shared__ __align__(16) float scale_of_key[W][STEP], log_of_value[W][STEP];
+    __shared__ float top_of[W][HEADS], sum_of[W][HEADS], ref_of[W][HEADS];
     // `group` neighbouring heads (with their chunks) are a share, and an XCD has whole shares; 0: the pieces of a head one after the other
     const int slot = group > 1 ? blockIdx.x >> 3 : blockIdx.x, share = group > 1 ? slot / group * 8 + (blockIdx.x & 7) : slot;
     if (share >= shares) return;
@@ -99,7 +109,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_attn(const rwkv_paged8_args 
     f32x4_t o[D / 16];
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) o[d] = f32x4_t{};
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, ref = -INFINITY, l = 0.f;                   // (ref and l are a lane's own)
     int j0 = static_cast<int>(begin) + wave * STEP;
     if (j0 < end) load(j0);
     for (; j0 < end; j0 += W * STEP) {
@@ -120,13 +130,12 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_attn(const rwkv_paged8_args 
         if (lane < 32) {
             scale_of_key[wave][lane] = kscale;
             log_of_value[wave][lane] = __builtin_amdgcn_logf(vscale);
-            inverse_of_value[wave][lane] = __builtin_amdgcn_rcpf(vscale);
         }
         const uint32_t on = static_cast<uint32_t>(__ballot(on_of));  // which of the 32 tokens count (twice)
         const int now = j0;
         if (j0 + W * STEP < end) load(j0 + W * STEP);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // the wave's own writes above
-        float top = -INFINITY;
+        float top = -INFINITY, most = -INFINITY, x[2][4];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const f32x4_t ks = *reinterpret_cast<const f32x4_t*>(&scale_of_key[wave][16 * e + 4 * grp]), lv = *reinterpret_cast<const f32x4_t*>(&log_of_value[wave][16 * e + 4 * grp]);
@@ -134,10 +143,12 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_attn(const rwkv_paged8_args 
             for (int r = 0; r < 4; ++r) {
                 const int t = 16 * e + 4 * grp + r;
                 const float dot = s[e][r] * ks[r];
-                float x = dot * unit;
-                if (p.cap > 0.f) x = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(dot * in)), -2.f * out, out);
-                x = fmaf(static_cast<float>(all - 1 - now - t), -slope, x) + lv[r];
-                s[e][r] = on >> t & 1 ? x : -INFINITY;
+                float y = dot * unit;
+                if (p.cap > 0.f) y = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(dot * in)), -2.f * out, out);
+                y = fmaf(static_cast<float>(all - 1 - now - t), -slope, y);
+                x[e][r] = on >> t & 1 ? y : -INFINITY;
+                s[e][r] = x[e][r] + lv[r];
+                most = fmaxf(most, x[e][r]);
                 top = fmaxf(top, s[e][r]);
             }
         }
@@ -146,22 +157,20 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_attn(const rwkv_paged8_args 
         if (__ballot(top > m) != 0ull) {
             const float to = fmaxf(top, m), f = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
             m = to;
-            l *= f;
 #pragma unroll
             for (int d = 0; d < D / 16; ++d)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[d][r] *= f;
         }
-        const float base = m == -INFINITY ? 0.f : m;
+        if (__ballot(most > ref + FAR) != 0ull) raise(ref, l, most);
+        const float base = m == -INFINITY ? 0.f : m, low = ref == -INFINITY ? 0.f : ref;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const f32x4_t iv = *reinterpret_cast<const f32x4_t*>(&inverse_of_value[wave][16 * e + 4 * grp]);
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 s[e][r] = __builtin_amdgcn_exp2f(s[e][r] - base);
-                l = fmaf(s[e][r], iv[r], l);
+                l += __builtin_amdgcn_exp2f(x[e][r] - low);
             }
-        }
         const u32x4 w = {pack2<E>(s[0][0], s[0][1]), pack2<E>(s[0][2], s[0][3]), pack2<E>(s[1][0], s[1][1]), pack2<E>(s[1][2], s[1][3])};
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
@@ -173,37 +182,39 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_attn(const rwkv_paged8_args 
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
+    raise(ref, l, fmaxf(__shfl_xor(ref, 16, 64), ref));
+    raise(ref, l, fmaxf(__shfl_xor(ref, 32, 64), ref));
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     __syncthreads();
     float* sums = reinterpret_cast<float*>(smem);                    // [wave][head][D], pieces of four channels of a head turned by the head
-    if (grp == 0) top_of[wave][col] = m, sum_of[wave][col] = l;
+    if (grp == 0) top_of[wave][col] = m, sum_of[wave][col] = l, ref_of[wave][col] = ref;
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4_t*>(sums + (wave * HEADS + col) * D + 4 * ((4 * d + grp) ^ col)) = o[d];
     __syncthreads();
     for (int i = tid; i < HEADS * D / 4; i += 64 * W) {
         const int x = i / (D / 4), c = i % (D / 4), hd = chunk * HEADS + x;
         if (hd >= G || 4 * c >= p.N) continue;
-        float top = -INFINITY;
+        float top = -INFINITY, ref = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < W; ++k) top = fmaxf(top, top_of[k][x]);
-        const float base = top == -INFINITY ? 0.f : top;
+        for (int k = 0; k < W; ++k) top = fmaxf(top, top_of[k][x]), ref = fmaxf(ref, ref_of[k][x]);
+        const float base = top == -INFINITY ? 0.f : top, low = ref == -INFINITY ? 0.f : ref;
         float sum = 0.f;
         f32x4_t y = f32x4_t{};
 #pragma unroll
         for (int k = 0; k < W; ++k) {
             const float f = __builtin_amdgcn_exp2f(top_of[k][x] - base);
-            sum = fmaf(sum_of[k][x], f, sum);
+            sum = fmaf(sum_of[k][x], __builtin_amdgcn_exp2f(ref_of[k][x] - low), sum);
             y += *reinterpret_cast<const f32x4_t*>(sums + (k * HEADS + x) * D + 4 * (c ^ x)) * f;
         }
         const int64_t row = wide(b) * p.H + hk * G + hd;
         if (alone) {
-            const float f = sum == 0.f ? 0.f : 1.f / sum;
-            *reinterpret_cast<u32x2*>(static_cast<E*>(p.y) + row * p.N + 4 * c) = u32x2{pack2<E>(y[0] * f, y[1] * f), pack2<E>(y[2] * f, y[3] * f)};
+            const float f = sum == 0.f ? 0.f : 1.f / sum, g = __builtin_amdgcn_exp2f(0.5f * (base - low));     // (twice: up to 2^(120 + FAR))
+            *reinterpret_cast<u32x2*>(static_cast<E*>(p.y) + row * p.N + 4 * c) = u32x2{pack2<E>(y[0] * f * g * g, y[1] * f * g * g), pack2<E>(y[2] * f * g * g, y[3] * f * g * g)};
         } else {
             float* to = part + (row * pieces + piece) * (D + 4);
             *reinterpret_cast<f32x4_t*>(to + 4 + 4 * c) = y;
-            if (c == 0) to[0] = top, to[1] = sum;
+            if (c == 0) to[0] = top, to[1] = sum, to[2] = ref;
         }
     }
 }
@@ -216,7 +227,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_few(const rwkv_paged8_args p
     constexpr int PER = 16 / TILES, SETS = 4 / TILES, TOKENS = 64, ROWS = 64 / (D / 16), VSTEPS = TOKENS / ROWS, WPITCH = 2 * TOKENS + 16;
     __shared__ __align__(16) char smem[W * STEP * 2 * D];
     __shared__ __align__(16) char weights[W][PER * WPITCH];
-    __shared__ float top_of[W][PER], sum_of[W][PER];
+    __shared__ float top_of[W][PER], sum_of[W][PER], ref_of[W][PER];
     const int slot = group > 1 ? blockIdx.x >> 3 : blockIdx.x, share = group > 1 ? slot / group * 8 + (blockIdx.x & 7) : slot;
     if (share >= shares) return;
     const int of_piece = p.Hk / max(group, 1);
@@ -289,9 +300,9 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_few(const rwkv_paged8_args p
     f32x4_t o[D / 16];
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) o[d] = f32x4_t{};
-    float m[R], l[R];
+    float m[R], ref[R], l[R];                                        // (ref and l are a lane's own)
 #pragma unroll
-    for (int r = 0; r < R; ++r) m[r] = -INFINITY, l[r] = 0.f;
+    for (int r = 0; r < R; ++r) m[r] = ref[r] = -INFINITY, l[r] = 0.f;
     int j0 = static_cast<int>(begin) + wave * TOKENS;
     if (j0 < end) load_pages(j0), load_keys(j0), load_values(j0);
     for (; j0 < end; j0 += W * TOKENS) {
@@ -326,15 +337,15 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_few(const rwkv_paged8_args p
                 to = mma16<E>(q[t % TILES][2 * c + 1], widen8<E>(kr[t][c][2], kr[t][c][3]), to);
             }
         }
-        float ks[SETS], lv[SETS], iv[SETS];
+        float ks[SETS], lv[SETS];
         bool is[SETS];
 #pragma unroll
-        for (int a = 0; a < SETS; ++a) ks[a] = kscale[a], lv[a] = __builtin_amdgcn_logf(vscale[a]), iv[a] = __builtin_amdgcn_rcpf(vscale[a]), is[a] = on[a];
+        for (int a = 0; a < SETS; ++a) ks[a] = kscale[a], lv[a] = __builtin_amdgcn_logf(vscale[a]), is[a] = on[a];
         const int next = j0 + W * TOKENS;
         if (next < end) load_keys(next);
-        float x[SETS][R], top[R];
+        float x[SETS][R], top[R], most[R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) top[r] = -INFINITY;
+        for (int r = 0; r < R; ++r) top[r] = most[r] = -INFINITY;
 #pragma unroll
         for (int a = 0; a < SETS; ++a) {
             const float ago = static_cast<float>(all - 1 - j0 - 16 * TILES * a - own);
@@ -343,14 +354,15 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_few(const rwkv_paged8_args p
                 const float dot = s[a][r] * ks[a];
                 float y = dot * unit;
                 if (p.cap > 0.f) y = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(dot * in)), -2.f * out, out);
-                y = fmaf(ago, -slope[r], y) + lv[a];
+                y = fmaf(ago, -slope[r], y);
                 x[a][r] = is[a] ? y : -INFINITY;
-                top[r] = fmaxf(top[r], x[a][r]);
+                most[r] = fmaxf(most[r], x[a][r]);
+                top[r] = fmaxf(top[r], x[a][r] + lv[a]);
             }
         }
-        bool rises = false;
+        bool rises = false, leaves = false;
 #pragma unroll
-        for (int r = 0; r < R; ++r) rises |= top[r] > m[r];
+        for (int r = 0; r < R; ++r) rises |= top[r] > m[r], leaves |= most[r] > ref[r] + FAR;
         if (__ballot(rises) != 0ull) {
             float f[R], mine = 1.f;
 #pragma unroll
@@ -360,7 +372,6 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_few(const rwkv_paged8_args p
                 to = fmaxf(fmaxf(to, __shfl_xor(to, 32, 64)), m[r]);
                 f[r] = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - to);
                 m[r] = to;
-                l[r] *= f[r];
                 const float other = PER == 4 ? f[r] : __shfl(f[r], col % PER / 4 * 16, 64);
                 mine = R == 1 || (col & 3) == r ? other : mine;
             }
@@ -369,13 +380,16 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_few(const rwkv_paged8_args p
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[d][r] *= mine;
         }
+        if (__ballot(leaves) != 0ull)
+#pragma unroll
+            for (int r = 0; r < R; ++r) raise(ref[r], l[r], most[r]);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const float base = m[r] == -INFINITY ? 0.f : m[r];
+            const float base = m[r] == -INFINITY ? 0.f : m[r], low = ref[r] == -INFINITY ? 0.f : ref[r];
 #pragma unroll
             for (int a = 0; a < SETS; ++a) {
-                const float w = __builtin_amdgcn_exp2f(x[a][r] - base);
-                l[r] = fmaf(w, iv[a], l[r]);
+                const float w = __builtin_amdgcn_exp2f(x[a][r] + lv[a] - base);
+                l[r] += __builtin_amdgcn_exp2f(x[a][r] - low);
                 lds_st(weight + (4 * grp + r) % PER * WPITCH + 2 * (16 * TILES * a + own), __builtin_bit_cast(uint16_t, from_f<E>(w)));
             }
         }
@@ -404,6 +418,9 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_few(const rwkv_paged8_args p
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
+        float to = row_max(ref[r]);
+        if constexpr (TILES == 4) to = fmaxf(to, __shfl_xor(to, 16, 64));
+        raise(ref[r], l[r], fmaxf(to, __shfl_xor(to, 32, 64)));
         l[r] = row_add(l[r]);
         if constexpr (TILES == 4) l[r] += __shfl_xor(l[r], 16, 64);
         l[r] += __shfl_xor(l[r], 32, 64);
@@ -412,7 +429,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_few(const rwkv_paged8_args p
     float* sums = reinterpret_cast<float*>(smem);                    // [wave][head][D], pieces of four channels of a head turned by the head
     if (col == 0 && grp < PER / 4)
 #pragma unroll
-        for (int r = 0; r < R; ++r) top_of[wave][4 * grp + r] = m[r], sum_of[wave][4 * grp + r] = l[r];
+        for (int r = 0; r < R; ++r) top_of[wave][4 * grp + r] = m[r], sum_of[wave][4 * grp + r] = l[r], ref_of[wave][4 * grp + r] = ref[r];
     if (col < PER)
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4_t*>(sums + (wave * PER + col) * D + 4 * ((4 * d + grp) ^ col)) = o[d];
@@ -420,26 +437,26 @@ __global__ __launch_bounds__(64 * W, 2) void paged8_few(const rwkv_paged8_args p
     for (int i = tid; i < G * D / 4; i += 64 * W) {
         const int h = i / (D / 4), c = i % (D / 4);
         if (4 * c >= p.N) continue;
-        float top = -INFINITY;
+        float top = -INFINITY, ref = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < W; ++k) top = fmaxf(top, top_of[k][h]);
-        const float base = top == -INFINITY ? 0.f : top;
+        for (int k = 0; k < W; ++k) top = fmaxf(top, top_of[k][h]), ref = fmaxf(ref, ref_of[k][h]);
+        const float base = top == -INFINITY ? 0.f : top, low = ref == -INFINITY ? 0.f : ref;
         float sum = 0.f;
         f32x4_t y = f32x4_t{};
 #pragma unroll
         for (int k = 0; k < W; ++k) {
             const float f = __builtin_amdgcn_exp2f(top_of[k][h] - base);
-            sum = fmaf(sum_of[k][h], f, sum);
+            sum = fmaf(sum_of[k][h], __builtin_amdgcn_exp2f(ref_of[k][h] - low), sum);
             y += *reinterpret_cast<const f32x4_t*>(sums + (k * PER + h) * D + 4 * (c ^ h)) * f;
         }
         const int64_t row = wide(b) * p.H + hk * G + h;
         if (alone) {
-            const float f = sum == 0.f ? 0.f : 1.f / sum;
-            *reinterpret_cast<u32x2*>(static_cast<E*>(p.y) + row * p.N + 4 * c) = u32x2{pack2<E>(y[0] * f, y[1] * f), pack2<E>(y[2] * f, y[3] * f)};
+            const float f = sum == 0.f ? 0.f : 1.f / sum, g = __builtin_amdgcn_exp2f(0.5f * (base - low));     // (twice: up to 2^(120 + FAR))
+            *reinterpret_cast<u32x2*>(static_cast<E*>(p.y) + row * p.N + 4 * c) = u32x2{pack2<E>(y[0] * f * g * g, y[1] * f * g * g), pack2<E>(y[2] * f * g * g, y[3] * f * g * g)};
         } else {
             float* to = part + (row * pieces + piece) * (D + 4);
             *reinterpret_cast<f32x4_t*>(to + 4 + 4 * c) = y;
-            if (c == 0) to[0] = top, to[1] = sum;
+            if (c == 0) to[0] = top, to[1] = sum, to[2] = ref;
         }
     }
 }
@@ -484,7 +501,7 @@ template <class E, int D, int W> int run(hipStream_t st, const rwkv_paged8_args&
     else if (D == 64 && G == 2) few(integral_constant<int, 4>(), integral_constant<int, D == 64 ? 2 : 1>());
     else if (G <= 8 && (D == 64 || G > 4)) few(integral_constant<int, 2>(), integral_constant<int, 4>());
     else hipLaunchKernelGGL((paged8_attn<E, D, W>), dim3(static_cast<unsigned>(grid)), dim3(64 * W), 0, st, p, shift, pieces, chunks, group, static_cast<int>(shares), part);
-    if (pieces > 1) hipLaunchKernelGGL((paged_join<rwkv_paged8_args, E, D>), dim3(p.H, p.B), dim3(256), 0, st, p, shift, pieces, part);
+    if (pieces > 1) hipLaunchKernelGGL((paged_join<rwkv_paged8_args, E, D, true>), dim3(p.H, p.B), dim3(256), 0, st, p, shift, pieces, part);
     return launch_status();
 }
 template <class E> int run_any(hipStream_t st, const rwkv_paged8_args& p) {

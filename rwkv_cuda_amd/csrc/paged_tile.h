@@ -23,28 +23,32 @@ DEVINL int piece_of(const int n, const int pieces) { return max(1, (n + pieces *
 // 32 rows of D values: piece c of row r at place c ^ swap(r), so that 16 rows of two pieces are spread over all banks
 template <int D> DEVINL lds_t value_at(const int r, const int c) { return r * 2 * D + ((c ^ (D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3))) << 4); }
 
-// joins the pieces of a head: 256 threads, four channels a thread, the pieces dealt out
-template <class Args, class E, int D> __global__ __launch_bounds__(256) void paged_join(const Args p, const int shift, const int pieces, const float* part) {
+// joins the pieces of a head: 256 threads, four channels a thread, the pieces dealt out.  A piece is its maximum, sum and (APART: what the sum's terms are relative to, with the outputs' maximum beside it) output.
+template <class Args, class E, int D, bool APART = false> __global__ __launch_bounds__(256) void paged_join(const Args p, const int shift, const int pieces, const float* part) {
     constexpr int LANES = D / 4, SETS = 256 / LANES;
     __shared__ __align__(16) float sums[SETS][D];
-    __shared__ float total[SETS], tops[4];
+    __shared__ float total[SETS], tops[4], refs[4];
     const int h = blockIdx.x, b = blockIdx.y, c = threadIdx.x % LANES, set = threadIdx.x / LANES;
     const int n = tokens_of(p, b, shift), size = piece_of(n, pieces), used = n <= 0 ? 0 : (n + size - 1) / size;
     const int64_t row = wide(b) * p.H + h;
     const float* from = part + row * pieces * (D + 4);
-    float top = threadIdx.x < used ? from[wide(threadIdx.x) * (D + 4)] : -INFINITY;
+    float top = threadIdx.x < used ? from[wide(threadIdx.x) * (D + 4)] : -INFINITY, ref = APART && threadIdx.x < used ? from[wide(threadIdx.x) * (D + 4) + 2] : -INFINITY;
 #pragma unroll
-    for (int x = 32; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
-    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    for (int x = 32; x >= 1; x >>= 1) {
+        top = fmaxf(top, __shfl_xor(top, x, 64));
+        if (APART) ref = fmaxf(ref, __shfl_xor(ref, x, 64));
+    }
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top, refs[threadIdx.x >> 6] = ref;
     __syncthreads();
     top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    const float base = top == -INFINITY ? 0.f : top;
+    ref = fmaxf(fmaxf(refs[0], refs[1]), fmaxf(refs[2], refs[3]));
+    const float base = top == -INFINITY ? 0.f : top, low = ref == -INFINITY ? 0.f : ref;
     f32x4_t y = f32x4_t{};
     float sum = 0.f;
     for (int i = set; i < used; i += SETS) {
         const float* x = from + wide(i) * (D + 4);
         const float f = __builtin_amdgcn_exp2f(x[0] - base);
-        sum = fmaf(x[1], f, sum);
+        sum = fmaf(x[1], APART ? __builtin_amdgcn_exp2f(x[2] - low) : f, sum);
         if (4 * c < p.N) y += *reinterpret_cast<const f32x4_t*>(x + 4 + 4 * c) * f;
     }
     *reinterpret_cast<f32x4_t*>(&sums[set][4 * c]) = y;
@@ -56,7 +60,10 @@ template <class Args, class E, int D> __global__ __launch_bounds__(256) void pag
             sum += total[k];
         }
         const float f = sum == 0.f ? 0.f : 1.f / sum;
-        *reinterpret_cast<u32x2*>(static_cast<E*>(p.y) + row * p.N + 4 * c) = u32x2{pack2<E>(y[0] * f, y[1] * f), pack2<E>(y[2] * f, y[3] * f)};
+        const float g = APART ? __builtin_amdgcn_exp2f(0.5f * (base - low)) : 1.f;
+        if (APART) y = y * f * g * g;
+        if (APART) *reinterpret_cast<u32x2*>(static_cast<E*>(p.y) + row * p.N + 4 * c) = u32x2{pack2<E>(y[0], y[1]), pack2<E>(y[2], y[3])};
+        else *reinterpret_cast<u32x2*>(static_cast<E*>(p.y) + row * p.N + 4 * c) = u32x2{pack2<E>(y[0] * f, y[1] * f), pack2<E>(y[2] * f, y[3] * f)};
     }
 }
 

@@ -325,3 +325,22 @@ def test_what_memory_held_before_counts_nowhere(lib, H, Hk, N, lens):
             torch.cuda.synchronize()
             del held
         assert torch.equal(P8.RUN_CUDA(q, *kv, table, lens), want), value
+
+
+@pytest.mark.parametrize("H,Hk,N", [(8, 2, 64), (4, 4, 128), (32, 2, 64), (12, 2, 128)])
+@pytest.mark.parametrize("M", [8, 70, 500])
+def test_scales_as_far_apart_as_there_are(lib, H, Hk, N, M):
+    """Pages of zeros at the least scale beside pages at scales up to 2^110, in one wave and in several, one after the other either way round: every token keeps its share of the softmax's sum."""
+    page, n = 16, 16 * M - 3
+    for small_first in (True, False):
+        for big in (27.0, 60.0, 110.0):
+            q, kv, table, lens = cache([n, n // 2], H, Hk, N, page, torch.bfloat16, seed=M)
+            for b in range(2):
+                pages = table[b, :-(-int(lens[b]) // page)].long()
+                kv[3][pages] = 2.0 ** big
+                zeros = pages[:len(pages) // 2] if small_first else pages[len(pages) // 2:]
+                kv[1].view(torch.uint8)[zeros] = 0
+                kv[3][zeros] = 2.0 ** -100
+            print(f"\nscales 2^-100 and 2^{big}, {'small' if small_first else 'large'} ones first", flush=True)
+            check(q, kv, table, lens)
+            check(q, kv, table, lens, cap=20.0, slopes=torch.exp2(-torch.arange(1.0, H + 1)).to(DEV))
