@@ -690,7 +690,7 @@ int rwkv_delta_backward(void* stream, const rwkv_delta_args* args);
 
 /* A paged cache in 8 bits (e4m3: 4 bits of exponent, 3 of mantissa, largest 448): a value is its code times the scale of its page and head, a power of
  * two.  rwkv_cache8_write puts n tokens into their slots (page number times page size plus the place in the page; a slot outside the cache: the
- * token is left out).  New tokens of a page stand beside each other in the list, and none of its pages comes twice.  The scale is the least power of two, from 2^-100
+ * token is left out).  New tokens of a page stand beside each other in the list, without one that is left out between them, and none of its pages comes twice.  The scale is the least power of two, from 2^-100
  * on, that holds the finite values; where a page holds tokens before the first new one its scale does not fall, and where it grows those are rounded again.  What is
  * not finite becomes NaN.  N is a multiple of 16 up to 128, page a power of two; rows of the pages are 16-byte aligned. */
 typedef struct rwkv_cache8_args {

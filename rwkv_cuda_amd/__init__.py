@@ -18,7 +18,7 @@ and, without a counterpart there, what hybrid models put beside them:
     gated_delta       RUN_CUDA(q,k,v,g,beta,s0,doc) -> (y, sT), STEP bf16, fp16; matrix-valued state, a decay and a step a head
     paged_attention   RUN_CUDA(q,k_pages,v_pages,table,lens,k,v)     bf16, fp16; one token a sequence, for serving
     paged_attention8  WRITE(k,v,k_pages,v_pages,...), RUN_CUDA       the same over a cache in 8 bits
-    page_tables       EXTEND(lens,more,table,pool,taken,page,n)      tables and slots for both, from the requests' lengths
+    page_tables       EXTEND(lens,more,table,pool,taken,page,n)      tables for both, slots for the second, from the requests' lengths
 
 There is no CPU or eager fallback: the ops need the compiled library and a HIP device.
 """

@@ -99,6 +99,7 @@ template <class E> __global__ __launch_bounds__(256) void delta_sum(const rwkv_d
 
 // Few tokens go one by one: a chunk costs the same whatever it holds.  us with 1, 2, 4, 6, 8 tokens, 32 heads, a row and 32 rows: heads of 64 3.8 5.2 8.0 10.8 13.6 beside 6.8 of a chunk, and 9.0 12.6
 // 21 29 39 beside 26.5; heads of 128 4.5 6.5 10.0 13.5 17.3 beside 8.4, and 27 36 53 72 90 beside 65 (of whose first 27 are the states, read and written at 4.9 TB/s).
+// One number for all batches, so that a sequence's results do not depend on how many others there are; for a single row 3 would do, where four tokens take 1.2 and 1.6 us longer so.
 constexpr int FEW = 4;
 template <class E> int run_fwd(hipStream_t st, const rwkv_delta_args& p) {
     if (p.saved != nullptr || p.T > FEW) return launch_delta_fwd(st, p);

@@ -1,5 +1,5 @@
-"""Page tables and slots of a batch of requests, made on the GPU from their lengths: what paged_attention and paged_attention8 read and
-paged_attention8.WRITE writes to (no counterpart in the reference)."""
+"""Page tables and slots of a batch of requests, made on the GPU from their lengths: the tables that paged_attention and paged_attention8 read, and the
+slots that paged_attention8.WRITE writes to (no counterpart in the reference)."""
 
 from ._call import ops
 

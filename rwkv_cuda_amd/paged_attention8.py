@@ -8,8 +8,8 @@ from ._call import ops
 
 def WRITE(k, v, k_pages, v_pages, k_scales, v_scales, slots):
     """Puts k, v [n,Hk,N] (bf16 or fp16; strides multiples of 8) into the cache: token i at slots[i] (int32 [n]; as page_tables.EXTEND makes them), that
-    is page slots[i] // page, row slots[i] % page; one outside the cache is left out.  New tokens of a page stand beside each other in the list, no page comes
-    twice in it and no slot.
+    is page slots[i] // page, row slots[i] % page; one outside the cache is left out.  New tokens of a page stand beside each other in the list (with none that
+    is left out between them, either: two runs of a page would race for its scale), no page comes twice in it and no slot.
 
     The scale of a page and head is the least power of two, from 2^-100 on, that holds its finite values up to 448.  Where a page holds tokens before the first
     new one, its scale does not fall, and where it grows they are rounded once more.  What is not finite becomes NaN.  No gradients."""

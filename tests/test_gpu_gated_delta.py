@@ -462,3 +462,39 @@ def test_rows_walked_by_two_workgroups_of_two_column_tiles(lib, B, H, Hk, N, dty
         doc[:, c:] += 1
     doc[-1, cuts[0] - 1:cuts[0]] = -1
     check(t, s0, doc.to(DEV), dy, dsT)
+
+
+@pytest.mark.parametrize("B,T,H,Hk,N,dtype", [(4, 140, 40, 20, 64, "fp16"), (2, 140, 24, 24, 128, "bf16"), (3, 100, 30, 30, 112, "fp16"), (1, 768, 32, 16, 128, "bf16")])
+def test_what_is_no_number_in_one_row_and_head(lib, B, T, H, Hk, N, dtype):
+    """Walks of two and four column tiles, and by two workgroups: other rows and heads keep their bits, other documents of the row are as without it, twice the same."""
+    dt = DT[dtype]
+    t, s0, dy, dsT = inputs(B, T, H, Hk, N, dt, seed=21)
+    doc = torch.zeros(B, T, dtype=torch.int32)
+    doc[:, T // 3:] += 1
+    doc[:, T // 2 + 3:] += 1
+    doc = doc.to(DEV)
+
+    def once(t, s0, dy, dsT):
+        leaves = [z.detach().clone().requires_grad_(True) for z in (*t, s0)]
+        y, sT = G.RUN_CUDA(*leaves, doc)
+        return dict(zip(("y", "sT") + NAMES, (y.detach(), sT.detach(), *torch.autograd.grad([y, sT], leaves, [dy, dsT]))))
+    want = once(t, s0, dy, dsT)
+    bad, G_ = H - 1, H // Hk
+    v = t[2].clone()
+    v[B - 1, T // 3 + 7, bad, N - 1] = float("inf")
+    got, again = (once([t[0], t[1], v, *t[3:]], s0, dy, dsT) for _ in range(2))
+    of = lambda n, z: z.transpose(1, 2) if n not in ("sT", "ds0") else z          # [B, heads, ...]
+    exact = O.gated_delta(*[z[B - 1:] for z in t], s0=s0[B - 1:], doc=doc[B - 1:], dy=dy[B - 1:], dsT=dsT[B - 1:])
+    middle = doc[B - 1] == 1
+    for n in want:
+        a, b = of(n, got[n]), of(n, want[n])
+        assert torch.equal(torch.nan_to_num(got[n]), torch.nan_to_num(again[n])), n
+        assert torch.equal(a[:B - 1], b[:B - 1]), n
+        last = bad // G_ if n in ("dq", "dk") else bad
+        assert torch.equal(a[B - 1, :last], b[B - 1, :last]), n
+        assert torch.isfinite(got[n][B - 1]).all() if n in ("sT", "ds0") else torch.isfinite(got[n][B - 1, ~middle]).all(), n
+        if n in ("sT", "ds0"):
+            near(n, got[n][B - 1:], exact[n])
+        else:
+            near(n, got[n][B - 1, ~middle], exact[n][0, ~middle])
+    assert not torch.isfinite(got["y"][B - 1, middle]).all() and not torch.isfinite(got["dk"][B - 1, middle]).all()
